@@ -373,6 +373,61 @@ int ispa_prune_points_2d(double *coords, int B, int64_t n, const uint8_t *flags,
                          int n_vert, const int32_t *segments, const int32_t *n_seg, int max_seg, int thickness,
                          int H, int W, uint8_t *pruned, void *stream);
 
+/* Soft correspondence: softmax-weighted transfer of a template's value map to query cells, the differentiable
+ * counterpart of ispa_nn_topk (not in the reference, whose correlation layers feed a trunk instead).
+ *   x_ij = scale * sum_c q_ci r_cj;   y_ij = cap > 0 ? cap * tanh(x_ij / cap) : x_ij
+ *   z_ij = y_ij - falloff[head] * ((qx_i - jx)^2 + (qy_i - jy)^2),  cell j at (j % W, j / W)
+ *   P = softmax over the cells j that take part;   out_ci = sum_j P_ij v_cj;   lse_i = log sum_j exp(z_ij)
+ * q (B, heads*D, nq), r (B, heads*D, cells), v (B, heads*Dv, cells) of one dtype, ISPA_F32 or ISPA_BF16; head h has
+ * channels [h*D, (h+1)*D).  v NULL: r is the value map too (Dv = D).  D and Dv: 1 to ISPA_SOFT_MAX_CHANNELS.
+ * falloff (heads) f32 or NULL; query_xy (B,nq,2) f32 [x, y] in cells, or NULL: query i lies on cell i.
+ * mask (B,cells) u8 or NULL: a cell with 0 takes no part, whatever its features hold.
+ * num_query (B) i32 or NULL: only the first num_query[b] queries are real.
+ * out (B, heads*Dv, nq) of the dtype; out32 (optional) the same in float32 before its rounding, which the backward call
+ * wants; lse (optional) (B,heads,nq) f32.  A query that is not real or has no cell gets out 0 and lse -inf.
+ * Sums, maxima and log-sums are float32; with ISPA_BF16 the softmax weights are rounded to bfloat16 for the
+ * product with v.  Few queries: the cells are split over workgroups and the parts joined by a second launch, in a fixed
+ * order (results do not change from run to run).  workspace: ispa_soft_match_workspace_bytes(...) with views = 1. */
+#define ISPA_SOFT_MAX_CHANNELS 256
+size_t ispa_soft_match_workspace_bytes(int dtype, int B, int heads, int D, int Dv, int64_t nq, int views, int64_t cells);
+int ispa_soft_match(const void *q, const void *r, const void *v, int dtype, int B, int heads, int D, int Dv, int64_t nq,
+                    int64_t cells, int W, float scale, float cap, const float *falloff, const float *query_xy,
+                    const uint8_t *mask, const int32_t *num_query, void *out, float *out32, float *lse, void *workspace,
+                    size_t workspace_bytes, void *stream);
+
+/* Its gradients.  out32 and lse as the forward call wrote them (ISPA_F32: out itself is out32); d_out of the dtype,
+ * d_lse (optional) (B,heads,nq) f32.  dq, dr, dv have the shapes and dtype of q, r, v; without a value map dv is NULL
+ * and dr holds the sum of both uses.  Masked cells and queries that are not real get gradient 0, and what the latter
+ * hold in q and d_out is not read.  No atomics: two runs agree bit for bit. */
+size_t ispa_soft_match_backward_workspace_bytes(int dtype, int B, int heads, int D, int Dv, int64_t nq, int64_t cells);
+int ispa_soft_match_backward(const void *q, const void *r, const void *v, int dtype, int B, int heads, int D, int Dv,
+                             int64_t nq, int64_t cells, int W, float scale, float cap, const float *falloff,
+                             const float *query_xy, const uint8_t *mask, const int32_t *num_query, const float *out32,
+                             const float *lse, const void *d_out, const float *d_lse, void *dq, void *dr, void *dv,
+                             void *workspace, size_t workspace_bytes, void *stream);
+
+/* Template store: the feature maps of n_view rendered views in 8 bits, for the views proxy_renderer.py:100-106 selects.
+ * codes (n_view,C,cells) int8 (ISPA_STORE_INT8) or e4m3 (ISPA_STORE_FP8); scales (n_view,cells) f32;
+ * mask (n_view,cells) u8 = the cell holds features.  scale = max_c |x_c| * r with r the float32
+ * number next to 1 / 127 (e4m3: 1 / 448), rounded to float32; code = the exact quotient x / scale rounded to the nearest
+ * code value, ties to even; value = code * scale.
+ * write: features (n,C,cells) f32 or bf16 go to views[0..n); take (optional) (n,cells) u8 becomes the mask; a cell with a
+ * non-finite channel is stored as zeros, masked.  A view listed twice keeps its last entry; an index outside
+ * [0, n_view) is skipped.  read: out (n,C,cells) f32 or bf16; an index outside gives zeros. */
+enum { ISPA_STORE_INT8 = 0, ISPA_STORE_FP8 = 1 };
+int ispa_store_write(const void *features, int dtype, const uint8_t *take, const int32_t *views, int n, int kind, int n_view,
+                     int C, int64_t cells, void *codes, float *scales, uint8_t *mask, void *stream);
+int ispa_store_read(const void *codes, const float *scales, const int32_t *views, int n, int kind, int n_view, int C,
+                    int64_t cells, int dtype, void *out, void *stream);
+
+/* ispa_soft_match against stored views, read from their codes: item b matches the cells of views[b,0..V) (views (B,V)
+ * i32) jointly, r = v = their values; an index outside [0, n_view) stands for no view.  C = heads*D.  dtype is that of q
+ * and out.  workspace: ispa_soft_match_workspace_bytes(dtype, B, heads, D, D, nq, V, cells). */
+int ispa_store_match(const void *q, int dtype, const void *codes, const float *scales, const uint8_t *mask, int kind,
+                     const int32_t *views, int V, int n_view, int B, int heads, int D, int64_t nq, int64_t cells, int W,
+                     float scale, float cap, const float *falloff, const float *query_xy, const int32_t *num_query, void *out,
+                     float *lse, void *workspace, size_t workspace_bytes, void *stream);
+
 #ifdef __cplusplus
 }
 #endif

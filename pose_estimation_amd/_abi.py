@@ -23,12 +23,15 @@ NN_NORMALIZE = 256
 NN_NO_PAD = 512
 PCK_MAX_RADII = 8
 PRUNE_POLYGON, PRUNE_BAND, PRUNE_DROP = 1, 2, 4
+SOFT_MAX_CHANNELS = 256
+STORE_INT8, STORE_FP8 = 0, 1
 PRUNE_MAX_VERTICES, PRUNE_MAX_SEGMENTS = 64, 256
 
 _p = ctypes.c_void_p
 _i = ctypes.c_int
 _i64 = ctypes.c_int64
 _d = ctypes.c_double
+_f = ctypes.c_float
 _sz = ctypes.c_size_t
 
 # name -> (restype, argtypes); one entry per declaration in include/ispa_abi.h
@@ -70,6 +73,15 @@ SIGNATURES = {
     "ispa_nearest_view": (_i, [_p, _i, _p, _i, _p, _p, _p]),
     "ispa_pck_counts": (_i, [_p, _i, _i, _i64, _p, _i, _d, _i, _p, _i, _p, _p]),
     "ispa_hard_negatives": (_i, [_p, _i, _i, _i64, _p, _i, _d, _i, _d, _p, _p, _p]),
+    "ispa_soft_match_workspace_bytes": (_sz, [_i, _i, _i, _i, _i, _i64, _i, _i64]),
+    "ispa_soft_match": (_i, [_p, _p, _p, _i, _i, _i, _i, _i, _i64, _i64, _i, _f, _f, _p, _p, _p, _p, _p, _p, _p, _p, _sz, _p]),
+    "ispa_soft_match_backward_workspace_bytes": (_sz, [_i, _i, _i, _i, _i, _i64, _i64]),
+    "ispa_soft_match_backward": (_i, [_p, _p, _p, _i, _i, _i, _i, _i, _i64, _i64, _i, _f, _f, _p, _p, _p, _p, _p, _p, _p, _p,
+                                      _p, _p, _p, _p, _sz, _p]),
+    "ispa_store_write": (_i, [_p, _i, _p, _p, _i, _i, _i, _i, _i64, _p, _p, _p, _p]),
+    "ispa_store_read": (_i, [_p, _p, _p, _i, _i, _i, _i, _i64, _i, _p, _p]),
+    "ispa_store_match": (_i, [_p, _i, _p, _p, _p, _i, _p, _i, _i, _i, _i, _i, _i64, _i64, _i, _f, _f, _p, _p, _p, _p, _p, _p,
+                              _sz, _p]),
     "ispa_prune_points_2d": (_i, [_p, _i, _i64, _p, _p, _i, _p, _p, _i, _i, _i, _i, _p, _p]),
 }
 

@@ -1,0 +1,84 @@
+// Launchers of the backward kernels for one arithmetic (included by soft_backward_f32.hip and soft_backward_bf16.hip).
+#pragma once
+#include "soft_backward.h"
+#include "soft_launch.h"
+
+namespace ispa_soft {
+
+// channels of the gradients that one launch forms
+template <typename T, int DP>
+constexpr int kFormed = DP == 256 && std::is_same_v<T, F32> ? 128 : DP;
+
+template <typename T, int DP, int WQ>
+int dq_one(Params p, hipStream_t stream) {
+    static unsigned long long lds_allowed = 0;
+    const int lds = (p.shared ? 1 : 2) * DP * kRowBytes + 2 * 64 * (int)sizeof(float);
+    const unsigned grid = (unsigned)((int64_t)p.B * p.heads * p.splits * p.blocks);
+    constexpr int NC = kFormed<T, DP>;
+    for (p.c0 = 0; p.c0 < p.D; p.c0 += NC)
+        if (int rc = launch(soft_dq_kernel<T, DP, WQ, NC>, p, grid, 64 * WQ, lds, &lds_allowed, "soft_dq_kernel", stream))
+            return rc;
+    return ISPA_OK;
+}
+
+template <typename T, int DP, int WQ, int PART>
+int dkv_one(Params p, int channels, hipStream_t stream) {
+    static unsigned long long lds_allowed = 0;
+    const int lds = 2 * DP * kRowBytes + 4 * 64 * (int)sizeof(float);
+    const unsigned grid = (unsigned)((int64_t)p.B * p.heads * p.splits * p.blocks);
+    constexpr int NC = PART == 2 ? kFormed<T, DP> : DP;
+    for (p.c0 = 0; p.c0 < channels; p.c0 += NC)
+        if (int rc = launch(soft_dkv_kernel<T, DP, WQ, PART, NC>, p, grid, 64 * WQ, lds, &lds_allowed, "soft_dkv_kernel",
+                            stream))
+            return rc;
+    return ISPA_OK;
+}
+
+template <typename T, int DP, int WQ>
+int dkv_parts(const Params &p, hipStream_t stream) {
+    if constexpr (DP == 256) {
+        if (int rc = dkv_one<T, DP, WQ, 1>(p, p.Dv, stream)) return rc;
+        return dkv_one<T, DP, WQ, 2>(p, p.D, stream);
+    } else {
+        return dkv_one<T, DP, WQ, 0>(p, DP, stream);
+    }
+}
+
+template <typename T>
+int sum_parts(const float *a, const float *b, int splits, int64_t n, float factor, void *out, hipStream_t stream) {
+    soft_sum_kernel<T><<<(unsigned)((n + 255) / 256), 256, 0, stream>>>(a, b, splits, n, factor, (typename T::elem *)out);
+    return ispa::check_launch("soft_sum_kernel");
+}
+
+template <typename T, int DP>
+int backward_sized(Params p, const Plan &dq, const Plan &dkv, hipStream_t stream) {
+    typedef Math<T, DP> M;
+    p.splits = dq.splits;
+    p.parts = dq.splits > 1;
+    p.blocks = dq.blocks;
+    p.tiles = p.tiles_per_view = (int)((p.cells + M::kRows - 1) / M::kRows);
+    if (int rc = dq.waves == 1 ? dq_one<T, DP, 1>(p, stream) : dq_one<T, DP, 4>(p, stream)) return rc;
+    const int64_t bh = (int64_t)p.B * p.heads;
+    if (p.parts)
+        if (int rc = sum_parts<T>(p.part_a, nullptr, p.splits, bh * p.D * p.nq, p.scale, p.dq, stream)) return rc;
+    p.splits = dkv.splits;
+    p.parts = dkv_in_parts(p.D, p.Dv, p.shared, dkv.splits);
+    p.blocks = dkv.blocks;
+    if (int rc = dkv.waves == 1 ? dkv_parts<T, DP, 1>(p, stream) : dkv_parts<T, DP, 4>(p, stream)) return rc;
+    if (!p.parts) return ISPA_OK;
+    if (p.shared) return sum_parts<T>(p.part_a, p.part_b, p.splits, bh * p.D * p.cells, 1.f, p.dk, stream);
+    if (int rc = sum_parts<T>(p.part_a, nullptr, p.splits, bh * p.D * p.cells, 1.f, p.dk, stream)) return rc;
+    return sum_parts<T>(p.part_b, nullptr, p.splits, bh * p.Dv * p.cells, 1.f, p.dv, stream);
+}
+
+template <typename T>
+int backward_channels(const Params &p, const Plan &dq, const Plan &dkv, hipStream_t stream) {
+    switch (padded_channels(p.D, p.Dv)) {
+        case 32: return backward_sized<T, 32>(p, dq, dkv, stream);
+        case 64: return backward_sized<T, 64>(p, dq, dkv, stream);
+        case 128: return backward_sized<T, 128>(p, dq, dkv, stream);
+        default: return backward_sized<T, 256>(p, dq, dkv, stream);
+    }
+}
+
+}  // namespace ispa_soft

@@ -1,0 +1,268 @@
+// Soft correspondence, forward: out = softmax_j(z_ij) v_j in one pass over the streamed cells (see soft_tile.h), with a
+// running maximum m and sum l per query (float32, in units of log2).
+#pragma once
+#include "soft_tile.h"
+
+namespace ispa_soft {
+
+// The streamed cells of one item: tile t lies in view t / tiles_per_view of the item.
+template <typename M, typename SRC>
+struct KeyTiles {
+    static constexpr bool kCodes = std::is_same_v<SRC, I8> || std::is_same_v<SRC, FP8>;
+    const Params &p;
+    int b, head;
+    __device__ KeyTiles(const Params &p_, int b_, int head_) : p(p_), b(b_), head(head_) {}
+    struct At {
+        int64_t map;          // which map of the batch or store; -1 = none
+        int64_t cell0;
+    };
+    __device__ At at(int t) const {
+        At a;
+        if constexpr (kCodes) {
+            const int view = t / p.tiles_per_view;
+            const int id = p.views[(int64_t)b * p.V + view];
+            a.map = id >= 0 && id < p.n_view ? id : -1;
+            a.cell0 = (int64_t)(t - view * p.tiles_per_view) * M::kRows;
+        } else {
+            a.map = b;
+            a.cell0 = (int64_t)t * M::kRows;
+        }
+        return a;
+    }
+    __device__ const typename SRC::elem *base(const void *maps, const At &a, int d) const {
+        return (const typename SRC::elem *)maps + ((a.map < 0 ? 0 : a.map) * p.heads + head) * (int64_t)d * p.cells;
+    }
+    // this lane's cell (lane % kRows) of the tile: takes part?  its scale
+    __device__ bool live(const At &a, int lane) const {
+        const int64_t c = a.cell0 + (lane & (M::kRows - 1));
+        if (a.map < 0 || c >= p.cells) return false;
+        return p.mask == nullptr || p.mask[a.map * p.cells + c] != 0;
+    }
+    __device__ float scale(const At &a, int lane, bool ok) const {
+        if constexpr (kCodes) return ok ? p.kscale[a.map * p.cells + a.cell0 + (lane & (M::kRows - 1))] : 0.f;
+        return 0.f;
+    }
+};
+
+__device__ __forceinline__ void query_place(const Params &p, int b, int64_t i, float &x, float &y) {
+    if (p.query_xy != nullptr) {
+        const float *xy = p.query_xy + ((int64_t)b * p.nq + i) * 2;
+        x = xy[0];
+        y = xy[1];
+    } else {
+        x = (float)((int)i % p.W);
+        y = (float)((int)i / p.W);
+    }
+}
+
+template <int DP, bool SHARED>
+constexpr int forward_lds() {
+    return (SHARED ? 1 : 2) * DP * kRowBytes + 3 * 64 * (int)sizeof(float);
+}
+
+// NC: value channels that one launch forms, from p.c0 on (256 float32 channels take two launches, for the registers).
+template <typename T, typename SRC, int DP, int WQ, int NC>
+__global__ __launch_bounds__(64 * WQ) void soft_forward_kernel(const Params p) {
+    typedef Math<T, DP> M;
+    constexpr int NT = 64 * WQ;
+    constexpr int kBlocks = M::kRows / 32;
+    constexpr bool kCodes = KeyTiles<M, SRC>::kCodes;
+    constexpr bool kScaled = kCodes && std::is_same_v<T, BF16>;        // scales applied to scores and weights
+    extern __shared__ __attribute__((aligned(16))) char lds[];
+    char *ktile = lds;
+    char *vtile = p.shared ? lds : lds + DP * kRowBytes;
+    float *sarr = reinterpret_cast<float *>(vtile + DP * kRowBytes);
+    float *xarr = sarr + 64, *yarr = sarr + 128;
+
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, h = lane >> 5;
+    int id = blockIdx.x;
+    const int qblk = id % p.blocks;
+    id /= p.blocks;
+    const int split = id % p.splits;
+    const int bh = id / p.splits;
+    const int b = bh / p.heads, head = bh - b * p.heads;
+    const int t0 = (int)((int64_t)p.tiles * split / p.splits), t1 = (int)((int64_t)p.tiles * (split + 1) / p.splits);
+    const int64_t live_q = live_queries(p, b);
+    const int64_t q = ((int64_t)qblk * WQ + wave) * 32 + (lane & 31);
+    const bool q_ok = q < live_q;
+    const bool idle = (int64_t)qblk * WQ * 32 >= live_q;       // no live query in the whole workgroup
+
+    typename M::Owned qf;
+    M::load_owned(qf, (const typename T::elem *)p.q + (int64_t)bh * p.D * p.nq + (q < p.nq ? q : 0), p.nq, p.D, q_ok, h);
+    const typename M::Addr addr = M::addr(lane);
+    const Score<T> score(p, head);
+    float qx = 0.f, qy = 0.f;
+    if (p.falloff != nullptr && q_ok) query_place(p, b, q, qx, qy);
+
+    f32x16 o[NC / 32];
+#pragma unroll
+    for (int c = 0; c < NC / 32; ++c)
+#pragma unroll
+        for (int i = 0; i < 16; ++i) o[c][i] = 0.f;
+    float m = -__builtin_inff(), l = 0.f;                      // l: this lane's half of the cells
+
+    const KeyTiles<M, SRC> keys(p, b, head);
+    for (int t = t0; t < (idle ? t0 : t1); ++t) {
+        const typename KeyTiles<M, SRC>::At at = keys.at(t);
+        const bool ok = keys.live(at, lane);
+        uint64_t live = __ballot(ok);
+        if constexpr (M::kRows == 32) live &= 0xffffffffull;
+        if (live == 0) continue;                               // the same in every wave
+        const float sc = keys.scale(at, lane, ok);
+        __syncthreads();
+        load_tile<M, SRC, DP, NT>(ktile, keys.base(p.k, at, p.D), p.cells, p.D, at.cell0, p.cells, live, sc);
+        if (!p.shared)
+            load_tile<M, SRC, DP, NT>(vtile, keys.base(p.v, at, p.Dv), p.cells, p.Dv, at.cell0, p.cells, live, sc);
+        if (kScaled && wave == 0) sarr[lane] = sc;
+        if (p.falloff != nullptr && threadIdx.x < M::kRows) {
+            const int c = (int)at.cell0 + threadIdx.x;
+            xarr[threadIdx.x] = (float)(c % p.W);
+            yarr[threadIdx.x] = (float)(c / p.W);
+        }
+        __syncthreads();
+
+        float z[kBlocks][16], ks[kBlocks][16];
+        float top = -__builtin_inff();
+#pragma unroll
+        for (int k = 0; k < kBlocks; ++k) {
+            if (DP == 256) __builtin_amdgcn_sched_barrier(0);
+            f32x16 acc = M::first(ktile, addr, k, qf);
+            if constexpr (kScaled) {
+                M::per_cell(sarr, k, h, ks[k]);
+#pragma unroll
+                for (int i = 0; i < 16; ++i) acc[i] *= ks[k][i];
+            }
+            if (p.falloff != nullptr) {
+                M::per_cell(xarr, k, h, z[k]);
+#pragma unroll
+                for (int i = 0; i < 16; ++i) z[k][i] = (z[k][i] - qx) * (z[k][i] - qx);
+                float cy[16];
+                M::per_cell(yarr, k, h, cy);
+#pragma unroll
+                for (int i = 0; i < 16; ++i) z[k][i] = -score.fall * fmaf(cy[i] - qy, cy[i] - qy, z[k][i]);
+            } else {
+#pragma unroll
+                for (int i = 0; i < 16; ++i) z[k][i] = 0.f;
+            }
+            if (score.cap) {
+#pragma unroll
+                for (int i = 0; i < 16; ++i) z[k][i] = fmaf(score.top, score.bend(acc[i]), z[k][i]);
+            } else {
+#pragma unroll
+                for (int i = 0; i < 16; ++i) z[k][i] = fmaf(score.in, acc[i], z[k][i]);
+            }
+            if (live != (M::kRows == 64 ? ~0ull : 0xffffffffull)) {
+                const unsigned bits = (unsigned)(live >> (32 * k));
+#pragma unroll
+                for (int i = 0; i < 16; ++i)
+                    z[k][i] = (bits >> M::cell(i, h)) & 1u ? z[k][i] : -__builtin_inff();
+            }
+#pragma unroll
+            for (int i = 0; i < 16; ++i) top = fmaxf(top, z[k][i]);
+        }
+        top = fmaxf(top, __shfl_xor(top, 32));
+        const float m_new = fmaxf(m, top);
+        const float m_use = m_new == -__builtin_inff() ? 0.f : m_new;
+        const float fix = exp2_(m - m_use);
+        m = m_new;
+        l *= fix;
+#pragma unroll
+        for (int c = 0; c < NC / 32; ++c)
+#pragma unroll
+            for (int i = 0; i < 16; ++i) o[c][i] *= fix;
+#pragma unroll
+        for (int k = 0; k < kBlocks; ++k) {
+            float w[16];
+#pragma unroll
+            for (int i = 0; i < 16; ++i) {
+                w[i] = exp2_(z[k][i] - m_use);
+                l += w[i];
+                if constexpr (kScaled) w[i] *= ks[k][i];
+            }
+            // weights in [0, 1] are rounded to the maps' type for the second product, the sum l is not
+            M::second(vtile + p.c0 * kRowBytes, addr, k, M::weights(w), o);
+        }
+    }
+    l += __shfl_xor(l, 32);
+
+    if (q >= p.nq) return;
+    if (p.splits > 1) {
+        const int64_t part = (int64_t)split * p.B * p.heads + bh;
+        if (h == 0) {
+            const float2 ml = q_ok ? make_float2(m, l) : make_float2(-__builtin_inff(), 0.f);
+            *reinterpret_cast<float2 *>(p.part_ml + (part * p.nq + q) * 2) = ml;
+        }
+        float *dst = p.part_o + part * p.Dv * p.nq + q;
+#pragma unroll
+        for (int c = 0; c < NC / 32; ++c)
+#pragma unroll
+            for (int i = 0; i < 16; ++i) {
+                const int ch = p.c0 + 32 * c + out_channel(i, h);
+                if (ch < p.Dv) dst[ch * p.nq] = o[c][i];
+            }
+        return;
+    }
+    const bool some = q_ok && l != 0.f;                        // l is 0 only where no cell takes part (NaN is not)
+    const float inv = some ? 1.f / l : 0.f;
+    typename T::elem *dst = (typename T::elem *)p.out + (int64_t)bh * p.Dv * p.nq + q;
+#pragma unroll
+    for (int c = 0; c < NC / 32; ++c)
+#pragma unroll
+        for (int i = 0; i < 16; ++i) {
+            const int ch = p.c0 + 32 * c + out_channel(i, h);
+            const float v = some ? o[c][i] * inv : 0.f;
+            if (ch < p.Dv) {
+                store_float(dst + ch * p.nq, v);
+                if (p.out32 != nullptr) p.out32[((int64_t)bh * p.Dv + ch) * p.nq + q] = v;
+            }
+        }
+    if (h == 0 && p.lse != nullptr)
+        p.lse[(int64_t)bh * p.nq + q] = some ? (m + log2f(l)) * kLn2 : -__builtin_inff();
+}
+
+// Joins the partial results of a split call: M = max m_s, out = sum_s 2^(m_s - M) o_s / sum_s 2^(m_s - M) l_s.
+constexpr int kMaxSplits = 512;
+template <typename T>
+__global__ __launch_bounds__(256) void soft_join_kernel(const Params p, int channels_per_block) {
+    __shared__ float w[kMaxSplits][8], ls[kMaxSplits][8];
+    // 8 queries x 32 channel lanes
+    const int qi = threadIdx.x & 7, g = threadIdx.x >> 3;
+    const int bh = blockIdx.y;
+    const int64_t q = (int64_t)blockIdx.x * 8 + qi;
+    const bool in = q < p.nq;
+    const int64_t bhn = (int64_t)p.B * p.heads;
+    for (int s = g; s < p.splits; s += 32) {
+        const float2 ml = in ? *reinterpret_cast<const float2 *>(p.part_ml + ((s * bhn + bh) * p.nq + q) * 2)
+                             : make_float2(-__builtin_inff(), 0.f);
+        w[s][qi] = ml.x;
+        ls[s][qi] = ml.y;
+    }
+    __syncthreads();
+    float top = -__builtin_inff();
+    for (int s = 0; s < p.splits; ++s) top = fmaxf(top, w[s][qi]);
+    __syncthreads();
+    if (top == -__builtin_inff()) top = 0.f;                   // no part has a cell, or all scores are NaN
+    for (int s = g; s < p.splits; s += 32) w[s][qi] = exp2_(w[s][qi] - top);
+    __syncthreads();
+    float l = 0.f;
+    for (int s = 0; s < p.splits; ++s) l = fmaf(w[s][qi], ls[s][qi], l);
+    if (!in) return;
+    const bool some = l != 0.f;
+    const float inv = some ? 1.f / l : 0.f;
+    const int c1 = min(p.Dv, ((int)blockIdx.z + 1) * channels_per_block);
+    for (int c = (int)blockIdx.z * channels_per_block + g; c < c1; c += 32) {
+        float v = 0.f;
+        const float *src = p.part_o + ((int64_t)bh * p.Dv + c) * p.nq + q;
+        const int64_t step = bhn * p.Dv * p.nq;
+#pragma unroll 8
+        for (int s = 0; s < p.splits; ++s) v = fmaf(w[s][qi], src[s * step], v);
+        v = some ? v * inv : 0.f;
+        const int64_t at = ((int64_t)bh * p.Dv + c) * p.nq + q;
+        store_float((typename T::elem *)p.out + at, v);
+        if (p.out32 != nullptr) p.out32[at] = v;
+    }
+    if (blockIdx.z == 0 && g == 0 && p.lse != nullptr)
+        p.lse[(int64_t)bh * p.nq + q] = some ? (top + log2f(l)) * kLn2 : -__builtin_inff();
+}
+
+}  // namespace ispa_soft

@@ -1,0 +1,49 @@
+// Launchers of the forward kernels for one arithmetic (included by soft_forward_f32.hip and soft_forward_bf16.hip).
+#pragma once
+#include "soft_forward.h"
+#include "soft_launch.h"
+
+namespace ispa_soft {
+
+template <typename T, typename SRC, int DP, int WQ>
+int forward_one(Params p, hipStream_t stream) {
+    static unsigned long long lds_allowed = 0;
+    const int lds = p.shared ? forward_lds<DP, true>() : forward_lds<DP, false>();
+    const unsigned grid = (unsigned)((int64_t)p.B * p.heads * p.splits * p.blocks);
+    constexpr int NC = DP == 256 && std::is_same_v<T, F32> ? 128 : DP;
+    for (p.c0 = 0; p.c0 < p.Dv; p.c0 += NC)
+        if (int rc = launch(soft_forward_kernel<T, SRC, DP, WQ, NC>, p, grid, 64 * WQ, lds, &lds_allowed, "soft_forward_kernel",
+                            stream))
+            return rc;
+    if (p.splits == 1) return ISPA_OK;
+    const int per = 32;                                   // channels of a join block
+    const dim3 join((unsigned)((p.nq + 7) / 8), (unsigned)(p.B * p.heads), (unsigned)((p.Dv + per - 1) / per));
+    soft_join_kernel<T><<<join, 256, 0, stream>>>(p, per);
+    return ispa::check_launch("soft_join_kernel");
+}
+
+template <typename T, typename SRC, int DP>
+int forward_waves(const Params &p, int waves, hipStream_t stream) {
+    return waves == 1 ? forward_one<T, SRC, DP, 1>(p, stream) : forward_one<T, SRC, DP, 4>(p, stream);
+}
+
+template <typename T, typename SRC>
+int forward_channels(const Params &p, int waves, hipStream_t stream) {
+    switch (padded_channels(p.D, p.Dv)) {
+        case 32: return forward_waves<T, SRC, 32>(p, waves, stream);
+        case 64: return forward_waves<T, SRC, 64>(p, waves, stream);
+        case 128: return forward_waves<T, SRC, 128>(p, waves, stream);
+        default: return forward_waves<T, SRC, 256>(p, waves, stream);
+    }
+}
+
+template <typename T>
+int forward_source(const Params &p, int source, int waves, hipStream_t stream) {
+    switch (source) {
+        case kSourceMap: return forward_channels<T, T>(p, waves, stream);
+        case kSourceInt8: return forward_channels<T, I8>(p, waves, stream);
+        default: return forward_channels<T, FP8>(p, waves, stream);
+    }
+}
+
+}  // namespace ispa_soft

@@ -1,0 +1,212 @@
+// Soft correspondence: C entry points (argument checks, workgroup plans, workspace layout).
+#include <cmath>
+
+#include "soft_backward.h"
+#include "soft_launch.h"
+
+namespace {
+using namespace ispa_soft;
+
+int64_t tile_cells(int dtype) { return dtype == ISPA_F32 ? Math<F32, 32>::kRows : Math<BF16, 32>::kRows; }
+
+bool sizes_ok(int dtype, int B, int heads, int D, int Dv, int64_t nq, int V, int64_t cells) {
+    return (dtype == ISPA_F32 || dtype == ISPA_BF16) && B >= 0 && heads >= 1 && D >= 1 && D <= ISPA_SOFT_MAX_CHANNELS && Dv >= 1 &&
+           Dv <= ISPA_SOFT_MAX_CHANNELS && nq >= 0 && nq < (1ll << 30) && V >= 0 && cells >= 1 && cells < (1ll << 30) &&
+           (int64_t)B * heads < 65536 && V * ((cells + 31) / 32) < (1ll << 30) &&
+           (int64_t)B * heads * ((nq > cells ? nq : cells) / 32 + 1) < (1ll << 31) / kMaxSplitCount * 4;
+}
+
+int check_sizes(int dtype, int B, int heads, int D, int Dv, int64_t nq, int V, int64_t cells) {
+    ISPA_REQUIRE(dtype == ISPA_F32 || dtype == ISPA_BF16, "dtype %d is neither float32 nor bfloat16", dtype);
+    ISPA_REQUIRE(heads >= 1 && D >= 1 && Dv >= 1 && D <= ISPA_SOFT_MAX_CHANNELS && Dv <= ISPA_SOFT_MAX_CHANNELS,
+                 "heads %d of %d query and %d value channels (1 to %d each)", heads, D, Dv, ISPA_SOFT_MAX_CHANNELS);
+    ISPA_REQUIRE(sizes_ok(dtype, B, heads, D, Dv, nq, V, cells),
+                 "sizes out of range: batch %d, heads %d, %lld queries, %d views of %lld cells", B, heads, (long long)nq, V,
+                 (long long)cells);
+    return ISPA_OK;
+}
+
+Plan forward_plan(int dtype, int B, int heads, int64_t nq, int V, int64_t cells) {
+    const int64_t per = (cells + tile_cells(dtype) - 1) / tile_cells(dtype);
+    return make_plan(nq, (int64_t)B * heads, per * V);
+}
+
+size_t forward_bytes(const Plan &plan, int B, int heads, int Dv, int64_t nq) {
+    return plan.splits == 1 ? 0 : (size_t)plan.splits * B * heads * nq * (Dv + 2) * sizeof(float);
+}
+
+void backward_plans(int dtype, int B, int heads, int64_t nq, int64_t cells, Plan *dq, Plan *dkv) {
+    const int64_t r = tile_cells(dtype);
+    *dq = make_plan(nq, (int64_t)B * heads, (cells + r - 1) / r);
+    *dkv = make_plan(cells, (int64_t)B * heads, (nq + r - 1) / r);
+}
+
+size_t align256(size_t x) { return (x + 255) & ~(size_t)255; }
+
+size_t backward_bytes(const Plan &dq, const Plan &dkv, int B, int heads, int D, int Dv, int64_t nq, int64_t cells) {
+    const size_t bh = (size_t)B * heads;
+    const size_t a = dq.splits > 1 ? dq.splits * bh * D * nq : 0, k = dkv_in_parts(D, Dv, D == Dv, dkv.splits) ? dkv.splits * bh * (D + Dv) * cells : 0;
+    return align256(bh * nq * sizeof(float)) + (a > k ? a : k) * sizeof(float);
+}
+
+int check_score(float scale, float cap, const float *falloff, int W) {
+    ISPA_REQUIRE(std::isfinite(scale) && std::isfinite(cap) && cap >= 0.f, "scale %g, cap %g: finite, cap >= 0 wanted", scale, cap);
+    ISPA_REQUIRE(falloff == nullptr || W >= 1, "falloff needs the map's width");
+    return ISPA_OK;
+}
+
+int run_forward(Params &p, int dtype, int source, void *workspace, size_t workspace_bytes, hipStream_t stream) {
+    const Plan plan = forward_plan(dtype, p.B, p.heads, p.nq, p.V, p.cells);
+    const size_t need = forward_bytes(plan, p.B, p.heads, p.Dv, p.nq);
+    if (need > 0 && (workspace == nullptr || workspace_bytes < need))
+        return ispa::fail(ISPA_EWORKSPACE, "workspace of %zu bytes, %zu needed", workspace_bytes, need);
+    p.tiles_per_view = (int)((p.cells + tile_cells(dtype) - 1) / tile_cells(dtype));
+    p.tiles = p.tiles_per_view * p.V;
+    p.blocks = plan.blocks;
+    p.splits = plan.splits;
+    p.part_ml = (float *)workspace;
+    p.part_o = p.part_ml + (size_t)plan.splits * p.B * p.heads * p.nq * 2;
+    return dtype == ISPA_F32 ? forward_f32(p, source, plan.waves, stream) : forward_bf16(p, source, plan.waves, stream);
+}
+}  // namespace
+
+extern "C" size_t ispa_soft_match_workspace_bytes(int dtype, int B, int heads, int D, int Dv, int64_t nq, int views,
+                                                  int64_t cells) {
+    if (!sizes_ok(dtype, B, heads, D, Dv, nq, views, cells) || B == 0 || nq == 0) return 0;
+    return forward_bytes(forward_plan(dtype, B, heads, nq, views, cells), B, heads, Dv, nq);
+}
+
+extern "C" int ispa_soft_match(const void *q, const void *r, const void *v, int dtype, int B, int heads, int D, int Dv,
+                               int64_t nq, int64_t cells, int W, float scale, float cap, const float *falloff,
+                               const float *query_xy, const uint8_t *mask, const int32_t *num_query, void *out, float *out32,
+                               float *lse, void *workspace, size_t workspace_bytes, void *stream) {
+    if (int rc = check_sizes(dtype, B, heads, D, Dv, nq, 1, cells)) return rc;
+    if (int rc = check_score(scale, cap, falloff, W)) return rc;
+    if (B == 0 || nq == 0) return ISPA_OK;
+    ISPA_REQUIRE(q && r && out, "null pointer");
+    ISPA_REQUIRE(v != nullptr || D == Dv, "without a value map the reference map is the value (%d != %d channels)", D, Dv);
+    Params p = {};
+    p.q = q;
+    p.k = r;
+    p.v = v ? v : r;
+    p.shared = v == nullptr;
+    p.mask = mask;
+    p.falloff = falloff;
+    p.query_xy = query_xy;
+    p.count = num_query;
+    p.out = out;
+    p.out32 = out32;
+    p.lse = lse;
+    p.nq = nq;
+    p.cells = cells;
+    p.B = B;
+    p.heads = heads;
+    p.D = D;
+    p.Dv = Dv;
+    p.W = W < 1 ? 1 : W;
+    p.V = 1;
+    p.scale = scale;
+    p.cap = cap;
+    return run_forward(p, dtype, kSourceMap, workspace, workspace_bytes, (hipStream_t)stream);
+}
+
+extern "C" int ispa_store_match(const void *q, int dtype, const void *codes, const float *scales, const uint8_t *mask, int kind,
+                                const int32_t *views, int V, int n_view, int B, int heads, int D, int64_t nq, int64_t cells,
+                                int W, float scale, float cap, const float *falloff, const float *query_xy,
+                                const int32_t *num_query, void *out, float *lse, void *workspace, size_t workspace_bytes,
+                                void *stream) {
+    if (int rc = check_sizes(dtype, B, heads, D, D, nq, V, cells)) return rc;
+    if (int rc = check_score(scale, cap, falloff, W)) return rc;
+    ISPA_REQUIRE(kind == ISPA_STORE_INT8 || kind == ISPA_STORE_FP8, "store kind %d is neither int8 nor e4m3", kind);
+    ISPA_REQUIRE(n_view >= 1, "a store of %d views", n_view);
+    if (B == 0 || nq == 0) return ISPA_OK;
+    ISPA_REQUIRE(q && codes && scales && mask && out && (views || V == 0), "null pointer");
+    Params p = {};
+    p.q = q;
+    p.k = p.v = codes;
+    p.shared = 1;
+    p.kscale = scales;
+    p.views = views;
+    p.n_view = n_view;
+    p.mask = mask;
+    p.falloff = falloff;
+    p.query_xy = query_xy;
+    p.count = num_query;
+    p.out = out;
+    p.lse = lse;
+    p.nq = nq;
+    p.cells = cells;
+    p.B = B;
+    p.heads = heads;
+    p.D = p.Dv = D;
+    p.W = W < 1 ? 1 : W;
+    p.V = V;
+    p.scale = scale;
+    p.cap = cap;
+    return run_forward(p, dtype, kind == ISPA_STORE_INT8 ? kSourceInt8 : kSourceFp8, workspace, workspace_bytes,
+                       (hipStream_t)stream);
+}
+
+extern "C" size_t ispa_soft_match_backward_workspace_bytes(int dtype, int B, int heads, int D, int Dv, int64_t nq,
+                                                           int64_t cells) {
+    if (!sizes_ok(dtype, B, heads, D, Dv, nq, 1, cells) || B == 0) return 0;
+    Plan dq, dkv;
+    backward_plans(dtype, B, heads, nq, cells, &dq, &dkv);
+    return backward_bytes(dq, dkv, B, heads, D, Dv, nq, cells);
+}
+
+extern "C" int ispa_soft_match_backward(const void *q, const void *r, const void *v, int dtype, int B, int heads, int D, int Dv,
+                                        int64_t nq, int64_t cells, int W, float scale, float cap, const float *falloff,
+                                        const float *query_xy, const uint8_t *mask, const int32_t *num_query,
+                                        const float *out32, const float *lse, const void *d_out, const float *d_lse, void *dq,
+                                        void *dr, void *dv, void *workspace, size_t workspace_bytes, void *stream) {
+    if (int rc = check_sizes(dtype, B, heads, D, Dv, nq, 1, cells)) return rc;
+    if (int rc = check_score(scale, cap, falloff, W)) return rc;
+    if (B == 0) return ISPA_OK;
+    ISPA_REQUIRE(r && dr, "null pointer");
+    ISPA_REQUIRE(nq == 0 || (q && out32 && lse && d_out && dq), "null pointer");
+    ISPA_REQUIRE((v == nullptr) == (dv == nullptr), "a value map and its gradient come together");
+    ISPA_REQUIRE(v != nullptr || D == Dv, "without a value map the reference map is the value (%d != %d channels)", D, Dv);
+    Plan pq, pkv;
+    backward_plans(dtype, B, heads, nq, cells, &pq, &pkv);
+    const size_t need = backward_bytes(pq, pkv, B, heads, D, Dv, nq, cells);
+    if (workspace_bytes < need || (need > 0 && workspace == nullptr))
+        return ispa::fail(ISPA_EWORKSPACE, "workspace of %zu bytes, %zu needed", workspace_bytes, need);
+    Params p = {};
+    p.q = q;
+    p.k = r;
+    p.v = v ? v : r;
+    p.shared = v == nullptr;
+    p.mask = mask;
+    p.falloff = falloff;
+    p.query_xy = query_xy;
+    p.count = num_query;
+    p.lse = const_cast<float *>(lse);
+    p.d_out = d_out;
+    p.dq = dq;
+    p.dk = dr;
+    p.dv = dv;
+    p.nq = nq;
+    p.cells = cells;
+    p.B = B;
+    p.heads = heads;
+    p.D = D;
+    p.Dv = Dv;
+    p.W = W < 1 ? 1 : W;
+    p.V = 1;
+    p.scale = scale;
+    p.cap = cap;
+    hipStream_t s = (hipStream_t)stream;
+    const int64_t bh = (int64_t)B * heads;
+    float *delta = (float *)workspace;
+    p.delta = delta;
+    p.part_a = (float *)((char *)workspace + align256(bh * nq * sizeof(float)));
+    p.part_b = p.part_a + (size_t)pkv.splits * bh * D * cells;
+    if (nq > 0) {
+        const unsigned grid = (unsigned)((nq + 63) / 64 * bh);
+        if (dtype == ISPA_F32) soft_delta_kernel<F32><<<grid, 256, 0, s>>>(p, out32, d_lse, delta);
+        else soft_delta_kernel<BF16><<<grid, 256, 0, s>>>(p, out32, d_lse, delta);
+        if (int rc = ispa::check_launch("soft_delta_kernel")) return rc;
+    }
+    return dtype == ISPA_F32 ? backward_f32(p, pq, pkv, s) : backward_bf16(p, pq, pkv, s);
+}

@@ -1,0 +1,424 @@
+// Soft correspondence: the tile format, operand fragments and loaders that the forward and backward kernels share.
+//
+// All three kernels are the same two chained products.  One side's cells are OWNED: a wave keeps 32 of them as the
+// columns of its MFMA tiles, channels in registers.  The other side's cells are STREAMED through LDS in tiles of
+// kRows cells.  The first product contracts channels (scores: rows = streamed cells, columns = owned cells), the
+// second contracts the streamed cells (rows = channels, columns = owned cells).  The 32x32 MFMA accumulator holds
+// one owned column per lane and 16 streamed rows in its registers, which is already the second product's B operand, so
+// probabilities never leave the registers.  Forward and the query gradient own queries, the key/value gradient owns
+// keys.
+//
+// LDS tile: channel rows of 128 bytes (64 bfloat16 or 32 float32 cells), as the maps lie in memory.  The 16-byte
+// segments of a row are permuted by swz(row), so that both readers are free of bank conflicts: the transposed read of
+// the first product touches 4 rows x 64 bytes at a time (row bit 0 picks the bank half, bit 1 the segment half), the
+// plain 16-byte read of the second one touches one segment of 16 or 32 successive rows (bits 1 to 3 pick 8 segments).
+#pragma once
+#include <type_traits>
+
+#include "common.h"
+
+namespace ispa_soft {
+
+typedef float f32x16 __attribute__((ext_vector_type(16)));
+typedef float f32x4 __attribute__((ext_vector_type(4)));
+typedef short s16x4 __attribute__((ext_vector_type(4)));
+typedef __bf16 bf16x8 __attribute__((ext_vector_type(8)));
+typedef unsigned u32x4 __attribute__((ext_vector_type(4)));
+typedef unsigned u32x2 __attribute__((ext_vector_type(2)));
+
+constexpr float kLog2e = 1.44269504088896340736f;
+constexpr float kLn2 = 0.69314718055994530942f;
+constexpr int kRowBytes = 128;
+
+__device__ __forceinline__ int swz(int row) { return ((row & 2) << 1) | ((row >> 2) & 3); }
+
+__device__ __forceinline__ float bf16_to_float(unsigned short u) { return __builtin_bit_cast(float, (unsigned)u << 16); }
+
+// Round to nearest, ties to even, two at a time (v_cvt_pk_bf16_f32).
+__device__ __forceinline__ unsigned pack_bf16(float lo, float hi) {
+    typedef __bf16 bf16x2 __attribute__((ext_vector_type(2)));
+    typedef float f32x2 __attribute__((ext_vector_type(2)));
+    const f32x2 v = {lo, hi};
+    return __builtin_bit_cast(unsigned, __builtin_convertvector(v, bf16x2));
+}
+
+// ------------------------------------------------------------------------------------------------
+// Element types of the maps in memory.
+struct F32 {
+    typedef float elem;
+};
+struct BF16 {
+    typedef unsigned short elem;
+};
+struct I8 {                 // codes of a template store; the value is code * scale[cell]
+    typedef signed char elem;
+};
+struct FP8 {                // e4m3
+    typedef unsigned char elem;
+};
+
+__device__ __forceinline__ float load_float(const float *p) { return *p; }
+__device__ __forceinline__ float load_float(const unsigned short *p) { return bf16_to_float(*p); }
+__device__ __forceinline__ void store_float(float *p, float v) { *p = v; }
+__device__ __forceinline__ void store_float(unsigned short *p, float v) { *p = (unsigned short)pack_bf16(v, 0.f); }
+
+template <typename S>
+__device__ __forceinline__ void decode4(unsigned w, float (&f)[4]) {
+    if constexpr (std::is_same_v<S, I8>) {
+#pragma unroll
+        for (int i = 0; i < 4; ++i) f[i] = (float)(int)(signed char)(w >> (8 * i));
+    } else {
+        const auto a = __builtin_amdgcn_cvt_pk_f32_fp8((int)w, false);
+        const auto b = __builtin_amdgcn_cvt_pk_f32_fp8((int)w, true);
+        f[0] = a[0];
+        f[1] = a[1];
+        f[2] = b[0];
+        f[3] = b[1];
+    }
+}
+
+// ------------------------------------------------------------------------------------------------
+// Arithmetic of a kernel: float32 MFMAs for float32 maps, bfloat16 MFMAs (float32 accumulation) for bfloat16 maps.
+template <typename T, int DP>
+struct Math;
+
+template <int DP>
+struct Math<BF16, DP> {
+    static constexpr int kRows = 64;             // streamed cells per tile
+    static constexpr int kCells = 8;             // cells of a 16-byte segment
+    typedef BF16 map;
+    struct Owned {                               // B operand of the first product: channels 16 s + 8 h .. + 7
+        bf16x8 f[DP / 16];
+    };
+    // base: a column of the map (always a real one); !ok: zeros
+    __device__ static void load_owned(Owned &o, const unsigned short *base, int64_t ld, int d, bool ok, int h) {
+#pragma unroll
+        for (int s = 0; s < DP / 16; ++s) {
+            unsigned short e[8];
+#pragma unroll
+            for (int j = 0; j < 8; ++j) {
+                const int c = 16 * s + 8 * h + j;
+                const unsigned short x = base[(int64_t)(c < d ? c : d - 1) * ld];
+                e[j] = ok && c < d ? x : (unsigned short)0;
+            }
+            u32x4 w;
+#pragma unroll
+            for (int j = 0; j < 4; ++j) w[j] = (unsigned)e[2 * j] | ((unsigned)e[2 * j + 1] << 16);
+            o.f[s] = __builtin_bit_cast(bf16x8, w);
+        }
+    }
+    // The transposed 8-byte read hands lane i of a 16-lane group element i of the group's four 8-byte pieces, for
+    // 4 channel rows.  The pieces are addressed so that accumulator row 16 s + 8 e + 4 h + j belongs to streamed cell
+    // 16 s + 8 h + 4 e + j: a lane then holds 8 successive cells per 16-cell step, what one plain 16-byte read of the
+    // second product's A operand gives.
+    struct Addr {
+        int tr[2];           // first, second four channels of a 16-channel step (swz repeats every 16 rows)
+        int nat;
+    };
+    __device__ static Addr addr(int lane) {
+        const int h = lane >> 5, g = (lane >> 4) & 1, p = lane & 3;
+        const int seg = 2 * g + (p & 1), half = p >> 1;
+        Addr a;
+#pragma unroll
+        for (int x = 0; x < 2; ++x) {
+            const int row = 8 * h + ((lane & 15) >> 2) + 4 * x;
+            a.tr[x] = row * kRowBytes + ((seg ^ swz(row)) << 4) + half * 8;
+        }
+        const int row = lane & 31;
+        a.nat = row * kRowBytes + ((h ^ swz(row)) << 4);
+        return a;
+    }
+    // Scores of streamed cells 32 b .. 32 b + 31 of a tile.
+    __device__ static f32x16 first(const char *tile, const Addr &a, int b, const Owned &o) {
+        typedef __attribute__((address_space(3))) s16x4 *lds_ptr;
+        f32x16 acc;
+#pragma unroll
+        for (int i = 0; i < 16; ++i) acc[i] = 0.f;
+#pragma unroll
+        for (int s = 0; s < DP / 16; ++s) {
+            union {
+                s16x4 q[2];
+                bf16x8 v;
+            } u;
+#pragma unroll
+            for (int x = 0; x < 2; ++x)
+                u.q[x] = __builtin_amdgcn_ds_read_tr16_b64_v4i16(
+                    (lds_ptr)(tile + (a.tr[x] ^ (b << 6)) + s * 16 * kRowBytes));
+            acc = __builtin_amdgcn_mfma_f32_32x32x16_bf16(u.v, o.f[s], acc, 0, 0, 0);
+            if (DP == 256 && s % 4 == 3) __builtin_amdgcn_sched_barrier(0);    // bounds the reads in flight: registers
+        }
+        return acc;
+    }
+    struct Weights {
+        bf16x8 f[2];
+    };
+    __device__ static Weights weights(const float (&p)[16]) {
+        Weights w;
+#pragma unroll
+        for (int s = 0; s < 2; ++s) {
+            u32x4 v;
+#pragma unroll
+            for (int j = 0; j < 4; ++j) v[j] = pack_bf16(p[8 * s + 2 * j], p[8 * s + 2 * j + 1]);
+            w.f[s] = __builtin_bit_cast(bf16x8, v);
+        }
+        return w;
+    }
+    // out += (channels x cells 32 b .. 32 b + 31 of the tile) x weights, for the first 32 N channel rows from `tile` on
+    template <int N>
+    __device__ static void second(const char *tile, const Addr &a, int b, const Weights &w, f32x16 (&out)[N]) {
+#pragma unroll
+        for (int c = 0; c < N; ++c)
+#pragma unroll
+            for (int s = 0; s < 2; ++s) {
+                const bf16x8 v = *reinterpret_cast<const bf16x8 *>(tile + (a.nat ^ ((4 * b + 2 * s) << 4)) + c * 32 * kRowBytes);
+                out[c] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(v, w.f[s], out[c], 0, 0, 0);
+                if (DP == 256 && s == 1 && c % 2 == 1) __builtin_amdgcn_sched_barrier(0);
+            }
+    }
+    // Streamed cell (inside its 32) of accumulator register i, i = 0 .. 15.
+    __device__ static constexpr int cell(int i, int h) { return 16 * (i >> 3) + 8 * h + (i & 7); }
+    // Per-cell floats of a tile's LDS array, in register order.
+    __device__ static void per_cell(const float *v, int b, int h, float (&out)[16]) {
+#pragma unroll
+        for (int s = 0; s < 2; ++s)
+#pragma unroll
+            for (int t = 0; t < 2; ++t) {
+                const f32x4 x = *reinterpret_cast<const f32x4 *>(v + 32 * b + 16 * s + 8 * h + 4 * t);
+#pragma unroll
+                for (int j = 0; j < 4; ++j) out[8 * s + 4 * t + j] = x[j];
+            }
+    }
+};
+
+template <int DP>
+struct Math<F32, DP> {
+    static constexpr int kRows = 32;
+    static constexpr int kCells = 4;
+    typedef F32 map;
+    struct Owned {                               // channel 2 s + h
+        float f[DP / 2];
+    };
+    __device__ static void load_owned(Owned &o, const float *base, int64_t ld, int d, bool ok, int h) {
+#pragma unroll
+        for (int s = 0; s < DP / 2; ++s) {
+            const int c = 2 * s + h;
+            const float x = base[(int64_t)(c < d ? c : d - 1) * ld];
+            o.f[s] = ok && c < d ? x : 0.f;
+            if (DP == 256 && s % 8 == 7) __builtin_amdgcn_sched_barrier(0);
+        }
+    }
+    struct Addr {
+        int one[8];          // row 2 s + h for s = 0 .. 7 (swz repeats every 16 rows)
+        int nat;
+    };
+    __device__ static Addr addr(int lane) {
+        const int h = lane >> 5, cell = lane & 31;
+        Addr a;
+#pragma unroll
+        for (int s = 0; s < 8; ++s) {
+            const int row = 2 * s + h;
+            a.one[s] = row * kRowBytes + (((cell >> 2) ^ swz(row)) << 4) + (cell & 3) * 4;
+        }
+        a.nat = cell * kRowBytes + ((h ^ swz(cell)) << 4);
+        return a;
+    }
+    __device__ static f32x16 first(const char *tile, const Addr &a, int, const Owned &o) {
+        f32x16 acc;
+#pragma unroll
+        for (int i = 0; i < 16; ++i) acc[i] = 0.f;
+#pragma unroll
+        for (int s = 0; s < DP / 2; ++s) {
+            const float x = *reinterpret_cast<const float *>(tile + a.one[s & 7] + (s >> 3) * 16 * kRowBytes);
+            acc = __builtin_amdgcn_mfma_f32_32x32x2f32(x, o.f[s], acc, 0, 0, 0);
+            if (DP == 256 && s % 4 == 3) __builtin_amdgcn_sched_barrier(0);
+        }
+        return acc;
+    }
+    struct Weights {
+        float f[16];
+    };
+    __device__ static Weights weights(const float (&p)[16]) {
+        Weights w;
+#pragma unroll
+        for (int i = 0; i < 16; ++i) w.f[i] = p[i];
+        return w;
+    }
+    template <int N>
+    __device__ static void second(const char *tile, const Addr &a, int, const Weights &w, f32x16 (&out)[N]) {
+#pragma unroll
+        for (int c = 0; c < N; ++c)
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {        // cells 8 i + 4 h + 0 .. 3
+                const f32x4 v = *reinterpret_cast<const f32x4 *>(tile + (a.nat ^ (i << 5)) + c * 32 * kRowBytes);
+#pragma unroll
+                for (int j = 0; j < 4; ++j)
+                    out[c] = __builtin_amdgcn_mfma_f32_32x32x2f32(v[j], w.f[4 * i + j], out[c], 0, 0, 0);
+                if (DP == 256) __builtin_amdgcn_sched_barrier(0);
+            }
+    }
+    __device__ static constexpr int cell(int i, int h) { return 8 * (i >> 2) + 4 * h + (i & 3); }
+    __device__ static void per_cell(const float *v, int, int h, float (&out)[16]) {
+#pragma unroll
+        for (int t = 0; t < 4; ++t) {
+            const f32x4 x = *reinterpret_cast<const f32x4 *>(v + 8 * t + 4 * h);
+#pragma unroll
+            for (int j = 0; j < 4; ++j) out[4 * t + j] = x[j];
+        }
+    }
+};
+
+// Channel of output accumulator register i of a 32-channel block.
+__device__ __forceinline__ int out_channel(int i, int h) { return 8 * (i >> 2) + 4 * h + (i & 3); }
+
+// ------------------------------------------------------------------------------------------------
+// Loads one tile: NT threads, thread t takes segment t & 7 of channel rows t / 8, t / 8 + NT / 8, ..., kBatch rows at a
+// time in registers.  live: bit j = cell j of the tile takes part; scale: the codes' scale of the tile's cell
+// lane % kRows (float32 arithmetic multiplies here, bfloat16 arithmetic keeps the codes, which bfloat16 holds exactly,
+// and scales the scores and weights).
+// Cells past the map's end, masked cells and channels past d are staged as zeros: whatever a masked cell holds
+// (infinities, NaN) meets a weight of zero in the second product and must not turn it into NaN.
+template <typename M, typename SRC, int DP, int NT>
+__device__ __forceinline__ void load_tile(char *tile, const typename SRC::elem *base, int64_t ld, int d, int64_t cell0,
+                                          int64_t n, uint64_t live, float scale) {
+    constexpr bool kCodes = std::is_same_v<SRC, I8> || std::is_same_v<SRC, FP8>;
+    constexpr bool kNarrow = std::is_same_v<typename M::map, BF16>;
+    constexpr int kN = M::kCells;
+    constexpr int kPer = DP * 8 / NT;
+    constexpr int kBatch = DP == 256 ? (kCodes || NT == 64 ? 1 : 2) : kPer < 8 ? kPer : 8;
+    typedef std::conditional_t<!kCodes, u32x4, std::conditional_t<kNarrow, u32x2, unsigned>> raw;
+    const int seg = threadIdx.x & 7, row0 = threadIdx.x >> 3;
+    const unsigned bits = (unsigned)(live >> (seg * kN)) & ((1u << kN) - 1u);
+    u32x4 keep;
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+        if constexpr (kNarrow)
+            keep[j] = ((bits >> (2 * j)) & 1u ? 0xffffu : 0u) | ((bits >> (2 * j + 1)) & 1u ? 0xffff0000u : 0u);
+        else
+            keep[j] = (bits >> j) & 1u ? 0xffffffffu : 0u;
+    }
+    float sc[4] = {};
+    if constexpr (kCodes && !kNarrow)
+#pragma unroll
+        for (int j = 0; j < 4; ++j) sc[j] = __shfl(scale, seg * 4 + j);
+    const int64_t at = cell0 + seg * kN;
+    const int64_t left = n - at;
+    const int ok = left >= kN ? kN : left > 0 ? (int)left : 0;
+    const typename SRC::elem *p = base + (int64_t)row0 * ld + at;
+    const int at0 = row0 * kRowBytes + ((seg ^ swz(row0)) << 4);
+    static_assert(NT == 64 || NT % 128 == 0, "");
+#pragma unroll 1
+    for (int i0 = 0; i0 < kPer; i0 += kBatch) {
+        raw r[kBatch];
+#pragma unroll
+        for (int i = 0; i < kBatch; ++i) {
+            raw v = {};
+            if (row0 + (i0 + i) * (NT / 8) < d) {
+                if (ok == kN) {
+                    __builtin_memcpy(&v, p, sizeof(raw));
+                } else if (ok > 0) {
+                    typename SRC::elem e[kN];
+#pragma unroll
+                    for (int j = 0; j < kN; ++j) e[j] = j < ok ? p[j] : (typename SRC::elem)0;
+                    __builtin_memcpy(&v, e, sizeof(raw));
+                }
+            }
+            r[i] = v;
+            p += (int64_t)(NT / 8) * ld;
+        }
+#pragma unroll
+        for (int i = 0; i < kBatch; ++i) {
+            u32x4 v;
+            if constexpr (!kCodes) {
+                v = r[i];
+            } else if constexpr (kNarrow) {
+                float f[8];
+                float x[4], y[4];
+                decode4<SRC>(r[i][0], x);
+                decode4<SRC>(r[i][1], y);
+#pragma unroll
+                for (int j = 0; j < 4; ++j) {
+                    f[j] = x[j];
+                    f[4 + j] = y[j];
+                }
+#pragma unroll
+                for (int j = 0; j < 4; ++j)      // 8-bit codes fit bfloat16: the upper halves are the values
+                    v[j] = (__builtin_bit_cast(unsigned, f[2 * j]) >> 16) |
+                           (__builtin_bit_cast(unsigned, f[2 * j + 1]) & 0xffff0000u);
+            } else {
+                float f[4];
+                decode4<SRC>(r[i], f);
+#pragma unroll
+                for (int j = 0; j < 4; ++j) v[j] = __builtin_bit_cast(unsigned, f[j] * sc[j]);
+            }
+            // swz repeats every 16 rows; 8 rows further (one wave) it differs by 2
+            const int at = at0 ^ (NT == 64 ? ((i0 + i) & 1) << 5 : 0);
+            *reinterpret_cast<u32x4 *>(tile + at + (i0 + i) * (NT / 8) * kRowBytes) = v & keep;
+        }
+    }
+}
+
+// ------------------------------------------------------------------------------------------------
+// What a call computes; device pointers as the C ABI hands them over.
+struct Params {
+    const void *q, *k, *v;                 // (B,heads D,nq), (B,heads D,cells), (B,heads Dv,cells); codes for a store
+    const float *kscale;                   // store: (n_view,cells)
+    const int32_t *views;                  // store: (B,V)
+    const uint8_t *mask;                   // (B,cells), store: (n_view,cells); NULL = all cells
+    const float *falloff;                  // (heads) or NULL
+    const float *query_xy;                 // (B,nq,2) or NULL: query i is cell (i % W, i / W)
+    const int32_t *count;                  // (B) live queries or NULL
+    void *out;
+    float *out32, *lse;
+    float *part_o, *part_ml;               // workspace of split calls
+    // backward
+    const void *d_out;
+    const float *delta;                    // (B,heads,nq)
+    void *dq, *dk, *dv;
+    float *part_a, *part_b;
+    int64_t nq, cells;
+    int B, heads, D, Dv, W, V, n_view;
+    int tiles_per_view, tiles, splits, blocks;       // streamed tiles of one item, split over `splits` workgroups
+    int shared;                            // the value map is the reference map
+    int parts;                             // gradients go to part_a (and part_b), to be summed by soft_sum_kernel
+    int c0;                                // first channel of the gradients this launch forms
+    float scale, cap;
+};
+
+// The scores of one item and head, in units of log2: z = fn(x) - falloff d^2 with x = scale (q . r).
+template <typename T>
+struct Score {
+    static constexpr bool kExact = std::is_same_v<T, F32>;
+    float in, top;                  // z = in acc, or top tanh(in acc)
+    float fall;
+    bool cap;
+    __device__ Score(const Params &p, int head) {
+        cap = p.cap > 0.f;
+        in = cap ? p.scale / p.cap : p.scale * kLog2e;
+        top = p.cap * kLog2e;
+        fall = p.falloff ? p.falloff[head] * kLog2e : 0.f;
+    }
+    // tanh(x / cap) = 1 - 2 / (exp(2 x / cap) + 1), whose absolute error of 2e-7 is far below what the inputs of the
+    // bfloat16 kernels leave.  float32 keeps the relative error near 1e-7 too: below 0.6 the odd polynomial
+    // y + y^3 r(y^2), r fitted to (tanh(y) / y - 1) / y^2 on [0, 0.36] by weighted least squares.
+    __device__ float bend(float acc) const {
+        const float y = in * acc;
+        const float far = fmaf(-2.f, __builtin_amdgcn_rcpf(__builtin_amdgcn_exp2f(y * (2.f * kLog2e)) + 1.f), 1.f);
+        if constexpr (!kExact) return far;
+        const float u = y * y;
+        float r = fmaf(u, -0.00589394523f, 0.020794617f);
+        r = fmaf(u, r, -0.0537832938f);
+        r = fmaf(u, r, 0.133319154f);
+        r = fmaf(u, r, -0.333332986f);
+        return fabsf(y) < 0.6f ? fmaf(y * u, r, y) : far;
+    }
+};
+
+__device__ __forceinline__ float exp2_(float x) { return __builtin_amdgcn_exp2f(x); }
+
+__device__ __forceinline__ int64_t live_queries(const Params &p, int b) {
+    if (p.count == nullptr) return p.nq;
+    const int64_t c = p.count[b];
+    return c < 0 ? 0 : c < p.nq ? c : p.nq;
+}
+
+}  // namespace ispa_soft

@@ -1,0 +1,409 @@
+"""Soft correspondence: the differentiable counterpart of `correspondence.dense_nn`, and a store of template features.
+
+  soft_match      softmax-weighted transfer of a template's features to query cells, with gradients
+  TemplateStore   feature maps of many rendered views in 8 bits: write, read back, and match against them
+
+The reference matches hard (the `KNN` layer of ucn_code/nets/train.prototxt:2116-2141) or hands correlation maps to a
+trunk (arch/eccv_net/eccv_net.py:161-231); it looks template views up one at a time (utils/proxy_renderer.py:100-151).
+Nothing here has a counterpart in it to be checked against.
+"""
+import contextlib
+import copy
+
+import numpy as np
+import torch
+
+from . import _abi, _device as dv
+
+_CODES = {torch.float32: _abi.F32, torch.bfloat16: _abi.BF16}
+MAX_CHANNELS = _abi.SOFT_MAX_CHANNELS
+
+
+def _dims(x):
+    return tuple(x.shape)
+
+
+def _elements(x, name):
+    """Shape check of a feature map given as array or tensor, before anything touches the device."""
+    if len(_dims(x)) < 3:
+        raise ValueError(f"{name} must be (B,C,H,W) or (B,C,n), got {_dims(x)}")
+    return int(np.prod(_dims(x)[2:], dtype=np.int64))
+
+
+def _dtype(x, name):
+    if not dv.is_tensor(x):
+        return torch.float32
+    if x.dtype not in _CODES:
+        raise ValueError(f"{name} must be float32 or bfloat16, got {x.dtype}")
+    return x.dtype
+
+
+def _place(x):
+    """Makes the device that a call runs on the current one: where its first tensor lives, else the current one."""
+    dv.device()
+    if dv.is_tensor(x) and x.is_cuda and x.device.index != torch.cuda.current_device():
+        return torch.cuda.device(x.device)
+    return contextlib.nullcontext()
+
+
+def _scores(heads, scale, cap, falloff, query_xy, grid, query_shape, batch, n):
+    """Checks of what turns products into scores; `grid` is the reference map's (H,W) or None."""
+    scale, cap = float(scale), float(cap or 0.0)
+    if not np.isfinite(scale):
+        raise ValueError(f"scale must be finite, got {scale}")
+    if not (np.isfinite(cap) and cap >= 0):
+        raise ValueError(f"cap must be finite and not negative (0 or None: no cap), got {cap}")
+    if falloff is not None:
+        if grid is None:
+            raise ValueError("falloff needs a reference map (B,C,H,W): distances are taken on its grid")
+        if query_xy is None and query_shape != grid:
+            raise ValueError(f"falloff: queries {query_shape} do not lie on the reference grid {grid}; give query_xy")
+        if not np.isscalar(falloff) and _dims(falloff if dv.is_tensor(falloff) else np.asarray(falloff)) != (heads,):
+            raise ValueError(f"falloff must be a number or hold one value per head ({heads})")
+        if query_xy is not None and _dims(query_xy) != (batch, n, 2):
+            raise ValueError(f"query_xy must be ({batch},{n},2), got {_dims(query_xy)}")
+    return scale, cap
+
+
+def _score_tensors(heads, falloff, query_xy):
+    if falloff is None:
+        return None, None
+    if np.isscalar(falloff):
+        f = torch.full((heads,), float(falloff), dtype=torch.float32, device=dv.device())
+    else:
+        f = dv.to_dev(falloff, torch.float32)
+    return f, (dv.to_dev(query_xy, torch.float32) if query_xy is not None else None)
+
+
+def _counts(num_query, batch):
+    if num_query is None:
+        return None
+    t = num_query if dv.is_tensor(num_query) else np.asarray(num_query)
+    if int(np.prod(_dims(t), dtype=np.int64)) != batch:
+        raise ValueError("num_query must hold one count per batch item")
+    return t.reshape(-1)
+
+
+def _count_tensor(num_query):
+    """Counts as int32; what int32 cannot hold is more than any query map has, or less than none."""
+    if num_query is None:
+        return None
+    low, high = -1, 2 ** 31 - 1
+    num_query = num_query.clamp(low, high) if dv.is_tensor(num_query) and num_query.dtype == torch.int64 else \
+        num_query if dv.is_tensor(num_query) else np.clip(num_query, low, high)
+    return dv.to_dev(num_query, torch.int32)
+
+
+def _mask(mask):
+    """Bytes, not 0 where the cell takes part.  A bool tensor is the byte array the kernels read."""
+    if mask is None:
+        return None
+    if not dv.is_tensor(mask):
+        mask = torch.from_numpy(np.asarray(mask) != 0)
+    elif mask.dtype not in (torch.bool, torch.uint8):
+        mask = mask != 0
+    if mask.dtype == torch.bool:
+        mask = mask.contiguous().view(torch.uint8)
+    return dv.to_dev(mask, torch.uint8)
+
+
+class _Call:
+    """One soft_match call: its arguments checked (nothing touches the device), then as device tensors."""
+
+    def __init__(self, query, ref, value, heads, scale, cap, falloff, query_xy, mask, num_query):
+        n, cells = _elements(query, "query"), _elements(ref, "ref")
+        b, c = _dims(query)[:2]
+        dtype = _dtype(query, "query")
+        heads = int(heads)
+        if _dims(ref)[:2] != (b, c):
+            raise ValueError(f"query {_dims(query)} and ref {_dims(ref)} must share batch and channels")
+        if value is not None and (_elements(value, "value") != cells or _dims(value)[0] != b):
+            raise ValueError(f"value {_dims(value)} must have the batch and cells of ref {_dims(ref)}")
+        for x, name in ((ref, "ref"), (value, "value")):
+            if x is not None and _dtype(x, name) != dtype:
+                raise ValueError(f"{name} must have query's dtype {dtype}")
+        cv = c if value is None else _dims(value)[1]
+        if heads < 1 or c < 1 or cv < 1 or c % heads or cv % heads:
+            raise ValueError(f"{c} and {cv} channels do not split into {heads} heads")
+        if c // heads > MAX_CHANNELS or cv // heads > MAX_CHANNELS:
+            raise ValueError(f"at most {MAX_CHANNELS} channels per head")
+        if cells < 1:
+            raise ValueError("ref has no cells")
+        if mask is not None and (_dims(mask)[0] != b or int(np.prod(_dims(mask), dtype=np.int64)) != b * cells):
+            raise ValueError(f"mask must be ({b},H,W) or ({b},1,H,W) over ref's cells, got {_dims(mask)}")
+        grid = _dims(ref)[2:] if len(_dims(ref)) == 4 else None
+        if scale is None:
+            scale = (c // heads) ** -0.5
+        self.scale, self.cap = _scores(heads, scale, cap, falloff, query_xy, grid, _dims(query)[2:], b, n)
+        num_query = _counts(num_query, b)
+        self.raw = (query, ref, value, falloff, query_xy, mask, num_query)
+        self.code = _CODES[dtype]
+        self.dtype, self.b, self.heads, self.d, self.dv, self.n, self.cells = dtype, b, heads, c // heads, cv // heads, n, cells
+        self.width = grid[1] if grid else cells
+        self.out_shape = (b, cv) + _dims(query)[2:]
+
+    def upload(self):
+        query, ref, value, falloff, query_xy, mask, num_query = self.raw
+        self.raw = None
+        f, xy = _score_tensors(self.heads, falloff, query_xy)
+        return self.bind(query, ref, value, f, xy, _mask(mask), _count_tensor(num_query))
+
+    def bind(self, query, ref, value, falloff, xy, mask, count):
+        self.q, self.r = dv.to_dev(query, self.dtype), dv.to_dev(ref, self.dtype)
+        self.v = dv.to_dev(value, self.dtype) if value is not None else None
+        self.falloff, self.xy, self.mask, self.count = falloff, xy, mask, count
+        return self
+
+    def release(self):
+        """The options as device tensors; the call keeps its sizes and settings alone."""
+        options = (self.falloff, self.xy, self.mask, self.count)
+        self.q = self.r = self.v = self.falloff = self.xy = self.mask = self.count = None
+        return options
+
+    def _common(self):
+        return (self.code, self.b, self.heads, self.d, self.dv, self.n, self.cells, self.width, self.scale, self.cap,
+                dv.ptr(self.falloff), dv.ptr(self.xy), dv.ptr(self.mask), dv.ptr(self.count))
+
+    def forward(self, exact):
+        """out, its float32 twin (`exact`; the same tensor for float32 maps) and lse.  The workspace is the call's own: calls
+        on two streams, or captured in two graphs, share nothing."""
+        out = dv.empty(self.out_shape, self.dtype)
+        out32 = None
+        if exact:
+            out32 = out if self.dtype == torch.float32 else dv.empty(self.out_shape, torch.float32)
+        lse = dv.empty((self.b, self.heads, self.n), torch.float32)
+        need = _abi.lib.ispa_soft_match_workspace_bytes(self.code, self.b, self.heads, self.d, self.dv, self.n, 1, self.cells)
+        ws = dv.empty((need,), torch.uint8) if need else None
+        _abi.check(_abi.lib.ispa_soft_match(dv.ptr(self.q), dv.ptr(self.r), dv.ptr(self.v), *self._common(), dv.ptr(out),
+                                            None if out32 is out else dv.ptr(out32), dv.ptr(lse), dv.ptr(ws), need,
+                                            dv.stream_ptr()))
+        return out, out32, lse
+
+    def backward(self, out32, lse, d_out, d_lse):
+        dq, dr = torch.empty_like(self.q), torch.empty_like(self.r)
+        dval = torch.empty_like(self.v) if self.v is not None else None
+        need = _abi.lib.ispa_soft_match_backward_workspace_bytes(self.code, self.b, self.heads, self.d, self.dv, self.n,
+                                                                 self.cells)
+        ws = dv.empty((need,), torch.uint8) if need else None
+        _abi.check(_abi.lib.ispa_soft_match_backward(dv.ptr(self.q), dv.ptr(self.r), dv.ptr(self.v), *self._common(),
+                                                     dv.ptr(out32), dv.ptr(lse), dv.ptr(d_out), dv.ptr(d_lse), dv.ptr(dq),
+                                                     dv.ptr(dr), dv.ptr(dval), dv.ptr(ws), need, dv.stream_ptr()))
+        return dq, dr, dval
+
+
+class _SoftMatch(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, query, ref, value, call):
+        with _place(query):
+            out, out32, lse = call.upload().forward(exact=True)
+        ctx.save_for_backward(query, ref, value, out32, lse, *call.release())
+        ctx.call = call
+        ctx.set_materialize_grads(False)
+        return out, lse
+
+    @staticmethod
+    @torch.autograd.function.once_differentiable
+    def backward(ctx, d_out, d_lse):
+        if d_out is None and d_lse is None:
+            return None, None, None, None
+        query, ref, value, out32, lse, *options = ctx.saved_tensors
+        with _place(query):
+            call = copy.copy(ctx.call).bind(query, ref, value, *options)
+            grads = _gradients(call, out32, lse, d_out, d_lse)
+        return (*(g.reshape(x.shape).to(x.device) if g is not None and need else None
+                  for g, x, need in zip(grads, (query, ref, value), ctx.needs_input_grad)), None)
+
+
+def _gradients(call, out32, lse, d_out, d_lse):
+    if d_out is None:
+        d_out = torch.zeros(call.out_shape, dtype=call.dtype, device=dv.device())
+    d_out = dv.to_dev(d_out, call.dtype)
+    d_lse = dv.to_dev(d_lse, torch.float32) if d_lse is not None else None
+    return call.backward(out32, lse, d_out, d_lse)
+
+
+def soft_match(query, ref, value=None, *, heads=1, scale=None, cap=0.0, falloff=None, query_xy=None, mask=None,
+               num_query=None, return_lse=False):
+    """For every query cell the average of `value` over the reference cells, weighted by the softmax of the match scores.
+
+    query (B,C,Hq,Wq) or (B,C,n); ref (B,C,H,W) or (B,C,cells); value (B,Cv,H,W) over the same cells, or None: ref
+    is the value too.  float32 arrays or tensors, or bfloat16 tensors (all of one dtype); channels split into `heads`
+    groups of at most 256 that are matched apart.  Scores of query i and cell j, per head:
+
+        x = scale * <q_i, r_j>             scale: 1 / sqrt(C / heads) unless given (features of unit length want 10 to 30)
+        y = cap * tanh(x / cap)            cap > 0; 0 or None: y = x
+        z = y - falloff * |xy_i - xy_j|^2  falloff: a number or one per head; a prior on where the match lies.  Distances are
+                                           in reference cells; queries lie on the reference grid unless query_xy (B,n,2)
+                                           gives [x, y]
+
+    mask (B,H,W) or (B,1,H,W): a cell with 0 / False takes no part, whatever its features hold (background of a
+    rendered template).  num_query (B,): only the first num_query[b] queries of item b are real, as in dense_nn.
+    Returns out (B,Cv,...) over query's cells in query's dtype, with return_lse also lse (B,heads,n) float32, the log of
+    the sum of exp(z): the match's confidence.  A query that is not real, or whose cells are all masked, gets 0 and -inf.
+
+    Tensors that require gradients get them (out and lse, once; value None: ref's is the sum of both uses); no gradient
+    flows to falloff, query_xy or the masks.  Scores, sums and log-sums are float32; bfloat16 maps round the weights to
+    bfloat16 for the product with the values.  Memory grows with the maps, not with their product, and results do
+    not change from run to run."""
+    as_tensor = dv.is_tensor(query)
+    call = _Call(query, ref, value, heads, scale, cap, falloff, query_xy, mask, num_query)
+    if torch.is_grad_enabled() and any(dv.is_tensor(x) and x.requires_grad for x in (query, ref, value)):
+        if not all(dv.is_tensor(x) for x in (query, ref, value) if x is not None):
+            raise ValueError("query, ref and value must be tensors where one of them requires gradients")
+        out, lse = _SoftMatch.apply(query, ref, value, call)
+        return (out, lse) if return_lse else out
+    with _place(query):
+        out, _, lse = call.upload().forward(exact=False)
+        out = dv.back(out, as_tensor)
+        return (out, dv.back(lse, as_tensor)) if return_lse else out
+
+
+_KINDS = {"int8": (_abi.STORE_INT8, torch.int8), "fp8": (_abi.STORE_FP8, torch.float8_e4m3fn)}
+
+
+class TemplateStore:
+    """Feature maps of rendered views in 8 bits: a quarter of float32's memory for a class's thousands of views, with the
+    views that `correspondence.nearest_view` names read back, or matched against, straight from their codes.
+
+    codes (n_view,C,H*W) int8 or float8_e4m3fn, scales (n_view,H*W) float32, mask (n_view,H*W) uint8, on one device.
+    A cell's channels share the scale max|x| / 127 ("fp8": / 448); the value is code * scale, so an int8 code is off
+    by at most half a scale, an e4m3 one by 2^-4 of itself.  Views not yet written have no cells.
+
+    Calls run on the current stream; a store that several streams use is ordered by the caller, like any tensor."""
+
+    def __init__(self, n_view, channels, size, kind="int8"):
+        self._set(kind, n_view, channels, size)
+        cells = self.size[0] * self.size[1]
+        dev = dv.device()
+        self.codes = torch.zeros((self.n_view, self.channels, cells), dtype=torch.uint8, device=dev).view(_KINDS[kind][1])
+        self.scales = torch.zeros((self.n_view, cells), dtype=torch.float32, device=dev)
+        self.mask = torch.zeros((self.n_view, cells), dtype=torch.uint8, device=dev)
+
+    def _set(self, kind, n_view, channels, size):
+        if kind not in _KINDS:
+            raise ValueError("kind must be 'int8' or 'fp8'")
+        h, w = (int(x) for x in size)
+        if n_view < 1 or channels < 1 or h < 1 or w < 1:
+            raise ValueError(f"a store of {n_view} views of {channels} x {h} x {w}")
+        self.kind, self.n_view, self.channels, self.size = kind, int(n_view), int(channels), (h, w)
+
+    @classmethod
+    def from_tensors(cls, codes, scales, mask, size):
+        """A store over existing tensors (kept, not copied), e.g. ones that were saved."""
+        kind = {torch.int8: "int8", torch.float8_e4m3fn: "fp8"}.get(codes.dtype)
+        if kind is None or codes.dim() != 3:
+            raise ValueError("codes must be (n_view,C,H*W) int8 or float8_e4m3fn")
+        store = cls.__new__(cls)
+        store._set(kind, codes.shape[0], codes.shape[1], size)
+        flat = (codes.shape[0], codes.shape[2])
+        if codes.shape[2] != store.size[0] * store.size[1]:
+            raise ValueError(f"codes of {codes.shape[2]} cells are no {store.size} maps")
+        if tuple(scales.shape) != flat or scales.dtype != torch.float32:
+            raise ValueError(f"scales must be {flat} float32")
+        if tuple(mask.shape) != flat or mask.dtype != torch.uint8:
+            raise ValueError(f"mask must be {flat} uint8")
+        if not (codes.is_cuda and scales.device == codes.device == mask.device):
+            raise ValueError("codes, scales and mask must lie on one GPU")
+        if not (codes.is_contiguous() and scales.is_contiguous() and mask.is_contiguous()):
+            raise ValueError("codes, scales and mask must be contiguous")
+        store.codes, store.scales, store.mask = codes, scales, mask
+        return store
+
+    def _views(self, views, dims):
+        """Host indices are checked here; device ones by the kernels, which take an index outside as no view."""
+        if not dv.is_tensor(views) or not views.is_cuda:
+            host = np.asarray(views)
+            if host.size and not np.issubdtype(host.dtype, np.integer):
+                raise ValueError("views must be integers")
+            if host.size and (host.min() < -1 or host.max() >= self.n_view):
+                raise IndexError(f"view index outside [0, {self.n_view}) (-1: no view)")
+            views = host.astype(np.int32)
+        elif views.dtype not in (torch.int32, torch.int64):
+            raise ValueError("views must be int32 or int64")
+        if len(_dims(views)) != dims:
+            raise ValueError(f"views must have {dims} dimension{'s' if dims > 1 else ''}, got {_dims(views)}")
+        return views
+
+    @staticmethod
+    def _index(views):
+        # an int64 index that int32 would wrap into the store must stay outside it
+        if dv.is_tensor(views) and views.dtype == torch.int64:
+            views = views.clamp(-1, 2 ** 31 - 1)
+        return dv.to_dev(views, torch.int32)
+
+    def write(self, views, features, mask=None):
+        """Quantises features (n,C,H,W) (float32, or bfloat16 tensors) into views (n,).  mask (n,H,W): the cells that hold
+        an object, all if None; a cell with a non-finite channel is masked as well.  A view listed twice keeps its
+        last entry; -1 skips an entry."""
+        views = self._views(views, 1)
+        n = _dims(views)[0]
+        dtype = _dtype(features, "features")
+        if _dims(features) != (n, self.channels) + self.size:
+            raise ValueError(f"features must be {(n, self.channels) + self.size}, got {_dims(features)}")
+        if mask is not None and int(np.prod(_dims(mask), dtype=np.int64)) != n * self.size[0] * self.size[1]:
+            raise ValueError(f"mask must be {(n,) + self.size}, got {_dims(mask)}")
+        with _place(self.codes):
+            v, f = self._index(views), dv.to_dev(features, dtype)
+            m = _mask(mask)
+            _abi.check(_abi.lib.ispa_store_write(dv.ptr(f), _CODES[dtype], dv.ptr(m), dv.ptr(v), n, _KINDS[self.kind][0],
+                                                 self.n_view, self.channels, self.codes.shape[2], dv.ptr(self.codes),
+                                                 dv.ptr(self.scales), dv.ptr(self.mask), dv.stream_ptr()))
+
+    def read(self, views, dtype=torch.float32):
+        """The features of views (n,), (n,C,H,W) of `dtype` (float32 or bfloat16), for dense_nn and the correlation layers.
+        Zeros for -1 and views not written."""
+        if dtype not in _CODES:
+            raise ValueError("dtype must be torch.float32 or torch.bfloat16")
+        views = self._views(views, 1)
+        with _place(self.codes):
+            v = self._index(views)
+            out = dv.empty((v.numel(), self.channels) + self.size, dtype)
+            _abi.check(_abi.lib.ispa_store_read(dv.ptr(self.codes), dv.ptr(self.scales), dv.ptr(v), v.numel(),
+                                                _KINDS[self.kind][0], self.n_view, self.channels, self.codes.shape[2],
+                                                _CODES[dtype], dv.ptr(out), dv.stream_ptr()))
+            return out
+
+    def read_mask(self, views):
+        """The masks of views (n,) as (n,H,W) uint8; zeros for -1 and views not written."""
+        views = self._views(views, 1)
+        with _place(self.codes):
+            v = self._index(views).long()
+            inside = (v >= 0) & (v < self.n_view)
+            return (self.mask[torch.where(inside, v, 0)] * inside[:, None]).view((v.numel(),) + self.size)
+
+    def soft_match(self, query, views, *, heads=1, scale=None, cap=0.0, falloff=None, query_xy=None, num_query=None,
+                   return_lse=False):
+        """soft_match of query (B,C,Hq,Wq) or (B,C,n) against the stored views (B,V) of each item: one softmax over the
+        cells of all V views, whose features are reference and value, read from their codes.  -1 stands for no
+        view, the store's masks apply, and the other arguments are soft_match's.  No gradients flow."""
+        n = _elements(query, "query")
+        b, c = _dims(query)[:2]
+        dtype = _dtype(query, "query")
+        heads = int(heads)
+        if c != self.channels:
+            raise ValueError(f"query has {c} channels, the store {self.channels}")
+        if heads < 1 or c % heads or c // heads > MAX_CHANNELS:
+            raise ValueError(f"{c} channels do not split into {heads} heads of at most {MAX_CHANNELS}")
+        views = self._views(views, 2)
+        if _dims(views)[0] != b:
+            raise ValueError(f"views must be ({b},V), got {_dims(views)}")
+        if scale is None:
+            scale = (c // heads) ** -0.5
+        scale, cap = _scores(heads, scale, cap, falloff, query_xy, self.size, _dims(query)[2:], b, n)
+        count = _counts(num_query, b)
+        as_tensor = dv.is_tensor(query)
+        with _place(self.codes):
+            q, v = dv.to_dev(query.detach() if as_tensor else query, dtype), self._index(views)
+            f, xy = _score_tensors(heads, falloff, query_xy)
+            count = _count_tensor(count)
+            out = dv.empty((b, c) + _dims(query)[2:], dtype)
+            lse = dv.empty((b, heads, n), torch.float32)
+            cells = self.codes.shape[2]
+            need = _abi.lib.ispa_soft_match_workspace_bytes(_CODES[dtype], b, heads, c // heads, c // heads, n, v.shape[1], cells)
+            ws = dv.empty((need,), torch.uint8) if need else None
+            _abi.check(_abi.lib.ispa_store_match(
+                dv.ptr(q), _CODES[dtype], dv.ptr(self.codes), dv.ptr(self.scales), dv.ptr(self.mask), _KINDS[self.kind][0],
+                dv.ptr(v), v.shape[1], self.n_view, b, heads, c // heads, n, cells, self.size[1], scale, cap, dv.ptr(f),
+                dv.ptr(xy), dv.ptr(count), dv.ptr(out), dv.ptr(lse), dv.ptr(ws), need, dv.stream_ptr()))
+            out = dv.back(out, as_tensor)
+            return (out, dv.back(lse, as_tensor)) if return_lse else out
