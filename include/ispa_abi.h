@@ -413,12 +413,13 @@ int ispa_soft_match_backward(const void *q, const void *r, const void *v, int dt
  * code value, ties to even; value = code * scale.
  * write: features (n,C,cells) f32 or bf16 go to views[0..n); take (optional) (n,cells) u8 becomes the mask; a cell with a
  * non-finite channel is stored as zeros, masked.  A view listed twice keeps its last entry; an index outside
- * [0, n_view) is skipped.  read: out (n,C,cells) f32 or bf16; an index outside gives zeros. */
+ * [0, n_view) is skipped.  read: out (n,C,cells) f32 or bf16 and mask_out (n,cells) u8, either may be NULL; an index outside
+ * gives zeros. */
 enum { ISPA_STORE_INT8 = 0, ISPA_STORE_FP8 = 1 };
 int ispa_store_write(const void *features, int dtype, const uint8_t *take, const int32_t *views, int n, int kind, int n_view,
                      int C, int64_t cells, void *codes, float *scales, uint8_t *mask, void *stream);
-int ispa_store_read(const void *codes, const float *scales, const int32_t *views, int n, int kind, int n_view, int C,
-                    int64_t cells, int dtype, void *out, void *stream);
+int ispa_store_read(const void *codes, const float *scales, const uint8_t *mask, const int32_t *views, int n, int kind,
+                    int n_view, int C, int64_t cells, int dtype, void *out, uint8_t *mask_out, void *stream);
 
 /* ispa_soft_match against stored views, read from their codes: item b matches the cells of views[b,0..V) (views (B,V)
  * i32) jointly, r = v = their values; an index outside [0, n_view) stands for no view.  C = heads*D.  dtype is that of q

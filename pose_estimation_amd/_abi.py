@@ -79,7 +79,7 @@ SIGNATURES = {
     "ispa_soft_match_backward": (_i, [_p, _p, _p, _i, _i, _i, _i, _i, _i64, _i64, _i, _f, _f, _p, _p, _p, _p, _p, _p, _p, _p,
                                       _p, _p, _p, _p, _sz, _p]),
     "ispa_store_write": (_i, [_p, _i, _p, _p, _i, _i, _i, _i, _i64, _p, _p, _p, _p]),
-    "ispa_store_read": (_i, [_p, _p, _p, _i, _i, _i, _i, _i64, _i, _p, _p]),
+    "ispa_store_read": (_i, [_p, _p, _p, _p, _i, _i, _i, _i, _i64, _i, _p, _p, _p]),
     "ispa_store_match": (_i, [_p, _i, _p, _p, _p, _i, _p, _i, _i, _i, _i, _i, _i64, _i64, _i, _f, _f, _p, _p, _p, _p, _p, _p,
                               _sz, _p]),
     "ispa_prune_points_2d": (_i, [_p, _i, _i64, _p, _p, _i, _p, _p, _i, _i, _i, _i, _p, _p]),

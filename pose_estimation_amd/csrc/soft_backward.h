@@ -88,9 +88,13 @@ __global__ __launch_bounds__(64 * WQ) void soft_dq_kernel(const Params p) {
         if constexpr (M::kRows == 32) live &= 0xffffffffull;
         if (live == 0) continue;                               // the same in every wave
         __syncthreads();
-        load_tile<M, T, DP, NT>(ktile, keys.base(p.k, at, p.D), p.cells, p.D, at.cell0, p.cells, live, 0.f);
-        if (!p.shared)
-            load_tile<M, T, DP, NT>(vtile, keys.base(p.v, at, p.Dv), p.cells, p.Dv, at.cell0, p.cells, live, 0.f);
+        Loader<M, T, DP, NT> kl, vl;
+        kl.load(keys.base(p.k, at, p.D), p.cells, p.D, at.cell0, p.cells);
+        kl.store(ktile, p.cells, p.D, live, 0.f);
+        if (!p.shared) {
+            vl.load(keys.base(p.v, at, p.Dv), p.cells, p.Dv, at.cell0, p.cells);
+            vl.store(vtile, p.cells, p.Dv, live, 0.f);
+        }
         if (p.falloff != nullptr && threadIdx.x < M::kRows) {
             const int c = (int)at.cell0 + threadIdx.x;
             xarr[threadIdx.x] = (float)(c % p.W);
@@ -203,8 +207,11 @@ __global__ __launch_bounds__(64 * WQ) void soft_dkv_kernel(const Params p) {
     for (int t = t0; t < t1; ++t) {
         const int64_t q0 = (int64_t)t * M::kRows;
         __syncthreads();
-        load_tile<M, T, DP, NT>(qtile, qmap, p.nq, p.D, q0, live_q, ~0ull, 0.f);
-        load_tile<M, T, DP, NT>(otile, omap, p.nq, p.Dv, q0, live_q, ~0ull, 0.f);
+        Loader<M, T, DP, NT> ql, ol;
+        ql.load(qmap, p.nq, p.D, q0, live_q);
+        ql.store(qtile, p.nq, p.D, ~0ull, 0.f);
+        ol.load(omap, p.nq, p.Dv, q0, live_q);
+        ol.store(otile, p.nq, p.Dv, ~0ull, 0.f);
         if (threadIdx.x < M::kRows) {
             const int64_t q = q0 + threadIdx.x;
             float lse2 = __builtin_inff(), delta = 0.f, x = 0.f, y = 0.f;      // no weight without cells

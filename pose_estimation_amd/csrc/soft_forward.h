@@ -55,37 +55,46 @@ __device__ __forceinline__ void query_place(const Params &p, int b, int64_t i, f
     }
 }
 
-template <int DP, bool SHARED>
-constexpr int forward_lds() {
-    return (SHARED ? 1 : 2) * DP * kRowBytes + 3 * 64 * (int)sizeof(float);
+// LDS of one buffer: the tiles, and per cell the scale and the place.
+template <int DP>
+constexpr int stage_bytes(bool shared) {
+    return (shared ? 1 : 2) * DP * kRowBytes + 3 * 64 * (int)sizeof(float);
 }
+// Two buffers where the loads run a tile ahead.
+template <typename T, typename SRC, int DP, int WQ>
+constexpr int kBuffers = Loader<Math<T, DP>, SRC, DP, 64 * WQ>::kAhead ? 2 : 1;
+
+// How far (in units of log2) a query's largest score may rise above the maximum that its sums are kept against before they
+// are rescaled: weights stay below 2^8, and nearly all tiles leave the accumulators alone.
+constexpr float kSlack = 8.f;
 
 // NC: value channels that one launch forms, from p.c0 on (256 float32 channels take two launches, for the registers).
 template <typename T, typename SRC, int DP, int WQ, int NC>
-__global__ __launch_bounds__(64 * WQ) void soft_forward_kernel(const Params p) {
+__global__ __launch_bounds__(64 * WQ, (DP <= 128 && std::is_same_v<SRC, BF16>) ? 2 : 1) void soft_forward_kernel(const Params p) {
     typedef Math<T, DP> M;
     constexpr int NT = 64 * WQ;
     constexpr int kBlocks = M::kRows / 32;
+    constexpr uint64_t kAll = M::kRows == 64 ? ~0ull : 0xffffffffull;
     constexpr bool kCodes = KeyTiles<M, SRC>::kCodes;
     constexpr bool kScaled = kCodes && std::is_same_v<T, BF16>;        // scales applied to scores and weights
+    typedef Loader<M, SRC, DP, NT> L;
     extern __shared__ __attribute__((aligned(16))) char lds[];
-    char *ktile = lds;
-    char *vtile = p.shared ? lds : lds + DP * kRowBytes;
-    float *sarr = reinterpret_cast<float *>(vtile + DP * kRowBytes);
-    float *xarr = sarr + 64, *yarr = sarr + 128;
+    const int v_at = p.shared ? 0 : DP * kRowBytes, cell_at = v_at + DP * kRowBytes;
+    const int stage = cell_at + 3 * 64 * (int)sizeof(float);
 
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, h = lane >> 5;
-    int id = blockIdx.x;
+    int id = die_major(blockIdx.x, gridDim.x);
     const int qblk = id % p.blocks;
     id /= p.blocks;
     const int split = id % p.splits;
     const int bh = id / p.splits;
     const int b = bh / p.heads, head = bh - b * p.heads;
-    const int t0 = (int)((int64_t)p.tiles * split / p.splits), t1 = (int)((int64_t)p.tiles * (split + 1) / p.splits);
     const int64_t live_q = live_queries(p, b);
     const int64_t q = ((int64_t)qblk * WQ + wave) * 32 + (lane & 31);
     const bool q_ok = q < live_q;
     const bool idle = (int64_t)qblk * WQ * 32 >= live_q;       // no live query in the whole workgroup
+    const int t0 = (int)((int64_t)p.tiles * split / p.splits);
+    const int t1 = idle ? t0 : (int)((int64_t)p.tiles * (split + 1) / p.splits);
 
     typename M::Owned qf;
     M::load_owned(qf, (const typename T::elem *)p.q + (int64_t)bh * p.D * p.nq + (q < p.nq ? q : 0), p.nq, p.D, q_ok, h);
@@ -102,85 +111,124 @@ __global__ __launch_bounds__(64 * WQ) void soft_forward_kernel(const Params p) {
     float m = -__builtin_inff(), l = 0.f;                      // l: this lane's half of the cells
 
     const KeyTiles<M, SRC> keys(p, b, head);
-    for (int t = t0; t < (idle ? t0 : t1); ++t) {
-        const typename KeyTiles<M, SRC>::At at = keys.at(t);
-        const bool ok = keys.live(at, lane);
-        uint64_t live = __ballot(ok);
-        if constexpr (M::kRows == 32) live &= 0xffffffffull;
-        if (live == 0) continue;                               // the same in every wave
-        const float sc = keys.scale(at, lane, ok);
-        __syncthreads();
-        load_tile<M, SRC, DP, NT>(ktile, keys.base(p.k, at, p.D), p.cells, p.D, at.cell0, p.cells, live, sc);
-        if (!p.shared)
-            load_tile<M, SRC, DP, NT>(vtile, keys.base(p.v, at, p.Dv), p.cells, p.Dv, at.cell0, p.cells, live, sc);
-        if (kScaled && wave == 0) sarr[lane] = sc;
+    L kl, vl;
+    typename KeyTiles<M, SRC>::At at{};
+    bool ok = false;
+    float sc = 0.f;
+    auto fetch = [&](int t) {
+        at = keys.at(t);
+        ok = keys.live(at, lane);
+        sc = keys.scale(at, lane, ok);
+        const int64_t n = at.map < 0 ? 0 : p.cells;
+        kl.load(keys.base(p.k, at, p.D), p.cells, p.D, at.cell0, n);
+        if (!p.shared) vl.load(keys.base(p.v, at, p.Dv), p.cells, p.Dv, at.cell0, n);
+    };
+    auto put = [&](char *buf) {                                // the fetched tile into LDS; its live cells
+        const uint64_t live = __ballot(ok) & kAll;
+        if (live == 0) return live;                            // the same in every wave
+        kl.store(buf, p.cells, p.D, live, sc);
+        if (!p.shared) vl.store(buf + v_at, p.cells, p.Dv, live, sc);
+        float *cell = reinterpret_cast<float *>(buf + cell_at);
+        if (kScaled && wave == 0) cell[lane] = sc;
         if (p.falloff != nullptr && threadIdx.x < M::kRows) {
             const int c = (int)at.cell0 + threadIdx.x;
-            xarr[threadIdx.x] = (float)(c % p.W);
-            yarr[threadIdx.x] = (float)(c / p.W);
+            cell[64 + threadIdx.x] = (float)(c % p.W);
+            cell[128 + threadIdx.x] = (float)(c / p.W);
+        }
+        return live;
+    };
+    uint64_t live = 0;
+    if constexpr (L::kAhead) {
+        if (t0 < t1) {
+            fetch(t0);
+            live = put(lds);
         }
         __syncthreads();
-
-        float z[kBlocks][16], ks[kBlocks][16];
-        float top = -__builtin_inff();
-#pragma unroll
-        for (int k = 0; k < kBlocks; ++k) {
-            if (DP == 256) __builtin_amdgcn_sched_barrier(0);
-            f32x16 acc = M::first(ktile, addr, k, qf);
-            if constexpr (kScaled) {
-                M::per_cell(sarr, k, h, ks[k]);
-#pragma unroll
-                for (int i = 0; i < 16; ++i) acc[i] *= ks[k][i];
-            }
-            if (p.falloff != nullptr) {
-                M::per_cell(xarr, k, h, z[k]);
-#pragma unroll
-                for (int i = 0; i < 16; ++i) z[k][i] = (z[k][i] - qx) * (z[k][i] - qx);
-                float cy[16];
-                M::per_cell(yarr, k, h, cy);
-#pragma unroll
-                for (int i = 0; i < 16; ++i) z[k][i] = -score.fall * fmaf(cy[i] - qy, cy[i] - qy, z[k][i]);
-            } else {
-#pragma unroll
-                for (int i = 0; i < 16; ++i) z[k][i] = 0.f;
-            }
-            if (score.cap) {
-#pragma unroll
-                for (int i = 0; i < 16; ++i) z[k][i] = fmaf(score.top, score.bend(acc[i]), z[k][i]);
-            } else {
-#pragma unroll
-                for (int i = 0; i < 16; ++i) z[k][i] = fmaf(score.in, acc[i], z[k][i]);
-            }
-            if (live != (M::kRows == 64 ? ~0ull : 0xffffffffull)) {
-                const unsigned bits = (unsigned)(live >> (32 * k));
-#pragma unroll
-                for (int i = 0; i < 16; ++i)
-                    z[k][i] = (bits >> M::cell(i, h)) & 1u ? z[k][i] : -__builtin_inff();
-            }
-#pragma unroll
-            for (int i = 0; i < 16; ++i) top = fmaxf(top, z[k][i]);
+    }
+    for (int t = t0; t < t1; ++t) {
+        const char *buf = lds + (L::kAhead ? ((t - t0) & 1) * stage : 0);
+        if constexpr (L::kAhead) {
+            if (t + 1 < t1) fetch(t + 1);
+        } else {
+            __syncthreads();
+            fetch(t);
+            live = put(lds);
+            __syncthreads();
         }
-        top = fmaxf(top, __shfl_xor(top, 32));
-        const float m_new = fmaxf(m, top);
-        const float m_use = m_new == -__builtin_inff() ? 0.f : m_new;
-        const float fix = exp2_(m - m_use);
-        m = m_new;
-        l *= fix;
+        if (live != 0) {
+            const char *ktile = buf, *vtile = buf + v_at;
+            const float *cell = reinterpret_cast<const float *>(buf + cell_at);
+            float z[kBlocks][16];
+            float ks[kScaled ? kBlocks : 1][16];
+            float top = -__builtin_inff();
 #pragma unroll
-        for (int c = 0; c < NC / 32; ++c)
+            for (int k = 0; k < kBlocks; ++k) {
+                if (DP == 256) __builtin_amdgcn_sched_barrier(0);
+                f32x16 acc = M::first(ktile, addr, k, qf);
+                if constexpr (kScaled) {
+                    M::per_cell(cell, k, h, ks[k]);
 #pragma unroll
-            for (int i = 0; i < 16; ++i) o[c][i] *= fix;
+                    for (int i = 0; i < 16; ++i) acc[i] *= ks[k][i];
+                }
+                if (p.falloff != nullptr) {
+                    M::per_cell(cell + 64, k, h, z[k]);
 #pragma unroll
-        for (int k = 0; k < kBlocks; ++k) {
-            float w[16];
+                    for (int i = 0; i < 16; ++i) z[k][i] = (z[k][i] - qx) * (z[k][i] - qx);
+                    float cy[16];
+                    M::per_cell(cell + 128, k, h, cy);
 #pragma unroll
-            for (int i = 0; i < 16; ++i) {
-                w[i] = exp2_(z[k][i] - m_use);
-                l += w[i];
-                if constexpr (kScaled) w[i] *= ks[k][i];
+                    for (int i = 0; i < 16; ++i) z[k][i] = -score.fall * fmaf(cy[i] - qy, cy[i] - qy, z[k][i]);
+                    if (score.cap) {
+#pragma unroll
+                        for (int i = 0; i < 16; ++i) z[k][i] = fmaf(score.top, score.bend(acc[i]), z[k][i]);
+                    } else {
+#pragma unroll
+                        for (int i = 0; i < 16; ++i) z[k][i] = fmaf(score.in, acc[i], z[k][i]);
+                    }
+                } else if (score.cap) {
+#pragma unroll
+                    for (int i = 0; i < 16; ++i) z[k][i] = score.top * score.bend(acc[i]);
+                } else {
+#pragma unroll
+                    for (int i = 0; i < 16; ++i) z[k][i] = score.in * acc[i];
+                }
+                if (live != kAll) {
+                    const unsigned bits = (unsigned)(live >> (32 * k)) >> M::cell(0, h);
+#pragma unroll
+                    for (int i = 0; i < 16; ++i)
+                        z[k][i] = bits & (1u << M::cell(i, 0)) ? z[k][i] : -__builtin_inff();
+                }
+#pragma unroll
+                for (int i = 0; i < 16; ++i) top = fmaxf(top, z[k][i]);
             }
-            // weights in [0, 1] are rounded to the maps' type for the second product, the sum l is not
-            M::second(vtile + p.c0 * kRowBytes, addr, k, M::weights(w), o);
+            top = fmaxf(top, __shfl_xor(top, 32));
+            if (__any(top > m + kSlack)) {
+                const float m_new = fmaxf(m, top);
+                const float fix = exp2_(m - (m_new == -__builtin_inff() ? 0.f : m_new));
+                m = m_new;
+                l *= fix;
+#pragma unroll
+                for (int c = 0; c < NC / 32; ++c)
+#pragma unroll
+                    for (int i = 0; i < 16; ++i) o[c][i] *= fix;
+            }
+            const float m_use = m == -__builtin_inff() ? 0.f : m;
+#pragma unroll
+            for (int k = 0; k < kBlocks; ++k) {
+                float w[16];
+#pragma unroll
+                for (int i = 0; i < 16; ++i) {
+                    w[i] = exp2_(z[k][i] - m_use);
+                    l += w[i];
+                    if constexpr (kScaled) w[i] *= ks[k][i];
+                }
+                // weights are rounded to the maps' type for the second product, the sum l is not
+                M::second(vtile + p.c0 * kRowBytes, addr, k, M::weights(w), o);
+            }
+        }
+        if constexpr (L::kAhead) {
+            if (t + 1 < t1) live = put(lds + ((t + 1 - t0) & 1) * stage);
+            __syncthreads();
         }
     }
     l += __shfl_xor(l, 32);

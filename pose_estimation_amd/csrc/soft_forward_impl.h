@@ -8,7 +8,7 @@ namespace ispa_soft {
 template <typename T, typename SRC, int DP, int WQ>
 int forward_one(Params p, hipStream_t stream) {
     static unsigned long long lds_allowed = 0;
-    const int lds = p.shared ? forward_lds<DP, true>() : forward_lds<DP, false>();
+    const int lds = kBuffers<T, SRC, DP, WQ> * stage_bytes<DP>(p.shared);
     const unsigned grid = (unsigned)((int64_t)p.B * p.heads * p.splits * p.blocks);
     constexpr int NC = DP == 256 && std::is_same_v<T, F32> ? 128 : DP;
     for (p.c0 = 0; p.c0 < p.Dv; p.c0 += NC)

@@ -271,44 +271,33 @@ struct Math<F32, DP> {
 __device__ __forceinline__ int out_channel(int i, int h) { return 8 * (i >> 2) + 4 * h + (i & 3); }
 
 // ------------------------------------------------------------------------------------------------
-// Loads one tile: NT threads, thread t takes segment t & 7 of channel rows t / 8, t / 8 + NT / 8, ..., kBatch rows at a
-// time in registers.  live: bit j = cell j of the tile takes part; scale: the codes' scale of the tile's cell
-// lane % kRows (float32 arithmetic multiplies here, bfloat16 arithmetic keeps the codes, which bfloat16 holds exactly,
-// and scales the scores and weights).
+// Loader of one tile: NT threads, thread t takes segment t & 7 of channel rows t / 8, t / 8 + NT / 8, ...
+// kAhead: the whole share of a thread fits a few registers, so that the loads of the next tile are issued (load) before
+// the products of the present one and written to LDS (store) after them; else store does both, a few rows at a time.
+// live: bit j = cell j of the tile takes part; scale: the codes' scale of the tile's cell lane % kRows (float32
+// arithmetic multiplies here, bfloat16 arithmetic keeps the codes, which bfloat16 holds exactly, and scales the scores
+// and weights).
 // Cells past the map's end, masked cells and channels past d are staged as zeros: whatever a masked cell holds
 // (infinities, NaN) meets a weight of zero in the second product and must not turn it into NaN.
 template <typename M, typename SRC, int DP, int NT>
-__device__ __forceinline__ void load_tile(char *tile, const typename SRC::elem *base, int64_t ld, int d, int64_t cell0,
-                                          int64_t n, uint64_t live, float scale) {
-    constexpr bool kCodes = std::is_same_v<SRC, I8> || std::is_same_v<SRC, FP8>;
-    constexpr bool kNarrow = std::is_same_v<typename M::map, BF16>;
-    constexpr int kN = M::kCells;
-    constexpr int kPer = DP * 8 / NT;
-    constexpr int kBatch = DP == 256 ? (kCodes || NT == 64 ? 1 : 2) : kPer < 8 ? kPer : 8;
+struct Loader {
+    static constexpr bool kCodes = std::is_same_v<SRC, I8> || std::is_same_v<SRC, FP8>;
+    static constexpr bool kNarrow = std::is_same_v<typename M::map, BF16>;
+    static constexpr int kN = M::kCells;
+    static constexpr int kPer = DP * 8 / NT;
+    typedef typename SRC::elem elem;
     typedef std::conditional_t<!kCodes, u32x4, std::conditional_t<kNarrow, u32x2, unsigned>> raw;
-    const int seg = threadIdx.x & 7, row0 = threadIdx.x >> 3;
-    const unsigned bits = (unsigned)(live >> (seg * kN)) & ((1u << kN) - 1u);
-    u32x4 keep;
-#pragma unroll
-    for (int j = 0; j < 4; ++j) {
-        if constexpr (kNarrow)
-            keep[j] = ((bits >> (2 * j)) & 1u ? 0xffffu : 0u) | ((bits >> (2 * j + 1)) & 1u ? 0xffff0000u : 0u);
-        else
-            keep[j] = (bits >> j) & 1u ? 0xffffffffu : 0u;
-    }
-    float sc[4] = {};
-    if constexpr (kCodes && !kNarrow)
-#pragma unroll
-        for (int j = 0; j < 4; ++j) sc[j] = __shfl(scale, seg * 4 + j);
-    const int64_t at = cell0 + seg * kN;
-    const int64_t left = n - at;
-    const int ok = left >= kN ? kN : left > 0 ? (int)left : 0;
-    const typename SRC::elem *p = base + (int64_t)row0 * ld + at;
-    const int at0 = row0 * kRowBytes + ((seg ^ swz(row0)) << 4);
+    static constexpr bool kAhead = kPer * (int)sizeof(raw) <= (DP == 256 ? 64 : 128);
+    static constexpr int kBatch = kAhead ? kPer : DP == 256 ? (kCodes || NT == 64 ? 1 : 2) : kPer < 8 ? kPer : 8;
+    static constexpr int kLoop = kAhead ? kPer / kBatch : 1;
     static_assert(NT == 64 || NT % 128 == 0, "");
-#pragma unroll 1
-    for (int i0 = 0; i0 < kPer; i0 += kBatch) {
-        raw r[kBatch];
+    raw r[kBatch];
+    const elem *from;          // this thread's first segment
+    int ok;                    // cells of the segment that the map has
+
+    __device__ void rows(int i0, int64_t ld, int d) {
+        const int row0 = threadIdx.x >> 3;
+        const elem *p = from + (int64_t)i0 * (NT / 8) * ld;
 #pragma unroll
         for (int i = 0; i < kBatch; ++i) {
             raw v = {};
@@ -316,45 +305,80 @@ __device__ __forceinline__ void load_tile(char *tile, const typename SRC::elem *
                 if (ok == kN) {
                     __builtin_memcpy(&v, p, sizeof(raw));
                 } else if (ok > 0) {
-                    typename SRC::elem e[kN];
+                    elem e[kN];
 #pragma unroll
-                    for (int j = 0; j < kN; ++j) e[j] = j < ok ? p[j] : (typename SRC::elem)0;
+                    for (int j = 0; j < kN; ++j) e[j] = j < ok ? p[j] : (elem)0;
                     __builtin_memcpy(&v, e, sizeof(raw));
                 }
             }
             r[i] = v;
             p += (int64_t)(NT / 8) * ld;
         }
+    }
+    __device__ void load(const elem *base, int64_t ld, int d, int64_t cell0, int64_t n) {
+        const int64_t at = cell0 + (threadIdx.x & 7) * kN;
+        const int64_t left = n - at;
+        ok = left >= kN ? kN : left > 0 ? (int)left : 0;
+        from = base + (int64_t)(threadIdx.x >> 3) * ld + at;
+        if constexpr (kAhead) rows(0, ld, d);
+    }
+    __device__ void store(char *tile, int64_t ld, int d, uint64_t live, float scale) {
+        const int seg = threadIdx.x & 7, row0 = threadIdx.x >> 3;
+        const unsigned bits = (unsigned)(live >> (seg * kN)) & ((1u << kN) - 1u);
+        const bool whole = live == (M::kRows == 64 ? ~0ull : 0xffffffffull);
+        u32x4 keep;
 #pragma unroll
-        for (int i = 0; i < kBatch; ++i) {
-            u32x4 v;
-            if constexpr (!kCodes) {
-                v = r[i];
-            } else if constexpr (kNarrow) {
-                float f[8];
-                float x[4], y[4];
-                decode4<SRC>(r[i][0], x);
-                decode4<SRC>(r[i][1], y);
+        for (int j = 0; j < 4; ++j) {
+            if constexpr (kNarrow)
+                keep[j] = ((bits >> (2 * j)) & 1u ? 0xffffu : 0u) | ((bits >> (2 * j + 1)) & 1u ? 0xffff0000u : 0u);
+            else
+                keep[j] = (bits >> j) & 1u ? 0xffffffffu : 0u;
+        }
+        float sc[4] = {};
+        if constexpr (kCodes && !kNarrow)
 #pragma unroll
-                for (int j = 0; j < 4; ++j) {
-                    f[j] = x[j];
-                    f[4 + j] = y[j];
+            for (int j = 0; j < 4; ++j) sc[j] = __shfl(scale, seg * 4 + j);
+        const int at0 = row0 * kRowBytes + ((seg ^ swz(row0)) << 4);
+#pragma unroll kLoop
+        for (int i0 = 0; i0 < kPer; i0 += kBatch) {
+            if constexpr (!kAhead) rows(i0, ld, d);
+#pragma unroll
+            for (int i = 0; i < kBatch; ++i) {
+                u32x4 v;
+                if constexpr (!kCodes) {
+                    v = r[i];
+                } else if constexpr (kNarrow) {
+                    float x[4], y[4];
+                    decode4<SRC>(r[i][0], x);
+                    decode4<SRC>(r[i][1], y);
+                    // 8-bit codes fit bfloat16: the upper halves are the values
+#pragma unroll
+                    for (int j = 0; j < 2; ++j) {
+                        v[j] = __builtin_amdgcn_perm(__builtin_bit_cast(unsigned, x[2 * j + 1]),
+                                                     __builtin_bit_cast(unsigned, x[2 * j]), 0x07060302u);
+                        v[2 + j] = __builtin_amdgcn_perm(__builtin_bit_cast(unsigned, y[2 * j + 1]),
+                                                         __builtin_bit_cast(unsigned, y[2 * j]), 0x07060302u);
+                    }
+                } else {
+                    float f[4];
+                    decode4<SRC>(r[i], f);
+#pragma unroll
+                    for (int j = 0; j < 4; ++j) v[j] = __builtin_bit_cast(unsigned, f[j] * sc[j]);
                 }
-#pragma unroll
-                for (int j = 0; j < 4; ++j)      // 8-bit codes fit bfloat16: the upper halves are the values
-                    v[j] = (__builtin_bit_cast(unsigned, f[2 * j]) >> 16) |
-                           (__builtin_bit_cast(unsigned, f[2 * j + 1]) & 0xffff0000u);
-            } else {
-                float f[4];
-                decode4<SRC>(r[i], f);
-#pragma unroll
-                for (int j = 0; j < 4; ++j) v[j] = __builtin_bit_cast(unsigned, f[j] * sc[j]);
+                if (!whole) v &= keep;
+                // swz repeats every 16 rows; 8 rows further (one wave) it differs by 2
+                const int at = at0 ^ (NT == 64 ? ((i0 + i) & 1) << 5 : 0);
+                *reinterpret_cast<u32x4 *>(tile + at + (i0 + i) * (NT / 8) * kRowBytes) = v;
             }
-            // swz repeats every 16 rows; 8 rows further (one wave) it differs by 2
-            const int at = at0 ^ (NT == 64 ? ((i0 + i) & 1) << 5 : 0);
-            *reinterpret_cast<u32x4 *>(tile + at + (i0 + i) * (NT / 8) * kRowBytes) = v & keep;
         }
     }
+};
+
+// Workgroups are dealt to the 8 dies in turn; this numbering gives each die a run of successive workgroups, so that those
+// that stream the same maps share one L2.
+__device__ __forceinline__ int die_major(int id, int n) {
+    const int die = id & 7, per = n >> 3, more = n & 7;
+    return die * per + (die < more ? die : more) + (id >> 3);
 }
 
 // ------------------------------------------------------------------------------------------------

@@ -85,8 +85,10 @@ __global__ __launch_bounds__(kThreads) void store_write_kernel(const typename T:
 template <typename T, typename S>
 __global__ __launch_bounds__(kThreads) void store_read_kernel(const unsigned char *__restrict__ codes,
                                                               const float *__restrict__ scales,
+                                                              const uint8_t *__restrict__ mask,
                                                               const int32_t *__restrict__ views, int n_view, int C,
-                                                              int64_t cells, typename T::elem *__restrict__ out) {
+                                                              int64_t cells, typename T::elem *__restrict__ out,
+                                                              uint8_t *__restrict__ mask_out) {
     const int64_t per = (cells + 63) / 64;
     const int item = (int)(blockIdx.x / per);
     const int id = views[item];
@@ -94,6 +96,8 @@ __global__ __launch_bounds__(kThreads) void store_read_kernel(const unsigned cha
     const int lane = threadIdx.x & 63, g = threadIdx.x >> 6;
     const int64_t cell = (blockIdx.x - item * per) * 64 + lane;
     if (cell >= cells) return;
+    if (mask_out != nullptr && g == 0) mask_out[item * cells + cell] = have && mask[(int64_t)id * cells + cell] != 0;
+    if (out == nullptr) return;                                // uniform
     const float s = have ? scales[(int64_t)id * cells + cell] : 0.f;
     const unsigned char *src = codes + (have ? (int64_t)id : 0) * C * cells + cell;
     typename T::elem *dst = out + (int64_t)item * C * cells + cell;
@@ -135,13 +139,14 @@ extern "C" int ispa_store_write(const void *features, int dtype, const uint8_t *
     return ispa::check_launch("store_write_kernel");
 }
 
-extern "C" int ispa_store_read(const void *codes, const float *scales, const int32_t *views, int n, int kind, int n_view,
-                               int C, int64_t cells, int dtype, void *out, void *stream) {
+extern "C" int ispa_store_read(const void *codes, const float *scales, const uint8_t *mask, const int32_t *views, int n,
+                               int kind, int n_view, int C, int64_t cells, int dtype, void *out, uint8_t *mask_out,
+                               void *stream) {
     if (int rc = check(dtype, kind, n, n_view, C, cells)) return rc;
     if (n == 0) return ISPA_OK;
-    ISPA_REQUIRE(codes && scales && views && out, "null pointer");
+    ISPA_REQUIRE(views && (out == nullptr || (codes && scales)) && (mask_out == nullptr || mask), "null pointer");
     const unsigned blocks = (unsigned)((cells + 63) / 64 * n);
     PICK(dtype, kind, (store_read_kernel<T, S><<<blocks, kThreads, 0, (hipStream_t)stream>>>(
-                           (const unsigned char *)codes, scales, views, n_view, C, cells, (T::elem *)out)));
+                           (const unsigned char *)codes, scales, mask, views, n_view, C, cells, (T::elem *)out, mask_out)));
     return ispa::check_launch("store_read_kernel");
 }

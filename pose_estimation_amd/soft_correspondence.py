@@ -9,6 +9,8 @@ Nothing here has a counterpart in it to be checked against.
 """
 import contextlib
 import copy
+import functools
+import math
 
 import numpy as np
 import torch
@@ -24,10 +26,11 @@ def _dims(x):
 
 
 def _elements(x, name):
-    """Shape check of a feature map given as array or tensor, before anything touches the device."""
-    if len(_dims(x)) < 3:
+    """Cells of a feature map given as array or tensor; a shape check before anything touches the device."""
+    shape = x.shape
+    if len(shape) < 3:
         raise ValueError(f"{name} must be (B,C,H,W) or (B,C,n), got {_dims(x)}")
-    return int(np.prod(_dims(x)[2:], dtype=np.int64))
+    return math.prod(shape[2:])
 
 
 def _dtype(x, name):
@@ -39,19 +42,44 @@ def _dtype(x, name):
 
 
 def _place(x):
-    """Makes the device that a call runs on the current one: where its first tensor lives, else the current one."""
-    dv.device()
-    if dv.is_tensor(x) and x.is_cuda and x.device.index != torch.cuda.current_device():
-        return torch.cuda.device(x.device)
-    return contextlib.nullcontext()
+    """(device of the call, context that makes it the current one): where its first tensor lives, else the current one."""
+    if dv.is_tensor(x) and x.is_cuda:
+        if x.device.index == torch.cuda.current_device():
+            return x.device, contextlib.nullcontext()
+        return x.device, torch.cuda.device(x.device)
+    return dv.device(), contextlib.nullcontext()
+
+
+def _on(x, dtype, device):
+    """`x` on `device` as a contiguous tensor of `dtype`; itself where it already is one (the usual case, kept short: a call
+    for a few queries is bounded by the host)."""
+    if x is None:
+        return None
+    if dv.is_tensor(x) and x.dtype == dtype and x.device == device and x.is_contiguous():
+        return x
+    return dv.to_dev(x, dtype)
+
+
+@functools.lru_cache(maxsize=4096)
+def _forward_bytes(*sizes):
+    return _abi.lib.ispa_soft_match_workspace_bytes(*sizes)
+
+
+@functools.lru_cache(maxsize=4096)
+def _backward_bytes(*sizes):
+    return _abi.lib.ispa_soft_match_backward_workspace_bytes(*sizes)
+
+
+def _bytes(n, device):
+    return torch.empty(n, dtype=torch.uint8, device=device) if n else None
 
 
 def _scores(heads, scale, cap, falloff, query_xy, grid, query_shape, batch, n):
     """Checks of what turns products into scores; `grid` is the reference map's (H,W) or None."""
     scale, cap = float(scale), float(cap or 0.0)
-    if not np.isfinite(scale):
+    if not math.isfinite(scale):
         raise ValueError(f"scale must be finite, got {scale}")
-    if not (np.isfinite(cap) and cap >= 0):
+    if not (math.isfinite(cap) and cap >= 0):
         raise ValueError(f"cap must be finite and not negative (0 or None: no cap), got {cap}")
     if falloff is not None:
         if grid is None:
@@ -65,36 +93,36 @@ def _scores(heads, scale, cap, falloff, query_xy, grid, query_shape, batch, n):
     return scale, cap
 
 
-def _score_tensors(heads, falloff, query_xy):
+def _score_tensors(heads, falloff, query_xy, device):
     if falloff is None:
         return None, None
     if np.isscalar(falloff):
-        f = torch.full((heads,), float(falloff), dtype=torch.float32, device=dv.device())
+        f = torch.full((heads,), float(falloff), dtype=torch.float32, device=device)
     else:
-        f = dv.to_dev(falloff, torch.float32)
-    return f, (dv.to_dev(query_xy, torch.float32) if query_xy is not None else None)
+        f = _on(falloff, torch.float32, device)
+    return f, _on(query_xy, torch.float32, device)
 
 
 def _counts(num_query, batch):
     if num_query is None:
         return None
     t = num_query if dv.is_tensor(num_query) else np.asarray(num_query)
-    if int(np.prod(_dims(t), dtype=np.int64)) != batch:
+    if math.prod(t.shape) != batch:
         raise ValueError("num_query must hold one count per batch item")
     return t.reshape(-1)
 
 
-def _count_tensor(num_query):
+def _count_tensor(num_query, device):
     """Counts as int32; what int32 cannot hold is more than any query map has, or less than none."""
     if num_query is None:
         return None
     low, high = -1, 2 ** 31 - 1
     num_query = num_query.clamp(low, high) if dv.is_tensor(num_query) and num_query.dtype == torch.int64 else \
         num_query if dv.is_tensor(num_query) else np.clip(num_query, low, high)
-    return dv.to_dev(num_query, torch.int32)
+    return _on(num_query, torch.int32, device)
 
 
-def _mask(mask):
+def _mask(mask, device):
     """Bytes, not 0 where the cell takes part.  A bool tensor is the byte array the kernels read."""
     if mask is None:
         return None
@@ -104,7 +132,7 @@ def _mask(mask):
         mask = mask != 0
     if mask.dtype == torch.bool:
         mask = mask.contiguous().view(torch.uint8)
-    return dv.to_dev(mask, torch.uint8)
+    return _on(mask, torch.uint8, device)
 
 
 class _Call:
@@ -129,7 +157,7 @@ class _Call:
             raise ValueError(f"at most {MAX_CHANNELS} channels per head")
         if cells < 1:
             raise ValueError("ref has no cells")
-        if mask is not None and (_dims(mask)[0] != b or int(np.prod(_dims(mask), dtype=np.int64)) != b * cells):
+        if mask is not None and (_dims(mask)[0] != b or math.prod(mask.shape) != b * cells):
             raise ValueError(f"mask must be ({b},H,W) or ({b},1,H,W) over ref's cells, got {_dims(mask)}")
         grid = _dims(ref)[2:] if len(_dims(ref)) == 4 else None
         if scale is None:
@@ -142,15 +170,15 @@ class _Call:
         self.width = grid[1] if grid else cells
         self.out_shape = (b, cv) + _dims(query)[2:]
 
-    def upload(self):
+    def upload(self, device):
         query, ref, value, falloff, query_xy, mask, num_query = self.raw
         self.raw = None
-        f, xy = _score_tensors(self.heads, falloff, query_xy)
-        return self.bind(query, ref, value, f, xy, _mask(mask), _count_tensor(num_query))
+        f, xy = _score_tensors(self.heads, falloff, query_xy, device)
+        return self.bind(device, query, ref, value, f, xy, _mask(mask, device), _count_tensor(num_query, device))
 
-    def bind(self, query, ref, value, falloff, xy, mask, count):
-        self.q, self.r = dv.to_dev(query, self.dtype), dv.to_dev(ref, self.dtype)
-        self.v = dv.to_dev(value, self.dtype) if value is not None else None
+    def bind(self, device, query, ref, value, falloff, xy, mask, count):
+        self.device = device
+        self.q, self.r, self.v = (_on(x, self.dtype, device) for x in (query, ref, value))
         self.falloff, self.xy, self.mask, self.count = falloff, xy, mask, count
         return self
 
@@ -164,16 +192,16 @@ class _Call:
         return (self.code, self.b, self.heads, self.d, self.dv, self.n, self.cells, self.width, self.scale, self.cap,
                 dv.ptr(self.falloff), dv.ptr(self.xy), dv.ptr(self.mask), dv.ptr(self.count))
 
-    def forward(self, exact):
+    def forward(self, exact, want_lse):
         """out, its float32 twin (`exact`; the same tensor for float32 maps) and lse.  The workspace is the call's own: calls
         on two streams, or captured in two graphs, share nothing."""
-        out = dv.empty(self.out_shape, self.dtype)
-        out32 = None
-        if exact:
-            out32 = out if self.dtype == torch.float32 else dv.empty(self.out_shape, torch.float32)
-        lse = dv.empty((self.b, self.heads, self.n), torch.float32)
-        need = _abi.lib.ispa_soft_match_workspace_bytes(self.code, self.b, self.heads, self.d, self.dv, self.n, 1, self.cells)
-        ws = dv.empty((need,), torch.uint8) if need else None
+        out = torch.empty(self.out_shape, dtype=self.dtype, device=self.device)
+        out32 = out if exact else None
+        if exact and self.dtype != torch.float32:
+            out32 = torch.empty(self.out_shape, dtype=torch.float32, device=self.device)
+        lse = torch.empty((self.b, self.heads, self.n), dtype=torch.float32, device=self.device) if want_lse else None
+        need = _forward_bytes(self.code, self.b, self.heads, self.d, self.dv, self.n, 1, self.cells)
+        ws = _bytes(need, self.device)
         _abi.check(_abi.lib.ispa_soft_match(dv.ptr(self.q), dv.ptr(self.r), dv.ptr(self.v), *self._common(), dv.ptr(out),
                                             None if out32 is out else dv.ptr(out32), dv.ptr(lse), dv.ptr(ws), need,
                                             dv.stream_ptr()))
@@ -182,9 +210,11 @@ class _Call:
     def backward(self, out32, lse, d_out, d_lse):
         dq, dr = torch.empty_like(self.q), torch.empty_like(self.r)
         dval = torch.empty_like(self.v) if self.v is not None else None
-        need = _abi.lib.ispa_soft_match_backward_workspace_bytes(self.code, self.b, self.heads, self.d, self.dv, self.n,
-                                                                 self.cells)
-        ws = dv.empty((need,), torch.uint8) if need else None
+        if d_out is None:
+            d_out = torch.zeros(self.out_shape, dtype=self.dtype, device=self.device)
+        d_out, d_lse = _on(d_out, self.dtype, self.device), _on(d_lse, torch.float32, self.device)
+        need = _backward_bytes(self.code, self.b, self.heads, self.d, self.dv, self.n, self.cells)
+        ws = _bytes(need, self.device)
         _abi.check(_abi.lib.ispa_soft_match_backward(dv.ptr(self.q), dv.ptr(self.r), dv.ptr(self.v), *self._common(),
                                                      dv.ptr(out32), dv.ptr(lse), dv.ptr(d_out), dv.ptr(d_lse), dv.ptr(dq),
                                                      dv.ptr(dr), dv.ptr(dval), dv.ptr(ws), need, dv.stream_ptr()))
@@ -194,8 +224,9 @@ class _Call:
 class _SoftMatch(torch.autograd.Function):
     @staticmethod
     def forward(ctx, query, ref, value, call):
-        with _place(query):
-            out, out32, lse = call.upload().forward(exact=True)
+        device, place = _place(query)
+        with place:
+            out, out32, lse = call.upload(device).forward(exact=True, want_lse=True)
         ctx.save_for_backward(query, ref, value, out32, lse, *call.release())
         ctx.call = call
         ctx.set_materialize_grads(False)
@@ -207,19 +238,11 @@ class _SoftMatch(torch.autograd.Function):
         if d_out is None and d_lse is None:
             return None, None, None, None
         query, ref, value, out32, lse, *options = ctx.saved_tensors
-        with _place(query):
-            call = copy.copy(ctx.call).bind(query, ref, value, *options)
-            grads = _gradients(call, out32, lse, d_out, d_lse)
+        device, place = _place(query)
+        with place:
+            grads = copy.copy(ctx.call).bind(device, query, ref, value, *options).backward(out32, lse, d_out, d_lse)
         return (*(g.reshape(x.shape).to(x.device) if g is not None and need else None
                   for g, x, need in zip(grads, (query, ref, value), ctx.needs_input_grad)), None)
-
-
-def _gradients(call, out32, lse, d_out, d_lse):
-    if d_out is None:
-        d_out = torch.zeros(call.out_shape, dtype=call.dtype, device=dv.device())
-    d_out = dv.to_dev(d_out, call.dtype)
-    d_lse = dv.to_dev(d_lse, torch.float32) if d_lse is not None else None
-    return call.backward(out32, lse, d_out, d_lse)
 
 
 def soft_match(query, ref, value=None, *, heads=1, scale=None, cap=0.0, falloff=None, query_xy=None, mask=None,
@@ -252,8 +275,9 @@ def soft_match(query, ref, value=None, *, heads=1, scale=None, cap=0.0, falloff=
             raise ValueError("query, ref and value must be tensors where one of them requires gradients")
         out, lse = _SoftMatch.apply(query, ref, value, call)
         return (out, lse) if return_lse else out
-    with _place(query):
-        out, _, lse = call.upload().forward(exact=False)
+    device, place = _place(query)
+    with place:
+        out, _, lse = call.upload(device).forward(exact=False, want_lse=return_lse)
         out = dv.back(out, as_tensor)
         return (out, dv.back(lse, as_tensor)) if return_lse else out
 
@@ -274,10 +298,10 @@ class TemplateStore:
     def __init__(self, n_view, channels, size, kind="int8"):
         self._set(kind, n_view, channels, size)
         cells = self.size[0] * self.size[1]
-        dev = dv.device()
-        self.codes = torch.zeros((self.n_view, self.channels, cells), dtype=torch.uint8, device=dev).view(_KINDS[kind][1])
-        self.scales = torch.zeros((self.n_view, cells), dtype=torch.float32, device=dev)
-        self.mask = torch.zeros((self.n_view, cells), dtype=torch.uint8, device=dev)
+        device = dv.device()
+        self.codes = torch.zeros((self.n_view, self.channels, cells), dtype=torch.uint8, device=device).view(_KINDS[kind][1])
+        self.scales = torch.zeros((self.n_view, cells), dtype=torch.float32, device=device)
+        self.mask = torch.zeros((self.n_view, cells), dtype=torch.uint8, device=device)
 
     def _set(self, kind, n_view, channels, size):
         if kind not in _KINDS:
@@ -324,12 +348,11 @@ class TemplateStore:
             raise ValueError(f"views must have {dims} dimension{'s' if dims > 1 else ''}, got {_dims(views)}")
         return views
 
-    @staticmethod
-    def _index(views):
+    def _index(self, views):
         # an int64 index that int32 would wrap into the store must stay outside it
         if dv.is_tensor(views) and views.dtype == torch.int64:
             views = views.clamp(-1, 2 ** 31 - 1)
-        return dv.to_dev(views, torch.int32)
+        return _on(views, torch.int32, self.codes.device)
 
     def write(self, views, features, mask=None):
         """Quantises features (n,C,H,W) (float32, or bfloat16 tensors) into views (n,).  mask (n,H,W): the cells that hold
@@ -340,36 +363,38 @@ class TemplateStore:
         dtype = _dtype(features, "features")
         if _dims(features) != (n, self.channels) + self.size:
             raise ValueError(f"features must be {(n, self.channels) + self.size}, got {_dims(features)}")
-        if mask is not None and int(np.prod(_dims(mask), dtype=np.int64)) != n * self.size[0] * self.size[1]:
+        if mask is not None and math.prod(mask.shape) != n * self.size[0] * self.size[1]:
             raise ValueError(f"mask must be {(n,) + self.size}, got {_dims(mask)}")
-        with _place(self.codes):
-            v, f = self._index(views), dv.to_dev(features, dtype)
-            m = _mask(mask)
+        device, place = _place(self.codes)
+        with place:
+            v, f, m = self._index(views), _on(features, dtype, device), _mask(mask, device)
             _abi.check(_abi.lib.ispa_store_write(dv.ptr(f), _CODES[dtype], dv.ptr(m), dv.ptr(v), n, _KINDS[self.kind][0],
                                                  self.n_view, self.channels, self.codes.shape[2], dv.ptr(self.codes),
                                                  dv.ptr(self.scales), dv.ptr(self.mask), dv.stream_ptr()))
+
+    def _read(self, views, dtype, features):
+        views = self._views(views, 1)
+        device, place = _place(self.codes)
+        with place:
+            v = self._index(views)
+            n = v.shape[0]
+            out = torch.empty((n, self.channels) + self.size, dtype=dtype, device=device) if features else None
+            mask = None if features else torch.empty((n,) + self.size, dtype=torch.uint8, device=device)
+            _abi.check(_abi.lib.ispa_store_read(dv.ptr(self.codes), dv.ptr(self.scales), dv.ptr(self.mask), dv.ptr(v), n,
+                                                _KINDS[self.kind][0], self.n_view, self.channels, self.codes.shape[2],
+                                                _CODES[dtype], dv.ptr(out), dv.ptr(mask), dv.stream_ptr()))
+            return out if features else mask
 
     def read(self, views, dtype=torch.float32):
         """The features of views (n,), (n,C,H,W) of `dtype` (float32 or bfloat16), for dense_nn and the correlation layers.
         Zeros for -1 and views not written."""
         if dtype not in _CODES:
             raise ValueError("dtype must be torch.float32 or torch.bfloat16")
-        views = self._views(views, 1)
-        with _place(self.codes):
-            v = self._index(views)
-            out = dv.empty((v.numel(), self.channels) + self.size, dtype)
-            _abi.check(_abi.lib.ispa_store_read(dv.ptr(self.codes), dv.ptr(self.scales), dv.ptr(v), v.numel(),
-                                                _KINDS[self.kind][0], self.n_view, self.channels, self.codes.shape[2],
-                                                _CODES[dtype], dv.ptr(out), dv.stream_ptr()))
-            return out
+        return self._read(views, dtype, True)
 
     def read_mask(self, views):
         """The masks of views (n,) as (n,H,W) uint8; zeros for -1 and views not written."""
-        views = self._views(views, 1)
-        with _place(self.codes):
-            v = self._index(views).long()
-            inside = (v >= 0) & (v < self.n_view)
-            return (self.mask[torch.where(inside, v, 0)] * inside[:, None]).view((v.numel(),) + self.size)
+        return self._read(views, torch.float32, False)
 
     def soft_match(self, query, views, *, heads=1, scale=None, cap=0.0, falloff=None, query_xy=None, num_query=None,
                    return_lse=False):
@@ -392,18 +417,19 @@ class TemplateStore:
         scale, cap = _scores(heads, scale, cap, falloff, query_xy, self.size, _dims(query)[2:], b, n)
         count = _counts(num_query, b)
         as_tensor = dv.is_tensor(query)
-        with _place(self.codes):
-            q, v = dv.to_dev(query.detach() if as_tensor else query, dtype), self._index(views)
-            f, xy = _score_tensors(heads, falloff, query_xy)
-            count = _count_tensor(count)
-            out = dv.empty((b, c) + _dims(query)[2:], dtype)
-            lse = dv.empty((b, heads, n), torch.float32)
-            cells = self.codes.shape[2]
-            need = _abi.lib.ispa_soft_match_workspace_bytes(_CODES[dtype], b, heads, c // heads, c // heads, n, v.shape[1], cells)
-            ws = dv.empty((need,), torch.uint8) if need else None
+        device, place = _place(self.codes)
+        with place:
+            q, v = _on(query.detach() if as_tensor else query, dtype, device), self._index(views)
+            f, xy = _score_tensors(heads, falloff, query_xy, device)
+            count = _count_tensor(count, device)
+            out = torch.empty((b, c) + _dims(query)[2:], dtype=dtype, device=device)
+            lse = torch.empty((b, heads, n), dtype=torch.float32, device=device) if return_lse else None
+            d, cells, code = c // heads, self.codes.shape[2], _CODES[dtype]
+            need = _forward_bytes(code, b, heads, d, d, n, v.shape[1], cells)
+            ws = _bytes(need, device)
             _abi.check(_abi.lib.ispa_store_match(
-                dv.ptr(q), _CODES[dtype], dv.ptr(self.codes), dv.ptr(self.scales), dv.ptr(self.mask), _KINDS[self.kind][0],
-                dv.ptr(v), v.shape[1], self.n_view, b, heads, c // heads, n, cells, self.size[1], scale, cap, dv.ptr(f),
-                dv.ptr(xy), dv.ptr(count), dv.ptr(out), dv.ptr(lse), dv.ptr(ws), need, dv.stream_ptr()))
+                dv.ptr(q), code, dv.ptr(self.codes), dv.ptr(self.scales), dv.ptr(self.mask), _KINDS[self.kind][0], dv.ptr(v),
+                v.shape[1], self.n_view, b, heads, d, n, cells, self.size[1], scale, cap, dv.ptr(f), dv.ptr(xy), dv.ptr(count),
+                dv.ptr(out), dv.ptr(lse), dv.ptr(ws), need, dv.stream_ptr()))
             out = dv.back(out, as_tensor)
             return (out, dv.back(lse, as_tensor)) if return_lse else out

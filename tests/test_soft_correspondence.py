@@ -708,6 +708,6 @@ def test_abi_refusals():
     assert back() == -3 and b"workspace" in lib.ispa_last_error()
     assert lib.ispa_store_write(1, 0, None, 1, 2, 2, 4, 8, 16, 1, 1, 1, None) == -1 and b"kind" in lib.ispa_last_error()
     assert lib.ispa_store_write(1, 0, None, 1, -1, 0, 4, 8, 16, 1, 1, 1, None) == -1
-    assert lib.ispa_store_read(None, 1, 1, 2, 0, 4, 8, 16, 0, 1, None) == -1 and b"null" in lib.ispa_last_error()
+    assert lib.ispa_store_read(None, 1, 1, 1, 2, 0, 4, 8, 16, 0, 1, None, None) == -1 and b"null" in lib.ispa_last_error()
     assert lib.ispa_store_match(1, 0, 1, 1, 1, 0, None, 2, 4, 1, 1, 64, 3, 100, 10, 1.0, 0.0, None, None, None, 1, None, None, 0,
                                 None) == -1
