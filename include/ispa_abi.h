@@ -387,7 +387,8 @@ int ispa_prune_points_2d(double *coords, int B, int64_t n, const uint8_t *flags,
  * wants; lse (optional) (B,heads,nq) f32.  A query that is not real or has no cell gets out 0 and lse -inf.
  * Sums, maxima and log-sums are float32; with ISPA_BF16 the softmax weights are rounded to bfloat16 for the
  * product with v.  Few queries: the cells are split over workgroups and the parts joined by a second launch, in a fixed
- * order (results do not change from run to run).  workspace: ispa_soft_match_workspace_bytes(...) with views = 1. */
+ * order (results do not change from run to run).  q, r, v (and d_out below) start on 16-byte borders.  workspace (256-byte
+ * aligned): ispa_soft_match_workspace_bytes(...) with views = 1. */
 #define ISPA_SOFT_MAX_CHANNELS 256
 size_t ispa_soft_match_workspace_bytes(int dtype, int B, int heads, int D, int Dv, int64_t nq, int views, int64_t cells);
 int ispa_soft_match(const void *q, const void *r, const void *v, int dtype, int B, int heads, int D, int Dv, int64_t nq,

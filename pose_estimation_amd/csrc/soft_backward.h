@@ -39,28 +39,28 @@ __global__ __launch_bounds__(256) void soft_delta_kernel(const Params p, const f
 //
 // Gradient of the queries: owned = queries, streamed = cells.
 template <typename T, int DP, int WQ, int NC>
-__global__ __launch_bounds__(64 * WQ) void soft_dq_kernel(const Params p) {
+__global__ __launch_bounds__(64 * WQ, (DP <= 128 && WQ > 1 && std::is_same_v<T, BF16>) ? 2 : 1) void soft_dq_kernel(const Params p) {
     typedef Math<T, DP> M;
-    constexpr int NT = 64 * WQ;
     constexpr int kBlocks = M::kRows / 32;
     constexpr int kUnroll = DP == 256 ? 1 : kBlocks;           // registers
+    constexpr uint64_t kAll = M::kRows == 64 ? ~0ull : 0xffffffffull;
     extern __shared__ __attribute__((aligned(16))) char lds[];
-    char *ktile = lds;
-    char *vtile = p.shared ? lds : lds + DP * kRowBytes;
-    float *xarr = reinterpret_cast<float *>(vtile + DP * kRowBytes), *yarr = xarr + 64;
+    const int v_at = p.shared ? 0 : DP * kRowBytes, cell_at = v_at + DP * kRowBytes;
+    const int stage = cell_at + 3 * 64 * (int)sizeof(float);
 
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, h = lane >> 5;
-    int id = blockIdx.x;
+    int id = die_major(blockIdx.x, gridDim.x);
     const int qblk = id % p.blocks;
     id /= p.blocks;
     const int split = id % p.splits;
     const int bh = id / p.splits;
     const int b = bh / p.heads, head = bh - b * p.heads;
-    const int t0 = (int)((int64_t)p.tiles * split / p.splits), t1 = (int)((int64_t)p.tiles * (split + 1) / p.splits);
     const int64_t live_q = live_queries(p, b);
     const int64_t q = ((int64_t)qblk * WQ + wave) * 32 + (lane & 31);
     const bool q_ok = q < live_q;
     const bool idle = (int64_t)qblk * WQ * 32 >= live_q;
+    const int t0 = (int)((int64_t)p.tiles * split / p.splits);
+    const int t1 = idle ? t0 : (int)((int64_t)p.tiles * (split + 1) / p.splits);
 
     typename M::Owned qf, of;
     M::load_owned(qf, (const typename T::elem *)p.q + (int64_t)bh * p.D * p.nq + (q < p.nq ? q : 0), p.nq, p.D, q_ok, h);
@@ -81,59 +81,58 @@ __global__ __launch_bounds__(64 * WQ) void soft_dq_kernel(const Params p) {
 #pragma unroll
         for (int i = 0; i < 16; ++i) g[c][i] = 0.f;
 
-    const KeyTiles<M, T> keys(p, b, head);
-    for (int t = t0; t < (idle ? t0 : t1); ++t) {
-        const typename KeyTiles<M, T>::At at = keys.at(t);
-        uint64_t live = __ballot(keys.live(at, lane));
-        if constexpr (M::kRows == 32) live &= 0xffffffffull;
-        if (live == 0) continue;                               // the same in every wave
-        __syncthreads();
-        Loader<M, T, DP, NT> kl, vl;
-        kl.load(keys.base(p.k, at, p.D), p.cells, p.D, at.cell0, p.cells);
-        kl.store(ktile, p.cells, p.D, live, 0.f);
-        if (!p.shared) {
-            vl.load(keys.base(p.v, at, p.Dv), p.cells, p.Dv, at.cell0, p.cells);
-            vl.store(vtile, p.cells, p.Dv, live, 0.f);
-        }
-        if (p.falloff != nullptr && threadIdx.x < M::kRows) {
-            const int c = (int)at.cell0 + threadIdx.x;
-            xarr[threadIdx.x] = (float)(c % p.W);
-            yarr[threadIdx.x] = (float)(c / p.W);
-        }
-        __syncthreads();
+    Feed<M, T, DP, WQ> feed(p, b, head, lds, stage);
+    uint64_t live = 0;
+    if (t0 < t1) {
+        feed.fetch(t0, lds);
+        live = feed.put(lds);
+    }
+    __syncthreads();
+    for (int t = t0; t < t1; ++t) {
+        const char *buf = lds + ((t - t0) & 1) * stage;
+        if (t + 1 < t1) feed.fetch(t + 1, lds + ((t + 1 - t0) & 1) * stage);
+        if (live != 0) {
+            const char *ktile = buf, *vtile = buf + v_at;
+            const float *cell = reinterpret_cast<const float *>(buf + cell_at);
 #pragma unroll kUnroll
-        for (int k = 0; k < kBlocks; ++k) {
-            const f32x16 acc = M::first(ktile, addr, k, qf);
-            const f32x16 dp = M::first(vtile, addr, k, of);
-            const unsigned bits = (unsigned)(live >> (32 * k));
-            float w[16];
-            if (p.falloff != nullptr) {
-                M::per_cell(xarr, k, h, w);
+            for (int k = 0; k < kBlocks; ++k) {
+                const f32x16 acc = M::first(ktile, addr, k, qf);
+                const f32x16 dp = M::first(vtile, addr, k, of);
+                float w[16];
+                if (p.falloff != nullptr) {
+                    M::per_cell(cell + 64, k, h, w);
 #pragma unroll
-                for (int i = 0; i < 16; ++i) w[i] = (w[i] - qx) * (w[i] - qx);
-                float cy[16];
-                M::per_cell(yarr, k, h, cy);
+                    for (int i = 0; i < 16; ++i) w[i] = (w[i] - qx) * (w[i] - qx);
+                    float cy[16];
+                    M::per_cell(cell + 128, k, h, cy);
 #pragma unroll
-                for (int i = 0; i < 16; ++i) w[i] = fmaf(-score.fall, fmaf(cy[i] - qy, cy[i] - qy, w[i]), -lse2);
-            } else {
-#pragma unroll
-                for (int i = 0; i < 16; ++i) w[i] = -lse2;
-            }
-#pragma unroll
-            for (int i = 0; i < 16; ++i) {
-                float ds = dp[i] - delta;
-                if (score.cap) {
-                    const float th = score.bend(acc[i]);
-                    w[i] = fmaf(score.top, th, w[i]);
-                    ds *= fmaf(-th, th, 1.f);
+                    for (int i = 0; i < 16; ++i) w[i] = fmaf(-score.fall, fmaf(cy[i] - qy, cy[i] - qy, w[i]), -lse2);
                 } else {
-                    w[i] = fmaf(score.in, acc[i], w[i]);
+#pragma unroll
+                    for (int i = 0; i < 16; ++i) w[i] = -lse2;
                 }
-                ds *= exp2_(w[i]);
-                w[i] = (bits >> M::cell(i, h)) & 1u ? ds : 0.f;
+#pragma unroll
+                for (int i = 0; i < 16; ++i) {
+                    float ds = dp[i] - delta;
+                    if (score.cap) {
+                        const float th = score.bend(acc[i]);
+                        w[i] = fmaf(score.top, th, w[i]);
+                        ds *= fmaf(-th, th, 1.f);
+                    } else {
+                        w[i] = fmaf(score.in, acc[i], w[i]);
+                    }
+                    w[i] = ds * exp2_(w[i]);
+                }
+                if (live != kAll) {
+                    const unsigned bits = (unsigned)(live >> (32 * k)) >> M::cell(0, h);
+#pragma unroll
+                    for (int i = 0; i < 16; ++i) w[i] = bits & (1u << M::cell(i, 0)) ? w[i] : 0.f;
+                }
+                M::second(ktile + p.c0 * kRowBytes, addr, k, M::weights(w), g);
             }
-            M::second(ktile + p.c0 * kRowBytes, addr, k, M::weights(w), g);
         }
+        if (t + 1 < t1) live = feed.put(lds + ((t + 1 - t0) & 1) * stage);
+        __syncthreads();
     }
     if (q >= p.nq) return;
     if (p.parts) {
@@ -157,22 +156,23 @@ __global__ __launch_bounds__(64 * WQ) void soft_dq_kernel(const Params p) {
         }
 }
 
+// LDS of one buffer: both tiles, and per query the log-sum, delta and the place.
+template <int DP>
+constexpr int dkv_stage_bytes = 2 * DP * kRowBytes + 4 * 64 * (int)sizeof(float);
+
 // Gradients of the reference and value maps: owned = cells, streamed = queries.  PART 0: both; 1: the value's, 2: the
 // reference's alone (maps of more than 128 channels, for the registers).
 template <typename T, int DP, int WQ, int PART, int NC>
 __global__ __launch_bounds__(64 * WQ) void soft_dkv_kernel(const Params p) {
     typedef Math<T, DP> M;
-    constexpr int NT = 64 * WQ;
     constexpr int kBlocks = M::kRows / 32;
     constexpr int kUnroll = DP == 256 ? 1 : kBlocks;           // registers
     constexpr bool kDv = PART != 2, kDk = PART != 1;
+    constexpr int kStage = dkv_stage_bytes<DP>;
     extern __shared__ __attribute__((aligned(16))) char lds[];
-    char *qtile = lds, *otile = lds + DP * kRowBytes;
-    float *larr = reinterpret_cast<float *>(otile + DP * kRowBytes);
-    float *darr = larr + 64, *xarr = larr + 128, *yarr = larr + 192;
 
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, h = lane >> 5;
-    int id = blockIdx.x;
+    int id = die_major(blockIdx.x, gridDim.x);
     const int blk = id % p.blocks;
     id /= p.blocks;
     const int split = id % p.splits;
@@ -202,31 +202,59 @@ __global__ __launch_bounds__(64 * WQ) void soft_dkv_kernel(const Params p) {
             if constexpr (kDv) gv[c][i] = 0.f;
         }
 
-    const typename T::elem *qmap = (const typename T::elem *)p.q + (int64_t)bh * p.D * p.nq;
-    const typename T::elem *omap = (const typename T::elem *)p.d_out + (int64_t)bh * p.Dv * p.nq;
-    for (int t = t0; t < t1; ++t) {
+    typedef Direct<M, DP, WQ> Copy;
+    Copy cq, co;
+    cq.init(p.sq.ld, p.sq.d);
+    co.init(p.so.ld, p.so.d);
+    const char *qmap = (const char *)p.sq.map + (int64_t)bh * p.sq.d * p.sq.ld * Copy::kSize;
+    const char *omap = (const char *)p.so.map + (int64_t)bh * p.so.d * p.so.ld * Copy::kSize;
+    for (int i = 0; i < 2; ++i) {
+        cq.clear_rest(lds + i * kStage);
+        co.clear_rest(lds + i * kStage + DP * kRowBytes);
+    }
+    float lse2 = 0.f, delta = 0.f, px = 0.f, py = 0.f;
+    auto fetch = [&](int t, char *buf) {
         const int64_t q0 = (int64_t)t * M::kRows;
-        __syncthreads();
-        Loader<M, T, DP, NT> ql, ol;
-        ql.load(qmap, p.nq, p.D, q0, live_q);
-        ql.store(qtile, p.nq, p.D, ~0ull, 0.f);
-        ol.load(omap, p.nq, p.Dv, q0, live_q);
-        ol.store(otile, p.nq, p.Dv, ~0ull, 0.f);
         if (threadIdx.x < M::kRows) {
             const int64_t q = q0 + threadIdx.x;
-            float lse2 = __builtin_inff(), delta = 0.f, x = 0.f, y = 0.f;      // no weight without cells
+            lse2 = __builtin_inff();                           // no weight without cells
+            delta = 0.f;
             if (q < live_q) {
-                const float l = p.lse[(int64_t)bh * p.nq + q];
-                lse2 = l == -__builtin_inff() ? __builtin_inff() : l * kLog2e;
+                const float x = p.lse[(int64_t)bh * p.nq + q];
+                lse2 = x == -__builtin_inff() ? __builtin_inff() : x * kLog2e;
                 delta = p.delta[(int64_t)bh * p.nq + q];
-                if (p.falloff != nullptr) query_place(p, b, q, x, y);
+                if (p.falloff != nullptr) query_place(p, b, q, px, py);
             }
-            larr[threadIdx.x] = lse2;
-            darr[threadIdx.x] = delta;
-            xarr[threadIdx.x] = x;
-            yarr[threadIdx.x] = y;
         }
-        __syncthreads();
+        cq.issue(qmap, q0, p.sq.ld, buf);
+        co.issue(omap, q0, p.so.ld, buf + DP * kRowBytes);
+    };
+    auto put = [&](int t, char *buf) {
+        Copy::wait();
+        const int64_t left = live_q - (int64_t)t * M::kRows;
+        if (left < M::kRows) {                                 // what lies behind the live queries counts as zeros
+            const uint64_t live = (1ull << left) - 1;
+            cq.mask(buf, live);
+            co.mask(buf + DP * kRowBytes, live);
+        }
+        if (threadIdx.x < M::kRows) {
+            float *cell = reinterpret_cast<float *>(buf + 2 * DP * kRowBytes) + threadIdx.x;
+            cell[0] = lse2;
+            cell[64] = delta;
+            cell[128] = px;
+            cell[192] = py;
+        }
+    };
+    if (t0 < t1) {
+        fetch(t0, lds);
+        put(t0, lds);
+    }
+    __syncthreads();
+    for (int t = t0; t < t1; ++t) {
+        const char *qtile = lds + ((t - t0) & 1) * kStage, *otile = qtile + DP * kRowBytes;
+        const float *larr = reinterpret_cast<const float *>(otile + DP * kRowBytes);
+        const float *darr = larr + 64, *xarr = larr + 128, *yarr = larr + 192;
+        if (t + 1 < t1) fetch(t + 1, lds + ((t + 1 - t0) & 1) * kStage);
 #pragma unroll kUnroll
         for (int k = 0; k < kBlocks; ++k) {
             const f32x16 acc = M::first(qtile, addr, k, kf);
@@ -268,6 +296,8 @@ __global__ __launch_bounds__(64 * WQ) void soft_dkv_kernel(const Params p) {
                 M::second(qtile + p.c0 * kRowBytes, addr, k, M::weights(w), gk);
             }
         }
+        if (t + 1 < t1) put(t + 1, lds + ((t + 1 - t0) & 1) * kStage);
+        __syncthreads();
     }
     if (cell >= p.cells) return;
     // masked cells take no part: their columns hold zeros' products and are dropped here

@@ -12,7 +12,7 @@ constexpr int kFormed = DP == 256 && std::is_same_v<T, F32> ? 128 : DP;
 template <typename T, int DP, int WQ>
 int dq_one(Params p, hipStream_t stream) {
     static unsigned long long lds_allowed = 0;
-    const int lds = (p.shared ? 1 : 2) * DP * kRowBytes + 2 * 64 * (int)sizeof(float);
+    const int lds = 2 * stage_bytes<DP>(p.shared);
     const unsigned grid = (unsigned)((int64_t)p.B * p.heads * p.splits * p.blocks);
     constexpr int NC = kFormed<T, DP>;
     for (p.c0 = 0; p.c0 < p.D; p.c0 += NC)
@@ -24,7 +24,7 @@ int dq_one(Params p, hipStream_t stream) {
 template <typename T, int DP, int WQ, int PART>
 int dkv_one(Params p, int channels, hipStream_t stream) {
     static unsigned long long lds_allowed = 0;
-    const int lds = 2 * DP * kRowBytes + 4 * 64 * (int)sizeof(float);
+    const int lds = 2 * dkv_stage_bytes<DP>;
     const unsigned grid = (unsigned)((int64_t)p.B * p.heads * p.splits * p.blocks);
     constexpr int NC = PART == 2 ? kFormed<T, DP> : DP;
     for (p.c0 = 0; p.c0 < channels; p.c0 += NC)

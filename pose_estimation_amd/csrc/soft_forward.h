@@ -60,9 +60,81 @@ template <int DP>
 constexpr int stage_bytes(bool shared) {
     return (shared ? 1 : 2) * DP * kRowBytes + 3 * 64 * (int)sizeof(float);
 }
-// Two buffers where the loads run a tile ahead.
+// Two buffers where the loads run a tile ahead: always from maps, from codes where they fit a thread's registers.
 template <typename T, typename SRC, int DP, int WQ>
-constexpr int kBuffers = Loader<Math<T, DP>, SRC, DP, 64 * WQ>::kAhead ? 2 : 1;
+constexpr bool kAhead = std::is_same_v<T, SRC> || Loader<Math<T, DP>, SRC, DP, 64 * WQ>::kAhead;
+template <typename T, typename SRC, int DP, int WQ>
+constexpr int kBuffers = kAhead<T, SRC, DP, WQ> ? 2 : 1;
+
+// The tiles of one item and head: fetch starts a tile's way into a buffer, put ends it and returns its live cells.
+template <typename M, typename SRC, int DP, int WQ>
+struct Feed {
+    typedef typename M::map T;
+    typedef KeyTiles<M, SRC> Keys;
+    static constexpr bool kCodes = Keys::kCodes;
+    static constexpr uint64_t kAll = M::kRows == 64 ? ~0ull : 0xffffffffull;
+    typedef Loader<M, SRC, DP, 64 * WQ> L;
+    typedef Direct<M, DP, WQ> D;
+    struct None {};
+    const Params &p;
+    const Keys keys;
+    std::conditional_t<kCodes, L, None> codes;
+    std::conditional_t<kCodes, None, D> dk, dv;
+    const char *kmap, *vmap;
+    typename Keys::At at{};
+    bool ok = false;
+    float sc = 0.f;
+    int v_at, cell_at;
+    __device__ Feed(const Params &p_, int b, int head, char *lds, int stage) : p(p_), keys(p_, b, head) {
+        v_at = p.shared ? 0 : DP * kRowBytes;
+        cell_at = v_at + DP * kRowBytes;
+        if constexpr (!kCodes) {
+            const int64_t bh = (int64_t)b * p.heads + head;
+            dk.init(p.sk.ld, p.sk.d);
+            kmap = (const char *)p.sk.map + bh * p.sk.d * p.sk.ld * D::kSize;
+            dk.clear_rest(lds);
+            dk.clear_rest(lds + stage);
+            if (!p.shared) {
+                dv.init(p.sv.ld, p.sv.d);
+                vmap = (const char *)p.sv.map + bh * p.sv.d * p.sv.ld * D::kSize;
+                dv.clear_rest(lds + v_at);
+                dv.clear_rest(lds + stage + v_at);
+            }
+        }
+    }
+    __device__ void fetch(int t, char *buf) {
+        const int lane = threadIdx.x & 63;
+        at = keys.at(t);
+        ok = keys.live(at, lane);
+        if constexpr (kCodes) {
+            sc = keys.scale(at, lane, ok);
+            codes.load(keys.base(p.k, at, p.D), p.cells, p.D, at.cell0, at.map < 0 ? 0 : p.cells);
+        } else {
+            dk.issue(kmap, at.cell0, p.sk.ld, buf);
+            if (!p.shared) dv.issue(vmap, at.cell0, p.sv.ld, buf + v_at);
+        }
+    }
+    __device__ uint64_t put(char *buf) {
+        const uint64_t live = __ballot(ok) & kAll;
+        if constexpr (!kCodes) D::wait();
+        if (live == 0) return live;                            // the same in every wave
+        const int lane = threadIdx.x & 63;
+        float *cell = reinterpret_cast<float *>(buf + cell_at);
+        if constexpr (kCodes) {
+            codes.store(buf, p.cells, p.D, live, sc);
+            if (std::is_same_v<T, BF16> && threadIdx.x < 64) cell[lane] = sc;
+        } else if (live != kAll) {
+            dk.mask(buf, live);
+            if (!p.shared) dv.mask(buf + v_at, live);
+        }
+        if (p.falloff != nullptr && threadIdx.x < M::kRows) {
+            const int c = (int)at.cell0 + threadIdx.x;
+            cell[64 + threadIdx.x] = (float)(c % p.W);
+            cell[128 + threadIdx.x] = (float)(c / p.W);
+        }
+        return live;
+    }
+};
 
 // How far (in units of log2) a query's largest score may rise above the maximum that its sums are kept against before they
 // are rescaled: weights stay below 2^8, and nearly all tiles leave the accumulators alone.
@@ -72,12 +144,11 @@ constexpr float kSlack = 8.f;
 template <typename T, typename SRC, int DP, int WQ, int NC>
 __global__ __launch_bounds__(64 * WQ, (DP <= 128 && std::is_same_v<SRC, BF16>) ? 2 : 1) void soft_forward_kernel(const Params p) {
     typedef Math<T, DP> M;
-    constexpr int NT = 64 * WQ;
     constexpr int kBlocks = M::kRows / 32;
     constexpr uint64_t kAll = M::kRows == 64 ? ~0ull : 0xffffffffull;
     constexpr bool kCodes = KeyTiles<M, SRC>::kCodes;
     constexpr bool kScaled = kCodes && std::is_same_v<T, BF16>;        // scales applied to scores and weights
-    typedef Loader<M, SRC, DP, NT> L;
+    constexpr bool kAheadHere = kAhead<T, SRC, DP, WQ>;
     extern __shared__ __attribute__((aligned(16))) char lds[];
     const int v_at = p.shared ? 0 : DP * kRowBytes, cell_at = v_at + DP * kRowBytes;
     const int stage = cell_at + 3 * 64 * (int)sizeof(float);
@@ -110,49 +181,23 @@ __global__ __launch_bounds__(64 * WQ, (DP <= 128 && std::is_same_v<SRC, BF16>) ?
         for (int i = 0; i < 16; ++i) o[c][i] = 0.f;
     float m = -__builtin_inff(), l = 0.f;                      // l: this lane's half of the cells
 
-    const KeyTiles<M, SRC> keys(p, b, head);
-    L kl, vl;
-    typename KeyTiles<M, SRC>::At at{};
-    bool ok = false;
-    float sc = 0.f;
-    auto fetch = [&](int t) {
-        at = keys.at(t);
-        ok = keys.live(at, lane);
-        sc = keys.scale(at, lane, ok);
-        const int64_t n = at.map < 0 ? 0 : p.cells;
-        kl.load(keys.base(p.k, at, p.D), p.cells, p.D, at.cell0, n);
-        if (!p.shared) vl.load(keys.base(p.v, at, p.Dv), p.cells, p.Dv, at.cell0, n);
-    };
-    auto put = [&](char *buf) {                                // the fetched tile into LDS; its live cells
-        const uint64_t live = __ballot(ok) & kAll;
-        if (live == 0) return live;                            // the same in every wave
-        kl.store(buf, p.cells, p.D, live, sc);
-        if (!p.shared) vl.store(buf + v_at, p.cells, p.Dv, live, sc);
-        float *cell = reinterpret_cast<float *>(buf + cell_at);
-        if (kScaled && wave == 0) cell[lane] = sc;
-        if (p.falloff != nullptr && threadIdx.x < M::kRows) {
-            const int c = (int)at.cell0 + threadIdx.x;
-            cell[64 + threadIdx.x] = (float)(c % p.W);
-            cell[128 + threadIdx.x] = (float)(c / p.W);
-        }
-        return live;
-    };
+    Feed<M, SRC, DP, WQ> feed(p, b, head, lds, stage);
     uint64_t live = 0;
-    if constexpr (L::kAhead) {
+    if constexpr (kAheadHere) {
         if (t0 < t1) {
-            fetch(t0);
-            live = put(lds);
+            feed.fetch(t0, lds);
+            live = feed.put(lds);
         }
         __syncthreads();
     }
     for (int t = t0; t < t1; ++t) {
-        const char *buf = lds + (L::kAhead ? ((t - t0) & 1) * stage : 0);
-        if constexpr (L::kAhead) {
-            if (t + 1 < t1) fetch(t + 1);
+        const char *buf = lds + (kAheadHere ? ((t - t0) & 1) * stage : 0);
+        if constexpr (kAheadHere) {
+            if (t + 1 < t1) feed.fetch(t + 1, lds + ((t + 1 - t0) & 1) * stage);
         } else {
             __syncthreads();
-            fetch(t);
-            live = put(lds);
+            feed.fetch(t, lds);
+            live = feed.put(lds);
             __syncthreads();
         }
         if (live != 0) {
@@ -226,8 +271,8 @@ __global__ __launch_bounds__(64 * WQ, (DP <= 128 && std::is_same_v<SRC, BF16>) ?
                 M::second(vtile + p.c0 * kRowBytes, addr, k, M::weights(w), o);
             }
         }
-        if constexpr (L::kAhead) {
-            if (t + 1 < t1) live = put(lds + ((t + 1 - t0) & 1) * stage);
+        if constexpr (kAheadHere) {
+            if (t + 1 < t1) live = feed.put(lds + ((t + 1 - t0) & 1) * stage);
             __syncthreads();
         }
     }

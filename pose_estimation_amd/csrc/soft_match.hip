@@ -11,7 +11,7 @@ int64_t tile_cells(int dtype) { return dtype == ISPA_F32 ? Math<F32, 32>::kRows 
 
 bool sizes_ok(int dtype, int B, int heads, int D, int Dv, int64_t nq, int V, int64_t cells) {
     return (dtype == ISPA_F32 || dtype == ISPA_BF16) && B >= 0 && heads >= 1 && D >= 1 && D <= ISPA_SOFT_MAX_CHANNELS && Dv >= 1 &&
-           Dv <= ISPA_SOFT_MAX_CHANNELS && nq >= 0 && nq < (1ll << 30) && V >= 0 && cells >= 1 && cells < (1ll << 30) &&
+           Dv <= ISPA_SOFT_MAX_CHANNELS && nq >= 0 && nq < (1ll << 22) && V >= 0 && cells >= 1 && cells < (1ll << 22) &&
            (int64_t)B * heads < 65536 && V * ((cells + 31) / 32) < (1ll << 30) &&
            (int64_t)B * heads * ((nq > cells ? nq : cells) / 32 + 1) < (1ll << 31) / kMaxSplitCount * 4;
 }
@@ -24,6 +24,43 @@ int check_sizes(int dtype, int B, int heads, int D, int Dv, int64_t nq, int V, i
                  "sizes out of range: batch %d, heads %d, %lld queries, %d views of %lld cells", B, heads, (long long)nq, V,
                  (long long)cells);
     return ISPA_OK;
+}
+
+size_t align256(size_t x) { return (x + 255) & ~(size_t)255; }
+
+// Copies of maps whose rows do not start on 16-byte borders or whose channels are no multiple of 8, in the workspace.
+struct Copies {
+    int64_t ld;
+    int d8;
+    size_t bytes;              // 0: the map is streamed as it is
+};
+
+Copies copies(int dtype, int64_t maps, int d, int64_t n) {
+    const int64_t unit = dtype == ISPA_F32 ? 4 : 8;
+    Copies c;
+    c.ld = (n + unit - 1) / unit * unit;
+    c.d8 = (d + 7) & ~7;
+    c.bytes = c.ld == n && c.d8 == d ? 0 : align256((size_t)maps * c.d8 * c.ld * (dtype == ISPA_F32 ? 4 : 2));
+    return c;
+}
+
+// The map for streaming; `at` moves past the copy, if there is one.
+int stream_map(Stream *s, int dtype, const void *map, int64_t maps, int d, int64_t n, char **at, hipStream_t stream) {
+    const Copies c = copies(dtype, maps, d, n);
+    s->ld = c.ld;
+    s->d = c.d8;
+    s->map = map;
+    if (c.bytes == 0) return ISPA_OK;
+    const int64_t rows = maps * c.d8, per = (c.ld + 255) / 256;
+    ISPA_REQUIRE(rows * per < (1ll << 31), "maps of %lld rows are too large for one call", (long long)rows);
+    if (dtype == ISPA_F32)
+        soft_pack_kernel<F32><<<(unsigned)(rows * per), 256, 0, stream>>>((const float *)map, (float *)*at, d, c.d8, n, c.ld, rows);
+    else
+        soft_pack_kernel<BF16><<<(unsigned)(rows * per), 256, 0, stream>>>((const unsigned short *)map, (unsigned short *)*at, d,
+                                                                           c.d8, n, c.ld, rows);
+    s->map = *at;
+    *at += c.bytes;
+    return ispa::check_launch("soft_pack_kernel");
 }
 
 Plan forward_plan(int dtype, int B, int heads, int64_t nq, int V, int64_t cells) {
@@ -41,12 +78,13 @@ void backward_plans(int dtype, int B, int heads, int64_t nq, int64_t cells, Plan
     *dkv = make_plan(cells, (int64_t)B * heads, (nq + r - 1) / r);
 }
 
-size_t align256(size_t x) { return (x + 255) & ~(size_t)255; }
 
-size_t backward_bytes(const Plan &dq, const Plan &dkv, int B, int heads, int D, int Dv, int64_t nq, int64_t cells) {
+size_t backward_bytes(int dtype, const Plan &dq, const Plan &dkv, int B, int heads, int D, int Dv, int64_t nq, int64_t cells) {
     const size_t bh = (size_t)B * heads;
+    const size_t copied = copies(dtype, bh, D, cells).bytes + copies(dtype, bh, Dv, cells).bytes + copies(dtype, bh, D, nq).bytes +
+                          copies(dtype, bh, Dv, nq).bytes;
     const size_t a = dq.splits > 1 ? dq.splits * bh * D * nq : 0, k = dkv_in_parts(D, Dv, D == Dv, dkv.splits) ? dkv.splits * bh * (D + Dv) * cells : 0;
-    return align256(bh * nq * sizeof(float)) + (a > k ? a : k) * sizeof(float);
+    return copied + align256(bh * nq * sizeof(float)) + (a > k ? a : k) * sizeof(float);
 }
 
 int check_score(float scale, float cap, const float *falloff, int W) {
@@ -55,16 +93,29 @@ int check_score(float scale, float cap, const float *falloff, int W) {
     return ISPA_OK;
 }
 
+size_t forward_copies(int dtype, int B, int heads, int D, int Dv, int64_t cells, bool shared) {
+    return copies(dtype, (int64_t)B * heads, D, cells).bytes + (shared ? 0 : copies(dtype, (int64_t)B * heads, Dv, cells).bytes);
+}
+
 int run_forward(Params &p, int dtype, int source, void *workspace, size_t workspace_bytes, hipStream_t stream) {
     const Plan plan = forward_plan(dtype, p.B, p.heads, p.nq, p.V, p.cells);
-    const size_t need = forward_bytes(plan, p.B, p.heads, p.Dv, p.nq);
+    const bool maps = source == kSourceMap;
+    const size_t copied = maps ? forward_copies(dtype, p.B, p.heads, p.D, p.Dv, p.cells, p.shared) : 0;
+    const size_t need = copied + forward_bytes(plan, p.B, p.heads, p.Dv, p.nq);
+    ISPA_REQUIRE(!maps || (((uintptr_t)p.k | (uintptr_t)p.v) & 15) == 0, "maps must start on 16-byte borders");
     if (need > 0 && (workspace == nullptr || workspace_bytes < need))
         return ispa::fail(ISPA_EWORKSPACE, "workspace of %zu bytes, %zu needed", workspace_bytes, need);
     p.tiles_per_view = (int)((p.cells + tile_cells(dtype) - 1) / tile_cells(dtype));
     p.tiles = p.tiles_per_view * p.V;
     p.blocks = plan.blocks;
     p.splits = plan.splits;
-    p.part_ml = (float *)workspace;
+    char *at = (char *)workspace;
+    if (maps) {
+        if (int rc = stream_map(&p.sk, dtype, p.k, (int64_t)p.B * p.heads, p.D, p.cells, &at, stream)) return rc;
+        if (!p.shared)
+            if (int rc = stream_map(&p.sv, dtype, p.v, (int64_t)p.B * p.heads, p.Dv, p.cells, &at, stream)) return rc;
+    }
+    p.part_ml = (float *)at;
     p.part_o = p.part_ml + (size_t)plan.splits * p.B * p.heads * p.nq * 2;
     return dtype == ISPA_F32 ? forward_f32(p, source, plan.waves, stream) : forward_bf16(p, source, plan.waves, stream);
 }
@@ -73,7 +124,8 @@ int run_forward(Params &p, int dtype, int source, void *workspace, size_t worksp
 extern "C" size_t ispa_soft_match_workspace_bytes(int dtype, int B, int heads, int D, int Dv, int64_t nq, int views,
                                                   int64_t cells) {
     if (!sizes_ok(dtype, B, heads, D, Dv, nq, views, cells) || B == 0 || nq == 0) return 0;
-    return forward_bytes(forward_plan(dtype, B, heads, nq, views, cells), B, heads, Dv, nq);
+    return forward_copies(dtype, B, heads, D, Dv, cells, false) + forward_bytes(forward_plan(dtype, B, heads, nq, views, cells), B,
+                                                                                heads, Dv, nq);
 }
 
 extern "C" int ispa_soft_match(const void *q, const void *r, const void *v, int dtype, int B, int heads, int D, int Dv,
@@ -152,7 +204,7 @@ extern "C" size_t ispa_soft_match_backward_workspace_bytes(int dtype, int B, int
     if (!sizes_ok(dtype, B, heads, D, Dv, nq, 1, cells) || B == 0) return 0;
     Plan dq, dkv;
     backward_plans(dtype, B, heads, nq, cells, &dq, &dkv);
-    return backward_bytes(dq, dkv, B, heads, D, Dv, nq, cells);
+    return backward_bytes(dtype, dq, dkv, B, heads, D, Dv, nq, cells);
 }
 
 extern "C" int ispa_soft_match_backward(const void *q, const void *r, const void *v, int dtype, int B, int heads, int D, int Dv,
@@ -169,7 +221,7 @@ extern "C" int ispa_soft_match_backward(const void *q, const void *r, const void
     ISPA_REQUIRE(v != nullptr || D == Dv, "without a value map the reference map is the value (%d != %d channels)", D, Dv);
     Plan pq, pkv;
     backward_plans(dtype, B, heads, nq, cells, &pq, &pkv);
-    const size_t need = backward_bytes(pq, pkv, B, heads, D, Dv, nq, cells);
+    const size_t need = backward_bytes(dtype, pq, pkv, B, heads, D, Dv, nq, cells);
     if (workspace_bytes < need || (need > 0 && workspace == nullptr))
         return ispa::fail(ISPA_EWORKSPACE, "workspace of %zu bytes, %zu needed", workspace_bytes, need);
     Params p = {};
@@ -198,9 +250,18 @@ extern "C" int ispa_soft_match_backward(const void *q, const void *r, const void
     p.cap = cap;
     hipStream_t s = (hipStream_t)stream;
     const int64_t bh = (int64_t)B * heads;
-    float *delta = (float *)workspace;
+    ISPA_REQUIRE((((uintptr_t)r | (uintptr_t)p.v | (uintptr_t)q | (uintptr_t)d_out) & 15) == 0, "maps must start on 16-byte borders");
+    char *at = (char *)workspace;
+    if (int rc = stream_map(&p.sk, dtype, r, bh, D, cells, &at, s)) return rc;
+    if (!p.shared)
+        if (int rc = stream_map(&p.sv, dtype, v, bh, Dv, cells, &at, s)) return rc;
+    if (nq > 0) {
+        if (int rc = stream_map(&p.sq, dtype, q, bh, D, nq, &at, s)) return rc;
+        if (int rc = stream_map(&p.so, dtype, d_out, bh, Dv, nq, &at, s)) return rc;
+    }
+    float *delta = (float *)at;
     p.delta = delta;
-    p.part_a = (float *)((char *)workspace + align256(bh * nq * sizeof(float)));
+    p.part_a = (float *)(at + align256(bh * nq * sizeof(float)));
     p.part_b = p.part_a + (size_t)pkv.splits * bh * D * cells;
     if (nq > 0) {
         const unsigned grid = (unsigned)((nq + 63) / 64 * bh);

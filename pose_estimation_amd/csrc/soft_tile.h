@@ -374,6 +374,108 @@ struct Loader {
     }
 };
 
+// Copies tiles of a map from memory into LDS without a register in between (global_load_lds, 16 bytes a lane), so that the
+// next tile is under way during the products of the present one.  Wave w of WQ moves channel rows 8 (w kShare + e) .. + 7
+// with instruction e; lane l lands on row l / 8, segment l % 8, and fetches the segment that swz keeps there.
+// The map: rows of `ld` cells that start on 16-byte borders (ld a multiple of kCells), `d` rows, a multiple of 8; what
+// does not come like that is copied into such a form first (soft_pack_kernel).
+template <typename M, int DP, int WQ>
+struct Direct {
+    static constexpr int kSize = std::is_same_v<typename M::map, BF16> ? 2 : 4;
+    static constexpr int kShare = DP / 8 / WQ;
+    static constexpr int kUnroll = kShare > 8 ? 4 : kShare / 2 < 1 ? 1 : kShare / 2;
+    static_assert(kShare == 1 || kShare % 2 == 0, "a wave moves 8 rows or pairs of 8");
+    unsigned off[2];           // byte offset of this lane's segment in rows 8 e .. 8 e + 7 for even, odd 8-row groups
+    unsigned row;              // byte offset of its row
+    unsigned ld8;              // bytes of 8 rows
+    int groups;                // 8-row groups of the map
+    __device__ void init(int64_t ld, int d) {
+        const int lane = threadIdx.x & 63;
+        row = (unsigned)((lane >> 3) * ld * kSize);
+#pragma unroll
+        for (int odd = 0; odd < 2; ++odd) off[odd] = row + (((lane & 7) ^ swz((lane >> 3) + 8 * odd)) << 4);
+        ld8 = (unsigned)(8 * ld * kSize);
+        groups = d >> 3;
+    }
+    // Rows past the map's are zero in LDS throughout.
+    __device__ void clear_rest(char *tile) const {
+        for (int i = groups * 8 * kRowBytes + (int)threadIdx.x * 16; i < DP * kRowBytes; i += 64 * WQ * 16)
+            *reinterpret_cast<u32x4 *>(tile + i) = u32x4{};
+    }
+    // Tile from `cell0` on, of a map with `cells` cells (a multiple of kCells) a row; asynchronous, wait() ends it.
+    __device__ void issue(const void *map, int64_t cell0, int64_t cells, const char *tile) const {
+        const int wave = __builtin_amdgcn_readfirstlane((int)threadIdx.x >> 6);
+        unsigned at[2] = {off[0], off[1]};
+        if (cells - cell0 < M::kRows) {                        // segments past the end: the row's first of this tile instead
+#pragma unroll
+            for (int odd = 0; odd < 2; ++odd)
+                if ((int64_t)((at[odd] - row) / kSize) >= cells - cell0) at[odd] = row;
+        }
+        const uint64_t base = (uint64_t)map + (uint64_t)cell0 * kSize;
+        const unsigned dst = (unsigned)(uintptr_t)(__attribute__((address_space(3))) const char *)tile;
+        if constexpr (kShare == 1) {
+            if (wave < groups) copy(wave & 1 ? at[1] : at[0], base + (uint64_t)wave * ld8, dst + wave * 1024);
+        } else {
+#pragma unroll kUnroll
+            for (int e = 0; e < kShare; e += 2) {
+                const int group = wave * kShare + e;
+                if (group < groups) copy(at[0], base + (uint64_t)group * ld8, dst + group * 1024);
+                if (group + 1 < groups) copy(at[1], base + (uint64_t)(group + 1) * ld8, dst + group * 1024 + 1024);
+            }
+        }
+    }
+    __device__ static void copy(unsigned voff, uint64_t sbase, unsigned dst) {
+        const uint32_t hi = (uint32_t)__builtin_amdgcn_readfirstlane((int)(uint32_t)(sbase >> 32));
+        const uint32_t lo = (uint32_t)__builtin_amdgcn_readfirstlane((int)(uint32_t)sbase);
+        const unsigned m0 = (unsigned)__builtin_amdgcn_readfirstlane((int)dst);
+        // nothing else in these kernels uses m0 (LDS instructions do not read it)
+        asm volatile("s_mov_b32 m0, %1\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %0, %2"
+                     :
+                     : "v"(voff), "s"(m0), "s"(((uint64_t)hi << 32) | lo)
+                     : "memory");
+    }
+    __device__ static void wait() { asm volatile("s_waitcnt vmcnt(0)" ::: "memory"); }
+    // After wait(): zeros for the cells that take no part (see Loader), in the segments this lane itself has copied.
+    __device__ void mask(char *tile, uint64_t live) const {
+        const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+#pragma unroll
+        for (int odd = 0; odd < 2; ++odd) {
+            const int seg = (lane & 7) ^ swz((lane >> 3) + 8 * odd);
+            const unsigned bits = (unsigned)(live >> (seg * M::kCells)) & ((1u << M::kCells) - 1u);
+            if (bits == (1u << M::kCells) - 1u) continue;
+            u32x4 keep;
+#pragma unroll
+            for (int j = 0; j < 4; ++j) {
+                if constexpr (kSize == 2)
+                    keep[j] = ((bits >> (2 * j)) & 1u ? 0xffffu : 0u) | ((bits >> (2 * j + 1)) & 1u ? 0xffff0000u : 0u);
+                else
+                    keep[j] = (bits >> j) & 1u ? 0xffffffffu : 0u;
+            }
+            if (kShare == 1 && (wave & 1) != odd) continue;
+#pragma unroll kUnroll
+            for (int e = kShare == 1 ? 0 : odd; e < kShare; e += 2) {
+                const int group = wave * kShare + e;
+                if (group >= groups) break;
+                u32x4 *p = reinterpret_cast<u32x4 *>(tile + group * 1024 + lane * 16);
+                *p = *p & keep;
+            }
+        }
+    }
+};
+
+// Copies maps (maps, d, n) into the form Direct wants: (maps, d8, ld) with d8 the next multiple of 8 rows and ld of kCells
+// cells, zeros beside.
+template <typename T>
+__global__ __launch_bounds__(256) void soft_pack_kernel(const typename T::elem *src, typename T::elem *dst, int d, int d8,
+                                                        int64_t n, int64_t ld, int64_t rows) {
+    const int64_t per = (ld + 255) / 256;
+    const int64_t row = blockIdx.x / per, cell = (blockIdx.x - row * per) * 256 + threadIdx.x;
+    if (row >= rows || cell >= ld) return;
+    const int64_t map = row / d8;
+    const int c = (int)(row - map * d8);
+    dst[row * ld + cell] = c < d && cell < n ? src[(map * d + c) * n + cell] : (typename T::elem)0;
+}
+
 // Workgroups are dealt to the 8 dies in turn; this numbering gives each die a run of successive workgroups, so that those
 // that stream the same maps share one L2.
 __device__ __forceinline__ int die_major(int id, int n) {
@@ -382,6 +484,13 @@ __device__ __forceinline__ int die_major(int id, int n) {
 }
 
 // ------------------------------------------------------------------------------------------------
+// A map as Direct streams it: `d` rows (a multiple of 8) of `ld` cells per item and head.
+struct Stream {
+    const void *map;
+    int64_t ld;
+    int d;
+};
+
 // What a call computes; device pointers as the C ABI hands them over.
 struct Params {
     const void *q, *k, *v;                 // (B,heads D,nq), (B,heads D,cells), (B,heads Dv,cells); codes for a store
@@ -402,6 +511,7 @@ struct Params {
     int64_t nq, cells;
     int B, heads, D, Dv, W, V, n_view;
     int tiles_per_view, tiles, splits, blocks;       // streamed tiles of one item, split over `splits` workgroups
+    Stream sk, sv, sq, so;                 // r, v, q, d_out for streaming: the maps themselves or their copies
     int shared;                            // the value map is the reference map
     int parts;                             // gradients go to part_a (and part_b), to be summed by soft_sum_kernel
     int c0;                                // first channel of the gradients this launch forms

@@ -60,6 +60,11 @@ def _on(x, dtype, device):
     return dv.to_dev(x, dtype)
 
 
+def _aligned(x):
+    """The kernels stream maps in 16-byte pieces: a view that starts between them is copied."""
+    return x if x is None or x.data_ptr() % 16 == 0 else x.clone()
+
+
 @functools.lru_cache(maxsize=4096)
 def _forward_bytes(*sizes):
     return _abi.lib.ispa_soft_match_workspace_bytes(*sizes)
@@ -178,7 +183,7 @@ class _Call:
 
     def bind(self, device, query, ref, value, falloff, xy, mask, count):
         self.device = device
-        self.q, self.r, self.v = (_on(x, self.dtype, device) for x in (query, ref, value))
+        self.q, self.r, self.v = (_aligned(_on(x, self.dtype, device)) for x in (query, ref, value))
         self.falloff, self.xy, self.mask, self.count = falloff, xy, mask, count
         return self
 
@@ -212,7 +217,7 @@ class _Call:
         dval = torch.empty_like(self.v) if self.v is not None else None
         if d_out is None:
             d_out = torch.zeros(self.out_shape, dtype=self.dtype, device=self.device)
-        d_out, d_lse = _on(d_out, self.dtype, self.device), _on(d_lse, torch.float32, self.device)
+        d_out, d_lse = _aligned(_on(d_out, self.dtype, self.device)), _on(d_lse, torch.float32, self.device)
         need = _backward_bytes(self.code, self.b, self.heads, self.d, self.dv, self.n, self.cells)
         ws = _bytes(need, self.device)
         _abi.check(_abi.lib.ispa_soft_match_backward(dv.ptr(self.q), dv.ptr(self.r), dv.ptr(self.v), *self._common(),
