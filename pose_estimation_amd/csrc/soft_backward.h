@@ -8,6 +8,10 @@
 
 namespace ispa_soft {
 
+// Registers for two waves a SIMD: one's products run under the other's exponentials.
+template <typename T, int DP, int WQ>
+constexpr bool two_waves = DP <= 128 && WQ > 1 && std::is_same_v<T, BF16>;
+
 // delta (B,heads,nq); 0 for queries that are not live or have no cell.
 template <typename T>
 __global__ __launch_bounds__(256) void soft_delta_kernel(const Params p, const float *o32, const float *d_lse,
@@ -34,12 +38,63 @@ __global__ __launch_bounds__(256) void soft_delta_kernel(const Params p, const f
     delta[bh * p.nq + q] = some ? s : 0.f;
 }
 
+// From products `acc` and w = -(falloff d^2) + minus_lse: w = P and the slope 1 - tanh^2, or at once dx / scale with dP in `dp`.
+template <typename T, int MODE>
+__device__ __forceinline__ void probabilities(const Score<T> &score, const f32x16 &acc, float (&w)[16], float (&slope)[16]) {
+    if (MODE == kPlain || MODE == kRows || (MODE == kGeneral && !score.cap)) {
+#pragma unroll
+        for (int i = 0; i < 16; ++i) w[i] = exp2_(fmaf(score.in, acc[i], w[i]));
+    } else if constexpr (Score<T>::kExact) {
+#pragma unroll
+        for (int i = 0; i < 16; ++i) {
+            const float th = score.bend(acc[i]);
+            slope[i] = fmaf(-th, th, 1.f);
+            w[i] = exp2_(fmaf(score.top, th, w[i]));
+        }
+    } else {
+        // tanh = 1 - 2 r: 1 - tanh^2 = 4 (r - r^2); the cap itself is in w
+#pragma unroll
+        for (int i = 0; i < 16; ++i) {
+            const float r = score.r(acc[i]);
+            slope[i] = 4.f * fmaf(-r, r, r);
+            w[i] = exp2_(fmaf(-2.f * score.top, r, w[i]));
+        }
+    }
+}
+template <typename T, int MODE>
+__device__ __forceinline__ void weights(const Score<T> &score, const f32x16 &acc, float (&w)[16], const f32x16 &dp,
+                                        const float (&delta)[16]) {
+    if (MODE == kPlain || MODE == kRows || (MODE == kGeneral && !score.cap)) {
+#pragma unroll
+        for (int i = 0; i < 16; ++i) w[i] = exp2_(fmaf(score.in, acc[i], w[i])) * (dp[i] - delta[i]);
+    } else if constexpr (Score<T>::kExact) {
+#pragma unroll
+        for (int i = 0; i < 16; ++i) {
+            const float th = score.bend(acc[i]);
+            w[i] = exp2_(fmaf(score.top, th, w[i])) * ((dp[i] - delta[i]) * fmaf(-th, th, 1.f));
+        }
+    } else {
+#pragma unroll
+        for (int i = 0; i < 16; ++i) {
+            const float r = score.r(acc[i]);
+            w[i] = exp2_(fmaf(-2.f * score.top, r, w[i])) * ((dp[i] - delta[i]) * (4.f * fmaf(-r, r, r)));
+        }
+    }
+}
+// -lse in log2 units, with what probabilities() expects beside: the cap where tanh is taken as 1 - 2 r.
+template <typename T, int MODE>
+__device__ __forceinline__ float minus_lse(const Score<T> &score, float lse) {
+    if (lse == -__builtin_inff()) return -__builtin_inff();    // no cells: weights 0
+    const bool cap = MODE == kCapped || (MODE == kGeneral && score.cap);
+    return fmaf(-kLog2e, lse, !Score<T>::kExact && cap ? score.top : 0.f);
+}
+
 // Both kernels can form their gradients for NC channels at a time, from p.c0 on.  A launch per half is what 256 float32
 // channels take: two owned operands and a whole accumulator would need more than a lane's 512 registers.
 //
 // Gradient of the queries: owned = queries, streamed = cells.
-template <typename T, int DP, int WQ, int NC>
-__global__ __launch_bounds__(64 * WQ, (DP <= 128 && WQ > 1 && std::is_same_v<T, BF16>) ? 2 : 1) void soft_dq_kernel(const Params p) {
+template <typename T, int DP, int WQ, int NC, int MODE>
+__global__ __launch_bounds__(64 * WQ, (two_waves<T, DP, WQ>) ? 2 : 1) void soft_dq_kernel(const Params p) {
     typedef Math<T, DP> M;
     constexpr int kBlocks = M::kRows / 32;
     constexpr int kUnroll = DP == 256 ? 1 : kBlocks;           // registers
@@ -69,10 +124,9 @@ __global__ __launch_bounds__(64 * WQ, (DP <= 128 && WQ > 1 && std::is_same_v<T, 
     const Score<T> score(p, head);
     float qx = 0.f, qy = 0.f;
     if (p.falloff != nullptr && q_ok) query_place(p, b, q, qx, qy);
-    float lse2 = __builtin_inff(), delta = 0.f;                // a query without cells has weights 0
+    float minus = -__builtin_inff(), delta = 0.f;
     if (q_ok) {
-        const float x = p.lse[(int64_t)bh * p.nq + q];
-        lse2 = x == -__builtin_inff() ? __builtin_inff() : x * kLog2e;
+        minus = minus_lse<T, MODE>(score, p.lse[(int64_t)bh * p.nq + q]);
         delta = p.delta[(int64_t)bh * p.nq + q];
     }
     f32x16 g[NC / 32];
@@ -82,10 +136,13 @@ __global__ __launch_bounds__(64 * WQ, (DP <= 128 && WQ > 1 && std::is_same_v<T, 
         for (int i = 0; i < 16; ++i) g[c][i] = 0.f;
 
     Feed<M, T, DP, WQ> feed(p, b, head, lds, stage);
+    const Penalty<M, MODE> penalty(p, score.fall, qx, qy, true);
     uint64_t live = 0;
+    int cell0 = 0;
     if (t0 < t1) {
         feed.fetch(t0, lds);
         live = feed.put(lds);
+        cell0 = (int)feed.at.cell0;
     }
     __syncthreads();
     for (int t = t0; t < t1; ++t) {
@@ -96,33 +153,22 @@ __global__ __launch_bounds__(64 * WQ, (DP <= 128 && WQ > 1 && std::is_same_v<T, 
             const float *cell = reinterpret_cast<const float *>(buf + cell_at);
 #pragma unroll kUnroll
             for (int k = 0; k < kBlocks; ++k) {
-                const f32x16 acc = M::first(ktile, addr, k, qf);
-                const f32x16 dp = M::first(vtile, addr, k, of);
-                float w[16];
-                if (p.falloff != nullptr) {
-                    M::per_cell(cell + 64, k, h, w);
+                if (DP == 256) __builtin_amdgcn_sched_barrier(0);
+                f32x16 acc[1], dp[1];
+                M::first(ktile, addr, k, qf, acc);
+                M::first(vtile, addr, k, of, dp);
+                float w[16], dl[16];
+                if (MODE == kRows || penalty.on) {
+                    penalty(cell + 64, cell0, k, h, w);
 #pragma unroll
-                    for (int i = 0; i < 16; ++i) w[i] = (w[i] - qx) * (w[i] - qx);
-                    float cy[16];
-                    M::per_cell(cell + 128, k, h, cy);
-#pragma unroll
-                    for (int i = 0; i < 16; ++i) w[i] = fmaf(-score.fall, fmaf(cy[i] - qy, cy[i] - qy, w[i]), -lse2);
+                    for (int i = 0; i < 16; ++i) w[i] += minus;
                 } else {
 #pragma unroll
-                    for (int i = 0; i < 16; ++i) w[i] = -lse2;
+                    for (int i = 0; i < 16; ++i) w[i] = minus;
                 }
 #pragma unroll
-                for (int i = 0; i < 16; ++i) {
-                    float ds = dp[i] - delta;
-                    if (score.cap) {
-                        const float th = score.bend(acc[i]);
-                        w[i] = fmaf(score.top, th, w[i]);
-                        ds *= fmaf(-th, th, 1.f);
-                    } else {
-                        w[i] = fmaf(score.in, acc[i], w[i]);
-                    }
-                    w[i] = ds * exp2_(w[i]);
-                }
+                for (int i = 0; i < 16; ++i) dl[i] = delta;
+                weights<T, MODE>(score, acc[0], w, dp[0], dl);
                 if (live != kAll) {
                     const unsigned bits = (unsigned)(live >> (32 * k)) >> M::cell(0, h);
 #pragma unroll
@@ -131,7 +177,10 @@ __global__ __launch_bounds__(64 * WQ, (DP <= 128 && WQ > 1 && std::is_same_v<T, 
                 M::second(ktile + p.c0 * kRowBytes, addr, k, M::weights(w), g);
             }
         }
-        if (t + 1 < t1) live = feed.put(lds + ((t + 1 - t0) & 1) * stage);
+        if (t + 1 < t1) {
+            live = feed.put(lds + ((t + 1 - t0) & 1) * stage);
+            cell0 = (int)feed.at.cell0;
+        }
         __syncthreads();
     }
     if (q >= p.nq) return;
@@ -161,12 +210,13 @@ template <int DP>
 constexpr int dkv_stage_bytes = 2 * DP * kRowBytes + 4 * 64 * (int)sizeof(float);
 
 // Gradients of the reference and value maps: owned = cells, streamed = queries.  PART 0: both; 1: the value's, 2: the
-// reference's alone (maps of more than 128 channels, for the registers).
-template <typename T, int DP, int WQ, int PART, int NC>
-__global__ __launch_bounds__(64 * WQ) void soft_dkv_kernel(const Params p) {
+// reference's alone: two launches and a fifth product, which pays where it brings two waves to a SIMD, and which the
+// registers ask for above 128 channels.
+template <typename T, int DP, int WQ, int PART, int NC, int MODE>
+__global__ __launch_bounds__(64 * WQ, (two_waves<T, DP, WQ> && (DP <= 64 || PART != 0)) ? 2 : 1) void soft_dkv_kernel(const Params p) {
     typedef Math<T, DP> M;
     constexpr int kBlocks = M::kRows / 32;
-    constexpr int kUnroll = DP == 256 ? 1 : kBlocks;           // registers
+    constexpr int kUnroll = DP == 256 || (DP == 128 && PART == 2) ? 1 : kBlocks;           // registers
     constexpr bool kDv = PART != 2, kDk = PART != 1;
     constexpr int kStage = dkv_stage_bytes<DP>;
     extern __shared__ __attribute__((aligned(16))) char lds[];
@@ -202,6 +252,7 @@ __global__ __launch_bounds__(64 * WQ) void soft_dkv_kernel(const Params p) {
             if constexpr (kDv) gv[c][i] = 0.f;
         }
 
+    const Penalty<M, MODE> penalty(p, score.fall, cx, cy, p.query_xy == nullptr);
     typedef Direct<M, DP, WQ> Copy;
     Copy cq, co;
     cq.init(p.sq.ld, p.sq.d);
@@ -212,18 +263,17 @@ __global__ __launch_bounds__(64 * WQ) void soft_dkv_kernel(const Params p) {
         cq.clear_rest(lds + i * kStage);
         co.clear_rest(lds + i * kStage + DP * kRowBytes);
     }
-    float lse2 = 0.f, delta = 0.f, px = 0.f, py = 0.f;
+    float minus = 0.f, delta = 0.f, px = 0.f, py = 0.f;
     auto fetch = [&](int t, char *buf) {
         const int64_t q0 = (int64_t)t * M::kRows;
         if (threadIdx.x < M::kRows) {
             const int64_t q = q0 + threadIdx.x;
-            lse2 = __builtin_inff();                           // no weight without cells
+            minus = -__builtin_inff();
             delta = 0.f;
             if (q < live_q) {
-                const float x = p.lse[(int64_t)bh * p.nq + q];
-                lse2 = x == -__builtin_inff() ? __builtin_inff() : x * kLog2e;
+                minus = minus_lse<T, MODE>(score, p.lse[(int64_t)bh * p.nq + q]);
                 delta = p.delta[(int64_t)bh * p.nq + q];
-                if (p.falloff != nullptr) query_place(p, b, q, px, py);
+                if (penalty.wants_places()) query_place(p, b, q, px, py);
             }
         }
         cq.issue(qmap, q0, p.sq.ld, buf);
@@ -239,7 +289,7 @@ __global__ __launch_bounds__(64 * WQ) void soft_dkv_kernel(const Params p) {
         }
         if (threadIdx.x < M::kRows) {
             float *cell = reinterpret_cast<float *>(buf + 2 * DP * kRowBytes) + threadIdx.x;
-            cell[0] = lse2;
+            cell[0] = minus;
             cell[64] = delta;
             cell[128] = px;
             cell[192] = py;
@@ -253,48 +303,45 @@ __global__ __launch_bounds__(64 * WQ) void soft_dkv_kernel(const Params p) {
     for (int t = t0; t < t1; ++t) {
         const char *qtile = lds + ((t - t0) & 1) * kStage, *otile = qtile + DP * kRowBytes;
         const float *larr = reinterpret_cast<const float *>(otile + DP * kRowBytes);
-        const float *darr = larr + 64, *xarr = larr + 128, *yarr = larr + 192;
+        const float *darr = larr + 64, *xarr = larr + 128;
         if (t + 1 < t1) fetch(t + 1, lds + ((t + 1 - t0) & 1) * kStage);
 #pragma unroll kUnroll
         for (int k = 0; k < kBlocks; ++k) {
-            const f32x16 acc = M::first(qtile, addr, k, kf);
-            float w[16], slope[16], ls[16];
-            M::per_cell(larr, k, h, ls);
-            if (score.cap) {
+            f32x16 acc[1];
+            M::first(qtile, addr, k, kf, acc);
+            float w[16];
+            if (MODE == kRows || penalty.on) {
+                penalty(xarr, t * M::kRows, k, h, w);
+                float minus_l[16];
+                M::per_cell(larr, k, h, minus_l);
 #pragma unroll
-                for (int i = 0; i < 16; ++i) {
-                    const float th = score.bend(acc[i]);
-                    w[i] = score.top * th;
-                    slope[i] = fmaf(-th, th, 1.f);
+                for (int i = 0; i < 16; ++i) w[i] += minus_l[i];
+            } else {
+                M::per_cell(larr, k, h, w);
+            }
+            if constexpr (kDv) {
+                float slope[16];
+                probabilities<T, MODE>(score, acc[0], w, slope);
+                M::second(otile + p.c0 * kRowBytes, addr, k, M::weights(w), gv);
+                if constexpr (kDk) {
+                    f32x16 dp[1];
+                    M::first(otile, addr, k, vf, dp);
+                    float dl[16];
+                    M::per_cell(darr, k, h, dl);
+#pragma unroll
+                    for (int i = 0; i < 16; ++i) w[i] *= dp[0][i] - dl[i];
+                    if (MODE == kCapped || (MODE == kGeneral && score.cap))
+#pragma unroll
+                        for (int i = 0; i < 16; ++i) w[i] *= slope[i];
                 }
             } else {
-#pragma unroll
-                for (int i = 0; i < 16; ++i) {
-                    w[i] = score.in * acc[i];
-                    slope[i] = 1.f;
-                }
-            }
-            if (p.falloff != nullptr) {
-                float qx[16], qy[16];
-                M::per_cell(xarr, k, h, qx);
-                M::per_cell(yarr, k, h, qy);
-#pragma unroll
-                for (int i = 0; i < 16; ++i) {
-                    const float dx = cx - qx[i], dy = cy - qy[i];
-                    w[i] = fmaf(-score.fall, fmaf(dx, dx, dy * dy), w[i]);
-                }
-            }
-#pragma unroll
-            for (int i = 0; i < 16; ++i) w[i] = exp2_(w[i] - ls[i]);
-            if constexpr (kDv) M::second(otile + p.c0 * kRowBytes, addr, k, M::weights(w), gv);
-            if constexpr (kDk) {
-                const f32x16 dp = M::first(otile, addr, k, vf);
+                f32x16 dp[1];
+                M::first(otile, addr, k, vf, dp);
                 float dl[16];
                 M::per_cell(darr, k, h, dl);
-#pragma unroll
-                for (int i = 0; i < 16; ++i) w[i] = w[i] * (dp[i] - dl[i]) * slope[i];
-                M::second(qtile + p.c0 * kRowBytes, addr, k, M::weights(w), gk);
+                weights<T, MODE>(score, acc[0], w, dp[0], dl);
             }
+            if constexpr (kDk) M::second(qtile + p.c0 * kRowBytes, addr, k, M::weights(w), gk);
         }
         if (t + 1 < t1) put(t + 1, lds + ((t + 1 - t0) & 1) * kStage);
         __syncthreads();
@@ -310,16 +357,20 @@ __global__ __launch_bounds__(64 * WQ) void soft_dkv_kernel(const Params p) {
             float a = 0.f, v = 0.f;
             if constexpr (kDk) a = c_ok ? gk[c][i] * p.scale : 0.f;
             if constexpr (kDv) v = c_ok ? gv[c][i] : 0.f;
+            float *pv = p.part_b + (part * p.Dv + ch) * p.cells + cell;
             if (p.parts) {
                 if constexpr (kDk)
                     if (ch < p.D) p.part_a[(part * p.D + ch) * p.cells + cell] = a;
                 if constexpr (kDv)
-                    if (ch < p.Dv) p.part_b[(part * p.Dv + ch) * p.cells + cell] = v;
+                    if (ch < p.Dv) *pv = v;
                 continue;
             }
             typename T::elem *dk = (typename T::elem *)p.dk + ((int64_t)bh * p.D + ch) * p.cells + cell;
-            if (p.shared) {                                    // PART 0 only: the parts of a shared map go to part_a, part_b
-                if (ch < p.D) store_float(dk, a + v);
+            if (p.shared) {                                    // the sum of both uses, rounded once
+                if (ch >= p.D) continue;
+                if constexpr (PART == 1) *pv = v;              // float32, for the launch that forms the other one
+                else if constexpr (PART == 2) store_float(dk, a + *pv);
+                else store_float(dk, a + v);
                 continue;
             }
             if constexpr (kDk)

@@ -9,38 +9,38 @@ namespace ispa_soft {
 template <typename T, int DP>
 constexpr int kFormed = DP == 256 && std::is_same_v<T, F32> ? 128 : DP;
 
-template <typename T, int DP, int WQ>
+template <typename T, int DP, int WQ, int MODE>
 int dq_one(Params p, hipStream_t stream) {
     static unsigned long long lds_allowed = 0;
     const int lds = 2 * stage_bytes<DP>(p.shared);
     const unsigned grid = (unsigned)((int64_t)p.B * p.heads * p.splits * p.blocks);
     constexpr int NC = kFormed<T, DP>;
     for (p.c0 = 0; p.c0 < p.D; p.c0 += NC)
-        if (int rc = launch(soft_dq_kernel<T, DP, WQ, NC>, p, grid, 64 * WQ, lds, &lds_allowed, "soft_dq_kernel", stream))
+        if (int rc = launch(soft_dq_kernel<T, DP, WQ, NC, MODE>, p, grid, 64 * WQ, lds, &lds_allowed, "soft_dq_kernel", stream))
             return rc;
     return ISPA_OK;
 }
 
-template <typename T, int DP, int WQ, int PART>
+template <typename T, int DP, int WQ, int PART, int MODE>
 int dkv_one(Params p, int channels, hipStream_t stream) {
     static unsigned long long lds_allowed = 0;
     const int lds = 2 * dkv_stage_bytes<DP>;
     const unsigned grid = (unsigned)((int64_t)p.B * p.heads * p.splits * p.blocks);
     constexpr int NC = PART == 2 ? kFormed<T, DP> : DP;
     for (p.c0 = 0; p.c0 < channels; p.c0 += NC)
-        if (int rc = launch(soft_dkv_kernel<T, DP, WQ, PART, NC>, p, grid, 64 * WQ, lds, &lds_allowed, "soft_dkv_kernel",
+        if (int rc = launch(soft_dkv_kernel<T, DP, WQ, PART, NC, MODE>, p, grid, 64 * WQ, lds, &lds_allowed, "soft_dkv_kernel",
                             stream))
             return rc;
     return ISPA_OK;
 }
 
-template <typename T, int DP, int WQ>
+template <typename T, int DP, int WQ, int MODE>
 int dkv_parts(const Params &p, hipStream_t stream) {
-    if constexpr (DP == 256) {
-        if (int rc = dkv_one<T, DP, WQ, 1>(p, p.Dv, stream)) return rc;
-        return dkv_one<T, DP, WQ, 2>(p, p.D, stream);
+    if constexpr (dkv_two_launches(std::is_same_v<T, F32>, DP, WQ)) {
+        if (int rc = dkv_one<T, DP, WQ, 1, MODE>(p, p.Dv, stream)) return rc;
+        return dkv_one<T, DP, WQ, 2, MODE>(p, p.D, stream);
     } else {
-        return dkv_one<T, DP, WQ, 0>(p, DP, stream);
+        return dkv_one<T, DP, WQ, 0, MODE>(p, DP, stream);
     }
 }
 
@@ -57,14 +57,20 @@ int backward_sized(Params p, const Plan &dq, const Plan &dkv, hipStream_t stream
     p.parts = dq.splits > 1;
     p.blocks = dq.blocks;
     p.tiles = p.tiles_per_view = (int)((p.cells + M::kRows - 1) / M::kRows);
-    if (int rc = dq.waves == 1 ? dq_one<T, DP, 1>(p, stream) : dq_one<T, DP, 4>(p, stream)) return rc;
+    if (int rc = dq.waves == 1 ? dq_one<T, DP, 1, kGeneral>(p, stream)
+                               : with_mode<T, DP>(p, true, [&](auto mode) { return dq_one<T, DP, 4, decltype(mode)::value>(p, stream); }))
+        return rc;
     const int64_t bh = (int64_t)p.B * p.heads;
     if (p.parts)
         if (int rc = sum_parts<T>(p.part_a, nullptr, p.splits, bh * p.D * p.nq, p.scale, p.dq, stream)) return rc;
     p.splits = dkv.splits;
-    p.parts = dkv_in_parts(p.D, p.Dv, p.shared, dkv.splits);
+    p.parts = dkv.splits > 1;
     p.blocks = dkv.blocks;
-    if (int rc = dkv.waves == 1 ? dkv_parts<T, DP, 1>(p, stream) : dkv_parts<T, DP, 4>(p, stream)) return rc;
+    if (int rc = dkv.waves == 1 ? dkv_parts<T, DP, 1, kGeneral>(p, stream)
+                                : with_mode<T, DP>(p, p.query_xy == nullptr, [&](auto mode) {
+                                      return dkv_parts<T, DP, 4, decltype(mode)::value>(p, stream);
+                                  }))
+        return rc;
     if (!p.parts) return ISPA_OK;
     if (p.shared) return sum_parts<T>(p.part_a, p.part_b, p.splits, bh * p.D * p.cells, 1.f, p.dk, stream);
     if (int rc = sum_parts<T>(p.part_a, nullptr, p.splits, bh * p.D * p.cells, 1.f, p.dk, stream)) return rc;

@@ -127,7 +127,7 @@ struct Feed {
             dk.mask(buf, live);
             if (!p.shared) dv.mask(buf + v_at, live);
         }
-        if (p.falloff != nullptr && threadIdx.x < M::kRows) {
+        if (p.falloff != nullptr && p.W % M::kCells != 0 && threadIdx.x < M::kRows) {
             const int c = (int)at.cell0 + threadIdx.x;
             cell[64 + threadIdx.x] = (float)(c % p.W);
             cell[128 + threadIdx.x] = (float)(c / p.W);
@@ -141,7 +141,7 @@ struct Feed {
 constexpr float kSlack = 8.f;
 
 // NC: value channels that one launch forms, from p.c0 on (256 float32 channels take two launches, for the registers).
-template <typename T, typename SRC, int DP, int WQ, int NC>
+template <typename T, typename SRC, int DP, int WQ, int NC, int MODE>
 __global__ __launch_bounds__(64 * WQ, (DP <= 128 && std::is_same_v<SRC, BF16>) ? 2 : 1) void soft_forward_kernel(const Params p) {
     typedef Math<T, DP> M;
     constexpr int kBlocks = M::kRows / 32;
@@ -169,8 +169,13 @@ __global__ __launch_bounds__(64 * WQ, (DP <= 128 && std::is_same_v<SRC, BF16>) ?
 
     typename M::Owned qf;
     M::load_owned(qf, (const typename T::elem *)p.q + (int64_t)bh * p.D * p.nq + (q < p.nq ? q : 0), p.nq, p.D, q_ok, h);
+    Score<T> score(p, head);
+    if (MODE == kPlain && score.in < 0.f) {                        // largest product = largest score
+        M::negate(qf);
+        score.in = -score.in;
+    }
+    if (MODE == kPlain) score.in = fmaxf(score.in, 1e-37f);    // scale 0: products of a masked cell stay -inf
     const typename M::Addr addr = M::addr(lane);
-    const Score<T> score(p, head);
     float qx = 0.f, qy = 0.f;
     if (p.falloff != nullptr && q_ok) query_place(p, b, q, qx, qy);
 
@@ -182,11 +187,14 @@ __global__ __launch_bounds__(64 * WQ, (DP <= 128 && std::is_same_v<SRC, BF16>) ?
     float m = -__builtin_inff(), l = 0.f;                      // l: this lane's half of the cells
 
     Feed<M, SRC, DP, WQ> feed(p, b, head, lds, stage);
+    const Penalty<M, MODE> penalty(p, score.fall, qx, qy, true);
     uint64_t live = 0;
+    int cell0 = 0;
     if constexpr (kAheadHere) {
         if (t0 < t1) {
             feed.fetch(t0, lds);
             live = feed.put(lds);
+            cell0 = (int)feed.at.cell0;
         }
         __syncthreads();
     }
@@ -198,81 +206,97 @@ __global__ __launch_bounds__(64 * WQ, (DP <= 128 && std::is_same_v<SRC, BF16>) ?
             __syncthreads();
             feed.fetch(t, lds);
             live = feed.put(lds);
+            cell0 = (int)feed.at.cell0;
             __syncthreads();
         }
         if (live != 0) {
             const char *ktile = buf, *vtile = buf + v_at;
             const float *cell = reinterpret_cast<const float *>(buf + cell_at);
-            float z[kBlocks][16];
+            // kPlain: z holds the products, scaled in the exponent.  kCapped: scores relative to the cap, which stands for
+            // the maximum: weights are 2^(-2 cap) > 2^-93 at least.
+            f32x16 z[kBlocks];
             float ks[kScaled ? kBlocks : 1][16];
-            float top = -__builtin_inff();
+            M::first(ktile, addr, 0, qf, z);
 #pragma unroll
             for (int k = 0; k < kBlocks; ++k) {
-                if (DP == 256) __builtin_amdgcn_sched_barrier(0);
-                f32x16 acc = M::first(ktile, addr, k, qf);
                 if constexpr (kScaled) {
                     M::per_cell(cell, k, h, ks[k]);
 #pragma unroll
-                    for (int i = 0; i < 16; ++i) acc[i] *= ks[k][i];
+                    for (int i = 0; i < 16; ++i) z[k][i] *= ks[k][i];
                 }
-                if (p.falloff != nullptr) {
-                    M::per_cell(cell + 64, k, h, z[k]);
+                if constexpr (MODE == kCapped) {
 #pragma unroll
-                    for (int i = 0; i < 16; ++i) z[k][i] = (z[k][i] - qx) * (z[k][i] - qx);
-                    float cy[16];
-                    M::per_cell(cell + 128, k, h, cy);
-#pragma unroll
-                    for (int i = 0; i < 16; ++i) z[k][i] = -score.fall * fmaf(cy[i] - qy, cy[i] - qy, z[k][i]);
-                    if (score.cap) {
-#pragma unroll
-                        for (int i = 0; i < 16; ++i) z[k][i] = fmaf(score.top, score.bend(acc[i]), z[k][i]);
+                    for (int i = 0; i < 16; ++i) z[k][i] = (-2.f * score.top) * score.r(z[k][i]);
+                } else if constexpr (MODE != kPlain) {
+                    float d[16];
+                    if (MODE == kRows || penalty.on) {
+                        penalty(cell + 64, cell0, k, h, d);
                     } else {
 #pragma unroll
-                        for (int i = 0; i < 16; ++i) z[k][i] = fmaf(score.in, acc[i], z[k][i]);
+                        for (int i = 0; i < 16; ++i) d[i] = 0.f;
                     }
-                } else if (score.cap) {
+                    if (MODE == kGeneral && score.cap) {
 #pragma unroll
-                    for (int i = 0; i < 16; ++i) z[k][i] = score.top * score.bend(acc[i]);
-                } else {
+                        for (int i = 0; i < 16; ++i) z[k][i] = fmaf(score.top, score.bend(z[k][i]), d[i]);
+                    } else {
 #pragma unroll
-                    for (int i = 0; i < 16; ++i) z[k][i] = score.in * acc[i];
+                        for (int i = 0; i < 16; ++i) z[k][i] = fmaf(score.in, z[k][i], d[i]);
+                    }
                 }
-                if (live != kAll) {
+            }
+            if (live != kAll) {
+#pragma unroll
+                for (int k = 0; k < kBlocks; ++k) {
                     const unsigned bits = (unsigned)(live >> (32 * k)) >> M::cell(0, h);
 #pragma unroll
                     for (int i = 0; i < 16; ++i)
                         z[k][i] = bits & (1u << M::cell(i, 0)) ? z[k][i] : -__builtin_inff();
                 }
-#pragma unroll
-                for (int i = 0; i < 16; ++i) top = fmaxf(top, z[k][i]);
             }
-            top = fmaxf(top, __shfl_xor(top, 32));
-            if (__any(top > m + kSlack)) {
-                const float m_new = fmaxf(m, top);
-                const float fix = exp2_(m - (m_new == -__builtin_inff() ? 0.f : m_new));
-                m = m_new;
-                l *= fix;
+            if constexpr (MODE == kCapped) {
+                m = score.top;
+            } else {
+                float top = -__builtin_inff();
 #pragma unroll
-                for (int c = 0; c < NC / 32; ++c)
+                for (int k = 0; k < kBlocks; ++k)
 #pragma unroll
-                    for (int i = 0; i < 16; ++i) o[c][i] *= fix;
+                    for (int i = 0; i < 16; ++i) top = fmaxf(top, z[k][i]);
+                if (MODE == kPlain) top *= score.in;
+                top = fmaxf(top, __shfl_xor(top, 32));
+                if (__any(top > m + kSlack)) {
+                    const float m_new = fmaxf(m, top);
+                    const float fix = exp2_(m - (m_new == -__builtin_inff() ? 0.f : m_new));
+                    m = m_new;
+                    l *= fix;
+#pragma unroll
+                    for (int c = 0; c < NC / 32; ++c)
+#pragma unroll
+                        for (int i = 0; i < 16; ++i) o[c][i] *= fix;
+                }
             }
             const float m_use = m == -__builtin_inff() ? 0.f : m;
+            float sum[2] = {0.f, 0.f};
 #pragma unroll
             for (int k = 0; k < kBlocks; ++k) {
                 float w[16];
 #pragma unroll
                 for (int i = 0; i < 16; ++i) {
-                    w[i] = exp2_(z[k][i] - m_use);
-                    l += w[i];
+                    w[i] = exp2_(MODE == kCapped  ? z[k][i]
+                                 : MODE == kPlain ? fmaf(score.in, z[k][i], -m_use)
+                                                  : z[k][i] - m_use);
+                    sum[i & 1] += w[i];
                     if constexpr (kScaled) w[i] *= ks[k][i];
                 }
                 // weights are rounded to the maps' type for the second product, the sum l is not
                 M::second(vtile + p.c0 * kRowBytes, addr, k, M::weights(w), o);
             }
+            l += sum[0] + sum[1];
         }
         if constexpr (kAheadHere) {
-            if (t + 1 < t1) live = feed.put(lds + ((t + 1 - t0) & 1) * stage);
+            if (t + 1 < t1) {
+                live = feed.put(lds + ((t + 1 - t0) & 1) * stage);
+                cell0 = (int)feed.at.cell0;
+            }
             __syncthreads();
         }
     }
@@ -314,17 +338,18 @@ __global__ __launch_bounds__(64 * WQ, (DP <= 128 && std::is_same_v<SRC, BF16>) ?
 }
 
 // Joins the partial results of a split call: M = max m_s, out = sum_s 2^(m_s - M) o_s / sum_s 2^(m_s - M) l_s.
+// A block joins QB queries; their parts' weights lie in LDS.
 constexpr int kMaxSplits = 512;
-template <typename T>
+template <typename T, int QB>
 __global__ __launch_bounds__(256) void soft_join_kernel(const Params p, int channels_per_block) {
-    __shared__ float w[kMaxSplits][8], ls[kMaxSplits][8];
-    // 8 queries x 32 channel lanes
-    const int qi = threadIdx.x & 7, g = threadIdx.x >> 3;
+    constexpr int kMost = QB == 8 ? kMaxSplits : kMaxSplits / 8, kLanes = 256 / QB;
+    __shared__ float w[kMost][QB], ls[kMost][QB];
+    const int qi = threadIdx.x % QB, g = threadIdx.x / QB;
     const int bh = blockIdx.y;
-    const int64_t q = (int64_t)blockIdx.x * 8 + qi;
+    const int64_t q = (int64_t)blockIdx.x * QB + qi;
     const bool in = q < p.nq;
     const int64_t bhn = (int64_t)p.B * p.heads;
-    for (int s = g; s < p.splits; s += 32) {
+    for (int s = g; s < p.splits; s += kLanes) {
         const float2 ml = in ? *reinterpret_cast<const float2 *>(p.part_ml + ((s * bhn + bh) * p.nq + q) * 2)
                              : make_float2(-__builtin_inff(), 0.f);
         w[s][qi] = ml.x;
@@ -335,7 +360,7 @@ __global__ __launch_bounds__(256) void soft_join_kernel(const Params p, int chan
     for (int s = 0; s < p.splits; ++s) top = fmaxf(top, w[s][qi]);
     __syncthreads();
     if (top == -__builtin_inff()) top = 0.f;                   // no part has a cell, or all scores are NaN
-    for (int s = g; s < p.splits; s += 32) w[s][qi] = exp2_(w[s][qi] - top);
+    for (int s = g; s < p.splits; s += kLanes) w[s][qi] = exp2_(w[s][qi] - top);
     __syncthreads();
     float l = 0.f;
     for (int s = 0; s < p.splits; ++s) l = fmaf(w[s][qi], ls[s][qi], l);
@@ -343,7 +368,7 @@ __global__ __launch_bounds__(256) void soft_join_kernel(const Params p, int chan
     const bool some = l != 0.f;
     const float inv = some ? 1.f / l : 0.f;
     const int c1 = min(p.Dv, ((int)blockIdx.z + 1) * channels_per_block);
-    for (int c = (int)blockIdx.z * channels_per_block + g; c < c1; c += 32) {
+    for (int c = (int)blockIdx.z * channels_per_block + g; c < c1; c += kLanes) {
         float v = 0.f;
         const float *src = p.part_o + ((int64_t)bh * p.Dv + c) * p.nq + q;
         const int64_t step = bhn * p.Dv * p.nq;

@@ -5,26 +5,29 @@
 
 namespace ispa_soft {
 
-template <typename T, typename SRC, int DP, int WQ>
+template <typename T, typename SRC, int DP, int WQ, int MODE>
 int forward_one(Params p, hipStream_t stream) {
     static unsigned long long lds_allowed = 0;
     const int lds = kBuffers<T, SRC, DP, WQ> * stage_bytes<DP>(p.shared);
     const unsigned grid = (unsigned)((int64_t)p.B * p.heads * p.splits * p.blocks);
     constexpr int NC = DP == 256 && std::is_same_v<T, F32> ? 128 : DP;
     for (p.c0 = 0; p.c0 < p.Dv; p.c0 += NC)
-        if (int rc = launch(soft_forward_kernel<T, SRC, DP, WQ, NC>, p, grid, 64 * WQ, lds, &lds_allowed, "soft_forward_kernel",
+        if (int rc = launch(soft_forward_kernel<T, SRC, DP, WQ, NC, MODE>, p, grid, 64 * WQ, lds, &lds_allowed, "soft_forward_kernel",
                             stream))
             return rc;
     if (p.splits == 1) return ISPA_OK;
-    const int per = 32;                                   // channels of a join block
-    const dim3 join((unsigned)((p.nq + 7) / 8), (unsigned)(p.B * p.heads), (unsigned)((p.Dv + per - 1) / per));
-    soft_join_kernel<T><<<join, 256, 0, stream>>>(p, per);
+    // 32 queries a block read their parts in 128-byte runs; few queries with many parts take blocks of 8
+    const int qb = p.nq <= 8 || p.splits > kMaxSplits / 8 ? 8 : 32, per = 32;       // per: channels of a block
+    const dim3 join((unsigned)((p.nq + qb - 1) / qb), (unsigned)(p.B * p.heads), (unsigned)((p.Dv + per - 1) / per));
+    if (qb == 8) soft_join_kernel<T, 8><<<join, 256, 0, stream>>>(p, per);
+    else soft_join_kernel<T, 32><<<join, 256, 0, stream>>>(p, per);
     return ispa::check_launch("soft_join_kernel");
 }
 
 template <typename T, typename SRC, int DP>
 int forward_waves(const Params &p, int waves, hipStream_t stream) {
-    return waves == 1 ? forward_one<T, SRC, DP, 1>(p, stream) : forward_one<T, SRC, DP, 4>(p, stream);
+    if (waves == 1) return forward_one<T, SRC, DP, 1, kGeneral>(p, stream);
+    return with_mode<T, DP>(p, true, [&](auto mode) { return forward_one<T, SRC, DP, 4, decltype(mode)::value>(p, stream); });
 }
 
 template <typename T, typename SRC>

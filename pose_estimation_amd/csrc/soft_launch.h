@@ -1,5 +1,7 @@
 // Host side of the soft-correspondence kernels: how a call is cut into workgroups, and the launchers per arithmetic.
 #pragma once
+#include <cstdint>
+
 #include "soft_tile.h"
 
 namespace ispa_soft {
@@ -19,29 +21,51 @@ struct Plan {
 
 constexpr int kMaxSplitCount = 512;
 
-inline Plan make_plan(int64_t owned, int64_t groups, int64_t tiles) {
+// resident: workgroups of four waves that a compute unit holds.  Up to 64 owned cells, workgroups of one wave: all the
+// parallelism lies in the streamed tiles, and four waves would stage for one.  The tiles are split so that the rounds of
+// workgroups that the 256 compute units work off, each as long as its tiles and about two more to start, are shortest; a
+// split costs its workgroup about four tiles more, for writing and joining its part.
+inline Plan make_plan(int64_t owned, int64_t groups, int64_t tiles, int resident) {
     Plan plan;
     plan.waves = owned <= 64 ? 1 : 4;
     plan.blocks = (int)((owned + 32 * plan.waves - 1) / (32 * plan.waves));
-    const int64_t base = groups * plan.blocks, want = plan.waves == 1 ? 2048 : 512;
-    int64_t s = base >= want / 2 ? 1 : (want + base - 1) / base;
-    if (s > tiles / 2) s = tiles / 2;
-    if (s > kMaxSplitCount) s = kMaxSplitCount;
-    plan.splits = s < 1 ? 1 : (int)s;
+    plan.splits = 1;
+    const int64_t base = groups * plan.blocks, room = 256 * (plan.waves == 1 ? 4 : resident);
+    int64_t best = INT64_MAX;
+    for (int64_t s = 1; s <= tiles && s <= kMaxSplitCount && (s == 1 || base * (s - 1) < 4 * room); ++s) {
+        const int64_t cost = (base * s + room - 1) / room * ((tiles + s - 1) / s + (s > 1 ? 6 : 2));
+        if (cost < best) {
+            best = cost;
+            plan.splits = (int)s;
+        }
+    }
     return plan;
 }
 
-// Whether the gradients of the reference and value maps are summed from float32 parts: where the queries are split, and
-// where two launches form the two uses of a shared map of more than 128 channels (one rounding of their sum).
-inline bool dkv_in_parts(int d, int dv, bool shared, int splits) {
-    return splits > 1 || (shared && padded_channels(d, dv) == 256);
-}
+// Whether the gradients of the reference and value maps take a launch each.
+constexpr bool dkv_two_launches(bool f32, int padded, int waves) { return padded == 256 || (padded == 128 && f32 == (waves == 1)); }
 
 // Every launcher expects p.blocks, p.splits, p.tiles and p.tiles_per_view to be set; 0 or a negative status.
 int forward_f32(const Params &p, int source, int waves, hipStream_t stream);
 int forward_bf16(const Params &p, int source, int waves, hipStream_t stream);
 int backward_f32(const Params &p, const Plan &dq, const Plan &dkv, hipStream_t stream);
 int backward_bf16(const Params &p, const Plan &dq, const Plan &dkv, hipStream_t stream);
+
+// Calls f with the mode that the kernels of four waves are built for; `grid`: the streamed cells lie on the grid.  float32
+// kernels are bound by their MFMAs and 256 channels by their registers: these have the general form, and the former the
+// plain one.
+template <typename T, int DP, typename F>
+int with_mode(const Params &p, bool grid, F f) {
+    const bool cap = p.cap > 0.f, pen = p.falloff != nullptr;
+    if constexpr (DP <= 128) {
+        if (!cap && !pen) return f(std::integral_constant<int, kPlain>{});
+        if constexpr (std::is_same_v<T, BF16>) {
+            if (cap && !pen && p.cap <= 32.f) return f(std::integral_constant<int, kCapped>{});
+            if (!cap && grid && p.W % Math<T, DP>::kCells == 0) return f(std::integral_constant<int, kRows>{});
+        }
+    }
+    return f(std::integral_constant<int, kGeneral>{});
+}
 
 template <typename K>
 int launch(K kernel, const Params &p, unsigned grid, int threads, int lds, unsigned long long *lds_allowed, const char *what,

@@ -63,27 +63,38 @@ int stream_map(Stream *s, int dtype, const void *map, int64_t maps, int d, int64
     return ispa::check_launch("soft_pack_kernel");
 }
 
-Plan forward_plan(int dtype, int B, int heads, int64_t nq, int V, int64_t cells) {
+// Workgroups of four waves a compute unit holds: two where a lane's registers allow it.
+int resident(int dtype, int D, int Dv) { return padded_channels(D, Dv) <= (dtype == ISPA_F32 ? 64 : 128) ? 2 : 1; }
+
+Plan forward_plan(int dtype, int B, int heads, int D, int Dv, int64_t nq, int V, int64_t cells) {
     const int64_t per = (cells + tile_cells(dtype) - 1) / tile_cells(dtype);
-    return make_plan(nq, (int64_t)B * heads, per * V);
+    return make_plan(nq, (int64_t)B * heads, per * V, resident(dtype, D, Dv));
 }
 
 size_t forward_bytes(const Plan &plan, int B, int heads, int Dv, int64_t nq) {
     return plan.splits == 1 ? 0 : (size_t)plan.splits * B * heads * nq * (Dv + 2) * sizeof(float);
 }
 
-void backward_plans(int dtype, int B, int heads, int64_t nq, int64_t cells, Plan *dq, Plan *dkv) {
+void backward_plans(int dtype, int B, int heads, int D, int Dv, int64_t nq, int64_t cells, Plan *dq, Plan *dkv) {
     const int64_t r = tile_cells(dtype);
-    *dq = make_plan(nq, (int64_t)B * heads, (cells + r - 1) / r);
-    *dkv = make_plan(cells, (int64_t)B * heads, (nq + r - 1) / r);
+    const int wgs = dtype == ISPA_F32 ? 1 : resident(dtype, D, Dv);
+    *dq = make_plan(nq, (int64_t)B * heads, (cells + r - 1) / r, wgs);
+    *dkv = make_plan(cells, (int64_t)B * heads, (nq + r - 1) / r, wgs);
 }
 
+
+// Channels of float32 parts per cell: every split's, or what the first of two launches leaves for the second (a map that is
+// reference and value; the size does not say which, so any map of equal channels).
+size_t dkv_parts(int dtype, const Plan &dkv, int D, int Dv) {
+    if (dkv.splits > 1) return (size_t)dkv.splits * (D + Dv);
+    return D == Dv && dkv_two_launches(dtype == ISPA_F32, padded_channels(D, Dv), dkv.waves) ? Dv : 0;
+}
 
 size_t backward_bytes(int dtype, const Plan &dq, const Plan &dkv, int B, int heads, int D, int Dv, int64_t nq, int64_t cells) {
     const size_t bh = (size_t)B * heads;
     const size_t copied = copies(dtype, bh, D, cells).bytes + copies(dtype, bh, Dv, cells).bytes + copies(dtype, bh, D, nq).bytes +
                           copies(dtype, bh, Dv, nq).bytes;
-    const size_t a = dq.splits > 1 ? dq.splits * bh * D * nq : 0, k = dkv_in_parts(D, Dv, D == Dv, dkv.splits) ? dkv.splits * bh * (D + Dv) * cells : 0;
+    const size_t a = dq.splits > 1 ? dq.splits * bh * D * nq : 0, k = dkv_parts(dtype, dkv, D, Dv) * bh * cells;
     return copied + align256(bh * nq * sizeof(float)) + (a > k ? a : k) * sizeof(float);
 }
 
@@ -98,7 +109,7 @@ size_t forward_copies(int dtype, int B, int heads, int D, int Dv, int64_t cells,
 }
 
 int run_forward(Params &p, int dtype, int source, void *workspace, size_t workspace_bytes, hipStream_t stream) {
-    const Plan plan = forward_plan(dtype, p.B, p.heads, p.nq, p.V, p.cells);
+    const Plan plan = forward_plan(dtype, p.B, p.heads, p.D, p.Dv, p.nq, p.V, p.cells);
     const bool maps = source == kSourceMap;
     const size_t copied = maps ? forward_copies(dtype, p.B, p.heads, p.D, p.Dv, p.cells, p.shared) : 0;
     const size_t need = copied + forward_bytes(plan, p.B, p.heads, p.Dv, p.nq);
@@ -124,7 +135,7 @@ int run_forward(Params &p, int dtype, int source, void *workspace, size_t worksp
 extern "C" size_t ispa_soft_match_workspace_bytes(int dtype, int B, int heads, int D, int Dv, int64_t nq, int views,
                                                   int64_t cells) {
     if (!sizes_ok(dtype, B, heads, D, Dv, nq, views, cells) || B == 0 || nq == 0) return 0;
-    return forward_copies(dtype, B, heads, D, Dv, cells, false) + forward_bytes(forward_plan(dtype, B, heads, nq, views, cells), B,
+    return forward_copies(dtype, B, heads, D, Dv, cells, false) + forward_bytes(forward_plan(dtype, B, heads, D, Dv, nq, views, cells), B,
                                                                                 heads, Dv, nq);
 }
 
@@ -203,7 +214,7 @@ extern "C" size_t ispa_soft_match_backward_workspace_bytes(int dtype, int B, int
                                                            int64_t cells) {
     if (!sizes_ok(dtype, B, heads, D, Dv, nq, 1, cells) || B == 0) return 0;
     Plan dq, dkv;
-    backward_plans(dtype, B, heads, nq, cells, &dq, &dkv);
+    backward_plans(dtype, B, heads, D, Dv, nq, cells, &dq, &dkv);
     return backward_bytes(dtype, dq, dkv, B, heads, D, Dv, nq, cells);
 }
 
@@ -220,7 +231,7 @@ extern "C" int ispa_soft_match_backward(const void *q, const void *r, const void
     ISPA_REQUIRE((v == nullptr) == (dv == nullptr), "a value map and its gradient come together");
     ISPA_REQUIRE(v != nullptr || D == Dv, "without a value map the reference map is the value (%d != %d channels)", D, Dv);
     Plan pq, pkv;
-    backward_plans(dtype, B, heads, nq, cells, &pq, &pkv);
+    backward_plans(dtype, B, heads, D, Dv, nq, cells, &pq, &pkv);
     const size_t need = backward_bytes(dtype, pq, pkv, B, heads, D, Dv, nq, cells);
     if (workspace_bytes < need || (need > 0 && workspace == nullptr))
         return ispa::fail(ISPA_EWORKSPACE, "workspace of %zu bytes, %zu needed", workspace_bytes, need);
@@ -262,7 +273,7 @@ extern "C" int ispa_soft_match_backward(const void *q, const void *r, const void
     float *delta = (float *)at;
     p.delta = delta;
     p.part_a = (float *)(at + align256(bh * nq * sizeof(float)));
-    p.part_b = p.part_a + (size_t)pkv.splits * bh * D * cells;
+    p.part_b = p.part_a + (pkv.splits > 1 ? (size_t)pkv.splits * bh * D * cells : 0);
     if (nq > 0) {
         const unsigned grid = (unsigned)((nq + 63) / 64 * bh);
         if (dtype == ISPA_F32) soft_delta_kernel<F32><<<grid, 256, 0, s>>>(p, out32, d_lse, delta);

@@ -107,6 +107,11 @@ struct Math<BF16, DP> {
             o.f[s] = __builtin_bit_cast(bf16x8, w);
         }
     }
+    __device__ static void negate(Owned &o) {
+#pragma unroll
+        for (int s = 0; s < DP / 16; ++s)
+            o.f[s] = __builtin_bit_cast(bf16x8, __builtin_bit_cast(u32x4, o.f[s]) ^ 0x80008000u);
+    }
     // The transposed 8-byte read hands lane i of a 16-lane group element i of the group's four 8-byte pieces, for
     // 4 channel rows.  The pieces are addressed so that accumulator row 16 s + 8 e + 4 h + j belongs to streamed cell
     // 16 s + 8 h + 4 e + j: a lane then holds 8 successive cells per 16-cell step, what one plain 16-byte read of the
@@ -128,14 +133,13 @@ struct Math<BF16, DP> {
         a.nat = row * kRowBytes + ((h ^ swz(row)) << 4);
         return a;
     }
-    // Scores of streamed cells 32 b .. 32 b + 31 of a tile.
-    __device__ static f32x16 first(const char *tile, const Addr &a, int b, const Owned &o) {
+    // Products of the owned cells with streamed cells 32 b .. 32 b + 31 of a tile, b = b0 .. b0 + N - 1.  The A fragments are
+    // read kAhead steps before their MFMAs.
+    template <int N>
+    __device__ static void first(const char *tile, const Addr &a, int b0, const Owned &o, f32x16 (&acc)[N]) {
         typedef __attribute__((address_space(3))) s16x4 *lds_ptr;
-        f32x16 acc;
-#pragma unroll
-        for (int i = 0; i < 16; ++i) acc[i] = 0.f;
-#pragma unroll
-        for (int s = 0; s < DP / 16; ++s) {
+        constexpr int kSteps = DP / 16, kAhead = DP == 256 ? 1 : 2;
+        auto frag = [&](int n, int s) {
             union {
                 s16x4 q[2];
                 bf16x8 v;
@@ -143,11 +147,27 @@ struct Math<BF16, DP> {
 #pragma unroll
             for (int x = 0; x < 2; ++x)
                 u.q[x] = __builtin_amdgcn_ds_read_tr16_b64_v4i16(
-                    (lds_ptr)(tile + (a.tr[x] ^ (b << 6)) + s * 16 * kRowBytes));
-            acc = __builtin_amdgcn_mfma_f32_32x32x16_bf16(u.v, o.f[s], acc, 0, 0, 0);
-            if (DP == 256 && s % 4 == 3) __builtin_amdgcn_sched_barrier(0);    // bounds the reads in flight: registers
+                    (lds_ptr)(tile + (a.tr[x] ^ ((b0 + n) << 6)) + s * 16 * kRowBytes));
+            return u.v;
+        };
+        bf16x8 f[kAhead + 1][N];
+#pragma unroll
+        for (int s = 0; s < kAhead && s < kSteps; ++s)
+#pragma unroll
+            for (int n = 0; n < N; ++n) f[s][n] = frag(n, s);
+#pragma unroll
+        for (int n = 0; n < N; ++n)
+#pragma unroll
+            for (int i = 0; i < 16; ++i) acc[n][i] = 0.f;
+#pragma unroll
+        for (int s = 0; s < kSteps; ++s) {
+#pragma unroll
+            for (int n = 0; n < N; ++n) {
+                if (s + kAhead < kSteps) f[(s + kAhead) % (kAhead + 1)][n] = frag(n, s + kAhead);
+                acc[n] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(f[s % (kAhead + 1)][n], o.f[s], acc[n], 0, 0, 0);
+            }
+            __builtin_amdgcn_sched_barrier(0);
         }
-        return acc;
     }
     struct Weights {
         bf16x8 f[2];
@@ -172,7 +192,7 @@ struct Math<BF16, DP> {
             for (int s = 0; s < 2; ++s) {
                 const bf16x8 v = *reinterpret_cast<const bf16x8 *>(tile + (a.nat ^ ((4 * b + 2 * s) << 4)) + c * 32 * kRowBytes);
                 out[c] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(v, w.f[s], out[c], 0, 0, 0);
-                if (DP == 256 && s == 1 && c % 2 == 1) __builtin_amdgcn_sched_barrier(0);
+                if (DP == 256 && s == 1 && c % 2 == 1) __builtin_amdgcn_sched_barrier(0);   // bounds the reads in flight
             }
     }
     // Streamed cell (inside its 32) of accumulator register i, i = 0 .. 15.
@@ -207,6 +227,10 @@ struct Math<F32, DP> {
             if (DP == 256 && s % 8 == 7) __builtin_amdgcn_sched_barrier(0);
         }
     }
+    __device__ static void negate(Owned &o) {
+#pragma unroll
+        for (int s = 0; s < DP / 2; ++s) o.f[s] = -o.f[s];
+    }
     struct Addr {
         int one[8];          // row 2 s + h for s = 0 .. 7 (swz repeats every 16 rows)
         int nat;
@@ -222,17 +246,16 @@ struct Math<F32, DP> {
         a.nat = cell * kRowBytes + ((h ^ swz(cell)) << 4);
         return a;
     }
-    __device__ static f32x16 first(const char *tile, const Addr &a, int, const Owned &o) {
-        f32x16 acc;
+    template <int N>
+    __device__ static void first(const char *tile, const Addr &a, int, const Owned &o, f32x16 (&acc)[N]) {
 #pragma unroll
-        for (int i = 0; i < 16; ++i) acc[i] = 0.f;
+        for (int i = 0; i < 16; ++i) acc[0][i] = 0.f;
 #pragma unroll
         for (int s = 0; s < DP / 2; ++s) {
             const float x = *reinterpret_cast<const float *>(tile + a.one[s & 7] + (s >> 3) * 16 * kRowBytes);
-            acc = __builtin_amdgcn_mfma_f32_32x32x2f32(x, o.f[s], acc, 0, 0, 0);
+            acc[0] = __builtin_amdgcn_mfma_f32_32x32x2f32(x, o.f[s], acc[0], 0, 0, 0);
             if (DP == 256 && s % 4 == 3) __builtin_amdgcn_sched_barrier(0);
         }
-        return acc;
     }
     struct Weights {
         float f[16];
@@ -287,7 +310,7 @@ struct Loader {
     static constexpr int kPer = DP * 8 / NT;
     typedef typename SRC::elem elem;
     typedef std::conditional_t<!kCodes, u32x4, std::conditional_t<kNarrow, u32x2, unsigned>> raw;
-    static constexpr bool kAhead = kPer * (int)sizeof(raw) <= (DP == 256 ? 64 : 128);
+    static constexpr bool kAhead = kPer * (int)sizeof(raw) <= (DP == 256 ? 32 : 128);
     static constexpr int kBatch = kAhead ? kPer : DP == 256 ? (kCodes || NT == 64 ? 1 : 2) : kPer < 8 ? kPer : 8;
     static constexpr int kLoop = kAhead ? kPer / kBatch : 1;
     static_assert(NT == 64 || NT % 128 == 0, "");
@@ -518,32 +541,81 @@ struct Params {
     float scale, cap;
 };
 
-// The scores of one item and head, in units of log2: z = fn(x) - falloff d^2 with x = scale (q . r).
+// What a kernel is built for: each sort of score has its own straight code, general ones branch at run time.
+enum Mode {
+    kPlain = 0,       // no cap, no falloff
+    kCapped = 1,      // bfloat16, a cap of at most 32, no falloff
+    kRows = 2,        // no cap, falloff on a grid whose rows the streamed groups of cells do not leave
+    kGeneral = 3
+};
+
+// The scores of one item and head, in units of log2: z = bent - falloff d^2 with bent = in acc, or top tanh(in acc).
 template <typename T>
 struct Score {
+    // tanh(y) = 1 - 2 r, r = 1 / (exp(2 y) + 1), whose absolute error of 2e-7 is far below what the inputs of the bfloat16
+    // kernels leave.  float32 keeps the relative error near 1e-7 too: below 0.6 the odd polynomial y + y^3 c(y^2), c
+    // fitted to (tanh(y) / y - 1) / y^2 on [0, 0.36] by weighted least squares.
     static constexpr bool kExact = std::is_same_v<T, F32>;
-    float in, top;                  // z = in acc, or top tanh(in acc)
-    float fall;
+    float in, top, fall, in2;
     bool cap;
     __device__ Score(const Params &p, int head) {
         cap = p.cap > 0.f;
         in = cap ? p.scale / p.cap : p.scale * kLog2e;
+        in2 = in * (2.f * kLog2e);
         top = p.cap * kLog2e;
         fall = p.falloff ? p.falloff[head] * kLog2e : 0.f;
     }
-    // tanh(x / cap) = 1 - 2 / (exp(2 x / cap) + 1), whose absolute error of 2e-7 is far below what the inputs of the
-    // bfloat16 kernels leave.  float32 keeps the relative error near 1e-7 too: below 0.6 the odd polynomial
-    // y + y^3 r(y^2), r fitted to (tanh(y) / y - 1) / y^2 on [0, 0.36] by weighted least squares.
+    __device__ float r(float acc) const { return __builtin_amdgcn_rcpf(__builtin_amdgcn_exp2f(acc * in2) + 1.f); }
     __device__ float bend(float acc) const {
-        const float y = in * acc;
-        const float far = fmaf(-2.f, __builtin_amdgcn_rcpf(__builtin_amdgcn_exp2f(y * (2.f * kLog2e)) + 1.f), 1.f);
+        const float far = fmaf(-2.f, r(acc), 1.f);
         if constexpr (!kExact) return far;
-        const float u = y * y;
-        float r = fmaf(u, -0.00589394523f, 0.020794617f);
-        r = fmaf(u, r, -0.0537832938f);
-        r = fmaf(u, r, 0.133319154f);
-        r = fmaf(u, r, -0.333332986f);
-        return fabsf(y) < 0.6f ? fmaf(y * u, r, y) : far;
+        const float y = in * acc, u = y * y;
+        float c = fmaf(u, -0.00589394523f, 0.020794617f);
+        c = fmaf(u, c, -0.0537832938f);
+        c = fmaf(u, c, 0.133319154f);
+        c = fmaf(u, c, -0.333332986f);
+        return fabsf(y) < 0.6f ? fmaf(y * u, c, y) : far;
+    }
+};
+
+// falloff d^2 of one owned cell at (x, y) to the 16 streamed cells of a lane, negative.  Streamed cells that lie on the grid
+// (`grid`) come in groups of kCells successive ones; where the width is a multiple of that, a group stays in one row
+// and d^2 grows along it by a quadratic: two operations a cell.  Else the places are read from LDS (`cell`: 64 x, 64 y).
+template <typename M, int MODE>
+struct Penalty {
+    bool on, rows;
+    float fall, x, y, width, per_width;
+    __device__ Penalty(const Params &p, float fall_, float x_, float y_, bool grid) {
+        on = MODE == kRows || (MODE == kGeneral && p.falloff != nullptr);
+        rows = MODE == kRows || (grid && p.W % M::kCells == 0);
+        fall = fall_;
+        x = x_;
+        y = y_;
+        width = (float)p.W;
+        per_width = 1.f / width;
+    }
+    __device__ bool wants_places() const { return on && !rows; }
+    __device__ void operator()(const float *cell, int cell0, int k, int h, float (&z)[16]) const {
+        if (rows) {
+#pragma unroll
+            for (int g = 0; g < 16; g += M::kCells) {
+                // cells are fewer than 2^22: c + 0.5 is exact and the quotient's error cannot reach the next integer
+                const float c = (float)(cell0 + 32 * k + M::cell(g, h));
+                const float cy = floorf((c + 0.5f) * per_width);
+                const float dx = fmaf(-width, cy, c) - x, dy = cy - y;
+                const float base = -fall * fmaf(dx, dx, dy * dy), step = -2.f * fall * dx;
+#pragma unroll
+                for (int j = 0; j < M::kCells; ++j) z[g + j] = fmaf((float)j, step, fmaf((float)(-j * j), fall, base));
+            }
+        } else {
+            M::per_cell(cell, k, h, z);
+#pragma unroll
+            for (int i = 0; i < 16; ++i) z[i] = (z[i] - x) * (z[i] - x);
+            float cy[16];
+            M::per_cell(cell + 64, k, h, cy);
+#pragma unroll
+            for (int i = 0; i < 16; ++i) z[i] = -fall * fmaf(cy[i] - y, cy[i] - y, z[i]);
+        }
     }
 };
 
