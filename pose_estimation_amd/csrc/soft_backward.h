@@ -100,6 +100,7 @@ __global__ __launch_bounds__(64 * WQ, (two_waves<T, DP, WQ>) ? 2 : 1) void soft_
     constexpr int kUnroll = DP == 256 ? 1 : kBlocks;           // registers
     constexpr uint64_t kAll = M::kRows == 64 ? ~0ull : 0xffffffffull;
     extern __shared__ __attribute__((aligned(16))) char lds[];
+    out_of_step();
     const int v_at = p.shared ? 0 : DP * kRowBytes, cell_at = v_at + DP * kRowBytes;
     const int stage = cell_at + 3 * 64 * (int)sizeof(float);
 
@@ -136,7 +137,8 @@ __global__ __launch_bounds__(64 * WQ, (two_waves<T, DP, WQ>) ? 2 : 1) void soft_
         for (int i = 0; i < 16; ++i) g[c][i] = 0.f;
 
     Feed<M, T, DP, WQ> feed(p, b, head, lds, stage);
-    const Penalty<M, MODE> penalty(p, score.fall, qx, qy, true);
+    const Penalty<M, MODE, false> penalty(p, score.fall, qx, qy, true);
+    const f32x16 from = penalty.from(score.in);
     uint64_t live = 0;
     int cell0 = 0;
     if (t0 < t1) {
@@ -155,13 +157,11 @@ __global__ __launch_bounds__(64 * WQ, (two_waves<T, DP, WQ>) ? 2 : 1) void soft_
             for (int k = 0; k < kBlocks; ++k) {
                 if (DP == 256) __builtin_amdgcn_sched_barrier(0);
                 f32x16 acc[1], dp[1];
-                M::first(ktile, addr, k, qf, acc);
+                M::first(ktile, addr, k, qf, acc, from);
                 M::first(vtile, addr, k, of, dp);
                 float w[16], dl[16];
                 if (MODE == kRows || penalty.on) {
-                    penalty(cell + 64, cell0, k, h, w);
-#pragma unroll
-                    for (int i = 0; i < 16; ++i) w[i] += minus;
+                    penalty(cell + 64, cell0, k, h, minus, w);
                 } else {
 #pragma unroll
                     for (int i = 0; i < 16; ++i) w[i] = minus;
@@ -170,6 +170,7 @@ __global__ __launch_bounds__(64 * WQ, (two_waves<T, DP, WQ>) ? 2 : 1) void soft_
                 for (int i = 0; i < 16; ++i) dl[i] = delta;
                 weights<T, MODE>(score, acc[0], w, dp[0], dl);
                 if (live != kAll) {
+                    stay_branch();
                     const unsigned bits = (unsigned)(live >> (32 * k)) >> M::cell(0, h);
 #pragma unroll
                     for (int i = 0; i < 16; ++i) w[i] = bits & (1u << M::cell(i, 0)) ? w[i] : 0.f;
@@ -185,24 +186,18 @@ __global__ __launch_bounds__(64 * WQ, (two_waves<T, DP, WQ>) ? 2 : 1) void soft_
     }
     if (q >= p.nq) return;
     if (p.parts) {
-        float *dst = p.part_a + ((int64_t)split * p.B * p.heads + bh) * p.D * p.nq + q;
 #pragma unroll
         for (int c = 0; c < NC / 32; ++c)
 #pragma unroll
-            for (int i = 0; i < 16; ++i) {
-                const int ch = p.c0 + 32 * c + out_channel(i, h);
-                if (ch < p.D) dst[ch * p.nq] = q_ok ? g[c][i] : 0.f;
-            }
+            for (int i = 0; i < 16; ++i) g[c][i] = q_ok ? g[c][i] : 0.f;
+        store_columns<NC>(p.part_a + ((int64_t)split * p.B * p.heads + bh) * p.D * p.nq, p.nq, q, h, p.c0, p.D, g);
         return;
     }
-    typename T::elem *dst = (typename T::elem *)p.dq + (int64_t)bh * p.D * p.nq + q;
 #pragma unroll
     for (int c = 0; c < NC / 32; ++c)
 #pragma unroll
-        for (int i = 0; i < 16; ++i) {
-            const int ch = p.c0 + 32 * c + out_channel(i, h);
-            if (ch < p.D) store_float(dst + ch * p.nq, q_ok ? g[c][i] * p.scale : 0.f);
-        }
+        for (int i = 0; i < 16; ++i) g[c][i] = q_ok ? g[c][i] * p.scale : 0.f;
+    store_columns<NC>((typename T::elem *)p.dq + (int64_t)bh * p.D * p.nq, p.nq, q, h, p.c0, p.D, g);
 }
 
 // LDS of one buffer: both tiles, and per query the log-sum, delta and the place.
@@ -220,6 +215,7 @@ __global__ __launch_bounds__(64 * WQ, (two_waves<T, DP, WQ> && (DP <= 64 || PART
     constexpr bool kDv = PART != 2, kDk = PART != 1;
     constexpr int kStage = dkv_stage_bytes<DP>;
     extern __shared__ __attribute__((aligned(16))) char lds[];
+    out_of_step();
 
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, h = lane >> 5;
     int id = die_major(blockIdx.x, gridDim.x);
@@ -253,12 +249,11 @@ __global__ __launch_bounds__(64 * WQ, (two_waves<T, DP, WQ> && (DP <= 64 || PART
         }
 
     const Penalty<M, MODE> penalty(p, score.fall, cx, cy, p.query_xy == nullptr);
+    const f32x16 from = penalty.from(score.in);
     typedef Direct<M, DP, WQ> Copy;
     Copy cq, co;
-    cq.init(p.sq.ld, p.sq.d);
-    co.init(p.so.ld, p.so.d);
-    const char *qmap = (const char *)p.sq.map + (int64_t)bh * p.sq.d * p.sq.ld * Copy::kSize;
-    const char *omap = (const char *)p.so.map + (int64_t)bh * p.so.d * p.so.ld * Copy::kSize;
+    cq.init((const char *)p.sq.map + (int64_t)bh * p.sq.d * p.sq.ld * Copy::kSize, p.sq.ld, p.sq.d);
+    co.init((const char *)p.so.map + (int64_t)bh * p.so.d * p.so.ld * Copy::kSize, p.so.ld, p.so.d);
     for (int i = 0; i < 2; ++i) {
         cq.clear_rest(lds + i * kStage);
         co.clear_rest(lds + i * kStage + DP * kRowBytes);
@@ -276,8 +271,8 @@ __global__ __launch_bounds__(64 * WQ, (two_waves<T, DP, WQ> && (DP <= 64 || PART
                 if (penalty.wants_places()) query_place(p, b, q, px, py);
             }
         }
-        cq.issue(qmap, q0, p.sq.ld, buf);
-        co.issue(omap, q0, p.so.ld, buf + DP * kRowBytes);
+        cq.issue((int)q0, (int)p.sq.ld, buf);
+        co.issue((int)q0, (int)p.so.ld, buf + DP * kRowBytes);
     };
     auto put = [&](int t, char *buf) {
         Copy::wait();
@@ -308,10 +303,10 @@ __global__ __launch_bounds__(64 * WQ, (two_waves<T, DP, WQ> && (DP <= 64 || PART
 #pragma unroll kUnroll
         for (int k = 0; k < kBlocks; ++k) {
             f32x16 acc[1];
-            M::first(qtile, addr, k, kf, acc);
+            M::first(qtile, addr, k, kf, acc, from);
             float w[16];
             if (MODE == kRows || penalty.on) {
-                penalty(xarr, t * M::kRows, k, h, w);
+                penalty(xarr, t * M::kRows, k, h, 0.f, w);
                 float minus_l[16];
                 M::per_cell(larr, k, h, minus_l);
 #pragma unroll
@@ -348,36 +343,36 @@ __global__ __launch_bounds__(64 * WQ, (two_waves<T, DP, WQ> && (DP <= 64 || PART
     }
     if (cell >= p.cells) return;
     // masked cells take no part: their columns hold zeros' products and are dropped here
-    const int64_t part = ((int64_t)split * p.B * p.heads + bh);
+    const int64_t part = (int64_t)split * p.B * p.heads + bh;
 #pragma unroll
     for (int c = 0; c < NC / 32; ++c)
 #pragma unroll
         for (int i = 0; i < 16; ++i) {
-            const int ch = p.c0 + 32 * c + out_channel(i, h);
-            float a = 0.f, v = 0.f;
-            if constexpr (kDk) a = c_ok ? gk[c][i] * p.scale : 0.f;
-            if constexpr (kDv) v = c_ok ? gv[c][i] : 0.f;
-            float *pv = p.part_b + (part * p.Dv + ch) * p.cells + cell;
-            if (p.parts) {
-                if constexpr (kDk)
-                    if (ch < p.D) p.part_a[(part * p.D + ch) * p.cells + cell] = a;
-                if constexpr (kDv)
-                    if (ch < p.Dv) *pv = v;
-                continue;
-            }
-            typename T::elem *dk = (typename T::elem *)p.dk + ((int64_t)bh * p.D + ch) * p.cells + cell;
-            if (p.shared) {                                    // the sum of both uses, rounded once
-                if (ch >= p.D) continue;
-                if constexpr (PART == 1) *pv = v;              // float32, for the launch that forms the other one
-                else if constexpr (PART == 2) store_float(dk, a + *pv);
-                else store_float(dk, a + v);
-                continue;
-            }
-            if constexpr (kDk)
-                if (ch < p.D) store_float(dk, a);
-            if constexpr (kDv)
-                if (ch < p.Dv) store_float((typename T::elem *)p.dv + ((int64_t)bh * p.Dv + ch) * p.cells + cell, v);
+            if constexpr (kDk) gk[c][i] = c_ok ? gk[c][i] * p.scale : 0.f;
+            if constexpr (kDv) gv[c][i] = c_ok ? gv[c][i] : 0.f;
         }
+    typedef typename T::elem elem;
+    float *pv = p.part_b + part * p.Dv * p.cells;
+    elem *dk = (elem *)p.dk + (int64_t)bh * p.D * p.cells, *dv = (elem *)p.dv + (int64_t)bh * p.Dv * p.cells;
+    if (p.parts) {
+        if constexpr (kDk) store_columns<NC>(p.part_a + part * p.D * p.cells, p.cells, cell, h, p.c0, p.D, gk);
+        if constexpr (kDv) store_columns<NC>(pv, p.cells, cell, h, p.c0, p.Dv, gv);
+    } else if (!p.shared) {
+        if constexpr (kDk) store_columns<NC>(dk, p.cells, cell, h, p.c0, p.D, gk);
+        if constexpr (kDv) store_columns<NC>(dv, p.cells, cell, h, p.c0, p.Dv, gv);
+    } else if constexpr (PART == 1) {                          // shared: the sum of both uses, rounded once
+        store_columns<NC>(pv, p.cells, cell, h, p.c0, p.Dv, gv);       // float32, for the launch that forms the other one
+    } else {
+#pragma unroll
+        for (int c = 0; c < NC / 32; ++c)
+#pragma unroll
+            for (int i = 0; i < 16; ++i) {
+                const int ch = p.c0 + 32 * c + out_channel(i, h);
+                if constexpr (PART == 2) gk[c][i] += ch < p.D ? pv[ch * p.cells + cell] : 0.f;
+                else gk[c][i] += gv[c][i];
+            }
+        store_columns<NC>(dk, p.cells, cell, h, p.c0, p.D, gk);
+    }
 }
 
 // out[i] = factor * sum_s a[s][i] (+ sum_s b[s][i]), in the order of s, rounded once.

@@ -11,12 +11,12 @@ struct KeyTiles {
     static constexpr bool kCodes = std::is_same_v<SRC, I8> || std::is_same_v<SRC, FP8>;
     const Params &p;
     int b, head;
-    __device__ KeyTiles(const Params &p_, int b_, int head_) : p(p_), b(b_), head(head_) {}
+    __device__ __forceinline__ KeyTiles(const Params &p_, int b_, int head_) : p(p_), b(b_), head(head_) {}
     struct At {
         int64_t map;          // which map of the batch or store; -1 = none
         int64_t cell0;
     };
-    __device__ At at(int t) const {
+    __device__ __forceinline__ At at(int t) const {
         At a;
         if constexpr (kCodes) {
             const int view = t / p.tiles_per_view;
@@ -29,16 +29,16 @@ struct KeyTiles {
         }
         return a;
     }
-    __device__ const typename SRC::elem *base(const void *maps, const At &a, int d) const {
+    __device__ __forceinline__ const typename SRC::elem *base(const void *maps, const At &a, int d) const {
         return (const typename SRC::elem *)maps + ((a.map < 0 ? 0 : a.map) * p.heads + head) * (int64_t)d * p.cells;
     }
     // this lane's cell (lane % kRows) of the tile: takes part?  its scale
-    __device__ bool live(const At &a, int lane) const {
+    __device__ __forceinline__ bool live(const At &a, int lane) const {
         const int64_t c = a.cell0 + (lane & (M::kRows - 1));
         if (a.map < 0 || c >= p.cells) return false;
         return p.mask == nullptr || p.mask[a.map * p.cells + c] != 0;
     }
-    __device__ float scale(const At &a, int lane, bool ok) const {
+    __device__ __forceinline__ float scale(const At &a, int lane, bool ok) const {
         if constexpr (kCodes) return ok ? p.kscale[a.map * p.cells + a.cell0 + (lane & (M::kRows - 1))] : 0.f;
         return 0.f;
     }
@@ -80,29 +80,26 @@ struct Feed {
     const Keys keys;
     std::conditional_t<kCodes, L, None> codes;
     std::conditional_t<kCodes, None, D> dk, dv;
-    const char *kmap, *vmap;
     typename Keys::At at{};
     bool ok = false;
     float sc = 0.f;
     int v_at, cell_at;
-    __device__ Feed(const Params &p_, int b, int head, char *lds, int stage) : p(p_), keys(p_, b, head) {
+    __device__ __forceinline__ Feed(const Params &p_, int b, int head, char *lds, int stage) : p(p_), keys(p_, b, head) {
         v_at = p.shared ? 0 : DP * kRowBytes;
         cell_at = v_at + DP * kRowBytes;
         if constexpr (!kCodes) {
             const int64_t bh = (int64_t)b * p.heads + head;
-            dk.init(p.sk.ld, p.sk.d);
-            kmap = (const char *)p.sk.map + bh * p.sk.d * p.sk.ld * D::kSize;
+            dk.init((const char *)p.sk.map + bh * p.sk.d * p.sk.ld * D::kSize, p.sk.ld, p.sk.d);
             dk.clear_rest(lds);
             dk.clear_rest(lds + stage);
             if (!p.shared) {
-                dv.init(p.sv.ld, p.sv.d);
-                vmap = (const char *)p.sv.map + bh * p.sv.d * p.sv.ld * D::kSize;
+                dv.init((const char *)p.sv.map + bh * p.sv.d * p.sv.ld * D::kSize, p.sv.ld, p.sv.d);
                 dv.clear_rest(lds + v_at);
                 dv.clear_rest(lds + stage + v_at);
             }
         }
     }
-    __device__ void fetch(int t, char *buf) {
+    __device__ __forceinline__ void fetch(int t, char *buf) {
         const int lane = threadIdx.x & 63;
         at = keys.at(t);
         ok = keys.live(at, lane);
@@ -110,11 +107,11 @@ struct Feed {
             sc = keys.scale(at, lane, ok);
             codes.load(keys.base(p.k, at, p.D), p.cells, p.D, at.cell0, at.map < 0 ? 0 : p.cells);
         } else {
-            dk.issue(kmap, at.cell0, p.sk.ld, buf);
-            if (!p.shared) dv.issue(vmap, at.cell0, p.sv.ld, buf + v_at);
+            dk.issue((int)at.cell0, (int)p.sk.ld, buf);
+            if (!p.shared) dv.issue((int)at.cell0, (int)p.sv.ld, buf + v_at);
         }
     }
-    __device__ uint64_t put(char *buf) {
+    __device__ __forceinline__ uint64_t put(char *buf) {
         const uint64_t live = __ballot(ok) & kAll;
         if constexpr (!kCodes) D::wait();
         if (live == 0) return live;                            // the same in every wave
@@ -150,6 +147,7 @@ __global__ __launch_bounds__(64 * WQ, (DP <= 128 && std::is_same_v<SRC, BF16>) ?
     constexpr bool kScaled = kCodes && std::is_same_v<T, BF16>;        // scales applied to scores and weights
     constexpr bool kAheadHere = kAhead<T, SRC, DP, WQ>;
     extern __shared__ __attribute__((aligned(16))) char lds[];
+    out_of_step();
     const int v_at = p.shared ? 0 : DP * kRowBytes, cell_at = v_at + DP * kRowBytes;
     const int stage = cell_at + 3 * 64 * (int)sizeof(float);
 
@@ -185,9 +183,12 @@ __global__ __launch_bounds__(64 * WQ, (DP <= 128 && std::is_same_v<SRC, BF16>) ?
 #pragma unroll
         for (int i = 0; i < 16; ++i) o[c][i] = 0.f;
     float m = -__builtin_inff(), l = 0.f;                      // l: this lane's half of the cells
+    // what scores are taken relative to (m once there is one), and how far above it they may lie
+    float off = 0.f, room = -__builtin_inff();
 
     Feed<M, SRC, DP, WQ> feed(p, b, head, lds, stage);
     const Penalty<M, MODE> penalty(p, score.fall, qx, qy, true);
+    const f32x16 from = penalty.from(score.in);
     uint64_t live = 0;
     int cell0 = 0;
     if constexpr (kAheadHere) {
@@ -212,17 +213,17 @@ __global__ __launch_bounds__(64 * WQ, (DP <= 128 && std::is_same_v<SRC, BF16>) ?
         if (live != 0) {
             const char *ktile = buf, *vtile = buf + v_at;
             const float *cell = reinterpret_cast<const float *>(buf + cell_at);
-            // kPlain: z holds the products, scaled in the exponent.  kCapped: scores relative to the cap, which stands for
-            // the maximum: weights are 2^(-2 cap) > 2^-93 at least.
+            // z: scores relative to off.  kPlain: the products, scaled in the exponent.  kCapped: relative to the cap, which
+            // stands for the maximum: weights are 2^(-2 cap) > 2^-93 at least.
             f32x16 z[kBlocks];
-            float ks[kScaled ? kBlocks : 1][16];
-            M::first(ktile, addr, 0, qf, z);
+            M::first(ktile, addr, 0, qf, z, from);
 #pragma unroll
             for (int k = 0; k < kBlocks; ++k) {
                 if constexpr (kScaled) {
-                    M::per_cell(cell, k, h, ks[k]);
+                    float ks[16];
+                    M::per_cell(cell, k, h, ks);
 #pragma unroll
-                    for (int i = 0; i < 16; ++i) z[k][i] *= ks[k][i];
+                    for (int i = 0; i < 16; ++i) z[k][i] *= ks[i];
                 }
                 if constexpr (MODE == kCapped) {
 #pragma unroll
@@ -230,10 +231,10 @@ __global__ __launch_bounds__(64 * WQ, (DP <= 128 && std::is_same_v<SRC, BF16>) ?
                 } else if constexpr (MODE != kPlain) {
                     float d[16];
                     if (MODE == kRows || penalty.on) {
-                        penalty(cell + 64, cell0, k, h, d);
+                        penalty(cell + 64, cell0, k, h, -off, d);
                     } else {
 #pragma unroll
-                        for (int i = 0; i < 16; ++i) d[i] = 0.f;
+                        for (int i = 0; i < 16; ++i) d[i] = -off;
                     }
                     if (MODE == kGeneral && score.cap) {
 #pragma unroll
@@ -245,6 +246,7 @@ __global__ __launch_bounds__(64 * WQ, (DP <= 128 && std::is_same_v<SRC, BF16>) ?
                 }
             }
             if (live != kAll) {
+                stay_branch();
 #pragma unroll
                 for (int k = 0; k < kBlocks; ++k) {
                     const unsigned bits = (unsigned)(live >> (32 * k)) >> M::cell(0, h);
@@ -261,31 +263,42 @@ __global__ __launch_bounds__(64 * WQ, (DP <= 128 && std::is_same_v<SRC, BF16>) ?
                 for (int k = 0; k < kBlocks; ++k)
 #pragma unroll
                     for (int i = 0; i < 16; ++i) top = fmaxf(top, z[k][i]);
-                if (MODE == kPlain) top *= score.in;
+                if (MODE == kPlain) top = fmaf(top, score.in, -off);
                 top = fmaxf(top, __shfl_xor(top, 32));
-                if (__any(top > m + kSlack)) {
-                    const float m_new = fmaxf(m, top);
-                    const float fix = exp2_(m - (m_new == -__builtin_inff() ? 0.f : m_new));
+                if (__any(top > room)) {
+                    stay_branch();
+                    const float m_new = fmaxf(m, top + off);
+                    const float fix = m == -__builtin_inff() ? 0.f : exp2_(m - m_new);
                     m = m_new;
+                    room = m == -__builtin_inff() ? m : kSlack;
+                    const float was = off;
+                    off = m == -__builtin_inff() ? 0.f : m;
                     l *= fix;
 #pragma unroll
                     for (int c = 0; c < NC / 32; ++c)
 #pragma unroll
                         for (int i = 0; i < 16; ++i) o[c][i] *= fix;
+                    if constexpr (MODE != kPlain)
+#pragma unroll
+                        for (int k = 0; k < kBlocks; ++k)
+#pragma unroll
+                            for (int i = 0; i < 16; ++i) z[k][i] -= off - was;
                 }
             }
-            const float m_use = m == -__builtin_inff() ? 0.f : m;
             float sum[2] = {0.f, 0.f};
 #pragma unroll
             for (int k = 0; k < kBlocks; ++k) {
                 float w[16];
 #pragma unroll
                 for (int i = 0; i < 16; ++i) {
-                    w[i] = exp2_(MODE == kCapped  ? z[k][i]
-                                 : MODE == kPlain ? fmaf(score.in, z[k][i], -m_use)
-                                                  : z[k][i] - m_use);
+                    w[i] = exp2_(MODE == kPlain ? fmaf(score.in, z[k][i], -off) : z[k][i]);
                     sum[i & 1] += w[i];
-                    if constexpr (kScaled) w[i] *= ks[k][i];
+                }
+                if constexpr (kScaled) {
+                    float ks[16];
+                    M::per_cell(cell, k, h, ks);
+#pragma unroll
+                    for (int i = 0; i < 16; ++i) w[i] *= ks[i];
                 }
                 // weights are rounded to the maps' type for the second product, the sum l is not
                 M::second(vtile + p.c0 * kRowBytes, addr, k, M::weights(w), o);
@@ -309,30 +322,17 @@ __global__ __launch_bounds__(64 * WQ, (DP <= 128 && std::is_same_v<SRC, BF16>) ?
             const float2 ml = q_ok ? make_float2(m, l) : make_float2(-__builtin_inff(), 0.f);
             *reinterpret_cast<float2 *>(p.part_ml + (part * p.nq + q) * 2) = ml;
         }
-        float *dst = p.part_o + part * p.Dv * p.nq + q;
-#pragma unroll
-        for (int c = 0; c < NC / 32; ++c)
-#pragma unroll
-            for (int i = 0; i < 16; ++i) {
-                const int ch = p.c0 + 32 * c + out_channel(i, h);
-                if (ch < p.Dv) dst[ch * p.nq] = o[c][i];
-            }
+        store_columns<NC>(p.part_o + part * p.Dv * p.nq, p.nq, q, h, p.c0, p.Dv, o);
         return;
     }
     const bool some = q_ok && l != 0.f;                        // l is 0 only where no cell takes part (NaN is not)
     const float inv = some ? 1.f / l : 0.f;
-    typename T::elem *dst = (typename T::elem *)p.out + (int64_t)bh * p.Dv * p.nq + q;
 #pragma unroll
     for (int c = 0; c < NC / 32; ++c)
 #pragma unroll
-        for (int i = 0; i < 16; ++i) {
-            const int ch = p.c0 + 32 * c + out_channel(i, h);
-            const float v = some ? o[c][i] * inv : 0.f;
-            if (ch < p.Dv) {
-                store_float(dst + ch * p.nq, v);
-                if (p.out32 != nullptr) p.out32[((int64_t)bh * p.Dv + ch) * p.nq + q] = v;
-            }
-        }
+        for (int i = 0; i < 16; ++i) o[c][i] = some ? o[c][i] * inv : 0.f;
+    store_columns<NC>((typename T::elem *)p.out + (int64_t)bh * p.Dv * p.nq, p.nq, q, h, p.c0, p.Dv, o);
+    if (p.out32 != nullptr) store_columns<NC>(p.out32 + (int64_t)bh * p.Dv * p.nq, p.nq, q, h, p.c0, p.Dv, o);
     if (h == 0 && p.lse != nullptr)
         p.lse[(int64_t)bh * p.nq + q] = some ? (m + log2f(l)) * kLn2 : -__builtin_inff();
 }

@@ -1,5 +1,6 @@
 // Host side of the soft-correspondence kernels: how a call is cut into workgroups, and the launchers per arithmetic.
 #pragma once
+#include <cmath>
 #include <cstdint>
 
 #include "soft_tile.h"
@@ -61,7 +62,7 @@ int with_mode(const Params &p, bool grid, F f) {
         if (!cap && !pen) return f(std::integral_constant<int, kPlain>{});
         if constexpr (std::is_same_v<T, BF16>) {
             if (cap && !pen && p.cap <= 32.f) return f(std::integral_constant<int, kCapped>{});
-            if (!cap && grid && p.W % Math<T, DP>::kCells == 0) return f(std::integral_constant<int, kRows>{});
+            if (!cap && grid && p.W % Math<T, DP>::kCells == 0 && std::fabs(p.scale) > 1e-6f) return f(std::integral_constant<int, kRows>{});
         }
     }
     return f(std::integral_constant<int, kGeneral>{});

@@ -14,6 +14,7 @@
 // plain 16-byte read of the second one touches one segment of 16 or 32 successive rows (bits 1 to 3 pick 8 segments).
 #pragma once
 #include <type_traits>
+#include <utility>
 
 #include "common.h"
 
@@ -30,6 +31,16 @@ constexpr float kLog2e = 1.44269504088896340736f;
 constexpr float kLn2 = 0.69314718055994530942f;
 constexpr int kRowBytes = 128;
 
+// f(0) .. f(N - 1) with constant arguments: loops over register arrays that the optimiser must not keep as loops.
+template <typename F, int... I>
+__device__ __forceinline__ void each(F &&f, std::integer_sequence<int, I...>) {
+    (f(std::integral_constant<int, I>{}), ...);
+}
+template <int N, typename F>
+__device__ __forceinline__ void each(F &&f) {
+    each(f, std::make_integer_sequence<int, N>{});
+}
+
 __device__ __forceinline__ int swz(int row) { return ((row & 2) << 1) | ((row >> 2) & 3); }
 
 __device__ __forceinline__ float bf16_to_float(unsigned short u) { return __builtin_bit_cast(float, (unsigned)u << 16); }
@@ -41,6 +52,9 @@ __device__ __forceinline__ unsigned pack_bf16(float lo, float hi) {
     const f32x2 v = {lo, hi};
     return __builtin_bit_cast(unsigned, __builtin_convertvector(v, bf16x2));
 }
+
+// Keeps the code of a rare case behind its branch: turned into selects it would cost every tile three operations a cell.
+__device__ __forceinline__ void stay_branch() { asm volatile(""); }
 
 // ------------------------------------------------------------------------------------------------
 // Element types of the maps in memory.
@@ -91,23 +105,24 @@ struct Math<BF16, DP> {
         bf16x8 f[DP / 16];
     };
     // base: a column of the map (always a real one); !ok: zeros
-    __device__ static void load_owned(Owned &o, const unsigned short *base, int64_t ld, int d, bool ok, int h) {
-#pragma unroll
-        for (int s = 0; s < DP / 16; ++s) {
+    __device__ __forceinline__ static void load_owned(Owned &o, const unsigned short *base, int64_t ld, int d, bool ok, int h) {
+        const int64_t lane = 8 * h * ld;
+        each<DP / 16>([&](auto step) {
+            constexpr int s = decltype(step)::value;
             unsigned short e[8];
+            const bool whole = 16 * s + 16 <= d;               // uniform: a row's address is a scalar's distance away
 #pragma unroll
             for (int j = 0; j < 8; ++j) {
-                const int c = 16 * s + 8 * h + j;
-                const unsigned short x = base[(int64_t)(c < d ? c : d - 1) * ld];
-                e[j] = ok && c < d ? x : (unsigned short)0;
+                if (whole) e[j] = base[(16 * s + j) * ld + lane];
+                else e[j] = 16 * s + 8 * h + j < d ? base[(16 * s + j) * ld + lane] : (unsigned short)0;
             }
             u32x4 w;
 #pragma unroll
-            for (int j = 0; j < 4; ++j) w[j] = (unsigned)e[2 * j] | ((unsigned)e[2 * j + 1] << 16);
+            for (int j = 0; j < 4; ++j) w[j] = ok ? (unsigned)e[2 * j] | ((unsigned)e[2 * j + 1] << 16) : 0u;
             o.f[s] = __builtin_bit_cast(bf16x8, w);
-        }
+        });
     }
-    __device__ static void negate(Owned &o) {
+    __device__ __forceinline__ static void negate(Owned &o) {
 #pragma unroll
         for (int s = 0; s < DP / 16; ++s)
             o.f[s] = __builtin_bit_cast(bf16x8, __builtin_bit_cast(u32x4, o.f[s]) ^ 0x80008000u);
@@ -120,7 +135,7 @@ struct Math<BF16, DP> {
         int tr[2];           // first, second four channels of a 16-channel step (swz repeats every 16 rows)
         int nat;
     };
-    __device__ static Addr addr(int lane) {
+    __device__ __forceinline__ static Addr addr(int lane) {
         const int h = lane >> 5, g = (lane >> 4) & 1, p = lane & 3;
         const int seg = 2 * g + (p & 1), half = p >> 1;
         Addr a;
@@ -134,9 +149,10 @@ struct Math<BF16, DP> {
         return a;
     }
     // Products of the owned cells with streamed cells 32 b .. 32 b + 31 of a tile, b = b0 .. b0 + N - 1.  The A fragments are
-    // read kAhead steps before their MFMAs.
+    // read kAhead steps before their MFMAs.  `from`: what the products are added to.
     template <int N>
-    __device__ static void first(const char *tile, const Addr &a, int b0, const Owned &o, f32x16 (&acc)[N]) {
+    __device__ __forceinline__ static void first(const char *tile, const Addr &a, int b0, const Owned &o, f32x16 (&acc)[N],
+                                 const f32x16 &from = f32x16{}) {
         typedef __attribute__((address_space(3))) s16x4 *lds_ptr;
         constexpr int kSteps = DP / 16, kAhead = DP == 256 ? 1 : 2;
         auto frag = [&](int n, int s) {
@@ -155,24 +171,21 @@ struct Math<BF16, DP> {
         for (int s = 0; s < kAhead && s < kSteps; ++s)
 #pragma unroll
             for (int n = 0; n < N; ++n) f[s][n] = frag(n, s);
-#pragma unroll
-        for (int n = 0; n < N; ++n)
-#pragma unroll
-            for (int i = 0; i < 16; ++i) acc[n][i] = 0.f;
-#pragma unroll
-        for (int s = 0; s < kSteps; ++s) {
+        each<kSteps>([&](auto step) {
+            constexpr int s = decltype(step)::value;
 #pragma unroll
             for (int n = 0; n < N; ++n) {
-                if (s + kAhead < kSteps) f[(s + kAhead) % (kAhead + 1)][n] = frag(n, s + kAhead);
+                if constexpr (s + kAhead < kSteps) f[(s + kAhead) % (kAhead + 1)][n] = frag(n, s + kAhead);
+                if constexpr (s == 0) acc[n] = from;
                 acc[n] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(f[s % (kAhead + 1)][n], o.f[s], acc[n], 0, 0, 0);
             }
             __builtin_amdgcn_sched_barrier(0);
-        }
+        });
     }
     struct Weights {
         bf16x8 f[2];
     };
-    __device__ static Weights weights(const float (&p)[16]) {
+    __device__ __forceinline__ static Weights weights(const float (&p)[16]) {
         Weights w;
 #pragma unroll
         for (int s = 0; s < 2; ++s) {
@@ -185,7 +198,7 @@ struct Math<BF16, DP> {
     }
     // out += (channels x cells 32 b .. 32 b + 31 of the tile) x weights, for the first 32 N channel rows from `tile` on
     template <int N>
-    __device__ static void second(const char *tile, const Addr &a, int b, const Weights &w, f32x16 (&out)[N]) {
+    __device__ __forceinline__ static void second(const char *tile, const Addr &a, int b, const Weights &w, f32x16 (&out)[N]) {
 #pragma unroll
         for (int c = 0; c < N; ++c)
 #pragma unroll
@@ -198,7 +211,7 @@ struct Math<BF16, DP> {
     // Streamed cell (inside its 32) of accumulator register i, i = 0 .. 15.
     __device__ static constexpr int cell(int i, int h) { return 16 * (i >> 3) + 8 * h + (i & 7); }
     // Per-cell floats of a tile's LDS array, in register order.
-    __device__ static void per_cell(const float *v, int b, int h, float (&out)[16]) {
+    __device__ __forceinline__ static void per_cell(const float *v, int b, int h, float (&out)[16]) {
 #pragma unroll
         for (int s = 0; s < 2; ++s)
 #pragma unroll
@@ -218,16 +231,16 @@ struct Math<F32, DP> {
     struct Owned {                               // channel 2 s + h
         float f[DP / 2];
     };
-    __device__ static void load_owned(Owned &o, const float *base, int64_t ld, int d, bool ok, int h) {
-#pragma unroll
-        for (int s = 0; s < DP / 2; ++s) {
+    __device__ __forceinline__ static void load_owned(Owned &o, const float *base, int64_t ld, int d, bool ok, int h) {
+        each<DP / 2>([&](auto step) {
+            constexpr int s = decltype(step)::value;
             const int c = 2 * s + h;
             const float x = base[(int64_t)(c < d ? c : d - 1) * ld];
             o.f[s] = ok && c < d ? x : 0.f;
             if (DP == 256 && s % 8 == 7) __builtin_amdgcn_sched_barrier(0);
-        }
+        });
     }
-    __device__ static void negate(Owned &o) {
+    __device__ __forceinline__ static void negate(Owned &o) {
 #pragma unroll
         for (int s = 0; s < DP / 2; ++s) o.f[s] = -o.f[s];
     }
@@ -235,7 +248,7 @@ struct Math<F32, DP> {
         int one[8];          // row 2 s + h for s = 0 .. 7 (swz repeats every 16 rows)
         int nat;
     };
-    __device__ static Addr addr(int lane) {
+    __device__ __forceinline__ static Addr addr(int lane) {
         const int h = lane >> 5, cell = lane & 31;
         Addr a;
 #pragma unroll
@@ -247,27 +260,27 @@ struct Math<F32, DP> {
         return a;
     }
     template <int N>
-    __device__ static void first(const char *tile, const Addr &a, int, const Owned &o, f32x16 (&acc)[N]) {
-#pragma unroll
-        for (int i = 0; i < 16; ++i) acc[0][i] = 0.f;
-#pragma unroll
-        for (int s = 0; s < DP / 2; ++s) {
+    __device__ __forceinline__ static void first(const char *tile, const Addr &a, int, const Owned &o, f32x16 (&acc)[N],
+                                 const f32x16 &from = f32x16{}) {
+        acc[0] = from;
+        each<DP / 2>([&](auto step) {
+            constexpr int s = decltype(step)::value;
             const float x = *reinterpret_cast<const float *>(tile + a.one[s & 7] + (s >> 3) * 16 * kRowBytes);
             acc[0] = __builtin_amdgcn_mfma_f32_32x32x2f32(x, o.f[s], acc[0], 0, 0, 0);
             if (DP == 256 && s % 4 == 3) __builtin_amdgcn_sched_barrier(0);
-        }
+        });
     }
     struct Weights {
         float f[16];
     };
-    __device__ static Weights weights(const float (&p)[16]) {
+    __device__ __forceinline__ static Weights weights(const float (&p)[16]) {
         Weights w;
 #pragma unroll
         for (int i = 0; i < 16; ++i) w.f[i] = p[i];
         return w;
     }
     template <int N>
-    __device__ static void second(const char *tile, const Addr &a, int, const Weights &w, f32x16 (&out)[N]) {
+    __device__ __forceinline__ static void second(const char *tile, const Addr &a, int, const Weights &w, f32x16 (&out)[N]) {
 #pragma unroll
         for (int c = 0; c < N; ++c)
 #pragma unroll
@@ -280,7 +293,7 @@ struct Math<F32, DP> {
             }
     }
     __device__ static constexpr int cell(int i, int h) { return 8 * (i >> 2) + 4 * h + (i & 3); }
-    __device__ static void per_cell(const float *v, int, int h, float (&out)[16]) {
+    __device__ __forceinline__ static void per_cell(const float *v, int, int h, float (&out)[16]) {
 #pragma unroll
         for (int t = 0; t < 4; ++t) {
             const f32x4 x = *reinterpret_cast<const f32x4 *>(v + 8 * t + 4 * h);
@@ -293,7 +306,23 @@ struct Math<F32, DP> {
 // Channel of output accumulator register i of a 32-channel block.
 __device__ __forceinline__ int out_channel(int i, int h) { return 8 * (i >> 2) + 4 * h + (i & 3); }
 
-// ------------------------------------------------------------------------------------------------
+// Stores 32-channel blocks of accumulators: channels c0 .. c0 + NC - 1 of column q of a map (d, n).
+template <int NC, typename E>
+__device__ __forceinline__ void store_columns(E *map, int64_t n, int64_t q, int h, int c0, int d, const f32x16 (&o)[NC / 32]) {
+    E *at = map + 4 * h * n + q;
+    each<NC / 32>([&](auto block) {
+        constexpr int c = decltype(block)::value;
+        if (c0 + 32 * c + 32 <= d) {                           // uniform: a channel's address is a scalar's distance away
+#pragma unroll
+            for (int i = 0; i < 16; ++i) store_float(at + (c0 + 32 * c + out_channel(i, 0)) * n, o[c][i]);
+        } else {
+#pragma unroll
+            for (int i = 0; i < 16; ++i)
+                if (c0 + 32 * c + out_channel(i, h) < d) store_float(at + (c0 + 32 * c + out_channel(i, 0)) * n, o[c][i]);
+        }
+    });
+}
+
 // Loader of one tile: NT threads, thread t takes segment t & 7 of channel rows t / 8, t / 8 + NT / 8, ...
 // kAhead: the whole share of a thread fits a few registers, so that the loads of the next tile are issued (load) before
 // the products of the present one and written to LDS (store) after them; else store does both, a few rows at a time.
@@ -318,7 +347,7 @@ struct Loader {
     const elem *from;          // this thread's first segment
     int ok;                    // cells of the segment that the map has
 
-    __device__ void rows(int i0, int64_t ld, int d) {
+    __device__ __forceinline__ void rows(int i0, int64_t ld, int d) {
         const int row0 = threadIdx.x >> 3;
         const elem *p = from + (int64_t)i0 * (NT / 8) * ld;
 #pragma unroll
@@ -338,14 +367,14 @@ struct Loader {
             p += (int64_t)(NT / 8) * ld;
         }
     }
-    __device__ void load(const elem *base, int64_t ld, int d, int64_t cell0, int64_t n) {
+    __device__ __forceinline__ void load(const elem *base, int64_t ld, int d, int64_t cell0, int64_t n) {
         const int64_t at = cell0 + (threadIdx.x & 7) * kN;
         const int64_t left = n - at;
         ok = left >= kN ? kN : left > 0 ? (int)left : 0;
         from = base + (int64_t)(threadIdx.x >> 3) * ld + at;
         if constexpr (kAhead) rows(0, ld, d);
     }
-    __device__ void store(char *tile, int64_t ld, int d, uint64_t live, float scale) {
+    __device__ __forceinline__ void store(char *tile, int64_t ld, int d, uint64_t live, float scale) {
         const int seg = threadIdx.x & 7, row0 = threadIdx.x >> 3;
         const unsigned bits = (unsigned)(live >> (seg * kN)) & ((1u << kN) - 1u);
         const bool whole = live == (M::kRows == 64 ? ~0ull : 0xffffffffull);
@@ -406,61 +435,77 @@ template <typename M, int DP, int WQ>
 struct Direct {
     static constexpr int kSize = std::is_same_v<typename M::map, BF16> ? 2 : 4;
     static constexpr int kShare = DP / 8 / WQ;
-    static constexpr int kUnroll = kShare > 8 ? 4 : kShare / 2 < 1 ? 1 : kShare / 2;
+    static constexpr int kUnroll = kShare > 8 ? 8 : kShare;
     static_assert(kShare == 1 || kShare % 2 == 0, "a wave moves 8 rows or pairs of 8");
     unsigned off[2];           // byte offset of this lane's segment in rows 8 e .. 8 e + 7 for even, odd 8-row groups
     unsigned row;              // byte offset of its row
     unsigned ld8;              // bytes of 8 rows
-    int groups;                // 8-row groups of the map
-    __device__ void init(int64_t ld, int d) {
+    uint64_t from;             // first row this wave moves
+    int first, groups;         // its 8-row group; the groups this wave moves that the map has
+    int rows;
+    __device__ __forceinline__ void init(const void *map, int64_t ld, int d) {
         const int lane = threadIdx.x & 63;
         row = (unsigned)((lane >> 3) * ld * kSize);
 #pragma unroll
         for (int odd = 0; odd < 2; ++odd) off[odd] = row + (((lane & 7) ^ swz((lane >> 3) + 8 * odd)) << 4);
         ld8 = (unsigned)(8 * ld * kSize);
-        groups = d >> 3;
+        rows = d;
+        first = __builtin_amdgcn_readfirstlane((int)threadIdx.x >> 6) * kShare;
+        groups = (d >> 3) - first;
+        const uint64_t at = (uint64_t)map + (uint64_t)first * ld8;
+        from = (uint64_t)(unsigned)__builtin_amdgcn_readfirstlane((int)(uint32_t)at) |
+               (uint64_t)(unsigned)__builtin_amdgcn_readfirstlane((int)(uint32_t)(at >> 32)) << 32;
     }
     // Rows past the map's are zero in LDS throughout.
-    __device__ void clear_rest(char *tile) const {
-        for (int i = groups * 8 * kRowBytes + (int)threadIdx.x * 16; i < DP * kRowBytes; i += 64 * WQ * 16)
+    __device__ __forceinline__ void clear_rest(char *tile) const {
+        for (int i = rows * kRowBytes + (int)threadIdx.x * 16; i < DP * kRowBytes; i += 64 * WQ * 16)
             *reinterpret_cast<u32x4 *>(tile + i) = u32x4{};
     }
     // Tile from `cell0` on, of a map with `cells` cells (a multiple of kCells) a row; asynchronous, wait() ends it.
-    __device__ void issue(const void *map, int64_t cell0, int64_t cells, const char *tile) const {
-        const int wave = __builtin_amdgcn_readfirstlane((int)threadIdx.x >> 6);
+    __device__ __forceinline__ void issue(int cell0, int cells, const char *tile) const {
         unsigned at[2] = {off[0], off[1]};
         if (cells - cell0 < M::kRows) {                        // segments past the end: the row's first of this tile instead
+            stay_branch();
 #pragma unroll
             for (int odd = 0; odd < 2; ++odd)
-                if ((int64_t)((at[odd] - row) / kSize) >= cells - cell0) at[odd] = row;
+                if ((int)((at[odd] - row) / kSize) >= cells - cell0) at[odd] = row;
         }
-        const uint64_t base = (uint64_t)map + (uint64_t)cell0 * kSize;
-        const unsigned dst = (unsigned)(uintptr_t)(__attribute__((address_space(3))) const char *)tile;
+        uint64_t src = from + (uint64_t)(unsigned)(cell0 * kSize);
+        unsigned dst = (unsigned)__builtin_amdgcn_readfirstlane(
+            (int)((unsigned)(uintptr_t)(__attribute__((address_space(3))) const char *)tile + first * 1024));
         if constexpr (kShare == 1) {
-            if (wave < groups) copy(wave & 1 ? at[1] : at[0], base + (uint64_t)wave * ld8, dst + wave * 1024);
-        } else {
+            if (groups > 0) copy(first & 1 ? at[1] : at[0], src, dst);
+        } else if (groups >= kShare) {
 #pragma unroll kUnroll
-            for (int e = 0; e < kShare; e += 2) {
-                const int group = wave * kShare + e;
-                if (group < groups) copy(at[0], base + (uint64_t)group * ld8, dst + group * 1024);
-                if (group + 1 < groups) copy(at[1], base + (uint64_t)(group + 1) * ld8, dst + group * 1024 + 1024);
+            for (int e = 0; e < kShare; ++e) {
+                copy(at[e & 1], src, dst);
+                src += ld8;
+                dst += 1024;
+            }
+        } else {
+#pragma unroll 1
+            for (int e = 0; e < groups; ++e) {
+                copy(e & 1 ? at[1] : at[0], src, dst);
+                src += ld8;
+                dst += 1024;
             }
         }
     }
-    __device__ static void copy(unsigned voff, uint64_t sbase, unsigned dst) {
+    __device__ __forceinline__ static void copy(unsigned voff, uint64_t sbase, unsigned dst) {
+        // uniform by construction; said so, whatever the optimiser concludes about the control flow around
         const uint32_t hi = (uint32_t)__builtin_amdgcn_readfirstlane((int)(uint32_t)(sbase >> 32));
         const uint32_t lo = (uint32_t)__builtin_amdgcn_readfirstlane((int)(uint32_t)sbase);
         const unsigned m0 = (unsigned)__builtin_amdgcn_readfirstlane((int)dst);
         // nothing else in these kernels uses m0 (LDS instructions do not read it)
         asm volatile("s_mov_b32 m0, %1\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %0, %2"
                      :
-                     : "v"(voff), "s"(m0), "s"(((uint64_t)hi << 32) | lo)
+                     : "v"(voff), "s"(m0), "s"((uint64_t)hi << 32 | lo)
                      : "memory");
     }
-    __device__ static void wait() { asm volatile("s_waitcnt vmcnt(0)" ::: "memory"); }
+    __device__ __forceinline__ static void wait() { asm volatile("s_waitcnt vmcnt(0)" ::: "memory"); }
     // After wait(): zeros for the cells that take no part (see Loader), in the segments this lane itself has copied.
-    __device__ void mask(char *tile, uint64_t live) const {
-        const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+    __device__ __forceinline__ void mask(char *tile, uint64_t live) const {
+        const int lane = threadIdx.x & 63;
 #pragma unroll
         for (int odd = 0; odd < 2; ++odd) {
             const int seg = (lane & 7) ^ swz((lane >> 3) + 8 * odd);
@@ -474,13 +519,13 @@ struct Direct {
                 else
                     keep[j] = (bits >> j) & 1u ? 0xffffffffu : 0u;
             }
-            if (kShare == 1 && (wave & 1) != odd) continue;
+            if (kShare == 1 && (first & 1) != odd) continue;
 #pragma unroll kUnroll
             for (int e = kShare == 1 ? 0 : odd; e < kShare; e += 2) {
-                const int group = wave * kShare + e;
-                if (group >= groups) break;
-                u32x4 *p = reinterpret_cast<u32x4 *>(tile + group * 1024 + lane * 16);
-                *p = *p & keep;
+                if (e < groups) {
+                    u32x4 *p = reinterpret_cast<u32x4 *>(tile + (first + e) * 1024 + lane * 16);
+                    *p = *p & keep;
+                }
             }
         }
     }
@@ -558,15 +603,15 @@ struct Score {
     static constexpr bool kExact = std::is_same_v<T, F32>;
     float in, top, fall, in2;
     bool cap;
-    __device__ Score(const Params &p, int head) {
+    __device__ __forceinline__ Score(const Params &p, int head) {
         cap = p.cap > 0.f;
         in = cap ? p.scale / p.cap : p.scale * kLog2e;
         in2 = in * (2.f * kLog2e);
         top = p.cap * kLog2e;
         fall = p.falloff ? p.falloff[head] * kLog2e : 0.f;
     }
-    __device__ float r(float acc) const { return __builtin_amdgcn_rcpf(__builtin_amdgcn_exp2f(acc * in2) + 1.f); }
-    __device__ float bend(float acc) const {
+    __device__ __forceinline__ float r(float acc) const { return __builtin_amdgcn_rcpf(__builtin_amdgcn_exp2f(acc * in2) + 1.f); }
+    __device__ __forceinline__ float bend(float acc) const {
         const float far = fmaf(-2.f, r(acc), 1.f);
         if constexpr (!kExact) return far;
         const float y = in * acc, u = y * y;
@@ -578,14 +623,16 @@ struct Score {
     }
 };
 
-// falloff d^2 of one owned cell at (x, y) to the 16 streamed cells of a lane, negative.  Streamed cells that lie on the grid
-// (`grid`) come in groups of kCells successive ones; where the width is a multiple of that, a group stays in one row
-// and d^2 grows along it by a quadratic: two operations a cell.  Else the places are read from LDS (`cell`: 64 x, 64 y).
-template <typename M, int MODE>
+// offset - falloff d^2 of one owned cell at (x, y) to the 16 streamed cells of a lane.  Streamed cells that lie on the grid
+// come in groups of kCells successive ones; where the width is a multiple of that, a group stays in one row and d^2 grows
+// along it by a quadratic.  kRows: the quadratic's own part, -falloff j^2, is the same in every group and lies in the
+// accumulators' start (`from`), so that one operation a cell is left (FROM: where 16 registers are left for it).  kGeneral: without that, or from places read from
+// LDS (`cell`: 64 x, 64 y).
+template <typename M, int MODE, bool FROM = true>
 struct Penalty {
     bool on, rows;
     float fall, x, y, width, per_width;
-    __device__ Penalty(const Params &p, float fall_, float x_, float y_, bool grid) {
+    __device__ __forceinline__ Penalty(const Params &p, float fall_, float x_, float y_, bool grid) {
         on = MODE == kRows || (MODE == kGeneral && p.falloff != nullptr);
         rows = MODE == kRows || (grid && p.W % M::kCells == 0);
         fall = fall_;
@@ -594,8 +641,17 @@ struct Penalty {
         width = (float)p.W;
         per_width = 1.f / width;
     }
-    __device__ bool wants_places() const { return on && !rows; }
-    __device__ void operator()(const float *cell, int cell0, int k, int h, float (&z)[16]) const {
+    __device__ __forceinline__ bool wants_places() const { return on && !rows; }
+    __device__ __forceinline__ f32x16 from(float in) const {
+        f32x16 v = {};
+        if constexpr (MODE == kRows && FROM) {
+            const float f = -fall / in;
+#pragma unroll
+            for (int i = 0; i < 16; ++i) v[i] = f * (float)((i % M::kCells) * (i % M::kCells));
+        }
+        return v;
+    }
+    __device__ __forceinline__ void operator()(const float *cell, int cell0, int k, int h, float offset, float (&z)[16]) const {
         if (rows) {
 #pragma unroll
             for (int g = 0; g < 16; g += M::kCells) {
@@ -603,9 +659,10 @@ struct Penalty {
                 const float c = (float)(cell0 + 32 * k + M::cell(g, h));
                 const float cy = floorf((c + 0.5f) * per_width);
                 const float dx = fmaf(-width, cy, c) - x, dy = cy - y;
-                const float base = -fall * fmaf(dx, dx, dy * dy), step = -2.f * fall * dx;
+                const float base = fmaf(-fall, fmaf(dx, dx, dy * dy), offset), step = -2.f * fall * dx;
 #pragma unroll
-                for (int j = 0; j < M::kCells; ++j) z[g + j] = fmaf((float)j, step, fmaf((float)(-j * j), fall, base));
+                for (int j = 0; j < M::kCells; ++j)
+                    z[g + j] = fmaf((float)j, step, MODE == kRows && FROM ? base : fmaf((float)(-j * j), fall, base));
             }
         } else {
             M::per_cell(cell, k, h, z);
@@ -614,10 +671,17 @@ struct Penalty {
             float cy[16];
             M::per_cell(cell + 64, k, h, cy);
 #pragma unroll
-            for (int i = 0; i < 16; ++i) z[i] = -fall * fmaf(cy[i] - y, cy[i] - y, z[i]);
+            for (int i = 0; i < 16; ++i) z[i] = fmaf(-fall, fmaf(cy[i] - y, cy[i] - y, z[i]), offset);
         }
     }
 };
+
+// Two waves that share a SIMD and run the same loop tend to fall into step: both want the matrix pipe, then both the vector
+// ALU, and neither hides the other.  Unequal priorities, by the parity of the hardware's wave slot, let one run ahead.
+__device__ __forceinline__ void out_of_step() {
+    constexpr int kHwId = 4, kWaveBits = 4;
+    if (__builtin_amdgcn_s_getreg(kHwId | ((kWaveBits - 1) << 11)) & 1) __builtin_amdgcn_s_setprio(1);
+}
 
 __device__ __forceinline__ float exp2_(float x) { return __builtin_amdgcn_exp2f(x); }
 
