@@ -101,8 +101,6 @@ __global__ __launch_bounds__(64 * WQ, (two_waves<T, DP, WQ>) ? 2 : 1) void soft_
     constexpr uint64_t kAll = M::kRows == 64 ? ~0ull : 0xffffffffull;
     extern __shared__ __attribute__((aligned(16))) char lds[];
     out_of_step();
-    const int v_at = p.shared ? 0 : DP * kRowBytes, cell_at = v_at + DP * kRowBytes;
-    const int stage = cell_at + 3 * 64 * (int)sizeof(float);
 
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, h = lane >> 5;
     int id = die_major(blockIdx.x, gridDim.x);
@@ -136,28 +134,51 @@ __global__ __launch_bounds__(64 * WQ, (two_waves<T, DP, WQ>) ? 2 : 1) void soft_
 #pragma unroll
         for (int i = 0; i < 16; ++i) g[c][i] = 0.f;
 
-    Feed<M, T, DP, WQ> feed(p, b, head, lds, stage);
+    Feed<T, T, DP, WQ, 2> feed(p, b, head, lds);
+    const bool phased = kMayPhase<M> && feed.phased;
     const Penalty<M, MODE, false> penalty(p, score.fall, qx, qy, true);
     const f32x16 from = penalty.from(score.in);
-    uint64_t live = 0;
-    int cell0 = 0;
+    uint64_t next = 0;                                         // live cells of the next tile
+    int next_cell0 = 0;
+    auto finish = [&](int i) {
+        next = feed.end_k(i);
+        if (!phased) feed.end_v(i, next);
+        next_cell0 = (int)feed.at.cell0;
+    };
     if (t0 < t1) {
-        feed.fetch(t0, lds);
-        live = feed.put(lds);
-        cell0 = (int)feed.at.cell0;
+        feed.begin_k(t0, 0);
+        if (!phased) feed.begin_v(0);
+        finish(0);
     }
     __syncthreads();
     for (int t = t0; t < t1; ++t) {
-        const char *buf = lds + ((t - t0) & 1) * stage;
-        if (t + 1 < t1) feed.fetch(t + 1, lds + ((t + 1 - t0) & 1) * stage);
+        const int i = (t - t0) & 1, j = i ^ 1;
+        if (phased) {
+            feed.begin_v(0);
+        } else if (t + 1 < t1) {
+            feed.begin_k(t + 1, j);
+            feed.begin_v(j);
+        }
+        const uint64_t live = next;
+        const int cell0 = next_cell0;
+        const char *ktile = feed.k(i), *vtile = feed.v(i);
+        const float *cell = feed.cell(i);
+        f32x16 ahead[kMayPhase<M> ? kBlocks : 1];              // products of the first map, where they come a phase before
+        if constexpr (kMayPhase<M>) {
+            if (live != 0) M::first(ktile, addr, 0, qf, ahead);
+            if (phased) {
+                feed.end_v(0, live);
+                __syncthreads();                               // the value's tile is there
+                if (t + 1 < t1) feed.begin_k(t + 1, j);
+            }
+        }
         if (live != 0) {
-            const char *ktile = buf, *vtile = buf + v_at;
-            const float *cell = reinterpret_cast<const float *>(buf + cell_at);
 #pragma unroll kUnroll
             for (int k = 0; k < kBlocks; ++k) {
                 if (DP == 256) __builtin_amdgcn_sched_barrier(0);
                 f32x16 acc[1], dp[1];
-                M::first(ktile, addr, k, qf, acc, from);
+                if constexpr (kMayPhase<M>) acc[0] = ahead[k];
+                else M::first(ktile, addr, k, qf, acc, from);
                 M::first(vtile, addr, k, of, dp);
                 float w[16], dl[16];
                 if (MODE == kRows || penalty.on) {
@@ -178,10 +199,7 @@ __global__ __launch_bounds__(64 * WQ, (two_waves<T, DP, WQ>) ? 2 : 1) void soft_
                 M::second(ktile + p.c0 * kRowBytes, addr, k, M::weights(w), g);
             }
         }
-        if (t + 1 < t1) {
-            live = feed.put(lds + ((t + 1 - t0) & 1) * stage);
-            cell0 = (int)feed.at.cell0;
-        }
+        if (t + 1 < t1) finish(j);
         __syncthreads();
     }
     if (q >= p.nq) return;
@@ -200,10 +218,6 @@ __global__ __launch_bounds__(64 * WQ, (two_waves<T, DP, WQ>) ? 2 : 1) void soft_
     store_columns<NC>((typename T::elem *)p.dq + (int64_t)bh * p.D * p.nq, p.nq, q, h, p.c0, p.D, g);
 }
 
-// LDS of one buffer: both tiles, and per query the log-sum, delta and the place.
-template <int DP>
-constexpr int dkv_stage_bytes = 2 * DP * kRowBytes + 4 * 64 * (int)sizeof(float);
-
 // Gradients of the reference and value maps: owned = cells, streamed = queries.  PART 0: both; 1: the value's, 2: the
 // reference's alone: two launches and a fifth product, which pays where it brings two waves to a SIMD, and which the
 // registers ask for above 128 channels.
@@ -213,7 +227,7 @@ __global__ __launch_bounds__(64 * WQ, (two_waves<T, DP, WQ> && (DP <= 64 || PART
     constexpr int kBlocks = M::kRows / 32;
     constexpr int kUnroll = DP == 256 || (DP == 128 && PART == 2) ? 1 : kBlocks;           // registers
     constexpr bool kDv = PART != 2, kDk = PART != 1;
-    constexpr int kStage = dkv_stage_bytes<DP>;
+    constexpr uint64_t kAll = M::kRows == 64 ? ~0ull : 0xffffffffull;
     extern __shared__ __attribute__((aligned(16))) char lds[];
     out_of_step();
 
@@ -250,16 +264,24 @@ __global__ __launch_bounds__(64 * WQ, (two_waves<T, DP, WQ> && (DP <= 64 || PART
 
     const Penalty<M, MODE> penalty(p, score.fall, cx, cy, p.query_xy == nullptr);
     const f32x16 from = penalty.from(score.in);
+    // buffers as in Feed: twice (query tile, per query -log-sum, delta and place), then the gradient's tiles, of which
+    // three planes leave room for one
     typedef Direct<M, DP, WQ> Copy;
+    constexpr bool phased = kMayPhase<M>;
+    constexpr int kTile = kTileBytes<M, DP>, kStage = kTile + kCellBytes;
     Copy cq, co;
-    cq.init((const char *)p.sq.map + (int64_t)bh * p.sq.d * p.sq.ld * Copy::kSize, p.sq.ld, p.sq.d);
-    co.init((const char *)p.so.map + (int64_t)bh * p.so.d * p.so.ld * Copy::kSize, p.so.ld, p.so.d);
+    cq.init(p.sq, bh);
+    co.init(p.so, bh);
     for (int i = 0; i < 2; ++i) {
         cq.clear_rest(lds + i * kStage);
-        co.clear_rest(lds + i * kStage + DP * kRowBytes);
+        if (i == 0 || !phased) co.clear_rest(lds + 2 * kStage + i * kTile);
     }
     float minus = 0.f, delta = 0.f, px = 0.f, py = 0.f;
-    auto fetch = [&](int t, char *buf) {
+    auto live_of = [&](int t) {                                // what lies behind the live queries counts as zeros
+        const int64_t left = live_q - (int64_t)t * M::kRows;
+        return left < M::kRows ? (1ull << left) - 1 : kAll;
+    };
+    auto begin_q = [&](int t, int i) {
         const int64_t q0 = (int64_t)t * M::kRows;
         if (threadIdx.x < M::kRows) {
             const int64_t q = q0 + threadIdx.x;
@@ -271,39 +293,63 @@ __global__ __launch_bounds__(64 * WQ, (two_waves<T, DP, WQ> && (DP <= 64 || PART
                 if (penalty.wants_places()) query_place(p, b, q, px, py);
             }
         }
-        cq.issue((int)q0, (int)p.sq.ld, buf);
-        co.issue((int)q0, (int)p.so.ld, buf + DP * kRowBytes);
+        cq.issue((int)q0, (int)p.sq.ld, lds + i * kStage);
     };
-    auto put = [&](int t, char *buf) {
+    auto begin_o = [&](int t, int i) { co.issue(t * M::kRows, (int)p.so.ld, lds + 2 * kStage + i * kTile); };
+    auto end_q = [&](int t, int i) {
         Copy::wait();
-        const int64_t left = live_q - (int64_t)t * M::kRows;
-        if (left < M::kRows) {                                 // what lies behind the live queries counts as zeros
-            const uint64_t live = (1ull << left) - 1;
-            cq.mask(buf, live);
-            co.mask(buf + DP * kRowBytes, live);
-        }
+        const uint64_t live = live_of(t);
+        if (live != kAll) cq.mask(lds + i * kStage, live);
         if (threadIdx.x < M::kRows) {
-            float *cell = reinterpret_cast<float *>(buf + 2 * DP * kRowBytes) + threadIdx.x;
+            float *cell = reinterpret_cast<float *>(lds + i * kStage + kTile) + threadIdx.x;
             cell[0] = minus;
             cell[64] = delta;
             cell[128] = px;
             cell[192] = py;
         }
     };
+    auto end_o = [&](int t, int i) {
+        Copy::wait();
+        const uint64_t live = live_of(t);
+        if (live != kAll) co.mask(lds + 2 * kStage + i * kTile, live);
+    };
     if (t0 < t1) {
-        fetch(t0, lds);
-        put(t0, lds);
+        begin_q(t0, 0);
+        if (!phased) begin_o(t0, 0);
+        end_q(t0, 0);
+        if (!phased) end_o(t0, 0);
     }
     __syncthreads();
     for (int t = t0; t < t1; ++t) {
-        const char *qtile = lds + ((t - t0) & 1) * kStage, *otile = qtile + DP * kRowBytes;
-        const float *larr = reinterpret_cast<const float *>(otile + DP * kRowBytes);
+        const int i = (t - t0) & 1, j = i ^ 1;
+        const char *qtile = lds + i * kStage, *otile = lds + 2 * kStage + (phased ? 0 : i) * kTile;
+        const float *larr = reinterpret_cast<const float *>(qtile + kTile);
         const float *darr = larr + 64, *xarr = larr + 128;
-        if (t + 1 < t1) fetch(t + 1, lds + ((t + 1 - t0) & 1) * kStage);
+        f32x16 ahead[phased ? kBlocks : 1];                    // scores, where they come a phase before the rest
+        if constexpr (phased) {
+            begin_o(t, 0);
+            if constexpr (PART == 2) {                         // block by block: fewer fragments in registers
+#pragma unroll
+                for (int k = 0; k < kBlocks; ++k) {
+                    f32x16 acc[1];
+                    M::first(qtile, addr, k, kf, acc, from);
+                    ahead[k] = acc[0];
+                }
+            } else {
+                M::first(qtile, addr, 0, kf, ahead, from);
+            }
+            end_o(t, 0);
+            __syncthreads();                                   // the gradient's tile is there
+            if (t + 1 < t1) begin_q(t + 1, j);
+        } else if (t + 1 < t1) {
+            begin_q(t + 1, j);
+            begin_o(t + 1, j);
+        }
 #pragma unroll kUnroll
         for (int k = 0; k < kBlocks; ++k) {
             f32x16 acc[1];
-            M::first(qtile, addr, k, kf, acc, from);
+            if constexpr (phased) acc[0] = ahead[k];
+            else M::first(qtile, addr, k, kf, acc, from);
             float w[16];
             if (MODE == kRows || penalty.on) {
                 penalty(xarr, t * M::kRows, k, h, 0.f, w);
@@ -338,7 +384,10 @@ __global__ __launch_bounds__(64 * WQ, (two_waves<T, DP, WQ> && (DP <= 64 || PART
             }
             if constexpr (kDk) M::second(qtile + p.c0 * kRowBytes, addr, k, M::weights(w), gk);
         }
-        if (t + 1 < t1) put(t + 1, lds + ((t + 1 - t0) & 1) * kStage);
+        if (t + 1 < t1) {
+            end_q(t + 1, j);
+            if (!phased) end_o(t + 1, j);
+        }
         __syncthreads();
     }
     if (cell >= p.cells) return;

@@ -12,7 +12,7 @@ constexpr int kFormed = DP == 256 && std::is_same_v<T, F32> ? 128 : DP;
 template <typename T, int DP, int WQ, int MODE>
 int dq_one(Params p, hipStream_t stream) {
     static unsigned long long lds_allowed = 0;
-    const int lds = 2 * stage_bytes<DP>(p.shared);
+    const int lds = lds_bytes<Math<T, DP>, DP>(p.shared, 2);
     const unsigned grid = (unsigned)((int64_t)p.B * p.heads * p.splits * p.blocks);
     constexpr int NC = kFormed<T, DP>;
     for (p.c0 = 0; p.c0 < p.D; p.c0 += NC)
@@ -24,7 +24,7 @@ int dq_one(Params p, hipStream_t stream) {
 template <typename T, int DP, int WQ, int PART, int MODE>
 int dkv_one(Params p, int channels, hipStream_t stream) {
     static unsigned long long lds_allowed = 0;
-    const int lds = 2 * dkv_stage_bytes<DP>;
+    const int lds = lds_bytes<Math<T, DP>, DP>(false, 2);
     const unsigned grid = (unsigned)((int64_t)p.B * p.heads * p.splits * p.blocks);
     constexpr int NC = PART == 2 ? kFormed<T, DP> : DP;
     for (p.c0 = 0; p.c0 < channels; p.c0 += NC)
@@ -36,7 +36,7 @@ int dkv_one(Params p, int channels, hipStream_t stream) {
 
 template <typename T, int DP, int WQ, int MODE>
 int dkv_parts(const Params &p, hipStream_t stream) {
-    if constexpr (dkv_two_launches(std::is_same_v<T, F32>, DP, WQ)) {
+    if constexpr (dkv_two_launches(!std::is_same_v<T, BF16>, DP, WQ)) {
         if (int rc = dkv_one<T, DP, WQ, 1, MODE>(p, p.Dv, stream)) return rc;
         return dkv_one<T, DP, WQ, 2, MODE>(p, p.D, stream);
     } else {
@@ -51,25 +51,50 @@ int sum_parts(const float *a, const float *b, int splits, int64_t n, float facto
 }
 
 template <typename T, int DP>
+int dq_waves(const Params &p, int waves, hipStream_t stream) {
+    if constexpr (!std::is_same_v<T, F32> || DP == 256)
+        if (waves > 1)
+            return with_mode<T, DP>(p, true, [&](auto mode) { return dq_one<T, DP, 4, decltype(mode)::value>(p, stream); });
+    if constexpr (!std::is_same_v<T, F32S>)
+        if (waves == 1) return dq_one<T, DP, 1, kGeneral>(p, stream);
+    return ispa::fail(ISPA_EUNSUPPORTED, "no gradient kernel for %d waves", waves);
+}
+
+template <typename T, int DP>
+int dkv_waves(const Params &p, int waves, hipStream_t stream) {
+    if constexpr (!std::is_same_v<T, F32> || DP == 256)
+        if (waves > 1)
+            return with_mode<T, DP>(p, p.query_xy == nullptr,
+                                    [&](auto mode) { return dkv_parts<T, DP, 4, decltype(mode)::value>(p, stream); });
+    if constexpr (!std::is_same_v<T, F32S>)
+        if (waves == 1) return dkv_parts<T, DP, 1, kGeneral>(p, stream);
+    return ispa::fail(ISPA_EUNSUPPORTED, "no gradient kernel for %d waves", waves);
+}
+
+// The arithmetic of each launch for float32 maps; bfloat16 has one.
+template <typename T, int DP, typename F>
+int with_arithmetic(int waves, F f) {
+    if constexpr (std::is_same_v<T, F32> && DP <= 128)
+        if (arithmetic(true, false, DP, waves) == kSplit) return f(F32S{});
+    return f(T{});
+}
+
+template <typename T, int DP>
 int backward_sized(Params p, const Plan &dq, const Plan &dkv, hipStream_t stream) {
-    typedef Math<T, DP> M;
+    const bool f32 = !std::is_same_v<T, BF16>;
     p.splits = dq.splits;
     p.parts = dq.splits > 1;
     p.blocks = dq.blocks;
-    p.tiles = p.tiles_per_view = (int)((p.cells + M::kRows - 1) / M::kRows);
-    if (int rc = dq.waves == 1 ? dq_one<T, DP, 1, kGeneral>(p, stream)
-                               : with_mode<T, DP>(p, true, [&](auto mode) { return dq_one<T, DP, 4, decltype(mode)::value>(p, stream); }))
-        return rc;
+    const int64_t rows = tile_rows(arithmetic(f32, false, DP, dq.waves));
+    p.tiles = p.tiles_per_view = (int)((p.cells + rows - 1) / rows);
+    if (int rc = with_arithmetic<T, DP>(dq.waves, [&](auto t) { return dq_waves<decltype(t), DP>(p, dq.waves, stream); })) return rc;
     const int64_t bh = (int64_t)p.B * p.heads;
     if (p.parts)
         if (int rc = sum_parts<T>(p.part_a, nullptr, p.splits, bh * p.D * p.nq, p.scale, p.dq, stream)) return rc;
     p.splits = dkv.splits;
     p.parts = dkv.splits > 1;
     p.blocks = dkv.blocks;
-    if (int rc = dkv.waves == 1 ? dkv_parts<T, DP, 1, kGeneral>(p, stream)
-                                : with_mode<T, DP>(p, p.query_xy == nullptr, [&](auto mode) {
-                                      return dkv_parts<T, DP, 4, decltype(mode)::value>(p, stream);
-                                  }))
+    if (int rc = with_arithmetic<T, DP>(dkv.waves, [&](auto t) { return dkv_waves<decltype(t), DP>(p, dkv.waves, stream); }))
         return rc;
     if (!p.parts) return ISPA_OK;
     if (p.shared) return sum_parts<T>(p.part_a, p.part_b, p.splits, bh * p.D * p.cells, 1.f, p.dk, stream);

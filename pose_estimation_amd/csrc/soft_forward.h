@@ -55,27 +55,38 @@ __device__ __forceinline__ void query_place(const Params &p, int b, int64_t i, f
     }
 }
 
-// LDS of one buffer: the tiles, and per cell the scale and the place.
-template <int DP>
-constexpr int stage_bytes(bool shared) {
-    return (shared ? 1 : 2) * DP * kRowBytes + 3 * 64 * (int)sizeof(float);
-}
-// Two buffers where the loads run a tile ahead: always from maps, from codes where they fit a thread's registers.
-template <typename T, typename SRC, int DP, int WQ>
-constexpr bool kAhead = std::is_same_v<T, SRC> || Loader<Math<T, DP>, SRC, DP, 64 * WQ>::kAhead;
-template <typename T, typename SRC, int DP, int WQ>
-constexpr int kBuffers = kAhead<T, SRC, DP, WQ> ? 2 : 1;
+// How tiles and products take turns.  Two buffers for each map, the next tile on its way during all products of the
+// present one: where that fits LDS.  Else (three planes a map, reference and value apart) the value's tile is copied
+// during the first products and the reference's next one during the second, with a barrier between: `phased`.
+template <typename M>
+constexpr bool kMayPhase = M::kPlanes == 3;
 
-// The tiles of one item and head: fetch starts a tile's way into a buffer, put ends it and returns its live cells.
-template <typename M, typename SRC, int DP, int WQ>
+// LDS: NK times (reference tile, 3 or 4 x 64 floats per cell), then the value tiles.
+constexpr int kCellBytes = 4 * 64 * (int)sizeof(float);
+template <typename M, int DP>
+constexpr int kTileBytes = M::kPlanes * DP * kRowBytes;
+template <typename M, int DP>
+constexpr int lds_bytes(bool shared, int phased_k) {
+    const bool phased = kMayPhase<M> && !shared;
+    return (phased ? phased_k : 2) * (kTileBytes<M, DP> + kCellBytes) + (shared ? 0 : phased ? 1 : 2) * kTileBytes<M, DP>;
+}
+
+// The tiles of one item and head: begin_* starts a tile's way into a buffer, end_* ends it.  Codes are reference and value.
+// PK: buffers of the reference's tiles where phased.
+template <typename T, typename SRC, int DP, int WQ, int PK>
 struct Feed {
-    typedef typename M::map T;
+    typedef Math<T, DP> M;
     typedef KeyTiles<M, SRC> Keys;
     static constexpr bool kCodes = Keys::kCodes;
     static constexpr uint64_t kAll = M::kRows == 64 ? ~0ull : 0xffffffffull;
+    static constexpr int kStage = kTileBytes<M, DP> + kCellBytes;
     typedef Loader<M, SRC, DP, 64 * WQ> L;
     typedef Direct<M, DP, WQ> D;
-    struct None {};
+    struct None {
+        static constexpr bool kAhead = true;
+    };
+    // the next tile's loads may run during the present tile's products
+    static constexpr bool kAhead = std::conditional_t<kCodes, L, None>::kAhead;
     const Params &p;
     const Keys keys;
     std::conditional_t<kCodes, L, None> codes;
@@ -83,23 +94,26 @@ struct Feed {
     typename Keys::At at{};
     bool ok = false;
     float sc = 0.f;
-    int v_at, cell_at;
-    __device__ __forceinline__ Feed(const Params &p_, int b, int head, char *lds, int stage) : p(p_), keys(p_, b, head) {
-        v_at = p.shared ? 0 : DP * kRowBytes;
-        cell_at = v_at + DP * kRowBytes;
+    char *lds;
+    int v_at;                  // of the first value tile
+    bool phased;
+    __device__ __forceinline__ Feed(const Params &p_, int b, int head, char *lds_) : p(p_), keys(p_, b, head), lds(lds_) {
+        phased = kMayPhase<M> && !p.shared;
+        v_at = (phased ? PK : 2) * kStage;
         if constexpr (!kCodes) {
             const int64_t bh = (int64_t)b * p.heads + head;
-            dk.init((const char *)p.sk.map + bh * p.sk.d * p.sk.ld * D::kSize, p.sk.ld, p.sk.d);
-            dk.clear_rest(lds);
-            dk.clear_rest(lds + stage);
+            dk.init(p.sk, bh);
+            for (int i = 0; i < (phased ? PK : 2); ++i) dk.clear_rest(lds + i * kStage);
             if (!p.shared) {
-                dv.init((const char *)p.sv.map + bh * p.sv.d * p.sv.ld * D::kSize, p.sv.ld, p.sv.d);
-                dv.clear_rest(lds + v_at);
-                dv.clear_rest(lds + stage + v_at);
+                dv.init(p.sv, bh);
+                for (int i = 0; i < (phased ? 1 : 2); ++i) dv.clear_rest(lds + v_at + i * kTileBytes<M, DP>);
             }
         }
     }
-    __device__ __forceinline__ void fetch(int t, char *buf) {
+    __device__ __forceinline__ char *k(int i) const { return lds + i * kStage; }
+    __device__ __forceinline__ char *v(int i) const { return p.shared ? k(i) : lds + v_at + (phased ? 0 : i) * kTileBytes<M, DP>; }
+    __device__ __forceinline__ const float *cell(int i) const { return reinterpret_cast<const float *>(k(i) + kTileBytes<M, DP>); }
+    __device__ __forceinline__ void begin_k(int t, int i) {
         const int lane = threadIdx.x & 63;
         at = keys.at(t);
         ok = keys.live(at, lane);
@@ -107,22 +121,23 @@ struct Feed {
             sc = keys.scale(at, lane, ok);
             codes.load(keys.base(p.k, at, p.D), p.cells, p.D, at.cell0, at.map < 0 ? 0 : p.cells);
         } else {
-            dk.issue((int)at.cell0, (int)p.sk.ld, buf);
-            if (!p.shared) dv.issue((int)at.cell0, (int)p.sv.ld, buf + v_at);
+            dk.issue((int)at.cell0, (int)p.sk.ld, k(i));
         }
     }
-    __device__ __forceinline__ uint64_t put(char *buf) {
+    __device__ __forceinline__ void begin_v(int i) {           // the tile of the last begin_k
+        if constexpr (!kCodes)
+            if (!p.shared) dv.issue((int)at.cell0, (int)p.sv.ld, v(i));
+    }
+    __device__ __forceinline__ uint64_t end_k(int i) {         // the tile's live cells
         const uint64_t live = __ballot(ok) & kAll;
         if constexpr (!kCodes) D::wait();
         if (live == 0) return live;                            // the same in every wave
-        const int lane = threadIdx.x & 63;
-        float *cell = reinterpret_cast<float *>(buf + cell_at);
+        float *cell = reinterpret_cast<float *>(k(i) + kTileBytes<M, DP>);
         if constexpr (kCodes) {
-            codes.store(buf, p.cells, p.D, live, sc);
-            if (std::is_same_v<T, BF16> && threadIdx.x < 64) cell[lane] = sc;
+            codes.store(k(i), p.cells, p.D, live);
+            if (threadIdx.x < 64) cell[threadIdx.x] = sc;
         } else if (live != kAll) {
-            dk.mask(buf, live);
-            if (!p.shared) dv.mask(buf + v_at, live);
+            dk.mask(k(i), live);
         }
         if (p.falloff != nullptr && p.W % M::kCells != 0 && threadIdx.x < M::kRows) {
             const int c = (int)at.cell0 + threadIdx.x;
@@ -130,6 +145,13 @@ struct Feed {
             cell[128 + threadIdx.x] = (float)(c / p.W);
         }
         return live;
+    }
+    __device__ __forceinline__ void end_v(int i, uint64_t live) {
+        if constexpr (!kCodes) {
+            if (p.shared) return;
+            D::wait();
+            if (live != 0 && live != kAll) dv.mask(v(i), live);
+        }
     }
 };
 
@@ -144,12 +166,9 @@ __global__ __launch_bounds__(64 * WQ, (DP <= 128 && std::is_same_v<SRC, BF16>) ?
     constexpr int kBlocks = M::kRows / 32;
     constexpr uint64_t kAll = M::kRows == 64 ? ~0ull : 0xffffffffull;
     constexpr bool kCodes = KeyTiles<M, SRC>::kCodes;
-    constexpr bool kScaled = kCodes && std::is_same_v<T, BF16>;        // scales applied to scores and weights
-    constexpr bool kAheadHere = kAhead<T, SRC, DP, WQ>;
+    typedef Feed<T, SRC, DP, WQ, 1> F;
     extern __shared__ __attribute__((aligned(16))) char lds[];
     out_of_step();
-    const int v_at = p.shared ? 0 : DP * kRowBytes, cell_at = v_at + DP * kRowBytes;
-    const int stage = cell_at + 3 * 64 * (int)sizeof(float);
 
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, h = lane >> 5;
     int id = die_major(blockIdx.x, gridDim.x);
@@ -186,40 +205,47 @@ __global__ __launch_bounds__(64 * WQ, (DP <= 128 && std::is_same_v<SRC, BF16>) ?
     // what scores are taken relative to (m once there is one), and how far above it they may lie
     float off = 0.f, room = -__builtin_inff();
 
-    Feed<M, SRC, DP, WQ> feed(p, b, head, lds, stage);
+    F feed(p, b, head, lds);
+    const bool phased = kMayPhase<M> && feed.phased;
     const Penalty<M, MODE> penalty(p, score.fall, qx, qy, true);
     const f32x16 from = penalty.from(score.in);
-    uint64_t live = 0;
-    int cell0 = 0;
-    if constexpr (kAheadHere) {
-        if (t0 < t1) {
-            feed.fetch(t0, lds);
-            live = feed.put(lds);
-            cell0 = (int)feed.at.cell0;
-        }
-        __syncthreads();
+    uint64_t next = 0;                                         // live cells of the next tile
+    int next_cell0 = 0;
+    auto finish = [&](int i) {
+        next = feed.end_k(i);
+        if (!phased) feed.end_v(i, next);
+        next_cell0 = (int)feed.at.cell0;
+    };
+    if (F::kAhead && t0 < t1) {
+        feed.begin_k(t0, 0);
+        if (!phased) feed.begin_v(0);
+        finish(0);
     }
+    __syncthreads();
     for (int t = t0; t < t1; ++t) {
-        const char *buf = lds + (kAheadHere ? ((t - t0) & 1) * stage : 0);
-        if constexpr (kAheadHere) {
-            if (t + 1 < t1) feed.fetch(t + 1, lds + ((t + 1 - t0) & 1) * stage);
-        } else {
+        const int i = phased || !F::kAhead ? 0 : (t - t0) & 1, j = phased || !F::kAhead ? 0 : i ^ 1;
+        if constexpr (!F::kAhead) {
+            feed.begin_k(t, 0);
+            finish(0);
             __syncthreads();
-            feed.fetch(t, lds);
-            live = feed.put(lds);
-            cell0 = (int)feed.at.cell0;
-            __syncthreads();
+        } else if (phased) {
+            feed.begin_v(0);
+        } else if (t + 1 < t1) {
+            feed.begin_k(t + 1, j);
+            feed.begin_v(j);
         }
+        const uint64_t live = next;
+        const int cell0 = next_cell0;
+        const char *ktile = feed.k(i), *vtile = feed.v(i);
+        const float *cell = feed.cell(i);
+        f32x16 z[kBlocks];
         if (live != 0) {
-            const char *ktile = buf, *vtile = buf + v_at;
-            const float *cell = reinterpret_cast<const float *>(buf + cell_at);
             // z: scores relative to off.  kPlain: the products, scaled in the exponent.  kCapped: relative to the cap, which
             // stands for the maximum: weights are 2^(-2 cap) > 2^-93 at least.
-            f32x16 z[kBlocks];
             M::first(ktile, addr, 0, qf, z, from);
 #pragma unroll
             for (int k = 0; k < kBlocks; ++k) {
-                if constexpr (kScaled) {
+                if constexpr (kCodes) {
                     float ks[16];
                     M::per_cell(cell, k, h, ks);
 #pragma unroll
@@ -285,6 +311,15 @@ __global__ __launch_bounds__(64 * WQ, (DP <= 128 && std::is_same_v<SRC, BF16>) ?
                             for (int i = 0; i < 16; ++i) z[k][i] -= off - was;
                 }
             }
+        }
+        if constexpr (kMayPhase<M>) {
+            if (phased) {
+                feed.end_v(0, live);
+                __syncthreads();                               // the reference tile is read, the value's is there
+                if (t + 1 < t1) feed.begin_k(t + 1, 0);
+            }
+        }
+        if (live != 0) {
             float sum[2] = {0.f, 0.f};
 #pragma unroll
             for (int k = 0; k < kBlocks; ++k) {
@@ -294,24 +329,19 @@ __global__ __launch_bounds__(64 * WQ, (DP <= 128 && std::is_same_v<SRC, BF16>) ?
                     w[i] = exp2_(MODE == kPlain ? fmaf(score.in, z[k][i], -off) : z[k][i]);
                     sum[i & 1] += w[i];
                 }
-                if constexpr (kScaled) {
+                if constexpr (kCodes) {
                     float ks[16];
                     M::per_cell(cell, k, h, ks);
 #pragma unroll
                     for (int i = 0; i < 16; ++i) w[i] *= ks[i];
                 }
-                // weights are rounded to the maps' type for the second product, the sum l is not
+                // weights are rounded to bfloat16 for the second product of bfloat16 maps, the sum l is not
                 M::second(vtile + p.c0 * kRowBytes, addr, k, M::weights(w), o);
             }
             l += sum[0] + sum[1];
         }
-        if constexpr (kAheadHere) {
-            if (t + 1 < t1) {
-                live = feed.put(lds + ((t + 1 - t0) & 1) * stage);
-                cell0 = (int)feed.at.cell0;
-            }
-            __syncthreads();
-        }
+        if (F::kAhead && t + 1 < t1) finish(j);
+        __syncthreads();
     }
     l += __shfl_xor(l, 32);
 

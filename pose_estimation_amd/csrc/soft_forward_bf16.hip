@@ -1,8 +1,6 @@
-// Soft correspondence, forward kernels on bfloat16 MFMAs.
+// Soft correspondence, forward kernels: bfloat16 maps.
 #include "soft_forward_impl.h"
 
 namespace ispa_soft {
-int forward_bf16(const Params &p, int source, int waves, hipStream_t stream) {
-    return forward_source<BF16>(p, source, waves, stream);
-}
+int forward_bf16(const Params &p, int waves, hipStream_t stream) { return forward_channels<BF16, BF16>(p, waves, stream); }
 }  // namespace ispa_soft

@@ -1,8 +1,9 @@
-// Soft correspondence, forward kernels on float32 MFMAs.
+// Soft correspondence, forward kernels: float32 maps.
 #include "soft_forward_impl.h"
 
 namespace ispa_soft {
-int forward_f32(const Params &p, int source, int waves, hipStream_t stream) {
-    return forward_source<F32>(p, source, waves, stream);
+int forward_f32(const Params &p, int waves, hipStream_t stream) {
+    return arithmetic(true, false, padded_channels(p.D, p.Dv), waves) == kSplit ? forward_channels<F32S, F32S>(p, waves, stream)
+                                                                               : forward_channels<F32, F32>(p, waves, stream);
 }
 }  // namespace ispa_soft

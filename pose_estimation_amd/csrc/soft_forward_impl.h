@@ -1,4 +1,4 @@
-// Launchers of the forward kernels for one arithmetic (included by soft_forward_f32.hip and soft_forward_bf16.hip).
+// Launchers of the forward kernels for one arithmetic (included by the soft_forward_*.hip files).
 #pragma once
 #include "soft_forward.h"
 #include "soft_launch.h"
@@ -8,9 +8,9 @@ namespace ispa_soft {
 template <typename T, typename SRC, int DP, int WQ, int MODE>
 int forward_one(Params p, hipStream_t stream) {
     static unsigned long long lds_allowed = 0;
-    const int lds = kBuffers<T, SRC, DP, WQ> * stage_bytes<DP>(p.shared);
+    const int lds = lds_bytes<Math<T, DP>, DP>(p.shared, 1);
     const unsigned grid = (unsigned)((int64_t)p.B * p.heads * p.splits * p.blocks);
-    constexpr int NC = DP == 256 && std::is_same_v<T, F32> ? 128 : DP;
+    constexpr int NC = DP == 256 && !std::is_same_v<T, BF16> ? 128 : DP;
     for (p.c0 = 0; p.c0 < p.Dv; p.c0 += NC)
         if (int rc = launch(soft_forward_kernel<T, SRC, DP, WQ, NC, MODE>, p, grid, 64 * WQ, lds, &lds_allowed, "soft_forward_kernel",
                             stream))
@@ -26,8 +26,13 @@ int forward_one(Params p, hipStream_t stream) {
 
 template <typename T, typename SRC, int DP>
 int forward_waves(const Params &p, int waves, hipStream_t stream) {
-    if (waves == 1) return forward_one<T, SRC, DP, 1, kGeneral>(p, stream);
-    return with_mode<T, DP>(p, true, [&](auto mode) { return forward_one<T, SRC, DP, 4, decltype(mode)::value>(p, stream); });
+    // F32S: more than 64 queries and up to 128 channels; F32: the rest
+    if constexpr (std::is_same_v<T, F32S> || (std::is_same_v<T, F32> && DP == 256) || !std::is_same_v<T, F32>)
+        if (waves > 1)
+            return with_mode<T, DP>(p, true, [&](auto mode) { return forward_one<T, SRC, DP, 4, decltype(mode)::value>(p, stream); });
+    if constexpr (!std::is_same_v<T, F32S>)
+        if (waves == 1) return forward_one<T, SRC, DP, 1, kGeneral>(p, stream);
+    return ispa::fail(ISPA_EUNSUPPORTED, "no forward kernel for %d waves", waves);
 }
 
 template <typename T, typename SRC>
@@ -36,17 +41,10 @@ int forward_channels(const Params &p, int waves, hipStream_t stream) {
         case 32: return forward_waves<T, SRC, 32>(p, waves, stream);
         case 64: return forward_waves<T, SRC, 64>(p, waves, stream);
         case 128: return forward_waves<T, SRC, 128>(p, waves, stream);
-        default: return forward_waves<T, SRC, 256>(p, waves, stream);
+        default:
+            if constexpr (!std::is_same_v<T, F32S>) return forward_waves<T, SRC, 256>(p, waves, stream);
     }
-}
-
-template <typename T>
-int forward_source(const Params &p, int source, int waves, hipStream_t stream) {
-    switch (source) {
-        case kSourceMap: return forward_channels<T, T>(p, waves, stream);
-        case kSourceInt8: return forward_channels<T, I8>(p, waves, stream);
-        default: return forward_channels<T, FP8>(p, waves, stream);
-    }
+    return ispa::fail(ISPA_EUNSUPPORTED, "no forward kernel for %d channels", p.D);
 }
 
 }  // namespace ispa_soft

@@ -7,9 +7,6 @@
 
 namespace ispa_soft {
 
-// Codes a template store holds, or the maps' own type.
-enum Source { kSourceMap = 0, kSourceInt8 = 1, kSourceFp8 = 2 };
-
 inline int padded_channels(int d, int dv) {
     const int m = d > dv ? d : dv;
     return m <= 32 ? 32 : m <= 64 ? 64 : m <= 128 ? 128 : 256;
@@ -22,13 +19,25 @@ struct Plan {
 
 constexpr int kMaxSplitCount = 512;
 
-// resident: workgroups of four waves that a compute unit holds.  Up to 64 owned cells, workgroups of one wave: all the
-// parallelism lies in the streamed tiles, and four waves would stage for one.  The tiles are split so that the rounds of
+// Workgroups of four waves for more than 64 owned cells.  Up to that all the parallelism lies in the streamed tiles, and
+// four waves would stage for one.
+inline int waves_for(int64_t owned) { return owned <= 64 ? 1 : 4; }
+
+// The arithmetic of a launch.  float32 maps run on bfloat16 MFMAs, six products for one (F32S), 2.7 times the rate of the
+// float32 MFMAs, but stream copies of three planes and keep them in registers: not for 256 channels, and not for few
+// queries, which read a map once.  Codes need no copies.
+enum Arithmetic { kNarrow, kSplit, kFloat };
+inline Arithmetic arithmetic(bool f32, bool codes, int padded, int waves) {
+    return !f32 ? kNarrow : codes || (padded <= 128 && waves > 1) ? kSplit : kFloat;
+}
+inline int64_t tile_rows(Arithmetic a) { return a == kFloat ? 32 : 64; }
+
+// resident: workgroups of four waves that a compute unit holds.  The tiles are split so that the rounds of
 // workgroups that the 256 compute units work off, each as long as its tiles and about two more to start, are shortest; a
 // split costs its workgroup about four tiles more, for writing and joining its part.
 inline Plan make_plan(int64_t owned, int64_t groups, int64_t tiles, int resident) {
     Plan plan;
-    plan.waves = owned <= 64 ? 1 : 4;
+    plan.waves = waves_for(owned);
     plan.blocks = (int)((owned + 32 * plan.waves - 1) / (32 * plan.waves));
     plan.splits = 1;
     const int64_t base = groups * plan.blocks, room = 256 * (plan.waves == 1 ? 4 : resident);
@@ -44,11 +53,13 @@ inline Plan make_plan(int64_t owned, int64_t groups, int64_t tiles, int resident
 }
 
 // Whether the gradients of the reference and value maps take a launch each.
-constexpr bool dkv_two_launches(bool f32, int padded, int waves) { return padded == 256 || (padded == 128 && f32 == (waves == 1)); }
+constexpr bool dkv_two_launches(bool f32, int padded, int waves) { return padded == 256 || (padded == 128 && (f32 || waves > 1)); }
 
 // Every launcher expects p.blocks, p.splits, p.tiles and p.tiles_per_view to be set; 0 or a negative status.
-int forward_f32(const Params &p, int source, int waves, hipStream_t stream);
-int forward_bf16(const Params &p, int source, int waves, hipStream_t stream);
+int forward_f32(const Params &p, int waves, hipStream_t stream);
+int forward_bf16(const Params &p, int waves, hipStream_t stream);
+int forward_codes_f32(const Params &p, bool fp8, int waves, hipStream_t stream);
+int forward_codes_bf16(const Params &p, bool fp8, int waves, hipStream_t stream);
 int backward_f32(const Params &p, const Plan &dq, const Plan &dkv, hipStream_t stream);
 int backward_bf16(const Params &p, const Plan &dq, const Plan &dkv, hipStream_t stream);
 

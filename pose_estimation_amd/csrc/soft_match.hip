@@ -7,8 +7,6 @@
 namespace {
 using namespace ispa_soft;
 
-int64_t tile_cells(int dtype) { return dtype == ISPA_F32 ? Math<F32, 32>::kRows : Math<BF16, 32>::kRows; }
-
 bool sizes_ok(int dtype, int B, int heads, int D, int Dv, int64_t nq, int V, int64_t cells) {
     return (dtype == ISPA_F32 || dtype == ISPA_BF16) && B >= 0 && heads >= 1 && D >= 1 && D <= ISPA_SOFT_MAX_CHANNELS && Dv >= 1 &&
            Dv <= ISPA_SOFT_MAX_CHANNELS && nq >= 0 && nq < (1ll << 22) && V >= 0 && cells >= 1 && cells < (1ll << 22) &&
@@ -28,47 +26,85 @@ int check_sizes(int dtype, int B, int heads, int D, int Dv, int64_t nq, int V, i
 
 size_t align256(size_t x) { return (x + 255) & ~(size_t)255; }
 
-// Copies of maps whose rows do not start on 16-byte borders or whose channels are no multiple of 8, in the workspace.
+// Copies maps (maps, d, n) into the form Direct wants: (maps, d8, ld) with d8 the next multiple of 8 rows and ld of kCells
+// cells, zeros beside.
+template <typename T>
+__global__ __launch_bounds__(256) void soft_pack_kernel(const typename T::elem *src, typename T::elem *dst, int d, int d8,
+                                                        int64_t n, int64_t ld, int64_t rows) {
+    const int64_t per = (ld + 255) / 256;
+    const int64_t row = blockIdx.x / per, cell = (blockIdx.x - row * per) * 256 + threadIdx.x;
+    if (row >= rows || cell >= ld) return;
+    const int64_t map = row / d8;
+    const int c = (int)(row - map * d8);
+    dst[row * ld + cell] = c < d && cell < n ? src[(map * d + c) * n + cell] : (typename T::elem)0;
+}
+
+// float32 maps as three planes of bfloat16 numbers (F32S), (maps, 3, d8, ld); two cells a thread.
+__global__ __launch_bounds__(256) void soft_split_kernel(const float *src, unsigned *dst, int d, int d8, int64_t n, int64_t ld,
+                                                         int64_t rows) {
+    const int64_t half = ld / 2, per = (half + 255) / 256;
+    const int64_t row = blockIdx.x / per, pair = (blockIdx.x - row * per) * 256 + threadIdx.x;
+    if (row >= rows || pair >= half) return;
+    const int64_t map = row / d8;
+    const int c = (int)(row - map * d8);
+    const float *at = src + (map * d + c) * n + 2 * pair;
+    const float x = c < d && 2 * pair < n ? at[0] : 0.f, y = c < d && 2 * pair + 1 < n ? at[1] : 0.f;
+    unsigned a[3], b[3];
+    split3(x, a[0], a[1], a[2]);
+    split3(y, b[0], b[1], b[2]);
+#pragma unroll
+    for (int k = 0; k < 3; ++k) dst[((map * 3 + k) * d8 + c) * half + pair] = uppers(a[k], b[k]);
+}
+
+// Copies of maps in the workspace: three planes for kSplit; else only maps whose rows do not start on 16-byte borders or
+// whose channels are no multiple of 8.
 struct Copies {
     int64_t ld;
     int d8;
     size_t bytes;              // 0: the map is streamed as it is
 };
 
-Copies copies(int dtype, int64_t maps, int d, int64_t n) {
-    const int64_t unit = dtype == ISPA_F32 ? 4 : 8;
+Copies copies(Arithmetic a, int64_t maps, int d, int64_t n) {
+    const int64_t unit = a == kFloat ? 4 : 8;
     Copies c;
     c.ld = (n + unit - 1) / unit * unit;
     c.d8 = (d + 7) & ~7;
-    c.bytes = c.ld == n && c.d8 == d ? 0 : align256((size_t)maps * c.d8 * c.ld * (dtype == ISPA_F32 ? 4 : 2));
+    const size_t numbers = (size_t)maps * c.d8 * c.ld;
+    c.bytes = a == kSplit ? align256(numbers * 6) : c.ld == n && c.d8 == d ? 0 : align256(numbers * (a == kFloat ? 4 : 2));
     return c;
 }
 
 // The map for streaming; `at` moves past the copy, if there is one.
-int stream_map(Stream *s, int dtype, const void *map, int64_t maps, int d, int64_t n, char **at, hipStream_t stream) {
-    const Copies c = copies(dtype, maps, d, n);
+int stream_map(Stream *s, Arithmetic a, const void *map, int64_t maps, int d, int64_t n, char **at, hipStream_t stream) {
+    const Copies c = copies(a, maps, d, n);
     s->ld = c.ld;
     s->d = c.d8;
     s->map = map;
     if (c.bytes == 0) return ISPA_OK;
-    const int64_t rows = maps * c.d8, per = (c.ld + 255) / 256;
+    const int64_t rows = maps * c.d8, per = (c.ld / (a == kSplit ? 2 : 1) + 255) / 256;
     ISPA_REQUIRE(rows * per < (1ll << 31), "maps of %lld rows are too large for one call", (long long)rows);
-    if (dtype == ISPA_F32)
-        soft_pack_kernel<F32><<<(unsigned)(rows * per), 256, 0, stream>>>((const float *)map, (float *)*at, d, c.d8, n, c.ld, rows);
+    const unsigned blocks = (unsigned)(rows * per);
+    if (a == kSplit)
+        soft_split_kernel<<<blocks, 256, 0, stream>>>((const float *)map, (unsigned *)*at, d, c.d8, n, c.ld, rows);
+    else if (a == kFloat)
+        soft_pack_kernel<F32><<<blocks, 256, 0, stream>>>((const float *)map, (float *)*at, d, c.d8, n, c.ld, rows);
     else
-        soft_pack_kernel<BF16><<<(unsigned)(rows * per), 256, 0, stream>>>((const unsigned short *)map, (unsigned short *)*at, d,
-                                                                           c.d8, n, c.ld, rows);
+        soft_pack_kernel<BF16><<<blocks, 256, 0, stream>>>((const unsigned short *)map, (unsigned short *)*at, d, c.d8, n, c.ld, rows);
     s->map = *at;
     *at += c.bytes;
     return ispa::check_launch("soft_pack_kernel");
 }
 
 // Workgroups of four waves a compute unit holds: two where a lane's registers allow it.
-int resident(int dtype, int D, int Dv) { return padded_channels(D, Dv) <= (dtype == ISPA_F32 ? 64 : 128) ? 2 : 1; }
+int resident(int dtype, int D, int Dv) { return dtype == ISPA_BF16 && padded_channels(D, Dv) <= 128 ? 2 : 1; }
 
-Plan forward_plan(int dtype, int B, int heads, int D, int Dv, int64_t nq, int V, int64_t cells) {
-    const int64_t per = (cells + tile_cells(dtype) - 1) / tile_cells(dtype);
-    return make_plan(nq, (int64_t)B * heads, per * V, resident(dtype, D, Dv));
+Arithmetic arithmetic_of(int dtype, bool codes, int D, int Dv, int64_t owned) {
+    return arithmetic(dtype == ISPA_F32, codes, padded_channels(D, Dv), waves_for(owned));
+}
+
+Plan plan_of(int dtype, bool codes, int64_t groups, int D, int Dv, int64_t owned, int V, int64_t streamed) {
+    const int64_t r = tile_rows(arithmetic_of(dtype, codes, D, Dv, owned));
+    return make_plan(owned, groups, (streamed + r - 1) / r * V, resident(dtype, D, Dv));
 }
 
 size_t forward_bytes(const Plan &plan, int B, int heads, int Dv, int64_t nq) {
@@ -76,10 +112,8 @@ size_t forward_bytes(const Plan &plan, int B, int heads, int Dv, int64_t nq) {
 }
 
 void backward_plans(int dtype, int B, int heads, int D, int Dv, int64_t nq, int64_t cells, Plan *dq, Plan *dkv) {
-    const int64_t r = tile_cells(dtype);
-    const int wgs = dtype == ISPA_F32 ? 1 : resident(dtype, D, Dv);
-    *dq = make_plan(nq, (int64_t)B * heads, (cells + r - 1) / r, wgs);
-    *dkv = make_plan(cells, (int64_t)B * heads, (nq + r - 1) / r, wgs);
+    *dq = plan_of(dtype, false, (int64_t)B * heads, D, Dv, nq, 1, cells);
+    *dkv = plan_of(dtype, false, (int64_t)B * heads, D, Dv, cells, 1, nq);
 }
 
 
@@ -92,8 +126,9 @@ size_t dkv_parts(int dtype, const Plan &dkv, int D, int Dv) {
 
 size_t backward_bytes(int dtype, const Plan &dq, const Plan &dkv, int B, int heads, int D, int Dv, int64_t nq, int64_t cells) {
     const size_t bh = (size_t)B * heads;
-    const size_t copied = copies(dtype, bh, D, cells).bytes + copies(dtype, bh, Dv, cells).bytes + copies(dtype, bh, D, nq).bytes +
-                          copies(dtype, bh, Dv, nq).bytes;
+    const Arithmetic aq = arithmetic_of(dtype, false, D, Dv, nq), akv = arithmetic_of(dtype, false, D, Dv, cells);
+    const size_t copied = copies(aq, bh, D, cells).bytes + copies(aq, bh, Dv, cells).bytes + copies(akv, bh, D, nq).bytes +
+                          copies(akv, bh, Dv, nq).bytes;
     const size_t a = dq.splits > 1 ? dq.splits * bh * D * nq : 0, k = dkv_parts(dtype, dkv, D, Dv) * bh * cells;
     return copied + align256(bh * nq * sizeof(float)) + (a > k ? a : k) * sizeof(float);
 }
@@ -104,39 +139,52 @@ int check_score(float scale, float cap, const float *falloff, int W) {
     return ISPA_OK;
 }
 
-size_t forward_copies(int dtype, int B, int heads, int D, int Dv, int64_t cells, bool shared) {
-    return copies(dtype, (int64_t)B * heads, D, cells).bytes + (shared ? 0 : copies(dtype, (int64_t)B * heads, Dv, cells).bytes);
+size_t forward_copies(int dtype, int B, int heads, int D, int Dv, int64_t nq, int64_t cells, bool shared) {
+    const Arithmetic a = arithmetic_of(dtype, false, D, Dv, nq);
+    return copies(a, (int64_t)B * heads, D, cells).bytes + (shared ? 0 : copies(a, (int64_t)B * heads, Dv, cells).bytes);
 }
 
-int run_forward(Params &p, int dtype, int source, void *workspace, size_t workspace_bytes, hipStream_t stream) {
-    const Plan plan = forward_plan(dtype, p.B, p.heads, p.D, p.Dv, p.nq, p.V, p.cells);
-    const bool maps = source == kSourceMap;
-    const size_t copied = maps ? forward_copies(dtype, p.B, p.heads, p.D, p.Dv, p.cells, p.shared) : 0;
+enum Source { kMaps, kInt8, kFp8 };
+
+int run_forward(Params &p, int dtype, Source source, void *workspace, size_t workspace_bytes, hipStream_t stream) {
+    const bool maps = source == kMaps;
+    const int64_t bh = (int64_t)p.B * p.heads;
+    const Plan plan = plan_of(dtype, !maps, bh, p.D, p.Dv, p.nq, p.V, p.cells);
+    const Arithmetic a = arithmetic_of(dtype, !maps, p.D, p.Dv, p.nq);
+    const size_t copied = maps ? forward_copies(dtype, p.B, p.heads, p.D, p.Dv, p.nq, p.cells, p.shared) : 0;
     const size_t need = copied + forward_bytes(plan, p.B, p.heads, p.Dv, p.nq);
     ISPA_REQUIRE(!maps || (((uintptr_t)p.k | (uintptr_t)p.v) & 15) == 0, "maps must start on 16-byte borders");
     if (need > 0 && (workspace == nullptr || workspace_bytes < need))
         return ispa::fail(ISPA_EWORKSPACE, "workspace of %zu bytes, %zu needed", workspace_bytes, need);
-    p.tiles_per_view = (int)((p.cells + tile_cells(dtype) - 1) / tile_cells(dtype));
+    p.tiles_per_view = (int)((p.cells + tile_rows(a) - 1) / tile_rows(a));
     p.tiles = p.tiles_per_view * p.V;
     p.blocks = plan.blocks;
     p.splits = plan.splits;
     char *at = (char *)workspace;
     if (maps) {
-        if (int rc = stream_map(&p.sk, dtype, p.k, (int64_t)p.B * p.heads, p.D, p.cells, &at, stream)) return rc;
+        if (int rc = stream_map(&p.sk, a, p.k, bh, p.D, p.cells, &at, stream)) return rc;
         if (!p.shared)
-            if (int rc = stream_map(&p.sv, dtype, p.v, (int64_t)p.B * p.heads, p.Dv, p.cells, &at, stream)) return rc;
+            if (int rc = stream_map(&p.sv, a, p.v, bh, p.Dv, p.cells, &at, stream)) return rc;
     }
     p.part_ml = (float *)at;
-    p.part_o = p.part_ml + (size_t)plan.splits * p.B * p.heads * p.nq * 2;
-    return dtype == ISPA_F32 ? forward_f32(p, source, plan.waves, stream) : forward_bf16(p, source, plan.waves, stream);
+    p.part_o = p.part_ml + (size_t)plan.splits * bh * p.nq * 2;
+    if (maps) return dtype == ISPA_F32 ? forward_f32(p, plan.waves, stream) : forward_bf16(p, plan.waves, stream);
+    return dtype == ISPA_F32 ? forward_codes_f32(p, source == kFp8, plan.waves, stream)
+                             : forward_codes_bf16(p, source == kFp8, plan.waves, stream);
 }
 }  // namespace
 
 extern "C" size_t ispa_soft_match_workspace_bytes(int dtype, int B, int heads, int D, int Dv, int64_t nq, int views,
                                                   int64_t cells) {
     if (!sizes_ok(dtype, B, heads, D, Dv, nq, views, cells) || B == 0 || nq == 0) return 0;
-    return forward_copies(dtype, B, heads, D, Dv, cells, false) + forward_bytes(forward_plan(dtype, B, heads, D, Dv, nq, views, cells), B,
-                                                                                heads, Dv, nq);
+    // codes may be cut into tiles of another size than maps: room for either
+    size_t most = 0;
+    for (int codes = 0; codes < 2; ++codes) {
+        const size_t n = (codes ? 0 : forward_copies(dtype, B, heads, D, Dv, nq, cells, false)) +
+                         forward_bytes(plan_of(dtype, codes, (int64_t)B * heads, D, Dv, nq, views, cells), B, heads, Dv, nq);
+        most = n > most ? n : most;
+    }
+    return most;
 }
 
 extern "C" int ispa_soft_match(const void *q, const void *r, const void *v, int dtype, int B, int heads, int D, int Dv,
@@ -170,7 +218,7 @@ extern "C" int ispa_soft_match(const void *q, const void *r, const void *v, int 
     p.V = 1;
     p.scale = scale;
     p.cap = cap;
-    return run_forward(p, dtype, kSourceMap, workspace, workspace_bytes, (hipStream_t)stream);
+    return run_forward(p, dtype, kMaps, workspace, workspace_bytes, (hipStream_t)stream);
 }
 
 extern "C" int ispa_store_match(const void *q, int dtype, const void *codes, const float *scales, const uint8_t *mask, int kind,
@@ -206,7 +254,7 @@ extern "C" int ispa_store_match(const void *q, int dtype, const void *codes, con
     p.V = V;
     p.scale = scale;
     p.cap = cap;
-    return run_forward(p, dtype, kind == ISPA_STORE_INT8 ? kSourceInt8 : kSourceFp8, workspace, workspace_bytes,
+    return run_forward(p, dtype, kind == ISPA_STORE_INT8 ? kInt8 : kFp8, workspace, workspace_bytes,
                        (hipStream_t)stream);
 }
 
@@ -263,12 +311,13 @@ extern "C" int ispa_soft_match_backward(const void *q, const void *r, const void
     const int64_t bh = (int64_t)B * heads;
     ISPA_REQUIRE((((uintptr_t)r | (uintptr_t)p.v | (uintptr_t)q | (uintptr_t)d_out) & 15) == 0, "maps must start on 16-byte borders");
     char *at = (char *)workspace;
-    if (int rc = stream_map(&p.sk, dtype, r, bh, D, cells, &at, s)) return rc;
+    const Arithmetic aq = arithmetic_of(dtype, false, D, Dv, nq), akv = arithmetic_of(dtype, false, D, Dv, cells);
+    if (int rc = stream_map(&p.sk, aq, r, bh, D, cells, &at, s)) return rc;
     if (!p.shared)
-        if (int rc = stream_map(&p.sv, dtype, v, bh, Dv, cells, &at, s)) return rc;
+        if (int rc = stream_map(&p.sv, aq, v, bh, Dv, cells, &at, s)) return rc;
     if (nq > 0) {
-        if (int rc = stream_map(&p.sq, dtype, q, bh, D, nq, &at, s)) return rc;
-        if (int rc = stream_map(&p.so, dtype, d_out, bh, Dv, nq, &at, s)) return rc;
+        if (int rc = stream_map(&p.sq, akv, q, bh, D, nq, &at, s)) return rc;
+        if (int rc = stream_map(&p.so, akv, d_out, bh, Dv, nq, &at, s)) return rc;
     }
     float *delta = (float *)at;
     p.delta = delta;

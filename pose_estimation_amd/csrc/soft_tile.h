@@ -64,6 +64,14 @@ struct F32 {
 struct BF16 {
     typedef unsigned short elem;
 };
+// float32 maps and codes on bfloat16 MFMAs: a float32 number is the exact sum of three bfloat16 numbers (its 24 bits cut
+// into three times 8), and six of the nine products of two such sums carry float32's precision.
+struct F32S {               // streamed maps in three planes
+    typedef float elem;
+};
+struct F32C {               // streamed codes, which one bfloat16 number holds exactly
+    typedef float elem;
+};
 struct I8 {                 // codes of a template store; the value is code * scale[cell]
     typedef signed char elem;
 };
@@ -100,7 +108,8 @@ template <int DP>
 struct Math<BF16, DP> {
     static constexpr int kRows = 64;             // streamed cells per tile
     static constexpr int kCells = 8;             // cells of a 16-byte segment
-    typedef BF16 map;
+    static constexpr int kBytes = 2;             // of a streamed number in LDS
+    static constexpr int kPlanes = 1;            // LDS tiles that hold one tile of the map
     struct Owned {                               // B operand of the first product: channels 16 s + 8 h .. + 7
         bf16x8 f[DP / 16];
     };
@@ -227,7 +236,8 @@ template <int DP>
 struct Math<F32, DP> {
     static constexpr int kRows = 32;
     static constexpr int kCells = 4;
-    typedef F32 map;
+    static constexpr int kBytes = 4;
+    static constexpr int kPlanes = 1;
     struct Owned {                               // channel 2 s + h
         float f[DP / 2];
     };
@@ -303,6 +313,148 @@ struct Math<F32, DP> {
     }
 };
 
+// x = hi + mid + lo exactly (up to bits below 2^-133), each a bfloat16 number in the upper half of the word.
+__device__ __forceinline__ void split3(float x, unsigned &hi, unsigned &mid, unsigned &lo) {
+    hi = __builtin_bit_cast(unsigned, x);
+    const float r = x - __builtin_bit_cast(float, hi & 0xffff0000u);
+    mid = __builtin_bit_cast(unsigned, r);
+    lo = __builtin_bit_cast(unsigned, r - __builtin_bit_cast(float, mid & 0xffff0000u));
+}
+// Upper halves of two words.
+__device__ __forceinline__ unsigned uppers(unsigned first, unsigned second) { return __builtin_amdgcn_perm(second, first, 0x07060302u); }
+
+// PLANES: of the streamed side, 3 (maps) or 1 (codes).
+template <int DP, int PLANES>
+struct SplitMath {
+    typedef Math<BF16, DP> Narrow;
+    static constexpr int kRows = 64;
+    static constexpr int kCells = 8;
+    static constexpr int kBytes = 2;
+    static constexpr int kPlanes = PLANES;
+    static constexpr int kTile = DP * kRowBytes;
+    struct Owned {
+        bf16x8 f[3][DP / 16];
+    };
+    typedef typename Narrow::Addr Addr;
+    __device__ __forceinline__ static Addr addr(int lane) { return Narrow::addr(lane); }
+    __device__ __forceinline__ static void load_owned(Owned &o, const float *base, int64_t ld, int d, bool ok, int h) {
+        const int64_t lane = 8 * h * ld;
+        each<DP / 16>([&](auto step) {
+            constexpr int s = decltype(step)::value;
+            float e[8];
+            const bool whole = 16 * s + 16 <= d;
+#pragma unroll
+            for (int j = 0; j < 8; ++j) {
+                if (whole) e[j] = base[(16 * s + j) * ld + lane];
+                else e[j] = 16 * s + 8 * h + j < d ? base[(16 * s + j) * ld + lane] : 0.f;
+            }
+            u32x4 w[3];
+#pragma unroll
+            for (int j = 0; j < 4; ++j) {
+                unsigned a[3], b[3];
+                split3(ok ? e[2 * j] : 0.f, a[0], a[1], a[2]);
+                split3(ok ? e[2 * j + 1] : 0.f, b[0], b[1], b[2]);
+#pragma unroll
+                for (int x = 0; x < 3; ++x) w[x][j] = uppers(a[x], b[x]);
+            }
+#pragma unroll
+            for (int x = 0; x < 3; ++x) o.f[x][s] = __builtin_bit_cast(bf16x8, w[x]);
+            if (DP == 256 && s % 2 == 1) __builtin_amdgcn_sched_barrier(0);
+        });
+    }
+    __device__ __forceinline__ static void negate(Owned &o) {
+        each<DP / 16>([&](auto step) {
+            constexpr int s = decltype(step)::value;
+#pragma unroll
+            for (int x = 0; x < 3; ++x)
+                o.f[x][s] = __builtin_bit_cast(bf16x8, __builtin_bit_cast(u32x4, o.f[x][s]) ^ 0x80008000u);
+        });
+    }
+    // Planes x of one side and y of the other are multiplied where x + y < 3: what is left out lies below 2^-24.
+    template <int N>
+    __device__ __forceinline__ static void first(const char *tile, const Addr &a, int b0, const Owned &o, f32x16 (&acc)[N],
+                                                 const f32x16 &from = f32x16{}) {
+        typedef __attribute__((address_space(3))) s16x4 *lds_ptr;
+        constexpr int kSteps = DP / 16;
+        auto frag = [&](int x, int n, int s) {
+            union {
+                s16x4 q[2];
+                bf16x8 v;
+            } u;
+#pragma unroll
+            for (int y = 0; y < 2; ++y)
+                u.q[y] = __builtin_amdgcn_ds_read_tr16_b64_v4i16(
+                    (lds_ptr)(tile + x * kTile + (a.tr[y] ^ ((b0 + n) << 6)) + s * 16 * kRowBytes));
+            return u.v;
+        };
+        bf16x8 f[2][PLANES][N];
+#pragma unroll
+        for (int x = 0; x < PLANES; ++x)
+#pragma unroll
+            for (int n = 0; n < N; ++n) f[0][x][n] = frag(x, n, 0);
+#pragma unroll
+        for (int n = 0; n < N; ++n) acc[n] = from;
+        each<kSteps>([&](auto step) {
+            constexpr int s = decltype(step)::value;
+            if constexpr (s + 1 < kSteps)
+#pragma unroll
+                for (int x = 0; x < PLANES; ++x)
+#pragma unroll
+                    for (int n = 0; n < N; ++n) f[(s + 1) & 1][x][n] = frag(x, n, s + 1);
+#pragma unroll
+            for (int x = PLANES - 1; x >= 0; --x)
+#pragma unroll
+                for (int y = 2 - x; y >= 0; --y)
+#pragma unroll
+                    for (int n = 0; n < N; ++n)
+                        acc[n] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(f[s & 1][x][n], o.f[y][s], acc[n], 0, 0, 0);
+            __builtin_amdgcn_sched_barrier(0);
+        });
+    }
+    struct Weights {
+        bf16x8 f[3][2];
+    };
+    __device__ __forceinline__ static Weights weights(const float (&p)[16]) {
+        Weights w;
+#pragma unroll
+        for (int s = 0; s < 2; ++s) {
+            u32x4 v[3];
+#pragma unroll
+            for (int j = 0; j < 4; ++j) {
+                unsigned a[3], b[3];
+                split3(p[8 * s + 2 * j], a[0], a[1], a[2]);
+                split3(p[8 * s + 2 * j + 1], b[0], b[1], b[2]);
+#pragma unroll
+                for (int x = 0; x < 3; ++x) v[x][j] = uppers(a[x], b[x]);
+            }
+#pragma unroll
+            for (int x = 0; x < 3; ++x) w.f[x][s] = __builtin_bit_cast(bf16x8, v[x]);
+        }
+        return w;
+    }
+    template <int N>
+    __device__ __forceinline__ static void second(const char *tile, const Addr &a, int b, const Weights &w, f32x16 (&out)[N]) {
+        each<2 * N>([&](auto step) {
+            constexpr int s = decltype(step)::value & 1, c = decltype(step)::value >> 1;
+            const char *at = tile + (a.nat ^ ((4 * b + 2 * s) << 4)) + c * 32 * kRowBytes;
+#pragma unroll
+            for (int x = PLANES - 1; x >= 0; --x) {
+                const bf16x8 v = *reinterpret_cast<const bf16x8 *>(at + x * kTile);
+#pragma unroll
+                for (int y = 2 - x; y >= 0; --y)
+                    out[c] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(v, w.f[y][s], out[c], 0, 0, 0);
+            }
+            if (s == 1 && c % 2 == 1) __builtin_amdgcn_sched_barrier(0);       // bounds the reads in flight
+        });
+    }
+    __device__ static constexpr int cell(int i, int h) { return Narrow::cell(i, h); }
+    __device__ __forceinline__ static void per_cell(const float *v, int b, int h, float (&out)[16]) { Narrow::per_cell(v, b, h, out); }
+};
+template <int DP>
+struct Math<F32S, DP> : SplitMath<DP, 3> {};
+template <int DP>
+struct Math<F32C, DP> : SplitMath<DP, 1> {};
+
 // Channel of output accumulator register i of a 32-channel block.
 __device__ __forceinline__ int out_channel(int i, int h) { return 8 * (i >> 2) + 4 * h + (i & 3); }
 
@@ -323,24 +475,21 @@ __device__ __forceinline__ void store_columns(E *map, int64_t n, int64_t q, int 
     });
 }
 
-// Loader of one tile: NT threads, thread t takes segment t & 7 of channel rows t / 8, t / 8 + NT / 8, ...
+// Loader of one tile of codes: NT threads, thread t takes segment t & 7 of channel rows t / 8, t / 8 + NT / 8, ... and
+// turns them into bfloat16, which holds an 8-bit code exactly; scales are applied to scores and weights.
 // kAhead: the whole share of a thread fits a few registers, so that the loads of the next tile are issued (load) before
 // the products of the present one and written to LDS (store) after them; else store does both, a few rows at a time.
-// live: bit j = cell j of the tile takes part; scale: the codes' scale of the tile's cell lane % kRows (float32
-// arithmetic multiplies here, bfloat16 arithmetic keeps the codes, which bfloat16 holds exactly, and scales the scores
-// and weights).
-// Cells past the map's end, masked cells and channels past d are staged as zeros: whatever a masked cell holds
-// (infinities, NaN) meets a weight of zero in the second product and must not turn it into NaN.
+// live: bit j = cell j of the tile takes part.  Cells past the map's end, masked cells and channels past d are staged as
+// zeros: whatever a masked cell holds (a NaN code) meets a weight of zero in the second product and must not turn it
+// into NaN.
 template <typename M, typename SRC, int DP, int NT>
 struct Loader {
-    static constexpr bool kCodes = std::is_same_v<SRC, I8> || std::is_same_v<SRC, FP8>;
-    static constexpr bool kNarrow = std::is_same_v<typename M::map, BF16>;
     static constexpr int kN = M::kCells;
     static constexpr int kPer = DP * 8 / NT;
     typedef typename SRC::elem elem;
-    typedef std::conditional_t<!kCodes, u32x4, std::conditional_t<kNarrow, u32x2, unsigned>> raw;
+    typedef u32x2 raw;
     static constexpr bool kAhead = kPer * (int)sizeof(raw) <= (DP == 256 ? 32 : 128);
-    static constexpr int kBatch = kAhead ? kPer : DP == 256 ? (kCodes || NT == 64 ? 1 : 2) : kPer < 8 ? kPer : 8;
+    static constexpr int kBatch = kAhead ? kPer : DP == 256 ? 1 : kPer < 8 ? kPer : 8;
     static constexpr int kLoop = kAhead ? kPer / kBatch : 1;
     static_assert(NT == 64 || NT % 128 == 0, "");
     raw r[kBatch];
@@ -374,50 +523,29 @@ struct Loader {
         from = base + (int64_t)(threadIdx.x >> 3) * ld + at;
         if constexpr (kAhead) rows(0, ld, d);
     }
-    __device__ __forceinline__ void store(char *tile, int64_t ld, int d, uint64_t live, float scale) {
+    __device__ __forceinline__ void store(char *tile, int64_t ld, int d, uint64_t live) {
         const int seg = threadIdx.x & 7, row0 = threadIdx.x >> 3;
         const unsigned bits = (unsigned)(live >> (seg * kN)) & ((1u << kN) - 1u);
-        const bool whole = live == (M::kRows == 64 ? ~0ull : 0xffffffffull);
         u32x4 keep;
 #pragma unroll
-        for (int j = 0; j < 4; ++j) {
-            if constexpr (kNarrow)
-                keep[j] = ((bits >> (2 * j)) & 1u ? 0xffffu : 0u) | ((bits >> (2 * j + 1)) & 1u ? 0xffff0000u : 0u);
-            else
-                keep[j] = (bits >> j) & 1u ? 0xffffffffu : 0u;
-        }
-        float sc[4] = {};
-        if constexpr (kCodes && !kNarrow)
-#pragma unroll
-            for (int j = 0; j < 4; ++j) sc[j] = __shfl(scale, seg * 4 + j);
+        for (int j = 0; j < 4; ++j)
+            keep[j] = ((bits >> (2 * j)) & 1u ? 0xffffu : 0u) | ((bits >> (2 * j + 1)) & 1u ? 0xffff0000u : 0u);
         const int at0 = row0 * kRowBytes + ((seg ^ swz(row0)) << 4);
 #pragma unroll kLoop
         for (int i0 = 0; i0 < kPer; i0 += kBatch) {
             if constexpr (!kAhead) rows(i0, ld, d);
 #pragma unroll
             for (int i = 0; i < kBatch; ++i) {
+                float x[4], y[4];
+                decode4<SRC>(r[i][0], x);
+                decode4<SRC>(r[i][1], y);
                 u32x4 v;
-                if constexpr (!kCodes) {
-                    v = r[i];
-                } else if constexpr (kNarrow) {
-                    float x[4], y[4];
-                    decode4<SRC>(r[i][0], x);
-                    decode4<SRC>(r[i][1], y);
-                    // 8-bit codes fit bfloat16: the upper halves are the values
 #pragma unroll
-                    for (int j = 0; j < 2; ++j) {
-                        v[j] = __builtin_amdgcn_perm(__builtin_bit_cast(unsigned, x[2 * j + 1]),
-                                                     __builtin_bit_cast(unsigned, x[2 * j]), 0x07060302u);
-                        v[2 + j] = __builtin_amdgcn_perm(__builtin_bit_cast(unsigned, y[2 * j + 1]),
-                                                         __builtin_bit_cast(unsigned, y[2 * j]), 0x07060302u);
-                    }
-                } else {
-                    float f[4];
-                    decode4<SRC>(r[i], f);
-#pragma unroll
-                    for (int j = 0; j < 4; ++j) v[j] = __builtin_bit_cast(unsigned, f[j] * sc[j]);
+                for (int j = 0; j < 2; ++j) {
+                    v[j] = uppers(__builtin_bit_cast(unsigned, x[2 * j]), __builtin_bit_cast(unsigned, x[2 * j + 1]));
+                    v[2 + j] = uppers(__builtin_bit_cast(unsigned, y[2 * j]), __builtin_bit_cast(unsigned, y[2 * j + 1]));
                 }
-                if (!whole) v &= keep;
+                if (live != ~0ull) v &= keep;
                 // swz repeats every 16 rows; 8 rows further (one wave) it differs by 2
                 const int at = at0 ^ (NT == 64 ? ((i0 + i) & 1) << 5 : 0);
                 *reinterpret_cast<u32x4 *>(tile + at + (i0 + i) * (NT / 8) * kRowBytes) = v;
@@ -426,14 +554,22 @@ struct Loader {
     }
 };
 
+// A map as Direct streams it: `d` rows (a multiple of 8) of `ld` cells per item, head and plane.
+struct Stream {
+    const void *map;
+    int64_t ld;
+    int d;
+};
+
 // Copies tiles of a map from memory into LDS without a register in between (global_load_lds, 16 bytes a lane), so that the
 // next tile is under way during the products of the present one.  Wave w of WQ moves channel rows 8 (w kShare + e) .. + 7
 // with instruction e; lane l lands on row l / 8, segment l % 8, and fetches the segment that swz keeps there.
 // The map: rows of `ld` cells that start on 16-byte borders (ld a multiple of kCells), `d` rows, a multiple of 8; what
-// does not come like that is copied into such a form first (soft_pack_kernel).
+// does not come like that is copied into such a form first.
 template <typename M, int DP, int WQ>
 struct Direct {
-    static constexpr int kSize = std::is_same_v<typename M::map, BF16> ? 2 : 4;
+    static constexpr int kSize = M::kBytes;
+    static constexpr int kTile = DP * kRowBytes;
     static constexpr int kShare = DP / 8 / WQ;
     static constexpr int kUnroll = kShare > 8 ? 8 : kShare;
     static_assert(kShare == 1 || kShare % 2 == 0, "a wave moves 8 rows or pairs of 8");
@@ -441,25 +577,29 @@ struct Direct {
     unsigned row;              // byte offset of its row
     unsigned ld8;              // bytes of 8 rows
     uint64_t from;             // first row this wave moves
+    uint64_t plane;            // bytes of a plane
     int first, groups;         // its 8-row group; the groups this wave moves that the map has
     int rows;
-    __device__ __forceinline__ void init(const void *map, int64_t ld, int d) {
+    // item: which of the maps (batch item and head)
+    __device__ __forceinline__ void init(const Stream &s, int64_t item) {
         const int lane = threadIdx.x & 63;
-        row = (unsigned)((lane >> 3) * ld * kSize);
+        row = (unsigned)((lane >> 3) * s.ld * kSize);
 #pragma unroll
         for (int odd = 0; odd < 2; ++odd) off[odd] = row + (((lane & 7) ^ swz((lane >> 3) + 8 * odd)) << 4);
-        ld8 = (unsigned)(8 * ld * kSize);
-        rows = d;
+        ld8 = (unsigned)(8 * s.ld * kSize);
+        rows = s.d;
+        plane = (uint64_t)(s.d >> 3) * ld8;
         first = __builtin_amdgcn_readfirstlane((int)threadIdx.x >> 6) * kShare;
-        groups = (d >> 3) - first;
-        const uint64_t at = (uint64_t)map + (uint64_t)first * ld8;
+        groups = (s.d >> 3) - first;
+        const uint64_t at = (uint64_t)s.map + (uint64_t)item * M::kPlanes * plane + (uint64_t)first * ld8;
         from = (uint64_t)(unsigned)__builtin_amdgcn_readfirstlane((int)(uint32_t)at) |
                (uint64_t)(unsigned)__builtin_amdgcn_readfirstlane((int)(uint32_t)(at >> 32)) << 32;
     }
     // Rows past the map's are zero in LDS throughout.
     __device__ __forceinline__ void clear_rest(char *tile) const {
-        for (int i = rows * kRowBytes + (int)threadIdx.x * 16; i < DP * kRowBytes; i += 64 * WQ * 16)
-            *reinterpret_cast<u32x4 *>(tile + i) = u32x4{};
+        for (int x = 0; x < M::kPlanes; ++x)
+            for (int i = rows * kRowBytes + (int)threadIdx.x * 16; i < kTile; i += 64 * WQ * 16)
+                *reinterpret_cast<u32x4 *>(tile + x * kTile + i) = u32x4{};
     }
     // Tile from `cell0` on, of a map with `cells` cells (a multiple of kCells) a row; asynchronous, wait() ends it.
     __device__ __forceinline__ void issue(int cell0, int cells, const char *tile) const {
@@ -470,25 +610,32 @@ struct Direct {
             for (int odd = 0; odd < 2; ++odd)
                 if ((int)((at[odd] - row) / kSize) >= cells - cell0) at[odd] = row;
         }
-        uint64_t src = from + (uint64_t)(unsigned)(cell0 * kSize);
-        unsigned dst = (unsigned)__builtin_amdgcn_readfirstlane(
+        uint64_t base = from + (uint64_t)(unsigned)(cell0 * kSize);
+        unsigned to = (unsigned)__builtin_amdgcn_readfirstlane(
             (int)((unsigned)(uintptr_t)(__attribute__((address_space(3))) const char *)tile + first * 1024));
-        if constexpr (kShare == 1) {
-            if (groups > 0) copy(first & 1 ? at[1] : at[0], src, dst);
-        } else if (groups >= kShare) {
+#pragma unroll
+        for (int x = 0; x < M::kPlanes; ++x) {
+            uint64_t src = base;
+            unsigned dst = to;
+            if constexpr (kShare == 1) {
+                if (groups > 0) copy(first & 1 ? at[1] : at[0], src, dst);
+            } else if (groups >= kShare) {
 #pragma unroll kUnroll
-            for (int e = 0; e < kShare; ++e) {
-                copy(at[e & 1], src, dst);
-                src += ld8;
-                dst += 1024;
-            }
-        } else {
+                for (int e = 0; e < kShare; ++e) {
+                    copy(at[e & 1], src, dst);
+                    src += ld8;
+                    dst += 1024;
+                }
+            } else {
 #pragma unroll 1
-            for (int e = 0; e < groups; ++e) {
-                copy(e & 1 ? at[1] : at[0], src, dst);
-                src += ld8;
-                dst += 1024;
+                for (int e = 0; e < groups; ++e) {
+                    copy(e & 1 ? at[1] : at[0], src, dst);
+                    src += ld8;
+                    dst += 1024;
+                }
             }
+            base += plane;
+            to += kTile;
         }
     }
     __device__ __forceinline__ static void copy(unsigned voff, uint64_t sbase, unsigned dst) {
@@ -520,29 +667,18 @@ struct Direct {
                     keep[j] = (bits >> j) & 1u ? 0xffffffffu : 0u;
             }
             if (kShare == 1 && (first & 1) != odd) continue;
+#pragma unroll
+            for (int x = 0; x < M::kPlanes; ++x)
 #pragma unroll kUnroll
-            for (int e = kShare == 1 ? 0 : odd; e < kShare; e += 2) {
-                if (e < groups) {
-                    u32x4 *p = reinterpret_cast<u32x4 *>(tile + (first + e) * 1024 + lane * 16);
-                    *p = *p & keep;
+                for (int e = kShare == 1 ? 0 : odd; e < kShare; e += 2) {
+                    if (e < groups) {
+                        u32x4 *p = reinterpret_cast<u32x4 *>(tile + x * kTile + (first + e) * 1024 + lane * 16);
+                        *p = *p & keep;
+                    }
                 }
-            }
         }
     }
 };
-
-// Copies maps (maps, d, n) into the form Direct wants: (maps, d8, ld) with d8 the next multiple of 8 rows and ld of kCells
-// cells, zeros beside.
-template <typename T>
-__global__ __launch_bounds__(256) void soft_pack_kernel(const typename T::elem *src, typename T::elem *dst, int d, int d8,
-                                                        int64_t n, int64_t ld, int64_t rows) {
-    const int64_t per = (ld + 255) / 256;
-    const int64_t row = blockIdx.x / per, cell = (blockIdx.x - row * per) * 256 + threadIdx.x;
-    if (row >= rows || cell >= ld) return;
-    const int64_t map = row / d8;
-    const int c = (int)(row - map * d8);
-    dst[row * ld + cell] = c < d && cell < n ? src[(map * d + c) * n + cell] : (typename T::elem)0;
-}
 
 // Workgroups are dealt to the 8 dies in turn; this numbering gives each die a run of successive workgroups, so that those
 // that stream the same maps share one L2.
@@ -552,13 +688,6 @@ __device__ __forceinline__ int die_major(int id, int n) {
 }
 
 // ------------------------------------------------------------------------------------------------
-// A map as Direct streams it: `d` rows (a multiple of 8) of `ld` cells per item and head.
-struct Stream {
-    const void *map;
-    int64_t ld;
-    int d;
-};
-
 // What a call computes; device pointers as the C ABI hands them over.
 struct Params {
     const void *q, *k, *v;                 // (B,heads D,nq), (B,heads D,cells), (B,heads Dv,cells); codes for a store
@@ -600,7 +729,7 @@ struct Score {
     // tanh(y) = 1 - 2 r, r = 1 / (exp(2 y) + 1), whose absolute error of 2e-7 is far below what the inputs of the bfloat16
     // kernels leave.  float32 keeps the relative error near 1e-7 too: below 0.6 the odd polynomial y + y^3 c(y^2), c
     // fitted to (tanh(y) / y - 1) / y^2 on [0, 0.36] by weighted least squares.
-    static constexpr bool kExact = std::is_same_v<T, F32>;
+    static constexpr bool kExact = !std::is_same_v<T, BF16>;
     float in, top, fall, in2;
     bool cap;
     __device__ __forceinline__ Score(const Params &p, int head) {
