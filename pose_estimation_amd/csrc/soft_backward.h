@@ -16,23 +16,24 @@ constexpr bool two_waves = DP <= 128 && WQ > 1 && std::is_same_v<T, BF16>;
 template <typename T>
 __global__ __launch_bounds__(256) void soft_delta_kernel(const Params p, const float *o32, const float *d_lse,
                                                          float *delta) {
-    __shared__ float part[4][64];
-    const int lane = threadIdx.x & 63, g = threadIdx.x >> 6;
-    const int64_t per = (p.nq + 63) / 64;
+    __shared__ float part[8][32];
+    const int lane = threadIdx.x & 31, g = threadIdx.x >> 5;
+    const int64_t per = (p.nq + 31) / 32;
     const int64_t bh = blockIdx.x / per;
-    const int64_t q = (blockIdx.x - bh * per) * 64 + lane;
+    const int64_t q = (blockIdx.x - bh * per) * 32 + lane;
     const bool in = q < p.nq && q < live_queries(p, (int)(bh / p.heads));
     float s = 0.f;
     if (in) {
         const typename T::elem *a = (const typename T::elem *)p.d_out + bh * p.Dv * p.nq + q;
         const float *o = o32 + bh * p.Dv * p.nq + q;
-#pragma unroll 4
-        for (int c = g; c < p.Dv; c += 4) s = fmaf(load_float(a + c * p.nq), o[c * p.nq], s);
+#pragma unroll 8
+        for (int c = g; c < p.Dv; c += 8) s = fmaf(load_float(a + c * p.nq), o[c * p.nq], s);
     }
     part[g][lane] = s;
     __syncthreads();
     if (g != 0 || q >= p.nq) return;
-    s = (part[0][lane] + part[1][lane]) + (part[2][lane] + part[3][lane]);
+    s = ((part[0][lane] + part[1][lane]) + (part[2][lane] + part[3][lane])) +
+        ((part[4][lane] + part[5][lane]) + (part[6][lane] + part[7][lane]));
     const bool some = in && p.lse[bh * p.nq + q] != -__builtin_inff();
     if (d_lse != nullptr && in) s -= d_lse[bh * p.nq + q];
     delta[bh * p.nq + q] = some ? s : 0.f;
@@ -63,21 +64,21 @@ __device__ __forceinline__ void probabilities(const Score<T> &score, const f32x1
 }
 template <typename T, int MODE>
 __device__ __forceinline__ void weights(const Score<T> &score, const f32x16 &acc, float (&w)[16], const f32x16 &dp,
-                                        const float (&delta)[16]) {
+                                        float delta) {
     if (MODE == kPlain || MODE == kRows || (MODE == kGeneral && !score.cap)) {
 #pragma unroll
-        for (int i = 0; i < 16; ++i) w[i] = exp2_(fmaf(score.in, acc[i], w[i])) * (dp[i] - delta[i]);
+        for (int i = 0; i < 16; ++i) w[i] = exp2_(fmaf(score.in, acc[i], w[i])) * (dp[i] - delta);
     } else if constexpr (Score<T>::kExact) {
 #pragma unroll
         for (int i = 0; i < 16; ++i) {
             const float th = score.bend(acc[i]);
-            w[i] = exp2_(fmaf(score.top, th, w[i])) * ((dp[i] - delta[i]) * fmaf(-th, th, 1.f));
+            w[i] = exp2_(fmaf(score.top, th, w[i])) * ((dp[i] - delta) * fmaf(-th, th, 1.f));
         }
     } else {
 #pragma unroll
         for (int i = 0; i < 16; ++i) {
             const float r = score.r(acc[i]);
-            w[i] = exp2_(fmaf(-2.f * score.top, r, w[i])) * ((dp[i] - delta[i]) * (4.f * fmaf(-r, r, r)));
+            w[i] = exp2_(fmaf(-2.f * score.top, r, w[i])) * ((dp[i] - delta) * (4.f * fmaf(-r, r, r)));
         }
     }
 }
@@ -109,16 +110,16 @@ __global__ __launch_bounds__(64 * WQ, (two_waves<T, DP, WQ>) ? 2 : 1) void soft_
     const int split = id % p.splits;
     const int bh = id / p.splits;
     const int b = bh / p.heads, head = bh - b * p.heads;
-    const int64_t live_q = live_queries(p, b);
-    const int64_t q = ((int64_t)qblk * WQ + wave) * 32 + (lane & 31);
+    const int live_q = (int)live_queries(p, b), nq = (int)p.nq;            // fewer than 2^22
+    const int q = (qblk * WQ + wave) * 32 + (lane & 31);
     const bool q_ok = q < live_q;
-    const bool idle = (int64_t)qblk * WQ * 32 >= live_q;
+    const bool idle = qblk * WQ * 32 >= live_q;
     const int t0 = (int)((int64_t)p.tiles * split / p.splits);
     const int t1 = idle ? t0 : (int)((int64_t)p.tiles * (split + 1) / p.splits);
 
     typename M::Owned qf, of;
-    M::load_owned(qf, (const typename T::elem *)p.q + (int64_t)bh * p.D * p.nq + (q < p.nq ? q : 0), p.nq, p.D, q_ok, h);
-    M::load_owned(of, (const typename T::elem *)p.d_out + (int64_t)bh * p.Dv * p.nq + (q < p.nq ? q : 0), p.nq, p.Dv, q_ok, h);
+    M::load_owned(qf, (const typename T::elem *)p.q + (int64_t)bh * p.D * p.nq + (q < nq ? q : 0), p.nq, p.D, q_ok, h);
+    M::load_owned(of, (const typename T::elem *)p.d_out + (int64_t)bh * p.Dv * p.nq + (q < nq ? q : 0), p.nq, p.Dv, q_ok, h);
     const typename M::Addr addr = M::addr(lane);
     const Score<T> score(p, head);
     float qx = 0.f, qy = 0.f;
@@ -134,19 +135,19 @@ __global__ __launch_bounds__(64 * WQ, (two_waves<T, DP, WQ>) ? 2 : 1) void soft_
 #pragma unroll
         for (int i = 0; i < 16; ++i) g[c][i] = 0.f;
 
-    Feed<T, T, DP, WQ, 2> feed(p, b, head, lds);
+    Feed<T, T, DP, WQ, 2> feed(p, b, head, t0, lds);
     const bool phased = kMayPhase<M> && feed.phased;
-    const Penalty<M, MODE, false> penalty(p, score.fall, qx, qy, true);
+    const Penalty<M, MODE, false> penalty(p, score.fall, qx, qy);
     const f32x16 from = penalty.from(score.in);
     uint64_t next = 0;                                         // live cells of the next tile
     int next_cell0 = 0;
     auto finish = [&](int i) {
-        next = feed.end_k(i);
+        next = feed.end_k(i, penalty.wants_places());
         if (!phased) feed.end_v(i, next);
-        next_cell0 = (int)feed.at.cell0;
+        next_cell0 = feed.keys.cell0;
     };
     if (t0 < t1) {
-        feed.begin_k(t0, 0);
+        feed.begin_k(0);
         if (!phased) feed.begin_v(0);
         finish(0);
     }
@@ -156,7 +157,7 @@ __global__ __launch_bounds__(64 * WQ, (two_waves<T, DP, WQ>) ? 2 : 1) void soft_
         if (phased) {
             feed.begin_v(0);
         } else if (t + 1 < t1) {
-            feed.begin_k(t + 1, j);
+            feed.begin_k(j);
             feed.begin_v(j);
         }
         const uint64_t live = next;
@@ -169,7 +170,7 @@ __global__ __launch_bounds__(64 * WQ, (two_waves<T, DP, WQ>) ? 2 : 1) void soft_
             if (phased) {
                 feed.end_v(0, live);
                 __syncthreads();                               // the value's tile is there
-                if (t + 1 < t1) feed.begin_k(t + 1, j);
+                if (t + 1 < t1) feed.begin_k(j);
             }
         }
         if (live != 0) {
@@ -180,16 +181,14 @@ __global__ __launch_bounds__(64 * WQ, (two_waves<T, DP, WQ>) ? 2 : 1) void soft_
                 if constexpr (kMayPhase<M>) acc[0] = ahead[k];
                 else M::first(ktile, addr, k, qf, acc, from);
                 M::first(vtile, addr, k, of, dp);
-                float w[16], dl[16];
+                float w[16];
                 if (MODE == kRows || penalty.on) {
                     penalty(cell + 64, cell0, k, h, minus, w);
                 } else {
 #pragma unroll
                     for (int i = 0; i < 16; ++i) w[i] = minus;
                 }
-#pragma unroll
-                for (int i = 0; i < 16; ++i) dl[i] = delta;
-                weights<T, MODE>(score, acc[0], w, dp[0], dl);
+                weights<T, MODE>(score, acc[0], w, dp[0], delta);
                 if (live != kAll) {
                     stay_branch();
                     const unsigned bits = (unsigned)(live >> (32 * k)) >> M::cell(0, h);
@@ -202,20 +201,21 @@ __global__ __launch_bounds__(64 * WQ, (two_waves<T, DP, WQ>) ? 2 : 1) void soft_
         if (t + 1 < t1) finish(j);
         __syncthreads();
     }
-    if (q >= p.nq) return;
-    if (p.parts) {
+    LateParams &e = late_params();
+    if (q >= e.nq) return;
+    if (e.parts) {
 #pragma unroll
         for (int c = 0; c < NC / 32; ++c)
 #pragma unroll
             for (int i = 0; i < 16; ++i) g[c][i] = q_ok ? g[c][i] : 0.f;
-        store_columns<NC>(p.part_a + ((int64_t)split * p.B * p.heads + bh) * p.D * p.nq, p.nq, q, h, p.c0, p.D, g);
+        store_columns<NC>(e.part_a + ((int64_t)split * e.B * e.heads + bh) * e.D * e.nq, e.nq, q, h, e.c0, e.D, g);
         return;
     }
 #pragma unroll
     for (int c = 0; c < NC / 32; ++c)
 #pragma unroll
-        for (int i = 0; i < 16; ++i) g[c][i] = q_ok ? g[c][i] * p.scale : 0.f;
-    store_columns<NC>((typename T::elem *)p.dq + (int64_t)bh * p.D * p.nq, p.nq, q, h, p.c0, p.D, g);
+        for (int i = 0; i < 16; ++i) g[c][i] = q_ok ? g[c][i] * e.scale : 0.f;
+    store_columns<NC>((typename T::elem *)e.dq + (int64_t)bh * e.D * e.nq, e.nq, q, h, e.c0, e.D, g);
 }
 
 // Gradients of the reference and value maps: owned = cells, streamed = queries.  PART 0: both; 1: the value's, 2: the
@@ -225,7 +225,7 @@ template <typename T, int DP, int WQ, int PART, int NC, int MODE>
 __global__ __launch_bounds__(64 * WQ, (two_waves<T, DP, WQ> && (DP <= 64 || PART != 0)) ? 2 : 1) void soft_dkv_kernel(const Params p) {
     typedef Math<T, DP> M;
     constexpr int kBlocks = M::kRows / 32;
-    constexpr int kUnroll = DP == 256 || (DP == 128 && PART == 2) ? 1 : kBlocks;           // registers
+    constexpr int kUnroll = !kMayPhase<M> && (DP == 256 || (DP == 128 && PART == 2)) ? 1 : kBlocks;           // registers
     constexpr bool kDv = PART != 2, kDk = PART != 1;
     constexpr uint64_t kAll = M::kRows == 64 ? ~0ull : 0xffffffffull;
     extern __shared__ __attribute__((aligned(16))) char lds[];
@@ -238,18 +238,18 @@ __global__ __launch_bounds__(64 * WQ, (two_waves<T, DP, WQ> && (DP <= 64 || PART
     const int split = id % p.splits;
     const int bh = id / p.splits;
     const int b = bh / p.heads, head = bh - b * p.heads;
-    const int64_t live_q = live_queries(p, b);
-    const int tiles = (int)((live_q + M::kRows - 1) / M::kRows);
+    const int live_q = (int)live_queries(p, b);                // fewer than 2^22
+    const int tiles = (live_q + M::kRows - 1) / M::kRows;
     const int t0 = (int)((int64_t)tiles * split / p.splits), t1 = (int)((int64_t)tiles * (split + 1) / p.splits);
-    const int64_t cell = ((int64_t)blk * WQ + wave) * 32 + (lane & 31);
-    const bool c_ok = cell < p.cells && (p.mask == nullptr || p.mask[(int64_t)b * p.cells + cell] != 0);
-    const float cx = (float)((int)cell % p.W), cy = (float)((int)cell / p.W);
+    const int cell = (blk * WQ + wave) * 32 + (lane & 31), cells = (int)p.cells;   // fewer than 2^22
+    const bool c_ok = cell < cells && (p.mask == nullptr || p.mask[(int64_t)b * p.cells + cell] != 0);
+    const float cx = (float)(cell % p.W), cy = (float)(cell / p.W);
 
     typename M::Owned kf, vf;
-    M::load_owned(kf, (const typename T::elem *)p.k + (int64_t)bh * p.D * p.cells + (cell < p.cells ? cell : 0), p.cells, p.D,
+    M::load_owned(kf, (const typename T::elem *)p.k + (int64_t)bh * p.D * p.cells + (cell < cells ? cell : 0), p.cells, p.D,
                   c_ok, h);
     if constexpr (kDk)
-        M::load_owned(vf, (const typename T::elem *)p.v + (int64_t)bh * p.Dv * p.cells + (cell < p.cells ? cell : 0), p.cells, p.Dv,
+        M::load_owned(vf, (const typename T::elem *)p.v + (int64_t)bh * p.Dv * p.cells + (cell < cells ? cell : 0), p.cells, p.Dv,
                       c_ok, h);
     const typename M::Addr addr = M::addr(lane);
     const Score<T> score(p, head);
@@ -262,9 +262,9 @@ __global__ __launch_bounds__(64 * WQ, (two_waves<T, DP, WQ> && (DP <= 64 || PART
             if constexpr (kDv) gv[c][i] = 0.f;
         }
 
-    const Penalty<M, MODE> penalty(p, score.fall, cx, cy, p.query_xy == nullptr);
+    const Penalty<M, MODE, std::is_same_v<T, BF16>> penalty(p, score.fall, cx, cy);
     const f32x16 from = penalty.from(score.in);
-    // buffers as in Feed: twice (query tile, per query -log-sum, delta and place), then the gradient's tiles, of which
+    // buffers as in Feed: twice (query tile, per query -log-sum, -delta and place), then the gradient's tiles, of which
     // three planes leave room for one
     typedef Direct<M, DP, WQ> Copy;
     constexpr bool phased = kMayPhase<M>;
@@ -278,13 +278,13 @@ __global__ __launch_bounds__(64 * WQ, (two_waves<T, DP, WQ> && (DP <= 64 || PART
     }
     float minus = 0.f, delta = 0.f, px = 0.f, py = 0.f;
     auto live_of = [&](int t) {                                // what lies behind the live queries counts as zeros
-        const int64_t left = live_q - (int64_t)t * M::kRows;
+        const int left = live_q - t * M::kRows;
         return left < M::kRows ? (1ull << left) - 1 : kAll;
     };
     auto begin_q = [&](int t, int i) {
-        const int64_t q0 = (int64_t)t * M::kRows;
+        const int q0 = t * M::kRows;
         if (threadIdx.x < M::kRows) {
-            const int64_t q = q0 + threadIdx.x;
+            const int q = q0 + (int)threadIdx.x;
             minus = -__builtin_inff();
             delta = 0.f;
             if (q < live_q) {
@@ -293,7 +293,7 @@ __global__ __launch_bounds__(64 * WQ, (two_waves<T, DP, WQ> && (DP <= 64 || PART
                 if (penalty.wants_places()) query_place(p, b, q, px, py);
             }
         }
-        cq.issue((int)q0, (int)p.sq.ld, lds + i * kStage);
+        cq.issue(q0, (int)p.sq.ld, lds + i * kStage);
     };
     auto begin_o = [&](int t, int i) { co.issue(t * M::kRows, (int)p.so.ld, lds + 2 * kStage + i * kTile); };
     auto end_q = [&](int t, int i) {
@@ -303,7 +303,7 @@ __global__ __launch_bounds__(64 * WQ, (two_waves<T, DP, WQ> && (DP <= 64 || PART
         if (threadIdx.x < M::kRows) {
             float *cell = reinterpret_cast<float *>(lds + i * kStage + kTile) + threadIdx.x;
             cell[0] = minus;
-            cell[64] = delta;
+            cell[64] = -delta;
             cell[128] = px;
             cell[192] = py;
         }
@@ -325,6 +325,14 @@ __global__ __launch_bounds__(64 * WQ, (two_waves<T, DP, WQ> && (DP <= 64 || PART
         const char *qtile = lds + i * kStage, *otile = lds + 2 * kStage + (phased ? 0 : i) * kTile;
         const float *larr = reinterpret_cast<const float *>(qtile + kTile);
         const float *darr = larr + 64, *xarr = larr + 128;
+        auto minus_delta = [&](int k) {                        // what dP is added to
+            float v[16];
+            M::per_cell(darr, k, h, v);
+            f32x16 x;
+#pragma unroll
+            for (int i = 0; i < 16; ++i) x[i] = v[i];
+            return x;
+        };
         f32x16 ahead[phased ? kBlocks : 1];                    // scores, where they come a phase before the rest
         if constexpr (phased) {
             begin_o(t, 0);
@@ -332,7 +340,7 @@ __global__ __launch_bounds__(64 * WQ, (two_waves<T, DP, WQ> && (DP <= 64 || PART
 #pragma unroll
                 for (int k = 0; k < kBlocks; ++k) {
                     f32x16 acc[1];
-                    M::first(qtile, addr, k, kf, acc, from);
+                    M::template first<1, MODE != kGeneral>(qtile, addr, k, kf, acc, from);
                     ahead[k] = acc[0];
                 }
             } else {
@@ -347,6 +355,7 @@ __global__ __launch_bounds__(64 * WQ, (two_waves<T, DP, WQ> && (DP <= 64 || PART
         }
 #pragma unroll kUnroll
         for (int k = 0; k < kBlocks; ++k) {
+            if constexpr (phased) __builtin_amdgcn_sched_barrier(0);
             f32x16 acc[1];
             if constexpr (phased) acc[0] = ahead[k];
             else M::first(qtile, addr, k, kf, acc, from);
@@ -366,21 +375,17 @@ __global__ __launch_bounds__(64 * WQ, (two_waves<T, DP, WQ> && (DP <= 64 || PART
                 M::second(otile + p.c0 * kRowBytes, addr, k, M::weights(w), gv);
                 if constexpr (kDk) {
                     f32x16 dp[1];
-                    M::first(otile, addr, k, vf, dp);
-                    float dl[16];
-                    M::per_cell(darr, k, h, dl);
+                    M::first(otile, addr, k, vf, dp, minus_delta(k));
 #pragma unroll
-                    for (int i = 0; i < 16; ++i) w[i] *= dp[0][i] - dl[i];
+                    for (int i = 0; i < 16; ++i) w[i] *= dp[0][i];
                     if (MODE == kCapped || (MODE == kGeneral && score.cap))
 #pragma unroll
                         for (int i = 0; i < 16; ++i) w[i] *= slope[i];
                 }
             } else {
                 f32x16 dp[1];
-                M::first(otile, addr, k, vf, dp);
-                float dl[16];
-                M::per_cell(darr, k, h, dl);
-                weights<T, MODE>(score, acc[0], w, dp[0], dl);
+                M::template first<1, !(phased && MODE == kGeneral)>(otile, addr, k, vf, dp, minus_delta(k));
+                weights<T, MODE>(score, acc[0], w, dp[0], 0.f);
             }
             if constexpr (kDk) M::second(qtile + p.c0 * kRowBytes, addr, k, M::weights(w), gk);
         }
@@ -390,37 +395,38 @@ __global__ __launch_bounds__(64 * WQ, (two_waves<T, DP, WQ> && (DP <= 64 || PART
         }
         __syncthreads();
     }
-    if (cell >= p.cells) return;
+    LateParams &e = late_params();
+    if (cell >= e.cells) return;
     // masked cells take no part: their columns hold zeros' products and are dropped here
-    const int64_t part = (int64_t)split * p.B * p.heads + bh;
+    const int64_t part = (int64_t)split * e.B * e.heads + bh;
 #pragma unroll
     for (int c = 0; c < NC / 32; ++c)
 #pragma unroll
         for (int i = 0; i < 16; ++i) {
-            if constexpr (kDk) gk[c][i] = c_ok ? gk[c][i] * p.scale : 0.f;
+            if constexpr (kDk) gk[c][i] = c_ok ? gk[c][i] * e.scale : 0.f;
             if constexpr (kDv) gv[c][i] = c_ok ? gv[c][i] : 0.f;
         }
     typedef typename T::elem elem;
-    float *pv = p.part_b + part * p.Dv * p.cells;
-    elem *dk = (elem *)p.dk + (int64_t)bh * p.D * p.cells, *dv = (elem *)p.dv + (int64_t)bh * p.Dv * p.cells;
-    if (p.parts) {
-        if constexpr (kDk) store_columns<NC>(p.part_a + part * p.D * p.cells, p.cells, cell, h, p.c0, p.D, gk);
-        if constexpr (kDv) store_columns<NC>(pv, p.cells, cell, h, p.c0, p.Dv, gv);
-    } else if (!p.shared) {
-        if constexpr (kDk) store_columns<NC>(dk, p.cells, cell, h, p.c0, p.D, gk);
-        if constexpr (kDv) store_columns<NC>(dv, p.cells, cell, h, p.c0, p.Dv, gv);
+    float *pv = e.part_b + part * e.Dv * e.cells;
+    elem *dk = (elem *)e.dk + (int64_t)bh * e.D * e.cells, *dv = (elem *)e.dv + (int64_t)bh * e.Dv * e.cells;
+    if (e.parts) {
+        if constexpr (kDk) store_columns<NC>(e.part_a + part * e.D * e.cells, e.cells, cell, h, e.c0, e.D, gk);
+        if constexpr (kDv) store_columns<NC>(pv, e.cells, cell, h, e.c0, e.Dv, gv);
+    } else if (!e.shared) {
+        if constexpr (kDk) store_columns<NC>(dk, e.cells, cell, h, e.c0, e.D, gk);
+        if constexpr (kDv) store_columns<NC>(dv, e.cells, cell, h, e.c0, e.Dv, gv);
     } else if constexpr (PART == 1) {                          // shared: the sum of both uses, rounded once
-        store_columns<NC>(pv, p.cells, cell, h, p.c0, p.Dv, gv);       // float32, for the launch that forms the other one
+        store_columns<NC>(pv, e.cells, cell, h, e.c0, e.Dv, gv);       // float32, for the launch that forms the other one
     } else {
 #pragma unroll
         for (int c = 0; c < NC / 32; ++c)
 #pragma unroll
             for (int i = 0; i < 16; ++i) {
-                const int ch = p.c0 + 32 * c + out_channel(i, h);
-                if constexpr (PART == 2) gk[c][i] += ch < p.D ? pv[ch * p.cells + cell] : 0.f;
+                const int ch = e.c0 + 32 * c + out_channel(i, h);
+                if constexpr (PART == 2) gk[c][i] += ch < e.D ? pv[ch * e.cells + cell] : 0.f;
                 else gk[c][i] += gv[c][i];
             }
-        store_columns<NC>(dk, p.cells, cell, h, p.c0, p.D, gk);
+        store_columns<NC>(dk, e.cells, cell, h, e.c0, e.D, gk);
     }
 }
 

@@ -5,41 +5,49 @@
 
 namespace ispa_soft {
 
-// The streamed cells of one item: tile t lies in view t / tiles_per_view of the item.
+// The streamed cells of one item, tile after tile; tile t lies in view t / tiles_per_view of the item.
 template <typename M, typename SRC>
 struct KeyTiles {
     static constexpr bool kCodes = std::is_same_v<SRC, I8> || std::is_same_v<SRC, FP8>;
     const Params &p;
     int b, head;
-    __device__ __forceinline__ KeyTiles(const Params &p_, int b_, int head_) : p(p_), b(b_), head(head_) {}
-    struct At {
-        int64_t map;          // which map of the batch or store; -1 = none
-        int64_t cell0;
-    };
-    __device__ __forceinline__ At at(int t) const {
-        At a;
+    int view, left;            // of the next tile: its view, the view's tiles from it on
+    int64_t map;               // the view's map in the store (-1: none); without a store the batch item's
+    int cell0;                 // of the present tile
+    __device__ __forceinline__ KeyTiles(const Params &p_, int b_, int head_, int t) : p(p_), b(b_), head(head_), map(b_) {
         if constexpr (kCodes) {
-            const int view = t / p.tiles_per_view;
-            const int id = p.views[(int64_t)b * p.V + view];
-            a.map = id >= 0 && id < p.n_view ? id : -1;
-            a.cell0 = (int64_t)(t - view * p.tiles_per_view) * M::kRows;
-        } else {
-            a.map = b;
-            a.cell0 = (int64_t)t * M::kRows;
+            view = t / p.tiles_per_view;
+            left = (view + 1) * p.tiles_per_view - t;
+            find();
         }
-        return a;
+        cell0 = (kCodes ? p.tiles_per_view - left : t) * M::kRows - M::kRows;
     }
-    __device__ __forceinline__ const typename SRC::elem *base(const void *maps, const At &a, int d) const {
-        return (const typename SRC::elem *)maps + ((a.map < 0 ? 0 : a.map) * p.heads + head) * (int64_t)d * p.cells;
+    __device__ __forceinline__ void find() {
+        const int id = view < p.V ? p.views[(int64_t)b * p.V + view] : -1;
+        map = id >= 0 && id < p.n_view ? id : -1;
     }
-    // this lane's cell (lane % kRows) of the tile: takes part?  its scale
-    __device__ __forceinline__ bool live(const At &a, int lane) const {
-        const int64_t c = a.cell0 + (lane & (M::kRows - 1));
-        if (a.map < 0 || c >= p.cells) return false;
-        return p.mask == nullptr || p.mask[a.map * p.cells + c] != 0;
+    __device__ __forceinline__ void next() {
+        cell0 += M::kRows;
+        if constexpr (kCodes) {
+            if (left == 0) {
+                ++view;
+                left = p.tiles_per_view;
+                cell0 = 0;
+                find();
+            }
+            --left;
+        }
     }
-    __device__ __forceinline__ float scale(const At &a, int lane, bool ok) const {
-        if constexpr (kCodes) return ok ? p.kscale[a.map * p.cells + a.cell0 + (lane & (M::kRows - 1))] : 0.f;
+    __device__ __forceinline__ const typename SRC::elem *base(const void *maps, int d) const {
+        return (const typename SRC::elem *)maps + ((map < 0 ? 0 : map) * p.heads + head) * (int64_t)d * p.cells;
+    }
+    // this lane's cell (lane % kRows) of the present tile: whether the map has it; then whether it takes part, its scale
+    __device__ __forceinline__ bool inside(int lane) const { return map >= 0 && cell0 + (lane & (M::kRows - 1)) < (int)p.cells; }
+    __device__ __forceinline__ uint8_t taken(int lane, bool in) const {
+        return p.mask == nullptr ? (uint8_t)1 : in ? p.mask[map * p.cells + cell0 + (lane & (M::kRows - 1))] : (uint8_t)0;
+    }
+    __device__ __forceinline__ float scale(int lane, bool in) const {
+        if constexpr (kCodes) return in ? p.kscale[map * p.cells + cell0 + (lane & (M::kRows - 1))] : 0.f;
         return 0.f;
     }
 };
@@ -88,16 +96,17 @@ struct Feed {
     // the next tile's loads may run during the present tile's products
     static constexpr bool kAhead = std::conditional_t<kCodes, L, None>::kAhead;
     const Params &p;
-    const Keys keys;
+    Keys keys;
     std::conditional_t<kCodes, L, None> codes;
     std::conditional_t<kCodes, None, D> dk, dv;
-    typename Keys::At at{};
-    bool ok = false;
+    bool in = false;           // of this lane's cell in the present tile, as KeyTiles says
+    uint8_t taken = 0;
     float sc = 0.f;
     char *lds;
     int v_at;                  // of the first value tile
     bool phased;
-    __device__ __forceinline__ Feed(const Params &p_, int b, int head, char *lds_) : p(p_), keys(p_, b, head), lds(lds_) {
+    __device__ __forceinline__ Feed(const Params &p_, int b, int head, int t, char *lds_)
+        : p(p_), keys(p_, b, head, t), lds(lds_) {
         phased = kMayPhase<M> && !p.shared;
         v_at = (phased ? PK : 2) * kStage;
         if constexpr (!kCodes) {
@@ -113,34 +122,37 @@ struct Feed {
     __device__ __forceinline__ char *k(int i) const { return lds + i * kStage; }
     __device__ __forceinline__ char *v(int i) const { return p.shared ? k(i) : lds + v_at + (phased ? 0 : i) * kTileBytes<M, DP>; }
     __device__ __forceinline__ const float *cell(int i) const { return reinterpret_cast<const float *>(k(i) + kTileBytes<M, DP>); }
-    __device__ __forceinline__ void begin_k(int t, int i) {
+    __device__ __forceinline__ void begin_k(int i) {           // the next tile
         const int lane = threadIdx.x & 63;
-        at = keys.at(t);
-        ok = keys.live(at, lane);
+        keys.next();
+        in = keys.inside(lane);
+        taken = keys.taken(lane, in);
         if constexpr (kCodes) {
-            sc = keys.scale(at, lane, ok);
-            codes.load(keys.base(p.k, at, p.D), p.cells, p.D, at.cell0, at.map < 0 ? 0 : p.cells);
+            sc = keys.scale(lane, in);
+            codes.load(keys.base(p.k, p.D), p.cells, p.D, keys.cell0, keys.map < 0 ? 0 : p.cells);
         } else {
-            dk.issue((int)at.cell0, (int)p.sk.ld, k(i));
+            dk.issue(keys.cell0, (int)p.sk.ld, k(i));
         }
     }
     __device__ __forceinline__ void begin_v(int i) {           // the tile of the last begin_k
         if constexpr (!kCodes)
-            if (!p.shared) dv.issue((int)at.cell0, (int)p.sv.ld, v(i));
+            if (!p.shared) dv.issue(keys.cell0, (int)p.sv.ld, v(i));
     }
-    __device__ __forceinline__ uint64_t end_k(int i) {         // the tile's live cells
+    // the tile's live cells; places: their coordinates are wanted in LDS
+    __device__ __forceinline__ uint64_t end_k(int i, bool places) {
+        const bool ok = in && taken != 0;
         const uint64_t live = __ballot(ok) & kAll;
         if constexpr (!kCodes) D::wait();
         if (live == 0) return live;                            // the same in every wave
         float *cell = reinterpret_cast<float *>(k(i) + kTileBytes<M, DP>);
         if constexpr (kCodes) {
             codes.store(k(i), p.cells, p.D, live);
-            if (threadIdx.x < 64) cell[threadIdx.x] = sc;
+            if (threadIdx.x < 64) cell[threadIdx.x] = ok ? sc : 0.f;
         } else if (live != kAll) {
             dk.mask(k(i), live);
         }
-        if (p.falloff != nullptr && p.W % M::kCells != 0 && threadIdx.x < M::kRows) {
-            const int c = (int)at.cell0 + threadIdx.x;
+        if (places && threadIdx.x < M::kRows) {
+            const int c = keys.cell0 + threadIdx.x;
             cell[64 + threadIdx.x] = (float)(c % p.W);
             cell[128 + threadIdx.x] = (float)(c / p.W);
         }
@@ -155,13 +167,17 @@ struct Feed {
     }
 };
 
+// Registers for two waves a SIMD: one's products run under the other's exponentials.
+template <typename T, typename SRC, int DP>
+constexpr bool two_resident = std::is_same_v<SRC, BF16> ? DP <= 128 : std::is_same_v<SRC, F32S> && DP <= 64;
+
 // How far (in units of log2) a query's largest score may rise above the maximum that its sums are kept against before they
 // are rescaled: weights stay below 2^8, and nearly all tiles leave the accumulators alone.
 constexpr float kSlack = 8.f;
 
 // NC: value channels that one launch forms, from p.c0 on (256 float32 channels take two launches, for the registers).
 template <typename T, typename SRC, int DP, int WQ, int NC, int MODE>
-__global__ __launch_bounds__(64 * WQ, (DP <= 128 && std::is_same_v<SRC, BF16>) ? 2 : 1) void soft_forward_kernel(const Params p) {
+__global__ __launch_bounds__(64 * WQ, (two_resident<T, SRC, DP>) ? 2 : 1) void soft_forward_kernel(const Params p) {
     typedef Math<T, DP> M;
     constexpr int kBlocks = M::kRows / 32;
     constexpr uint64_t kAll = M::kRows == 64 ? ~0ull : 0xffffffffull;
@@ -177,15 +193,15 @@ __global__ __launch_bounds__(64 * WQ, (DP <= 128 && std::is_same_v<SRC, BF16>) ?
     const int split = id % p.splits;
     const int bh = id / p.splits;
     const int b = bh / p.heads, head = bh - b * p.heads;
-    const int64_t live_q = live_queries(p, b);
-    const int64_t q = ((int64_t)qblk * WQ + wave) * 32 + (lane & 31);
+    const int live_q = (int)live_queries(p, b), nq = (int)p.nq;            // fewer than 2^22
+    const int q = (qblk * WQ + wave) * 32 + (lane & 31);
     const bool q_ok = q < live_q;
-    const bool idle = (int64_t)qblk * WQ * 32 >= live_q;       // no live query in the whole workgroup
+    const bool idle = qblk * WQ * 32 >= live_q;       // no live query in the whole workgroup
     const int t0 = (int)((int64_t)p.tiles * split / p.splits);
     const int t1 = idle ? t0 : (int)((int64_t)p.tiles * (split + 1) / p.splits);
 
     typename M::Owned qf;
-    M::load_owned(qf, (const typename T::elem *)p.q + (int64_t)bh * p.D * p.nq + (q < p.nq ? q : 0), p.nq, p.D, q_ok, h);
+    M::load_owned(qf, (const typename T::elem *)p.q + (int64_t)bh * p.D * p.nq + (q < nq ? q : 0), p.nq, p.D, q_ok, h);
     Score<T> score(p, head);
     if (MODE == kPlain && score.in < 0.f) {                        // largest product = largest score
         M::negate(qf);
@@ -205,19 +221,19 @@ __global__ __launch_bounds__(64 * WQ, (DP <= 128 && std::is_same_v<SRC, BF16>) ?
     // what scores are taken relative to (m once there is one), and how far above it they may lie
     float off = 0.f, room = -__builtin_inff();
 
-    F feed(p, b, head, lds);
+    F feed(p, b, head, t0, lds);
     const bool phased = kMayPhase<M> && feed.phased;
-    const Penalty<M, MODE> penalty(p, score.fall, qx, qy, true);
+    const Penalty<M, MODE> penalty(p, score.fall, qx, qy);
     const f32x16 from = penalty.from(score.in);
     uint64_t next = 0;                                         // live cells of the next tile
     int next_cell0 = 0;
     auto finish = [&](int i) {
-        next = feed.end_k(i);
+        next = feed.end_k(i, penalty.wants_places());
         if (!phased) feed.end_v(i, next);
-        next_cell0 = (int)feed.at.cell0;
+        next_cell0 = feed.keys.cell0;
     };
     if (F::kAhead && t0 < t1) {
-        feed.begin_k(t0, 0);
+        feed.begin_k(0);
         if (!phased) feed.begin_v(0);
         finish(0);
     }
@@ -225,13 +241,13 @@ __global__ __launch_bounds__(64 * WQ, (DP <= 128 && std::is_same_v<SRC, BF16>) ?
     for (int t = t0; t < t1; ++t) {
         const int i = phased || !F::kAhead ? 0 : (t - t0) & 1, j = phased || !F::kAhead ? 0 : i ^ 1;
         if constexpr (!F::kAhead) {
-            feed.begin_k(t, 0);
+            feed.begin_k(0);
             finish(0);
             __syncthreads();
         } else if (phased) {
             feed.begin_v(0);
         } else if (t + 1 < t1) {
-            feed.begin_k(t + 1, j);
+            feed.begin_k(j);
             feed.begin_v(j);
         }
         const uint64_t live = next;
@@ -242,7 +258,16 @@ __global__ __launch_bounds__(64 * WQ, (DP <= 128 && std::is_same_v<SRC, BF16>) ?
         if (live != 0) {
             // z: scores relative to off.  kPlain: the products, scaled in the exponent.  kCapped: relative to the cap, which
             // stands for the maximum: weights are 2^(-2 cap) > 2^-93 at least.
-            M::first(ktile, addr, 0, qf, z, from);
+            if constexpr (DP == 256 && kBlocks == 2) {         // block by block: fewer fragments in registers
+#pragma unroll
+                for (int k = 0; k < kBlocks; ++k) {
+                    f32x16 acc[1];
+                    M::first(ktile, addr, k, qf, acc, from);
+                    z[k] = acc[0];
+                }
+            } else {
+                M::first(ktile, addr, 0, qf, z, from);
+            }
 #pragma unroll
             for (int k = 0; k < kBlocks; ++k) {
                 if constexpr (kCodes) {
@@ -255,6 +280,7 @@ __global__ __launch_bounds__(64 * WQ, (DP <= 128 && std::is_same_v<SRC, BF16>) ?
 #pragma unroll
                     for (int i = 0; i < 16; ++i) z[k][i] = (-2.f * score.top) * score.r(z[k][i]);
                 } else if constexpr (MODE != kPlain) {
+                    if constexpr (!std::is_same_v<T, BF16>) __builtin_amdgcn_sched_barrier(0);
                     float d[16];
                     if (MODE == kRows || penalty.on) {
                         penalty(cell + 64, cell0, k, h, -off, d);
@@ -316,13 +342,14 @@ __global__ __launch_bounds__(64 * WQ, (DP <= 128 && std::is_same_v<SRC, BF16>) ?
             if (phased) {
                 feed.end_v(0, live);
                 __syncthreads();                               // the reference tile is read, the value's is there
-                if (t + 1 < t1) feed.begin_k(t + 1, 0);
+                if (t + 1 < t1) feed.begin_k(0);
             }
         }
         if (live != 0) {
             float sum[2] = {0.f, 0.f};
 #pragma unroll
             for (int k = 0; k < kBlocks; ++k) {
+                if constexpr (!std::is_same_v<T, BF16>) __builtin_amdgcn_sched_barrier(0);     // one block's weights at a time
                 float w[16];
 #pragma unroll
                 for (int i = 0; i < 16; ++i) {
@@ -344,15 +371,16 @@ __global__ __launch_bounds__(64 * WQ, (DP <= 128 && std::is_same_v<SRC, BF16>) ?
         __syncthreads();
     }
     l += __shfl_xor(l, 32);
+    LateParams &e = late_params();
 
-    if (q >= p.nq) return;
-    if (p.splits > 1) {
-        const int64_t part = (int64_t)split * p.B * p.heads + bh;
+    if (q >= e.nq) return;
+    if (e.splits > 1) {
+        const int64_t part = (int64_t)split * e.B * e.heads + bh;
         if (h == 0) {
             const float2 ml = q_ok ? make_float2(m, l) : make_float2(-__builtin_inff(), 0.f);
-            *reinterpret_cast<float2 *>(p.part_ml + (part * p.nq + q) * 2) = ml;
+            *reinterpret_cast<float2 *>(e.part_ml + (part * e.nq + q) * 2) = ml;
         }
-        store_columns<NC>(p.part_o + part * p.Dv * p.nq, p.nq, q, h, p.c0, p.Dv, o);
+        store_columns<NC>(e.part_o + part * e.Dv * e.nq, e.nq, q, h, e.c0, e.Dv, o);
         return;
     }
     const bool some = q_ok && l != 0.f;                        // l is 0 only where no cell takes part (NaN is not)
@@ -361,19 +389,20 @@ __global__ __launch_bounds__(64 * WQ, (DP <= 128 && std::is_same_v<SRC, BF16>) ?
     for (int c = 0; c < NC / 32; ++c)
 #pragma unroll
         for (int i = 0; i < 16; ++i) o[c][i] = some ? o[c][i] * inv : 0.f;
-    store_columns<NC>((typename T::elem *)p.out + (int64_t)bh * p.Dv * p.nq, p.nq, q, h, p.c0, p.Dv, o);
-    if (p.out32 != nullptr) store_columns<NC>(p.out32 + (int64_t)bh * p.Dv * p.nq, p.nq, q, h, p.c0, p.Dv, o);
-    if (h == 0 && p.lse != nullptr)
-        p.lse[(int64_t)bh * p.nq + q] = some ? (m + log2f(l)) * kLn2 : -__builtin_inff();
+    store_columns<NC>((typename T::elem *)e.out + (int64_t)bh * e.Dv * e.nq, e.nq, q, h, e.c0, e.Dv, o);
+    if (e.out32 != nullptr) store_columns<NC>(e.out32 + (int64_t)bh * e.Dv * e.nq, e.nq, q, h, e.c0, e.Dv, o);
+    if (h == 0 && e.lse != nullptr)
+        e.lse[(int64_t)bh * e.nq + q] = some ? (m + log2f(l)) * kLn2 : -__builtin_inff();
 }
 
 // Joins the partial results of a split call: M = max m_s, out = sum_s 2^(m_s - M) o_s / sum_s 2^(m_s - M) l_s.
-// A block joins QB queries; their parts' weights lie in LDS.
-constexpr int kMaxSplits = 512;
-template <typename T, int QB>
+// A block joins QB queries; their parts' weights lie in LDS.  The other 256 / QB threads of a query are dealt to channels
+// (many queries, few parts) or, for at most 64 queries, to parts, whose sums meet in LDS in a fixed order.
+constexpr int kMaxSplits = 512, kManySplits = 64;
+template <typename T>
 __global__ __launch_bounds__(256) void soft_join_kernel(const Params p, int channels_per_block) {
-    constexpr int kMost = QB == 8 ? kMaxSplits : kMaxSplits / 8, kLanes = 256 / QB;
-    __shared__ float w[kMost][QB], ls[kMost][QB];
+    constexpr int QB = 32, kLanes = 256 / QB;
+    __shared__ float w[kManySplits][QB], ls[kManySplits][QB];
     const int qi = threadIdx.x % QB, g = threadIdx.x / QB;
     const int bh = blockIdx.y;
     const int64_t q = (int64_t)blockIdx.x * QB + qi;
@@ -388,12 +417,9 @@ __global__ __launch_bounds__(256) void soft_join_kernel(const Params p, int chan
     __syncthreads();
     float top = -__builtin_inff();
     for (int s = 0; s < p.splits; ++s) top = fmaxf(top, w[s][qi]);
-    __syncthreads();
     if (top == -__builtin_inff()) top = 0.f;                   // no part has a cell, or all scores are NaN
-    for (int s = g; s < p.splits; s += kLanes) w[s][qi] = exp2_(w[s][qi] - top);
-    __syncthreads();
     float l = 0.f;
-    for (int s = 0; s < p.splits; ++s) l = fmaf(w[s][qi], ls[s][qi], l);
+    for (int s = 0; s < p.splits; ++s) l = fmaf(exp2_(w[s][qi] - top), ls[s][qi], l);
     if (!in) return;
     const bool some = l != 0.f;
     const float inv = some ? 1.f / l : 0.f;
@@ -403,13 +429,73 @@ __global__ __launch_bounds__(256) void soft_join_kernel(const Params p, int chan
         const float *src = p.part_o + ((int64_t)bh * p.Dv + c) * p.nq + q;
         const int64_t step = bhn * p.Dv * p.nq;
 #pragma unroll 8
-        for (int s = 0; s < p.splits; ++s) v = fmaf(w[s][qi], src[s * step], v);
+        for (int s = 0; s < p.splits; ++s) v = fmaf(exp2_(w[s][qi] - top), src[s * step], v);
         v = some ? v * inv : 0.f;
         const int64_t at = ((int64_t)bh * p.Dv + c) * p.nq + q;
         store_float((typename T::elem *)p.out + at, v);
         if (p.out32 != nullptr) p.out32[at] = v;
     }
     if (blockIdx.z == 0 && g == 0 && p.lse != nullptr)
+        p.lse[(int64_t)bh * p.nq + q] = some ? (top + log2f(l)) * kLn2 : -__builtin_inff();
+}
+
+// 8 queries x 32 part lanes, kJoinChannels channels a block.
+constexpr int kJoinChannels = 8;
+template <typename T>
+__global__ __launch_bounds__(256) void soft_join_few_kernel(const Params p) {
+    constexpr int kPer = kMaxSplits / 32;                      // parts of a lane
+    __shared__ float part[kJoinChannels][32][8];
+    const int qi = threadIdx.x & 7, g = threadIdx.x >> 3;
+    const int bh = blockIdx.y;
+    const int64_t q = (int64_t)blockIdx.x * 8 + qi;
+    const bool in = q < p.nq;
+    const int64_t bhn = (int64_t)p.B * p.heads;
+    const int c0 = (int)blockIdx.z * kJoinChannels;
+    float m[kPer], l = 0.f, v[kJoinChannels] = {}, top = -__builtin_inff();
+    float ls[kPer];
+#pragma unroll
+    for (int i = 0; i < kPer; ++i) {
+        const int s = g + 32 * i;
+        const float2 ml = in && s < p.splits ? *reinterpret_cast<const float2 *>(p.part_ml + ((s * bhn + bh) * p.nq + q) * 2)
+                                             : make_float2(-__builtin_inff(), 0.f);
+        m[i] = ml.x;
+        ls[i] = ml.y;
+        top = fmaxf(top, ml.x);
+    }
+    part[0][g][qi] = top;
+    __syncthreads();
+    for (int i = 0; i < 32; ++i) top = fmaxf(top, part[0][i][qi]);
+    if (top == -__builtin_inff()) top = 0.f;                   // no part has a cell, or all scores are NaN
+    __syncthreads();
+#pragma unroll
+    for (int i = 0; i < kPer; ++i) {
+        const int s = g + 32 * i;
+        if (s >= p.splits) break;
+        const float w = exp2_(m[i] - top);
+        l = fmaf(w, ls[i], l);
+        const float *src = p.part_o + ((s * bhn + bh) * p.Dv + c0) * p.nq + q;
+#pragma unroll
+        for (int c = 0; c < kJoinChannels; ++c)
+            if (in && c0 + c < p.Dv) v[c] = fmaf(w, src[c * p.nq], v[c]);
+    }
+    part[0][g][qi] = l;
+    __syncthreads();
+    l = 0.f;
+    for (int i = 0; i < 32; ++i) l += part[0][i][qi];
+    __syncthreads();
+#pragma unroll
+    for (int c = 0; c < kJoinChannels; ++c) part[c][g][qi] = v[c];
+    __syncthreads();
+    const bool some = l != 0.f;
+    if (in && g < kJoinChannels && c0 + g < p.Dv) {
+        float x = 0.f;
+        for (int i = 0; i < 32; ++i) x += part[g][i][qi];
+        x = some ? x / l : 0.f;
+        const int64_t at = ((int64_t)bh * p.Dv + c0 + g) * p.nq + q;
+        store_float((typename T::elem *)p.out + at, x);
+        if (p.out32 != nullptr) p.out32[at] = x;
+    }
+    if (in && blockIdx.z == 0 && g == 0 && p.lse != nullptr)
         p.lse[(int64_t)bh * p.nq + q] = some ? (top + log2f(l)) * kLn2 : -__builtin_inff();
 }
 

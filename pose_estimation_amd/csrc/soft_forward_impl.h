@@ -16,11 +16,14 @@ int forward_one(Params p, hipStream_t stream) {
                             stream))
             return rc;
     if (p.splits == 1) return ISPA_OK;
-    // 32 queries a block read their parts in 128-byte runs; few queries with many parts take blocks of 8
-    const int qb = p.nq <= 8 || p.splits > kMaxSplits / 8 ? 8 : 32, per = 32;       // per: channels of a block
-    const dim3 join((unsigned)((p.nq + qb - 1) / qb), (unsigned)(p.B * p.heads), (unsigned)((p.Dv + per - 1) / per));
-    if (qb == 8) soft_join_kernel<T, 8><<<join, 256, 0, stream>>>(p, per);
-    else soft_join_kernel<T, 32><<<join, 256, 0, stream>>>(p, per);
+    const unsigned bh = (unsigned)(p.B * p.heads);
+    if (WQ == 1 || p.splits > kManySplits) {
+        soft_join_few_kernel<T><<<dim3((unsigned)((p.nq + 7) / 8), bh, (unsigned)((p.Dv + kJoinChannels - 1) / kJoinChannels)), 256,
+                                  0, stream>>>(p);
+    } else {
+        const int per = 32;                                   // channels of a block
+        soft_join_kernel<T><<<dim3((unsigned)((p.nq + 31) / 32), bh, (unsigned)((p.Dv + per - 1) / per)), 256, 0, stream>>>(p, per);
+    }
     return ispa::check_launch("soft_join_kernel");
 }
 

@@ -63,18 +63,17 @@ int forward_codes_bf16(const Params &p, bool fp8, int waves, hipStream_t stream)
 int backward_f32(const Params &p, const Plan &dq, const Plan &dkv, hipStream_t stream);
 int backward_bf16(const Params &p, const Plan &dq, const Plan &dkv, hipStream_t stream);
 
-// Calls f with the mode that the kernels of four waves are built for; `grid`: the streamed cells lie on the grid.  float32
-// kernels are bound by their MFMAs and 256 channels by their registers: these have the general form, and the former the
-// plain one.
+// Calls f with the mode that the kernels of four waves are built for; `grid`: the streamed cells lie on the grid.  256
+// channels have the general form alone.
 template <typename T, int DP, typename F>
 int with_mode(const Params &p, bool grid, F f) {
     const bool cap = p.cap > 0.f, pen = p.falloff != nullptr;
     if constexpr (DP <= 128) {
         if (!cap && !pen) return f(std::integral_constant<int, kPlain>{});
-        if constexpr (std::is_same_v<T, BF16>) {
+        if constexpr (std::is_same_v<T, BF16>)
             if (cap && !pen && p.cap <= 32.f) return f(std::integral_constant<int, kCapped>{});
-            if (!cap && grid && p.W % Math<T, DP>::kCells == 0 && std::fabs(p.scale) > 1e-6f) return f(std::integral_constant<int, kRows>{});
-        }
+        if (!cap && grid && p.W % Math<T, DP>::kCells == 0 && std::fabs(p.scale) > 1e-6f)
+            return f(std::integral_constant<int, kRows>{});
     }
     return f(std::integral_constant<int, kGeneral>{});
 }

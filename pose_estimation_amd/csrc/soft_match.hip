@@ -96,15 +96,17 @@ int stream_map(Stream *s, Arithmetic a, const void *map, int64_t maps, int d, in
 }
 
 // Workgroups of four waves a compute unit holds: two where a lane's registers allow it.
-int resident(int dtype, int D, int Dv) { return dtype == ISPA_BF16 && padded_channels(D, Dv) <= 128 ? 2 : 1; }
+int resident(int dtype, int D, int Dv, bool backward) {
+    return padded_channels(D, Dv) <= (dtype == ISPA_BF16 ? 128 : backward ? 0 : 64) ? 2 : 1;
+}
 
 Arithmetic arithmetic_of(int dtype, bool codes, int D, int Dv, int64_t owned) {
     return arithmetic(dtype == ISPA_F32, codes, padded_channels(D, Dv), waves_for(owned));
 }
 
-Plan plan_of(int dtype, bool codes, int64_t groups, int D, int Dv, int64_t owned, int V, int64_t streamed) {
+Plan plan_of(int dtype, bool codes, bool backward, int64_t groups, int D, int Dv, int64_t owned, int V, int64_t streamed) {
     const int64_t r = tile_rows(arithmetic_of(dtype, codes, D, Dv, owned));
-    return make_plan(owned, groups, (streamed + r - 1) / r * V, resident(dtype, D, Dv));
+    return make_plan(owned, groups, (streamed + r - 1) / r * V, resident(dtype, D, Dv, codes || backward));
 }
 
 size_t forward_bytes(const Plan &plan, int B, int heads, int Dv, int64_t nq) {
@@ -112,8 +114,8 @@ size_t forward_bytes(const Plan &plan, int B, int heads, int Dv, int64_t nq) {
 }
 
 void backward_plans(int dtype, int B, int heads, int D, int Dv, int64_t nq, int64_t cells, Plan *dq, Plan *dkv) {
-    *dq = plan_of(dtype, false, (int64_t)B * heads, D, Dv, nq, 1, cells);
-    *dkv = plan_of(dtype, false, (int64_t)B * heads, D, Dv, cells, 1, nq);
+    *dq = plan_of(dtype, false, true, (int64_t)B * heads, D, Dv, nq, 1, cells);
+    *dkv = plan_of(dtype, false, true, (int64_t)B * heads, D, Dv, cells, 1, nq);
 }
 
 
@@ -149,7 +151,7 @@ enum Source { kMaps, kInt8, kFp8 };
 int run_forward(Params &p, int dtype, Source source, void *workspace, size_t workspace_bytes, hipStream_t stream) {
     const bool maps = source == kMaps;
     const int64_t bh = (int64_t)p.B * p.heads;
-    const Plan plan = plan_of(dtype, !maps, bh, p.D, p.Dv, p.nq, p.V, p.cells);
+    const Plan plan = plan_of(dtype, !maps, false, bh, p.D, p.Dv, p.nq, p.V, p.cells);
     const Arithmetic a = arithmetic_of(dtype, !maps, p.D, p.Dv, p.nq);
     const size_t copied = maps ? forward_copies(dtype, p.B, p.heads, p.D, p.Dv, p.nq, p.cells, p.shared) : 0;
     const size_t need = copied + forward_bytes(plan, p.B, p.heads, p.Dv, p.nq);
@@ -181,7 +183,7 @@ extern "C" size_t ispa_soft_match_workspace_bytes(int dtype, int B, int heads, i
     size_t most = 0;
     for (int codes = 0; codes < 2; ++codes) {
         const size_t n = (codes ? 0 : forward_copies(dtype, B, heads, D, Dv, nq, cells, false)) +
-                         forward_bytes(plan_of(dtype, codes, (int64_t)B * heads, D, Dv, nq, views, cells), B, heads, Dv, nq);
+                         forward_bytes(plan_of(dtype, codes, false, (int64_t)B * heads, D, Dv, nq, views, cells), B, heads, Dv, nq);
         most = n > most ? n : most;
     }
     return most;
@@ -324,7 +326,7 @@ extern "C" int ispa_soft_match_backward(const void *q, const void *r, const void
     p.part_a = (float *)(at + align256(bh * nq * sizeof(float)));
     p.part_b = p.part_a + (pkv.splits > 1 ? (size_t)pkv.splits * bh * D * cells : 0);
     if (nq > 0) {
-        const unsigned grid = (unsigned)((nq + 63) / 64 * bh);
+        const unsigned grid = (unsigned)((nq + 31) / 32 * bh);
         if (dtype == ISPA_F32) soft_delta_kernel<F32><<<grid, 256, 0, s>>>(p, out32, d_lse, delta);
         else soft_delta_kernel<BF16><<<grid, 256, 0, s>>>(p, out32, d_lse, delta);
         if (int rc = ispa::check_launch("soft_delta_kernel")) return rc;

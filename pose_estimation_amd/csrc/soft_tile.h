@@ -104,6 +104,13 @@ __device__ __forceinline__ void decode4(unsigned w, float (&f)[4]) {
 template <typename T, int DP>
 struct Math;
 
+// A lane's 512 registers are two halves of 256, and the vector ALU reaches one of them: operands that only MFMAs read are
+// put into the other where both are needed.
+__device__ __forceinline__ bf16x8 accumulator_side(bf16x8 v) {
+    asm("" : "+a"(v));
+    return v;
+}
+
 template <int DP>
 struct Math<BF16, DP> {
     static constexpr int kRows = 64;             // streamed cells per tile
@@ -129,6 +136,7 @@ struct Math<BF16, DP> {
 #pragma unroll
             for (int j = 0; j < 4; ++j) w[j] = ok ? (unsigned)e[2 * j] | ((unsigned)e[2 * j + 1] << 16) : 0u;
             o.f[s] = __builtin_bit_cast(bf16x8, w);
+            if constexpr (DP == 256) o.f[s] = accumulator_side(o.f[s]);
         });
     }
     __device__ __forceinline__ static void negate(Owned &o) {
@@ -159,11 +167,11 @@ struct Math<BF16, DP> {
     }
     // Products of the owned cells with streamed cells 32 b .. 32 b + 31 of a tile, b = b0 .. b0 + N - 1.  The A fragments are
     // read kAhead steps before their MFMAs.  `from`: what the products are added to.
-    template <int N>
+    template <int N, bool AHEAD = true>
     __device__ __forceinline__ static void first(const char *tile, const Addr &a, int b0, const Owned &o, f32x16 (&acc)[N],
                                  const f32x16 &from = f32x16{}) {
         typedef __attribute__((address_space(3))) s16x4 *lds_ptr;
-        constexpr int kSteps = DP / 16, kAhead = DP == 256 ? 1 : 2;
+        constexpr int kSteps = DP / 16, kAhead = DP == 256 ? 0 : 2;
         auto frag = [&](int n, int s) {
             union {
                 s16x4 q[2];
@@ -220,15 +228,16 @@ struct Math<BF16, DP> {
     // Streamed cell (inside its 32) of accumulator register i, i = 0 .. 15.
     __device__ static constexpr int cell(int i, int h) { return 16 * (i >> 3) + 8 * h + (i & 7); }
     // Per-cell floats of a tile's LDS array, in register order.
+    __device__ __forceinline__ static f32x4 four(const float *v, int b, int h, int t) {        // registers 4 t .. 4 t + 3
+        return *reinterpret_cast<const f32x4 *>(v + 32 * b + 16 * (t >> 1) + 8 * h + 4 * (t & 1));
+    }
     __device__ __forceinline__ static void per_cell(const float *v, int b, int h, float (&out)[16]) {
 #pragma unroll
-        for (int s = 0; s < 2; ++s)
+        for (int t = 0; t < 4; ++t) {
+            const f32x4 x = four(v, b, h, t);
 #pragma unroll
-            for (int t = 0; t < 2; ++t) {
-                const f32x4 x = *reinterpret_cast<const f32x4 *>(v + 32 * b + 16 * s + 8 * h + 4 * t);
-#pragma unroll
-                for (int j = 0; j < 4; ++j) out[8 * s + 4 * t + j] = x[j];
-            }
+            for (int j = 0; j < 4; ++j) out[4 * t + j] = x[j];
+        }
     }
 };
 
@@ -269,7 +278,7 @@ struct Math<F32, DP> {
         a.nat = cell * kRowBytes + ((h ^ swz(cell)) << 4);
         return a;
     }
-    template <int N>
+    template <int N, bool AHEAD = true>
     __device__ __forceinline__ static void first(const char *tile, const Addr &a, int, const Owned &o, f32x16 (&acc)[N],
                                  const f32x16 &from = f32x16{}) {
         acc[0] = from;
@@ -303,10 +312,13 @@ struct Math<F32, DP> {
             }
     }
     __device__ static constexpr int cell(int i, int h) { return 8 * (i >> 2) + 4 * h + (i & 3); }
-    __device__ __forceinline__ static void per_cell(const float *v, int, int h, float (&out)[16]) {
+    __device__ __forceinline__ static f32x4 four(const float *v, int, int h, int t) {
+        return *reinterpret_cast<const f32x4 *>(v + 8 * t + 4 * h);
+    }
+    __device__ __forceinline__ static void per_cell(const float *v, int b, int h, float (&out)[16]) {
 #pragma unroll
         for (int t = 0; t < 4; ++t) {
-            const f32x4 x = *reinterpret_cast<const f32x4 *>(v + 8 * t + 4 * h);
+            const f32x4 x = four(v, b, h, t);
 #pragma unroll
             for (int j = 0; j < 4; ++j) out[4 * t + j] = x[j];
         }
@@ -358,7 +370,10 @@ struct SplitMath {
                 for (int x = 0; x < 3; ++x) w[x][j] = uppers(a[x], b[x]);
             }
 #pragma unroll
-            for (int x = 0; x < 3; ++x) o.f[x][s] = __builtin_bit_cast(bf16x8, w[x]);
+            for (int x = 0; x < 3; ++x) {
+                o.f[x][s] = __builtin_bit_cast(bf16x8, w[x]);
+                if constexpr (DP >= 128) o.f[x][s] = accumulator_side(o.f[x][s]);
+            }
             if (DP == 256 && s % 2 == 1) __builtin_amdgcn_sched_barrier(0);
         });
     }
@@ -371,7 +386,7 @@ struct SplitMath {
         });
     }
     // Planes x of one side and y of the other are multiplied where x + y < 3: what is left out lies below 2^-24.
-    template <int N>
+    template <int N, bool AHEAD = true>
     __device__ __forceinline__ static void first(const char *tile, const Addr &a, int b0, const Owned &o, f32x16 (&acc)[N],
                                                  const f32x16 &from = f32x16{}) {
         typedef __attribute__((address_space(3))) s16x4 *lds_ptr;
@@ -387,27 +402,28 @@ struct SplitMath {
                     (lds_ptr)(tile + x * kTile + (a.tr[y] ^ ((b0 + n) << 6)) + s * 16 * kRowBytes));
             return u.v;
         };
-        bf16x8 f[2][PLANES][N];
+        constexpr int kBuf = AHEAD && DP <= 128 ? 2 : 1;       // fragments read a step ahead, where registers are left
+        bf16x8 f[kBuf][PLANES][N];
+        auto read = [&](int s) {
 #pragma unroll
-        for (int x = 0; x < PLANES; ++x)
+            for (int x = 0; x < PLANES; ++x)
 #pragma unroll
-            for (int n = 0; n < N; ++n) f[0][x][n] = frag(x, n, 0);
+                for (int n = 0; n < N; ++n) f[s % kBuf][x][n] = frag(x, n, s);
+        };
+        read(0);
 #pragma unroll
         for (int n = 0; n < N; ++n) acc[n] = from;
         each<kSteps>([&](auto step) {
             constexpr int s = decltype(step)::value;
-            if constexpr (s + 1 < kSteps)
-#pragma unroll
-                for (int x = 0; x < PLANES; ++x)
-#pragma unroll
-                    for (int n = 0; n < N; ++n) f[(s + 1) & 1][x][n] = frag(x, n, s + 1);
+            if constexpr (kBuf == 1 && s > 0) read(s);
+            if constexpr (kBuf == 2 && s + 1 < kSteps) read(s + 1);
 #pragma unroll
             for (int x = PLANES - 1; x >= 0; --x)
 #pragma unroll
                 for (int y = 2 - x; y >= 0; --y)
 #pragma unroll
                     for (int n = 0; n < N; ++n)
-                        acc[n] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(f[s & 1][x][n], o.f[y][s], acc[n], 0, 0, 0);
+                        acc[n] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(f[s % kBuf][x][n], o.f[y][s], acc[n], 0, 0, 0);
             __builtin_amdgcn_sched_barrier(0);
         });
     }
@@ -448,6 +464,7 @@ struct SplitMath {
         });
     }
     __device__ static constexpr int cell(int i, int h) { return Narrow::cell(i, h); }
+    __device__ __forceinline__ static f32x4 four(const float *v, int b, int h, int t) { return Narrow::four(v, b, h, t); }
     __device__ __forceinline__ static void per_cell(const float *v, int b, int h, float (&out)[16]) { Narrow::per_cell(v, b, h, out); }
 };
 template <int DP>
@@ -460,7 +477,7 @@ __device__ __forceinline__ int out_channel(int i, int h) { return 8 * (i >> 2) +
 
 // Stores 32-channel blocks of accumulators: channels c0 .. c0 + NC - 1 of column q of a map (d, n).
 template <int NC, typename E>
-__device__ __forceinline__ void store_columns(E *map, int64_t n, int64_t q, int h, int c0, int d, const f32x16 (&o)[NC / 32]) {
+__device__ __forceinline__ void store_columns(E *map, int64_t n, int q, int h, int c0, int d, const f32x16 (&o)[NC / 32]) {
     E *at = map + 4 * h * n + q;
     each<NC / 32>([&](auto block) {
         constexpr int c = decltype(block)::value;
@@ -472,6 +489,7 @@ __device__ __forceinline__ void store_columns(E *map, int64_t n, int64_t q, int 
             for (int i = 0; i < 16; ++i)
                 if (c0 + 32 * c + out_channel(i, h) < d) store_float(at + (c0 + 32 * c + out_channel(i, 0)) * n, o[c][i]);
         }
+        __builtin_amdgcn_sched_barrier(0);                     // bounds the addresses in registers
     });
 }
 
@@ -571,15 +589,13 @@ struct Direct {
     static constexpr int kSize = M::kBytes;
     static constexpr int kTile = DP * kRowBytes;
     static constexpr int kShare = DP / 8 / WQ;
-    static constexpr int kUnroll = kShare > 8 ? 8 : kShare;
+    static constexpr int kUnroll = kShare > 4 ? 4 : kShare;    // scalar registers
     static_assert(kShare == 1 || kShare % 2 == 0, "a wave moves 8 rows or pairs of 8");
     unsigned off[2];           // byte offset of this lane's segment in rows 8 e .. 8 e + 7 for even, odd 8-row groups
     unsigned row;              // byte offset of its row
     unsigned ld8;              // bytes of 8 rows
     uint64_t from;             // first row this wave moves
-    uint64_t plane;            // bytes of a plane
-    int first, groups;         // its 8-row group; the groups this wave moves that the map has
-    int rows;
+    int first, groups;         // its 8-row group; the groups that the map has from there on
     // item: which of the maps (batch item and head)
     __device__ __forceinline__ void init(const Stream &s, int64_t item) {
         const int lane = threadIdx.x & 63;
@@ -587,18 +603,16 @@ struct Direct {
 #pragma unroll
         for (int odd = 0; odd < 2; ++odd) off[odd] = row + (((lane & 7) ^ swz((lane >> 3) + 8 * odd)) << 4);
         ld8 = (unsigned)(8 * s.ld * kSize);
-        rows = s.d;
-        plane = (uint64_t)(s.d >> 3) * ld8;
         first = __builtin_amdgcn_readfirstlane((int)threadIdx.x >> 6) * kShare;
         groups = (s.d >> 3) - first;
-        const uint64_t at = (uint64_t)s.map + (uint64_t)item * M::kPlanes * plane + (uint64_t)first * ld8;
+        const uint64_t at = (uint64_t)s.map + (uint64_t)item * M::kPlanes * (uint64_t)(s.d >> 3) * ld8 + (uint64_t)first * ld8;
         from = (uint64_t)(unsigned)__builtin_amdgcn_readfirstlane((int)(uint32_t)at) |
                (uint64_t)(unsigned)__builtin_amdgcn_readfirstlane((int)(uint32_t)(at >> 32)) << 32;
     }
     // Rows past the map's are zero in LDS throughout.
     __device__ __forceinline__ void clear_rest(char *tile) const {
         for (int x = 0; x < M::kPlanes; ++x)
-            for (int i = rows * kRowBytes + (int)threadIdx.x * 16; i < kTile; i += 64 * WQ * 16)
+            for (int i = (first + groups) * 8 * kRowBytes + (int)threadIdx.x * 16; i < kTile; i += 64 * WQ * 16)
                 *reinterpret_cast<u32x4 *>(tile + x * kTile + i) = u32x4{};
     }
     // Tile from `cell0` on, of a map with `cells` cells (a multiple of kCells) a row; asynchronous, wait() ends it.
@@ -613,7 +627,7 @@ struct Direct {
         uint64_t base = from + (uint64_t)(unsigned)(cell0 * kSize);
         unsigned to = (unsigned)__builtin_amdgcn_readfirstlane(
             (int)((unsigned)(uintptr_t)(__attribute__((address_space(3))) const char *)tile + first * 1024));
-#pragma unroll
+#pragma unroll 1
         for (int x = 0; x < M::kPlanes; ++x) {
             uint64_t src = base;
             unsigned dst = to;
@@ -634,7 +648,7 @@ struct Direct {
                     dst += 1024;
                 }
             }
-            base += plane;
+            base += (uint64_t)(first + groups) * ld8;
             to += kTile;
         }
     }
@@ -715,6 +729,15 @@ struct Params {
     float scale, cap;
 };
 
+// The kernel's arguments read again: what only the end of a kernel wants need not wait in scalar registers through its loop
+// (the asm keeps the loads from being moved up).
+typedef const __attribute__((address_space(4))) Params LateParams;
+__device__ __forceinline__ LateParams &late_params() {
+    LateParams *p = (LateParams *)__builtin_amdgcn_kernarg_segment_ptr();
+    asm volatile("" : "+s"(p));
+    return *p;
+}
+
 // What a kernel is built for: each sort of score has its own straight code, general ones branch at run time.
 enum Mode {
     kPlain = 0,       // no cap, no falloff
@@ -752,25 +775,24 @@ struct Score {
     }
 };
 
-// offset - falloff d^2 of one owned cell at (x, y) to the 16 streamed cells of a lane.  Streamed cells that lie on the grid
-// come in groups of kCells successive ones; where the width is a multiple of that, a group stays in one row and d^2 grows
-// along it by a quadratic.  kRows: the quadratic's own part, -falloff j^2, is the same in every group and lies in the
-// accumulators' start (`from`), so that one operation a cell is left (FROM: where 16 registers are left for it).  kGeneral: without that, or from places read from
-// LDS (`cell`: 64 x, 64 y).
+// offset - falloff d^2 of one owned cell at (x, y) to the 16 streamed cells of a lane.
+// kRows: streamed cells lie on the grid in groups of kCells successive ones, whose rows' width is a multiple of that: a
+// group stays in one row and d^2 grows along it by a quadratic.  The quadratic's own part, -falloff j^2, is the same in
+// every group and lies in the accumulators' start (`from`), so that one operation a cell is left (FROM: where 16 registers
+// are left for it).  kGeneral: places read from LDS (`cell`: 64 x, 64 y).
 template <typename M, int MODE, bool FROM = true>
 struct Penalty {
-    bool on, rows;
+    bool on;
     float fall, x, y, width, per_width;
-    __device__ __forceinline__ Penalty(const Params &p, float fall_, float x_, float y_, bool grid) {
+    __device__ __forceinline__ Penalty(const Params &p, float fall_, float x_, float y_) {
         on = MODE == kRows || (MODE == kGeneral && p.falloff != nullptr);
-        rows = MODE == kRows || (grid && p.W % M::kCells == 0);
         fall = fall_;
         x = x_;
         y = y_;
         width = (float)p.W;
         per_width = 1.f / width;
     }
-    __device__ __forceinline__ bool wants_places() const { return on && !rows; }
+    __device__ __forceinline__ bool wants_places() const { return MODE == kGeneral && on; }
     __device__ __forceinline__ f32x16 from(float in) const {
         f32x16 v = {};
         if constexpr (MODE == kRows && FROM) {
@@ -781,7 +803,7 @@ struct Penalty {
         return v;
     }
     __device__ __forceinline__ void operator()(const float *cell, int cell0, int k, int h, float offset, float (&z)[16]) const {
-        if (rows) {
+        if constexpr (MODE == kRows) {
 #pragma unroll
             for (int g = 0; g < 16; g += M::kCells) {
                 // cells are fewer than 2^22: c + 0.5 is exact and the quotient's error cannot reach the next integer
@@ -791,16 +813,18 @@ struct Penalty {
                 const float base = fmaf(-fall, fmaf(dx, dx, dy * dy), offset), step = -2.f * fall * dx;
 #pragma unroll
                 for (int j = 0; j < M::kCells; ++j)
-                    z[g + j] = fmaf((float)j, step, MODE == kRows && FROM ? base : fmaf((float)(-j * j), fall, base));
+                    z[g + j] = fmaf((float)j, step, FROM ? base : fmaf((float)(-j * j), fall, base));
             }
         } else {
-            M::per_cell(cell, k, h, z);
 #pragma unroll
-            for (int i = 0; i < 16; ++i) z[i] = (z[i] - x) * (z[i] - x);
-            float cy[16];
-            M::per_cell(cell + 64, k, h, cy);
+            for (int t = 0; t < 4; ++t) {
+                const f32x4 cx = M::four(cell, k, h, t), cy = M::four(cell + 64, k, h, t);
 #pragma unroll
-            for (int i = 0; i < 16; ++i) z[i] = fmaf(-fall, fmaf(cy[i] - y, cy[i] - y, z[i]), offset);
+                for (int j = 0; j < 4; ++j) {
+                    const float dx = cx[j] - x, dy = cy[j] - y;
+                    z[4 * t + j] = fmaf(-fall, fmaf(dx, dx, dy * dy), offset);
+                }
+            }
         }
     }
 };

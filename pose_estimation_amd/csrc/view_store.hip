@@ -36,46 +36,56 @@ __device__ __forceinline__ unsigned char encode(float v) {
     return (unsigned char)(__builtin_amdgcn_cvt_pk_fp8_f32(v, v, 0, false) & 0xff);
 }
 
-// One block: 64 cells of one written view, 4 channel groups.
+// One block: kCellsPer cells of one written view; the other threads of a cell share its channels, at most kHeld each, and
+// hold them in registers between the maximum and the codes, so that features are read once.  Maps of more channels read
+// the rest again.
+constexpr int kCellsPer = 32, kGroups = kThreads / kCellsPer, kHeld = 16;
 template <typename T, typename S>
 __global__ __launch_bounds__(kThreads) void store_write_kernel(const typename T::elem *__restrict__ features,
                                                                const uint8_t *__restrict__ take,
                                                                const int32_t *__restrict__ views, int n, int n_view, int C,
                                                                int64_t cells, unsigned char *__restrict__ codes,
                                                                float *__restrict__ scales, uint8_t *__restrict__ mask) {
-    __shared__ float tops[4][64];
-    const int64_t per = (cells + 63) / 64;
+    __shared__ float tops[kGroups][kCellsPer];
+    const int64_t per = (cells + kCellsPer - 1) / kCellsPer;
     const int item = (int)(blockIdx.x / per);
     const int id = views[item];
     if (id < 0 || id >= n_view) return;                        // uniform
+    const int lane = threadIdx.x % kCellsPer, g = threadIdx.x / kCellsPer;
+    const int64_t cell = (blockIdx.x - item * per) * kCellsPer + lane;
+    const bool in = cell < cells;
+    const typename T::elem *src = features + (int64_t)item * C * cells + cell;
+    float held[kHeld], top = 0.f;
+#pragma unroll
+    for (int i = 0; i < kHeld; ++i) {
+        const int c = g + kGroups * i;
+        held[i] = in && c < C ? load_float(src + c * cells) : 0.f;
+    }
+    auto larger = [&](float x) {
+        const float a = fabsf(x);
+        top = a <= __builtin_inff() ? fmaxf(top, a) : __builtin_inff();        // NaN counts as infinite
+    };
+#pragma unroll
+    for (int i = 0; i < kHeld; ++i) larger(held[i]);
+    if (in)
+        for (int c = g + kGroups * kHeld; c < C; c += kGroups) larger(load_float(src + c * cells));
+    tops[g][lane] = top;
     // a view listed more than once keeps its last entry
     int later = 0;
     for (int i = item + 1 + (int)threadIdx.x; i < n; i += kThreads) later |= views[i] == id;
     if (__syncthreads_or(later)) return;
-    const int lane = threadIdx.x & 63, g = threadIdx.x >> 6;
-    const int64_t cell = (blockIdx.x - item * per) * 64 + lane;
-    const bool in = cell < cells;
-    const typename T::elem *src = features + (int64_t)item * C * cells + cell;
-    float top = 0.f;
-    if (in)
-#pragma unroll 8
-        for (int c = g; c < C; c += 4) {
-            const float a = fabsf(load_float(src + c * cells));
-            top = a <= __builtin_inff() ? fmaxf(top, a) : __builtin_inff();        // NaN counts as infinite
-        }
-    tops[g][lane] = top;
-    __syncthreads();
-    top = fmaxf(fmaxf(tops[0][lane], tops[1][lane]), fmaxf(tops[2][lane], tops[3][lane]));
+#pragma unroll
+    for (int i = 0; i < kGroups; ++i) top = fmaxf(top, tops[i][lane]);
     if (!in) return;
     const bool finite = top < __builtin_inff();
     const float s = finite ? top * kPerTop<S> : 0.f;
     const float inv = s > 1e-30f ? 1.f / s : 0.f;              // 1 / s may overflow below: divides there
     unsigned char *dst = codes + (int64_t)id * C * cells + cell;
-#pragma unroll 8
-    for (int c = g; c < C; c += 4) {
-        const float x = finite ? load_float(src + c * cells) : 0.f;
-        dst[c * cells] = s > 0.f ? encode<S>(quantised<S>(x, s, inv)) : (unsigned char)0;
-    }
+    auto write = [&](int c, float x) { dst[c * cells] = s > 0.f ? encode<S>(quantised<S>(x, s, inv)) : (unsigned char)0; };
+#pragma unroll
+    for (int i = 0; i < kHeld; ++i)
+        if (g + kGroups * i < C) write(g + kGroups * i, held[i]);
+    for (int c = g + kGroups * kHeld; c < C; c += kGroups) write(c, load_float(src + c * cells));
     if (g == 0) {
         scales[(int64_t)id * cells + cell] = s;
         mask[(int64_t)id * cells + cell] = finite && (take == nullptr || take[(int64_t)item * cells + cell] != 0);
@@ -114,7 +124,7 @@ int check(int dtype, int kind, int n, int n_view, int C, int64_t cells) {
     ISPA_REQUIRE(kind == ISPA_STORE_INT8 || kind == ISPA_STORE_FP8, "store kind %d is neither int8 nor e4m3", kind);
     ISPA_REQUIRE(n >= 0 && n_view >= 1 && C >= 1 && cells >= 1, "store sizes out of range (n %d, views %d, channels %d)", n,
                  n_view, C);
-    ISPA_REQUIRE((cells + 63) / 64 * (int64_t)(n > 1 ? n : 1) < 0x7fffffff && C * cells < 0x7fffffff,
+    ISPA_REQUIRE((cells + 31) / 32 * (int64_t)(n > 1 ? n : 1) < 0x7fffffff && C * cells < 0x7fffffff,
                  "maps of %lld cells are too large for one call", (long long)cells);
     return ISPA_OK;
 }
@@ -133,7 +143,7 @@ extern "C" int ispa_store_write(const void *features, int dtype, const uint8_t *
     if (int rc = check(dtype, kind, n, n_view, C, cells)) return rc;
     if (n == 0) return ISPA_OK;
     ISPA_REQUIRE(features && views && codes && scales && mask, "null pointer");
-    const unsigned blocks = (unsigned)((cells + 63) / 64 * n);
+    const unsigned blocks = (unsigned)((cells + kCellsPer - 1) / kCellsPer * n);
     PICK(dtype, kind, (store_write_kernel<T, S><<<blocks, kThreads, 0, (hipStream_t)stream>>>(
                            (const T::elem *)features, take, views, n, n_view, C, cells, (unsigned char *)codes, scales, mask)));
     return ispa::check_launch("store_write_kernel");
