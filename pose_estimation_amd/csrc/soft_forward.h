@@ -467,16 +467,20 @@ __global__ __launch_bounds__(256) void soft_join_few_kernel(const Params p) {
     for (int i = 0; i < 32; ++i) top = fmaxf(top, part[0][i][qi]);
     if (top == -__builtin_inff()) top = 0.f;                   // no part has a cell, or all scores are NaN
     __syncthreads();
+    // parts past the last one count with weight 0, from the last one's place: every load may go out at once
+    const int cq = in ? (int)q : 0;
 #pragma unroll
     for (int i = 0; i < kPer; ++i) {
+        if (32 * i >= p.splits) break;                         // uniform
         const int s = g + 32 * i;
-        if (s >= p.splits) break;
-        const float w = exp2_(m[i] - top);
+        const float w = s < p.splits ? exp2_(m[i] - top) : 0.f;
         l = fmaf(w, ls[i], l);
-        const float *src = p.part_o + ((s * bhn + bh) * p.Dv + c0) * p.nq + q;
+        const float *src = p.part_o + (((s < p.splits ? s : 0) * bhn + bh) * p.Dv + c0) * p.nq + cq;
+        float x[kJoinChannels];
 #pragma unroll
-        for (int c = 0; c < kJoinChannels; ++c)
-            if (in && c0 + c < p.Dv) v[c] = fmaf(w, src[c * p.nq], v[c]);
+        for (int c = 0; c < kJoinChannels; ++c) x[c] = src[(c0 + c < p.Dv ? c : 0) * p.nq];
+#pragma unroll
+        for (int c = 0; c < kJoinChannels; ++c) v[c] = s < p.splits ? fmaf(w, x[c], v[c]) : v[c];
     }
     part[0][g][qi] = l;
     __syncthreads();

@@ -26,34 +26,62 @@ int check_sizes(int dtype, int B, int heads, int D, int Dv, int64_t nq, int V, i
 
 size_t align256(size_t x) { return (x + 255) & ~(size_t)255; }
 
-// Copies maps (maps, d, n) into the form Direct wants: (maps, d8, ld) with d8 the next multiple of 8 rows and ld of kCells
-// cells, zeros beside.
+// Copies maps (maps, d, n) into the form Direct wants: (maps, d8, ld) with d8 the next multiple of 8 rows and ld of 16 bytes,
+// zeros beside.  16 bytes a thread, read as they lie.
 template <typename T>
-__global__ __launch_bounds__(256) void soft_pack_kernel(const typename T::elem *src, typename T::elem *dst, int d, int d8,
-                                                        int64_t n, int64_t ld, int64_t rows) {
-    const int64_t per = (ld + 255) / 256;
-    const int64_t row = blockIdx.x / per, cell = (blockIdx.x - row * per) * 256 + threadIdx.x;
-    if (row >= rows || cell >= ld) return;
-    const int64_t map = row / d8;
-    const int c = (int)(row - map * d8);
-    dst[row * ld + cell] = c < d && cell < n ? src[(map * d + c) * n + cell] : (typename T::elem)0;
+__global__ __launch_bounds__(256) void soft_pack_kernel(const typename T::elem *src, typename T::elem *dst, int d, int d8, int n,
+                                                        int segs, int64_t total) {
+    typedef typename T::elem elem;
+    constexpr int kN = 16 / sizeof(elem);
+    const int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x;
+    if (i >= total) return;
+    const int row = (int)(i / segs), cell = (int)(i - (int64_t)row * segs) * kN;
+    const int map = row / d8, c = row - map * d8;
+    elem e[kN] = {};
+    if (c < d) {
+        const elem *at = src + ((int64_t)map * d + c) * n + cell;
+        if (cell + kN <= n) {
+            __builtin_memcpy(e, at, 16);
+        } else {
+#pragma unroll
+            for (int j = 0; j < kN; ++j)
+                if (cell + j < n) e[j] = at[j];
+        }
+    }
+    u32x4 v;
+    __builtin_memcpy(&v, e, 16);
+    *reinterpret_cast<u32x4 *>(dst + i * kN) = v;
 }
 
-// float32 maps as three planes of bfloat16 numbers (F32S), (maps, 3, d8, ld); two cells a thread.
-__global__ __launch_bounds__(256) void soft_split_kernel(const float *src, unsigned *dst, int d, int d8, int64_t n, int64_t ld,
-                                                         int64_t rows) {
-    const int64_t half = ld / 2, per = (half + 255) / 256;
-    const int64_t row = blockIdx.x / per, pair = (blockIdx.x - row * per) * 256 + threadIdx.x;
-    if (row >= rows || pair >= half) return;
-    const int64_t map = row / d8;
-    const int c = (int)(row - map * d8);
-    const float *at = src + (map * d + c) * n + 2 * pair;
-    const float x = c < d && 2 * pair < n ? at[0] : 0.f, y = c < d && 2 * pair + 1 < n ? at[1] : 0.f;
-    unsigned a[3], b[3];
-    split3(x, a[0], a[1], a[2]);
-    split3(y, b[0], b[1], b[2]);
+// float32 maps as three planes of bfloat16 numbers (F32S), (maps, 3, d8, ld); 8 cells a thread.
+__global__ __launch_bounds__(256) void soft_split_kernel(const float *src, u32x4 *dst, int d, int d8, int n, int segs,
+                                                         int64_t total) {
+    const int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x;
+    if (i >= total) return;
+    const int row = (int)(i / segs), seg = (int)(i - (int64_t)row * segs), cell = seg * 8;
+    const int map = row / d8, c = row - map * d8;
+    float e[8] = {};
+    if (c < d) {
+        const float *at = src + ((int64_t)map * d + c) * n + cell;
+        if (cell + 8 <= n) {
+            __builtin_memcpy(e, at, 32);
+        } else {
 #pragma unroll
-    for (int k = 0; k < 3; ++k) dst[((map * 3 + k) * d8 + c) * half + pair] = uppers(a[k], b[k]);
+            for (int j = 0; j < 8; ++j)
+                if (cell + j < n) e[j] = at[j];
+        }
+    }
+    u32x4 v[3];
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+        unsigned x[3], y[3];
+        split3(e[2 * j], x[0], x[1], x[2]);
+        split3(e[2 * j + 1], y[0], y[1], y[2]);
+#pragma unroll
+        for (int k = 0; k < 3; ++k) v[k][j] = uppers(x[k], y[k]);
+    }
+#pragma unroll
+    for (int k = 0; k < 3; ++k) dst[(((int64_t)map * 3 + k) * d8 + c) * segs + seg] = v[k];
 }
 
 // Copies of maps in the workspace: three planes for kSplit; else only maps whose rows do not start on 16-byte borders or
@@ -81,15 +109,17 @@ int stream_map(Stream *s, Arithmetic a, const void *map, int64_t maps, int d, in
     s->d = c.d8;
     s->map = map;
     if (c.bytes == 0) return ISPA_OK;
-    const int64_t rows = maps * c.d8, per = (c.ld / (a == kSplit ? 2 : 1) + 255) / 256;
-    ISPA_REQUIRE(rows * per < (1ll << 31), "maps of %lld rows are too large for one call", (long long)rows);
-    const unsigned blocks = (unsigned)(rows * per);
+    const int segs = (int)(c.ld / (a == kFloat ? 4 : 8));
+    const int64_t rows = maps * c.d8, total = rows * segs;
+    ISPA_REQUIRE(rows < (1ll << 31) && total < (1ll << 38), "maps of %lld rows are too large for one call", (long long)rows);
+    const unsigned blocks = (unsigned)((total + 255) / 256);
     if (a == kSplit)
-        soft_split_kernel<<<blocks, 256, 0, stream>>>((const float *)map, (unsigned *)*at, d, c.d8, n, c.ld, rows);
+        soft_split_kernel<<<blocks, 256, 0, stream>>>((const float *)map, (u32x4 *)*at, d, c.d8, (int)n, segs, total);
     else if (a == kFloat)
-        soft_pack_kernel<F32><<<blocks, 256, 0, stream>>>((const float *)map, (float *)*at, d, c.d8, n, c.ld, rows);
+        soft_pack_kernel<F32><<<blocks, 256, 0, stream>>>((const float *)map, (float *)*at, d, c.d8, (int)n, segs, total);
     else
-        soft_pack_kernel<BF16><<<blocks, 256, 0, stream>>>((const unsigned short *)map, (unsigned short *)*at, d, c.d8, n, c.ld, rows);
+        soft_pack_kernel<BF16><<<blocks, 256, 0, stream>>>((const unsigned short *)map, (unsigned short *)*at, d, c.d8, (int)n, segs,
+                                                           total);
     s->map = *at;
     *at += c.bytes;
     return ispa::check_launch("soft_pack_kernel");
