@@ -185,9 +185,9 @@ int run_forward(Params &p, int dtype, Source source, void *workspace, size_t wor
     const Arithmetic a = arithmetic_of(dtype, !maps, p.D, p.Dv, p.nq);
     const size_t copied = maps ? forward_copies(dtype, p.B, p.heads, p.D, p.Dv, p.nq, p.cells, p.shared) : 0;
     const size_t need = copied + forward_bytes(plan, p.B, p.heads, p.Dv, p.nq);
-    ISPA_REQUIRE(!maps || (((uintptr_t)p.k | (uintptr_t)p.v) & 15) == 0, "maps must start on 16-byte borders");
     if (need > 0 && (workspace == nullptr || workspace_bytes < need))
         return ispa::fail(ISPA_EWORKSPACE, "workspace of %zu bytes, %zu needed", workspace_bytes, need);
+    ISPA_REQUIRE(!maps || (((uintptr_t)p.k | (uintptr_t)p.v) & 15) == 0, "maps must start on 16-byte borders");
     p.tiles_per_view = (int)((p.cells + tile_rows(a) - 1) / tile_rows(a));
     p.tiles = p.tiles_per_view * p.V;
     p.blocks = plan.blocks;
