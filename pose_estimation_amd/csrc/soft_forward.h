@@ -174,6 +174,10 @@ constexpr bool two_resident = std::is_same_v<SRC, BF16> ? DP <= 128 : std::is_sa
 // How far (in units of log2) a query's largest score may rise above the maximum that its sums are kept against before they
 // are rescaled: weights stay below 2^8, and nearly all tiles leave the accumulators alone.
 constexpr float kSlack = 8.f;
+// A tile whose scores rise by more than this over what they were formed against is formed anew: their rounding goes by the
+// rise, which a steep falloff makes far larger than the scores that count.  float32 only: 2^-24 of any rise below 2^16 is
+// lost in bfloat16's weights.
+constexpr float kFar = 64.f;
 
 // NC: value channels that one launch forms, from p.c0 on (256 float32 channels take two launches, for the registers).
 template <typename T, typename SRC, int DP, int WQ, int NC, int MODE>
@@ -223,7 +227,7 @@ __global__ __launch_bounds__(64 * WQ, (two_resident<T, SRC, DP>) ? 2 : 1) void s
 
     F feed(p, b, head, t0, lds);
     const bool phased = kMayPhase<M> && feed.phased;
-    const Penalty<M, MODE> penalty(p, score.fall, qx, qy);
+    const Penalty<M, MODE, !kCodes> penalty(p, score.fall, qx, qy);    // codes: products are yet to be scaled
     const f32x16 from = penalty.from(score.in);
     uint64_t next = 0;                                         // live cells of the next tile
     int next_cell0 = 0;
@@ -255,7 +259,9 @@ __global__ __launch_bounds__(64 * WQ, (two_resident<T, SRC, DP>) ? 2 : 1) void s
         const char *ktile = feed.k(i), *vtile = feed.v(i);
         const float *cell = feed.cell(i);
         f32x16 z[kBlocks];
-        if (live != 0) {
+        bool again = live != 0;
+        while (again) {
+            again = false;
             // z: scores relative to off.  kPlain: the products, scaled in the exponent.  kCapped: relative to the cap, which
             // stands for the maximum: weights are 2^(-2 cap) > 2^-93 at least.
             if constexpr (DP == 256 && kBlocks == 2) {         // block by block: fewer fragments in registers
@@ -330,6 +336,7 @@ __global__ __launch_bounds__(64 * WQ, (two_resident<T, SRC, DP>) ? 2 : 1) void s
                     for (int c = 0; c < NC / 32; ++c)
 #pragma unroll
                         for (int i = 0; i < 16; ++i) o[c][i] *= fix;
+                    if constexpr (M::kWide && MODE != kPlain) again = __any(was != 0.f && off - was > kFar);
                     if constexpr (MODE != kPlain)
 #pragma unroll
                         for (int k = 0; k < kBlocks; ++k)

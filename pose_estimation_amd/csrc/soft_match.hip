@@ -111,7 +111,7 @@ int stream_map(Stream *s, Arithmetic a, const void *map, int64_t maps, int d, in
     if (c.bytes == 0) return ISPA_OK;
     const int segs = (int)(c.ld / (a == kFloat ? 4 : 8));
     const int64_t rows = maps * c.d8, total = rows * segs;
-    ISPA_REQUIRE(rows < (1ll << 31) && total < (1ll << 38), "maps of %lld rows are too large for one call", (long long)rows);
+    ISPA_REQUIRE(rows < (1ll << 31) && total < (1ll << 32) - 256, "maps of %lld rows are too large for one call", (long long)rows);
     const unsigned blocks = (unsigned)((total + 255) / 256);
     if (a == kSplit)
         soft_split_kernel<<<blocks, 256, 0, stream>>>((const float *)map, (u32x4 *)*at, d, c.d8, (int)n, segs, total);
@@ -147,7 +147,6 @@ void backward_plans(int dtype, int B, int heads, int D, int Dv, int64_t nq, int6
     *dq = plan_of(dtype, false, true, (int64_t)B * heads, D, Dv, nq, 1, cells);
     *dkv = plan_of(dtype, false, true, (int64_t)B * heads, D, Dv, cells, 1, nq);
 }
-
 
 // Channels of float32 parts per cell: every split's, or what the first of two launches leaves for the second (a map that is
 // reference and value; the size does not say which, so any map of equal channels).

@@ -117,6 +117,7 @@ struct Math<BF16, DP> {
     static constexpr int kCells = 8;             // cells of a 16-byte segment
     static constexpr int kBytes = 2;             // of a streamed number in LDS
     static constexpr int kPlanes = 1;            // LDS tiles that hold one tile of the map
+    static constexpr bool kWide = false;         // float32 maps or queries
     struct Owned {                               // B operand of the first product: channels 16 s + 8 h .. + 7
         bf16x8 f[DP / 16];
     };
@@ -247,6 +248,7 @@ struct Math<F32, DP> {
     static constexpr int kCells = 4;
     static constexpr int kBytes = 4;
     static constexpr int kPlanes = 1;
+    static constexpr bool kWide = true;
     struct Owned {                               // channel 2 s + h
         float f[DP / 2];
     };
@@ -343,6 +345,7 @@ struct SplitMath {
     static constexpr int kCells = 8;
     static constexpr int kBytes = 2;
     static constexpr int kPlanes = PLANES;
+    static constexpr bool kWide = true;
     static constexpr int kTile = DP * kRowBytes;
     struct Owned {
         bf16x8 f[3][DP / 16];
@@ -777,11 +780,14 @@ struct Score {
 
 // offset - falloff d^2 of one owned cell at (x, y) to the 16 streamed cells of a lane.
 // kRows: streamed cells lie on the grid in groups of kCells successive ones, whose rows' width is a multiple of that: a
-// group stays in one row and d^2 grows along it by a quadratic.  The quadratic's own part, -falloff j^2, is the same in
-// every group and lies in the accumulators' start (`from`), so that one operation a cell is left (FROM: where 16 registers
-// are left for it).  kGeneral: places read from LDS (`cell`: 64 x, 64 y).
+// group stays in one row.  bfloat16: d^2 grows along it by a quadratic, whose own part, -falloff j^2, is the same in every
+// group and lies in the accumulators' start (`from`), so that one operation a cell is left (FROM: where 16 registers are
+// left for it).  Its parts cancel near the query, which leaves falloff 64 2^-23 of error in a score: below a weight's
+// rounding up to a falloff of 250, but not below float32's; float32 takes the distances as they are.
+// kGeneral: places read from LDS (`cell`: 64 x, 64 y).
 template <typename M, int MODE, bool FROM = true>
 struct Penalty {
+    static constexpr bool kQuadratic = !M::kWide;
     bool on;
     float fall, x, y, width, per_width;
     __device__ __forceinline__ Penalty(const Params &p, float fall_, float x_, float y_) {
@@ -795,7 +801,7 @@ struct Penalty {
     __device__ __forceinline__ bool wants_places() const { return MODE == kGeneral && on; }
     __device__ __forceinline__ f32x16 from(float in) const {
         f32x16 v = {};
-        if constexpr (MODE == kRows && FROM) {
+        if constexpr (MODE == kRows && FROM && kQuadratic) {
             const float f = -fall / in;
 #pragma unroll
             for (int i = 0; i < 16; ++i) v[i] = f * (float)((i % M::kCells) * (i % M::kCells));
@@ -809,7 +815,16 @@ struct Penalty {
                 // cells are fewer than 2^22: c + 0.5 is exact and the quotient's error cannot reach the next integer
                 const float c = (float)(cell0 + 32 * k + M::cell(g, h));
                 const float cy = floorf((c + 0.5f) * per_width);
-                const float dx = fmaf(-width, cy, c) - x, dy = cy - y;
+                const float cx = fmaf(-width, cy, c), dx = cx - x, dy = cy - y;
+                if constexpr (!kQuadratic) {
+                    const float yy = dy * dy;
+#pragma unroll
+                    for (int j = 0; j < M::kCells; ++j) {
+                        const float d = (cx + (float)j) - x;
+                        z[g + j] = fmaf(-fall, fmaf(d, d, yy), offset);
+                    }
+                    continue;
+                }
                 const float base = fmaf(-fall, fmaf(dx, dx, dy * dy), offset), step = -2.f * fall * dx;
 #pragma unroll
                 for (int j = 0; j < M::kCells; ++j)

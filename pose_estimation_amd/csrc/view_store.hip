@@ -148,7 +148,8 @@ int check(int dtype, int kind, int n, int n_view, int C, int64_t cells) {
     ISPA_REQUIRE(kind == ISPA_STORE_INT8 || kind == ISPA_STORE_FP8, "store kind %d is neither int8 nor e4m3", kind);
     ISPA_REQUIRE(n >= 0 && n_view >= 1 && C >= 1 && cells >= 1, "store sizes out of range (n %d, views %d, channels %d)", n,
                  n_view, C);
-    ISPA_REQUIRE((cells + kCellsPer - 1) / kCellsPer * (int64_t)(n > 1 ? n : 1) < 0x7fffffff && C * cells < 0x7fffffff,
+    ISPA_REQUIRE((cells + kCellsPer - 1) / kCellsPer * (int64_t)(n > 1 ? n : 1) < (1ll << 32) / (kWriters * kCellsPer) &&
+                     C * cells < 0x7fffffff,
                  "maps of %lld cells are too large for one call", (long long)cells);
     return ISPA_OK;
 }

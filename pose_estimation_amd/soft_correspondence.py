@@ -22,12 +22,12 @@ MAX_CHANNELS = _abi.SOFT_MAX_CHANNELS
 
 
 def _dims(x):
-    return tuple(x.shape)
+    return tuple(x.shape) if hasattr(x, "shape") else np.shape(x)
 
 
 def _elements(x, name):
     """Cells of a feature map given as array or tensor; a shape check before anything touches the device."""
-    shape = x.shape
+    shape = _dims(x)
     if len(shape) < 3:
         raise ValueError(f"{name} must be (B,C,H,W) or (B,C,n), got {_dims(x)}")
     return math.prod(shape[2:])
@@ -91,8 +91,10 @@ def _scores(heads, scale, cap, falloff, query_xy, grid, query_shape, batch, n):
             raise ValueError("falloff needs a reference map (B,C,H,W): distances are taken on its grid")
         if query_xy is None and query_shape != grid:
             raise ValueError(f"falloff: queries {query_shape} do not lie on the reference grid {grid}; give query_xy")
-        if not np.isscalar(falloff) and _dims(falloff if dv.is_tensor(falloff) else np.asarray(falloff)) != (heads,):
+        if not np.isscalar(falloff) and _dims(falloff) != (heads,):
             raise ValueError(f"falloff must be a number or hold one value per head ({heads})")
+        if not dv.is_tensor(falloff) and not np.isfinite(np.asarray(falloff, np.float64)).all():
+            raise ValueError(f"falloff must be finite, got {falloff}")
         if query_xy is not None and _dims(query_xy) != (batch, n, 2):
             raise ValueError(f"query_xy must be ({batch},{n},2), got {_dims(query_xy)}")
     return scale, cap
@@ -114,6 +116,8 @@ def _counts(num_query, batch):
     t = num_query if dv.is_tensor(num_query) else np.asarray(num_query)
     if math.prod(t.shape) != batch:
         raise ValueError("num_query must hold one count per batch item")
+    if t.dtype.is_floating_point if dv.is_tensor(t) else t.size and t.dtype.kind not in "iu":
+        raise ValueError("num_query must hold integers")
     return t.reshape(-1)
 
 
@@ -125,6 +129,11 @@ def _count_tensor(num_query, device):
     num_query = num_query.clamp(low, high) if dv.is_tensor(num_query) and num_query.dtype == torch.int64 else \
         num_query if dv.is_tensor(num_query) else np.clip(num_query, low, high)
     return _on(num_query, torch.int32, device)
+
+
+def _check_mask(mask, batch, size):
+    if mask is not None and _dims(mask) not in ((batch,) + size, (batch, 1) + size):
+        raise ValueError(f"mask must be {(batch,) + size} or {(batch, 1) + size}, got {_dims(mask)}")
 
 
 def _mask(mask, device):
@@ -162,8 +171,7 @@ class _Call:
             raise ValueError(f"at most {MAX_CHANNELS} channels per head")
         if cells < 1:
             raise ValueError("ref has no cells")
-        if mask is not None and (_dims(mask)[0] != b or math.prod(mask.shape) != b * cells):
-            raise ValueError(f"mask must be ({b},H,W) or ({b},1,H,W) over ref's cells, got {_dims(mask)}")
+        _check_mask(mask, b, _dims(ref)[2:])
         grid = _dims(ref)[2:] if len(_dims(ref)) == 4 else None
         if scale is None:
             scale = (c // heads) ** -0.5
@@ -265,7 +273,8 @@ def soft_match(query, ref, value=None, *, heads=1, scale=None, cap=0.0, falloff=
                                            gives [x, y]
 
     mask (B,H,W) or (B,1,H,W): a cell with 0 / False takes no part, whatever its features hold (background of a
-    rendered template).  num_query (B,): only the first num_query[b] queries of item b are real, as in dense_nn.
+    rendered template); all other features are to be finite.  num_query (B,): only the first num_query[b] queries of item
+    b are real, as in dense_nn; what lies behind them may be anything.
     Returns out (B,Cv,...) over query's cells in query's dtype, with return_lse also lse (B,heads,n) float32, the log of
     the sum of exp(z): the match's confidence.  A query that is not real, or whose cells are all masked, gets 0 and -inf.
 
@@ -360,7 +369,7 @@ class TemplateStore:
         return _on(views, torch.int32, self.codes.device)
 
     def write(self, views, features, mask=None):
-        """Quantises features (n,C,H,W) (float32, or bfloat16 tensors) into views (n,).  mask (n,H,W): the cells that hold
+        """Quantises features (n,C,H,W) (float32, or bfloat16 tensors) into views (n,).  mask (n,H,W) or (n,1,H,W): the cells that hold
         an object, all if None; a cell with a non-finite channel is masked as well.  A view listed twice keeps its
         last entry; -1 skips an entry."""
         views = self._views(views, 1)
@@ -368,8 +377,7 @@ class TemplateStore:
         dtype = _dtype(features, "features")
         if _dims(features) != (n, self.channels) + self.size:
             raise ValueError(f"features must be {(n, self.channels) + self.size}, got {_dims(features)}")
-        if mask is not None and math.prod(mask.shape) != n * self.size[0] * self.size[1]:
-            raise ValueError(f"mask must be {(n,) + self.size}, got {_dims(mask)}")
+        _check_mask(mask, n, self.size)
         device, place = _place(self.codes)
         with place:
             v, f, m = self._index(views), _on(features, dtype, device), _mask(mask, device)

@@ -65,7 +65,7 @@ def oracle(q, r, v, heads, scale, cap=0.0, falloff=None, xy=None, width=None, ma
             # a rounded product dp (float32) and delta: their errors go by magnitudes
             size = p * (np.abs(dp) + (p * np.abs(dp)).sum(1, keepdims=True) + (0 if d_lse is None else np.abs(np.asarray(d_lse, np.float64)[i, h, :live, None])))
             slope = scale * (1 - t * t) if cap else scale
-            g, size = g * slope, size * slope
+            g, size = g * slope, size * np.abs(slope)
             dq[i, a, :live] = rr @ g.T
             mq[i, a, :live] = np.abs(rr) @ size.T
             dr[i, a][:, js] += qq @ g
@@ -611,6 +611,175 @@ def test_templates_from_poses_to_matches(sc, kind):
     assert torch.allclose(out, same, rtol=1e-4, atol=1e-5)
 
 
+# ------------------------------------------------------------------------------------------------ every form of the kernels
+# More than 64 queries and cells take workgroups of four waves, with a form of their own for plain scores, for caps up to 32
+# (bfloat16), for a falloff on a grid whose width is a multiple of 8 cells, and for the rest.
+SCORES = {
+    "plain": dict(scale=15.0),
+    "negative scale": dict(scale=-15.0),
+    "no scale": dict(scale=0.0),
+    "cap": dict(scale=25.0, cap=6.0),
+    "large cap": dict(scale=25.0, cap=40.0),
+    "falloff": dict(scale=15.0, falloff=0.04),
+    "rising falloff": dict(scale=-15.0, falloff=-0.02),
+    "falloff alone": dict(scale=0.0, falloff=0.04),
+    "cap and falloff": dict(scale=25.0, cap=6.0, falloff=0.04),
+}
+FORMS = [  # channels, heads, value channels, queries (0: the grid)
+    (32, 1, 0, 0),
+    (128, 2, 64, 150),
+    (128, 1, 0, 150),
+    (100, 1, 128, 0),
+    (256, 1, 0, 0),
+    (200, 1, 256, 150),
+]
+
+
+@gpu
+@pytest.mark.parametrize("dtype", [F32, BF16])
+@pytest.mark.parametrize("form", FORMS)
+@pytest.mark.parametrize("scores", SCORES)
+def test_forms(sc, dtype, form, scores):
+    """Forward and gradients of an item of whole and one of partly masked, partly real rows."""
+    c, heads, cv, n = form
+    grid, nq = (15, 24), form[3] or 360
+    q, r, v = inputs(dtype, 2, c, grid, n, cv, seed=130)
+    opts = dict(SCORES[scores])
+    fall = xy = None
+    if "falloff" in opts:
+        fall = opts["falloff"] = torch.full((heads,), opts["falloff"])
+        if n:
+            xy = opts["query_xy"] = torch.rand((2, n, 2), generator=torch.Generator().manual_seed(3)) * torch.tensor([23.0, 14.0])
+    mask = torch.ones((2,) + grid, dtype=torch.bool)
+    mask[1] = silhouette(131, 1, *grid)[0]
+    count = torch.tensor([nq, nq - 47])
+    d_out, d_lse = rand(132, (2, cv or c) + tuple(q.shape[2:]), dtype, unit=False), rand(133, (2, heads, nq), F32, unit=False)
+    out, got = gradients(sc, *cuda(q, r, v, d_out, d_lse), heads=heads, mask=mask.cuda(), num_query=count, **opts)
+    want = oracle(flat(q), flat(r), flat(r if v is None else v), heads, opts["scale"], opts.get("cap", 0.0),
+                  None if fall is None else host(fall), None if xy is None else host(xy), grid[1], mask.numpy(), count.numpy(),
+                  flat(d_out), host(d_lse))
+    near(out, want[0], want[2], dtype, 1)
+    check_gradients(got, want, dtype, v is None)
+
+
+@gpu
+@pytest.mark.parametrize("grid", [(12, 16), (12, 15)])
+@pytest.mark.parametrize("falloff", [2.0, 50.0])
+def test_steep_falloff(sc, falloff, grid):
+    """Distances as exact as float32 has them: queries between cells, whose nearest ones weigh alike."""
+    q, r, v = inputs(F32, 1, 16, grid, 100, 8, seed=140)
+    xy = torch.rand((1, 100, 2), generator=torch.Generator().manual_seed(141)) * torch.tensor([grid[1] - 1.0, grid[0] - 1.0])
+    out, lse = sc.soft_match(*cuda(q, r, v), scale=4.0, falloff=falloff, query_xy=xy, return_lse=True)
+    want = oracle(flat(q), flat(r), flat(v), 1, 4.0, 0.0, [falloff], host(xy), grid[1])
+    # scores of the cells that count: up to falloff / 2 + 4 = 29, below the 60 of the tolerance's count
+    near(out, want[0], want[2], F32, 1)
+    near_lse(lse, want[1])
+
+
+@gpu
+@pytest.mark.parametrize("dtype", [F32, BF16])
+@pytest.mark.parametrize("n, grid, cv", [(100, (64, 80), 0), (70, (72, 70), 32), (900, (30, 34), 0), (3, (100, 100), 0), (64, (50, 41), 8)])
+def test_many_parts(sc, dtype, n, grid, cv):
+    """Few workgroups: the cells are split over many, whose parts are joined."""
+    q, r, v = inputs(dtype, 1, 32, grid, n, cv, seed=150)
+    mask = silhouette(151, 1, *grid)
+    mask[0, : grid[0] // 2] = False                      # parts without a cell
+    d_out, d_lse = rand(152, (1, cv or 32, n), dtype, unit=False), rand(153, (1, 1, n), F32, unit=False)
+    out, got = gradients(sc, *cuda(q, r, v, d_out, d_lse), scale=20.0, mask=mask[:, None].cuda())
+    want = oracle(flat(q), flat(r), flat(r if v is None else v), 1, 20.0, mask=mask.numpy(), d_out=flat(d_out), d_lse=host(d_lse))
+    near(out, want[0], want[2], dtype, 1)
+    check_gradients(got, want, dtype, v is None)
+
+
+@gpu
+@pytest.mark.parametrize("dtype", [F32, BF16])
+def test_one_cell_far_above_the_rest(sc, dtype):
+    """The largest score rises late, in steps beyond and within what the sums are kept for, in each tile of 64 cells."""
+    n, m, c = 130, 640, 32
+    q, r = rand(160, (1, c, n), dtype), rand(161, (1, c, m), dtype) * 0.01
+    for k, size in enumerate((0.05, 0.1, 0.3, 0.35, 0.9, 1.0)):
+        at = 5 + 101 * k
+        r[0, :, at] = q[0, :, 17 * k] * size
+    out, lse = sc.soft_match(q.cuda(), r.cuda(), scale=80.0, return_lse=True)
+    want = oracle(flat(q), flat(r), flat(r), 1, 80.0)
+    near(out, want[0], want[2], dtype, 1)
+    # scores up to 80: 80 2^-24 of a weight each, in the tolerance of near_lse
+    near_lse(lse, want[1])
+
+
+@gpu
+@pytest.mark.parametrize("dtype", [F32, BF16])
+@pytest.mark.parametrize("kind", ["int8", "fp8"])
+@pytest.mark.parametrize("c, heads, size, n", [(128, 1, (10, 16), 0), (128, 1, (9, 13), 100), (256, 1, (6, 8), 100), (64, 2, (7, 8), 20)])
+def test_store_match_falloff(sc, dtype, kind, c, heads, size, n):
+    """The grid's distances in every view, per head; the same as soft_match over the views side by side."""
+    h, w = size
+    store = sc.TemplateStore(5, c, size, kind)
+    store.write(range(5), rand(170, (5, c) + size, F32), mask=silhouette(171, 5, h, w))
+    views = [[4, 0, 2], [1, 1, -1]]
+    nq = n or h * w
+    q = rand(172, (2, c, n) if n else (2, c, h, w), dtype)
+    xy = torch.rand((2, n, 2), generator=torch.Generator().manual_seed(173)) * torch.tensor([w - 1.0, h - 1.0]) if n else None
+    fall = [0.03 * (i + 1) for i in range(heads)]
+    out, lse = store.soft_match(q.cuda(), views, heads=heads, scale=18.0, falloff=fall, query_xy=xy, num_query=[nq, nq - 7],
+                                return_lse=True)
+    ids = np.maximum(np.array(views).reshape(-1), 0)
+    values = flat(store.read(ids)).reshape(2, 3, c, -1).transpose(0, 2, 1, 3).reshape(2, c, -1)
+    masks = (host(store.read_mask(ids)).reshape(2, 3, -1) * (np.array(views) >= 0)[:, :, None]).reshape(2, -1)
+    # the oracle's grid is one map: per view, joined by the log-sums
+    want, mag, want_lse = 0, 0, None
+    parts = [oracle(flat(q), values[:, :, i * h * w:(i + 1) * h * w], values[:, :, i * h * w:(i + 1) * h * w], heads, 18.0, 0.0, fall,
+                    None if xy is None else host(xy), w, masks[:, i * h * w:(i + 1) * h * w], [nq, nq - 7]) for i in range(3)]
+    want_lse = np.logaddexp.reduce([p[1] for p in parts])
+    for p in parts:
+        share = np.where(np.isneginf(p[1]), 0, np.exp(p[1] - np.where(np.isneginf(want_lse), 0, want_lse)))
+        share = np.repeat(share, c // heads, 1)
+        want, mag = want + share * p[0], mag + share * p[2]
+    near(out, want, mag, dtype, 1)
+    near_lse(lse, want_lse)
+
+
+@gpu
+def test_store_over_a_part_of_another(sc):
+    """Views of a larger tensor, which start anywhere."""
+    store = sc.TemplateStore(4, 9, (5, 7))
+    store.write(range(4), rand(180, (4, 9, 5, 7), F32))
+    part = sc.TemplateStore.from_tensors(store.codes[1:], store.scales[1:], store.mask[1:], (5, 7))
+    assert torch.equal(part.read([0, 2]), store.read([1, 3]))
+    q = rand(181, (1, 9, 90), F32).cuda()
+    assert torch.equal(part.soft_match(q, [[0, 2]], scale=9.0), store.soft_match(q, [[1, 3]], scale=9.0))
+    part.write([1], rand(182, (1, 9, 5, 7), F32))
+    assert torch.equal(part.read([1]), store.read([2]))
+
+
+@gpu
+def test_captured_store(sc):
+    """Write, match and read in a graph, replayed on other views."""
+    feats = rand(190, (6, 32, 8, 9), F32).cuda()
+    store, twin = sc.TemplateStore(6, 32, (8, 9)), sc.TemplateStore(6, 32, (8, 9))
+    views, x, q = torch.zeros(2, dtype=torch.int32, device="cuda"), feats[:2].clone(), rand(191, (1, 32, 70), F32).cuda()
+
+    def step(s):
+        s.write(views, x)
+        return s.soft_match(q, views[None], scale=15.0), s.read(views), s.read_mask(views)
+
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        step(store)
+    torch.cuda.current_stream().wait_stream(side)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        got = step(store)
+    for i in range(3):
+        views.copy_(torch.tensor([5 - i, i]))
+        x.copy_(feats[2 * i:2 * i + 2])
+        want = step(twin)
+        graph.replay()
+        torch.cuda.synchronize()
+        assert all(torch.equal(a, b) for a, b in zip(got, want))
+
+
 # ------------------------------------------------------------------------------------------------ refusals (no GPU)
 def test_refusals(sc):
     q, r = torch.zeros((2, 8, 4, 4)), torch.zeros((2, 8, 5, 6))
@@ -639,6 +808,13 @@ def test_refusals(sc):
         (dict(mask=torch.ones((2, 5, 5))), "mask"),
         (dict(mask=torch.ones((1, 5, 6))), "mask"),
         (dict(num_query=[1, 2, 3]), "one count per"),
+        (dict(num_query=[1.5, 2.0]), "integers"),
+        (dict(num_query=torch.ones(2)), "integers"),
+        (dict(mask=[[True] * 6] * 5), "mask"),
+        (dict(mask=torch.ones((2, 6, 5))), "mask"),
+        (dict(query=q[..., :3, :3], falloff=math.nan, query_xy=torch.zeros((2, 9, 2))), "finite"),
+        (dict(falloff=[math.inf], query_xy=torch.zeros((2, 16, 2))), "finite"),
+        (dict(query=[[1.0, 2.0]]), "must be"),
         (dict(query=q.clone().requires_grad_(), ref=r.numpy()), "must be tensors"),
     ]
     for args, match in bad:
