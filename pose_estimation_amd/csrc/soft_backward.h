@@ -118,8 +118,8 @@ __global__ __launch_bounds__(64 * WQ, (two_waves<T, DP, WQ>) ? 2 : 1) void soft_
     const int t1 = idle ? t0 : (int)((int64_t)p.tiles * (split + 1) / p.splits);
 
     typename M::Owned qf, of;
-    M::load_owned(qf, (const typename T::elem *)p.q + (int64_t)bh * p.D * p.nq + (q < nq ? q : 0), p.nq, p.D, q_ok, h);
-    M::load_owned(of, (const typename T::elem *)p.d_out + (int64_t)bh * p.Dv * p.nq + (q < nq ? q : 0), p.nq, p.Dv, q_ok, h);
+    M::load_owned(qf, (const typename T::elem *)p.q + (int64_t)bh * p.D * p.nq, q < nq ? q : 0, p.nq, p.D, q_ok, h);
+    M::load_owned(of, (const typename T::elem *)p.d_out + (int64_t)bh * p.Dv * p.nq, q < nq ? q : 0, p.nq, p.Dv, q_ok, h);
     const typename M::Addr addr = M::addr(lane);
     const Score<T> score(p, head);
     float qx = 0.f, qy = 0.f;
@@ -246,10 +246,10 @@ __global__ __launch_bounds__(64 * WQ, (two_waves<T, DP, WQ> && (DP <= 64 || PART
     const float cx = (float)(cell % p.W), cy = (float)(cell / p.W);
 
     typename M::Owned kf, vf;
-    M::load_owned(kf, (const typename T::elem *)p.k + (int64_t)bh * p.D * p.cells + (cell < cells ? cell : 0), p.cells, p.D,
+    M::load_owned(kf, (const typename T::elem *)p.k + (int64_t)bh * p.D * p.cells, cell < cells ? cell : 0, p.cells, p.D,
                   c_ok, h);
     if constexpr (kDk)
-        M::load_owned(vf, (const typename T::elem *)p.v + (int64_t)bh * p.Dv * p.cells + (cell < cells ? cell : 0), p.cells, p.Dv,
+        M::load_owned(vf, (const typename T::elem *)p.v + (int64_t)bh * p.Dv * p.cells, cell < cells ? cell : 0, p.cells, p.Dv,
                       c_ok, h);
     const typename M::Addr addr = M::addr(lane);
     const Score<T> score(p, head);

@@ -73,10 +73,13 @@ constexpr bool kMayPhase = M::kPlanes == 3;
 constexpr int kCellBytes = 4 * 64 * (int)sizeof(float);
 template <typename M, int DP>
 constexpr int kTileBytes = M::kPlanes * DP * kRowBytes;
+// Codes of a lone wave take one buffer: the next tile waits in registers until the present one's products are done.
+template <typename SRC, int WQ>
+constexpr bool kOneBuffer = WQ == 1 && (std::is_same_v<SRC, I8> || std::is_same_v<SRC, FP8>);
 template <typename M, int DP>
-constexpr int lds_bytes(bool shared, int phased_k) {
+constexpr int lds_bytes(bool shared, int phased_k, bool one = false) {
     const bool phased = kMayPhase<M> && !shared;
-    return (phased ? phased_k : 2) * (kTileBytes<M, DP> + kCellBytes) + (shared ? 0 : phased ? 1 : 2) * kTileBytes<M, DP>;
+    return (phased ? phased_k : one ? 1 : 2) * (kTileBytes<M, DP> + kCellBytes) + (shared ? 0 : phased ? 1 : 2) * kTileBytes<M, DP>;
 }
 
 // The tiles of one item and head: begin_* starts a tile's way into a buffer, end_* ends it.  Codes are reference and value.
@@ -168,8 +171,9 @@ struct Feed {
 };
 
 // Registers for two waves a SIMD: one's products run under the other's exponentials.
-template <typename T, typename SRC, int DP>
-constexpr bool two_resident = std::is_same_v<SRC, BF16> ? DP <= 128 : std::is_same_v<SRC, F32S> && DP <= 64;
+template <typename T, typename SRC, int DP, int WQ>
+constexpr bool two_resident = std::is_same_v<SRC, BF16> || (kOneBuffer<SRC, WQ> && !std::is_same_v<T, F32C>)
+                                  ? DP <= 128 : std::is_same_v<SRC, F32S> && DP <= 64;
 
 // How far (in units of log2) a query's largest score may rise above the maximum that its sums are kept against before they
 // are rescaled: weights stay below 2^8, and nearly all tiles leave the accumulators alone.
@@ -181,7 +185,7 @@ constexpr float kFar = 64.f;
 
 // NC: value channels that one launch forms, from p.c0 on (256 float32 channels take two launches, for the registers).
 template <typename T, typename SRC, int DP, int WQ, int NC, int MODE>
-__global__ __launch_bounds__(64 * WQ, (two_resident<T, SRC, DP>) ? 2 : 1) void soft_forward_kernel(const Params p) {
+__global__ __launch_bounds__(64 * WQ, (two_resident<T, SRC, DP, WQ>) ? 2 : 1) void soft_forward_kernel(const Params p) {
     typedef Math<T, DP> M;
     constexpr int kBlocks = M::kRows / 32;
     constexpr uint64_t kAll = M::kRows == 64 ? ~0ull : 0xffffffffull;
@@ -198,14 +202,20 @@ __global__ __launch_bounds__(64 * WQ, (two_resident<T, SRC, DP>) ? 2 : 1) void s
     const int bh = id / p.splits;
     const int b = bh / p.heads, head = bh - b * p.heads;
     const int live_q = (int)live_queries(p, b), nq = (int)p.nq;            // fewer than 2^22
-    const int q = (qblk * WQ + wave) * 32 + (lane & 31);
+    const int q = (qblk * WQ + wave) * M::kColumns + (lane & (M::kColumns - 1));
     const bool q_ok = q < live_q;
-    const bool idle = qblk * WQ * 32 >= live_q;       // no live query in the whole workgroup
+    const bool idle = qblk * WQ * M::kColumns >= live_q;       // no live query in the whole workgroup
     const int t0 = (int)((int64_t)p.tiles * split / p.splits);
     const int t1 = idle ? t0 : (int)((int64_t)p.tiles * (split + 1) / p.splits);
 
+    F feed(p, b, head, t0, lds);
+    const bool phased = kMayPhase<M> && feed.phased;
+    if (F::kAhead && t0 < t1) {                                // the first tile's loads first: the rest hides in them
+        feed.begin_k(0);
+        if (!phased) feed.begin_v(0);
+    }
     typename M::Owned qf;
-    M::load_owned(qf, (const typename T::elem *)p.q + (int64_t)bh * p.D * p.nq + (q < nq ? q : 0), p.nq, p.D, q_ok, h);
+    M::load_owned(qf, (const typename T::elem *)p.q + (int64_t)bh * p.D * p.nq, q < nq ? q : 0, p.nq, p.D, q_ok, h);
     Score<T> score(p, head);
     if (MODE == kPlain && score.in < 0.f) {                        // largest product = largest score
         M::negate(qf);
@@ -225,8 +235,6 @@ __global__ __launch_bounds__(64 * WQ, (two_resident<T, SRC, DP>) ? 2 : 1) void s
     // what scores are taken relative to (m once there is one), and how far above it they may lie
     float off = 0.f, room = -__builtin_inff();
 
-    F feed(p, b, head, t0, lds);
-    const bool phased = kMayPhase<M> && feed.phased;
     const Penalty<M, MODE, !kCodes> penalty(p, score.fall, qx, qy);    // codes: products are yet to be scaled
     const f32x16 from = penalty.from(score.in);
     uint64_t next = 0;                                         // live cells of the next tile
@@ -236,14 +244,11 @@ __global__ __launch_bounds__(64 * WQ, (two_resident<T, SRC, DP>) ? 2 : 1) void s
         if (!phased) feed.end_v(i, next);
         next_cell0 = feed.keys.cell0;
     };
-    if (F::kAhead && t0 < t1) {
-        feed.begin_k(0);
-        if (!phased) feed.begin_v(0);
-        finish(0);
-    }
+    if (F::kAhead && t0 < t1) finish(0);
     __syncthreads();
     for (int t = t0; t < t1; ++t) {
-        const int i = phased || !F::kAhead ? 0 : (t - t0) & 1, j = phased || !F::kAhead ? 0 : i ^ 1;
+        constexpr bool kOne = !F::kAhead || kOneBuffer<SRC, WQ>;
+        const int i = phased || kOne ? 0 : (t - t0) & 1, j = phased || kOne ? 0 : i ^ 1;
         if constexpr (!F::kAhead) {
             feed.begin_k(0);
             finish(0);
@@ -272,10 +277,11 @@ __global__ __launch_bounds__(64 * WQ, (two_resident<T, SRC, DP>) ? 2 : 1) void s
                     z[k] = acc[0];
                 }
             } else {
-                M::first(ktile, addr, 0, qf, z, from);
+                M::template first<kBlocks, M::kColumns == 32>(ktile, addr, 0, qf, z, from);
             }
 #pragma unroll
             for (int k = 0; k < kBlocks; ++k) {
+                if constexpr (M::kColumns < 32) M::fold(z[k]);
                 if constexpr (kCodes) {
                     float ks[16];
                     M::per_cell(cell, k, h, ks);
@@ -288,6 +294,13 @@ __global__ __launch_bounds__(64 * WQ, (two_resident<T, SRC, DP>) ? 2 : 1) void s
                 } else if constexpr (MODE != kPlain) {
                     if constexpr (!std::is_same_v<T, BF16>) __builtin_amdgcn_sched_barrier(0);
                     float d[16];
+                    if (M::kColumns < 32 && score.cap) {       // tanh before there is a d: registers
+#pragma unroll
+                        for (int i = 0; i < 16; ++i) {
+                            z[k][i] = score.bend(z[k][i]);
+                            if (i % 8 == 7) __builtin_amdgcn_sched_barrier(0);
+                        }
+                    }
                     if (MODE == kRows || penalty.on) {
                         penalty(cell + 64, cell0, k, h, -off, d);
                     } else {
@@ -296,7 +309,7 @@ __global__ __launch_bounds__(64 * WQ, (two_resident<T, SRC, DP>) ? 2 : 1) void s
                     }
                     if (MODE == kGeneral && score.cap) {
 #pragma unroll
-                        for (int i = 0; i < 16; ++i) z[k][i] = fmaf(score.top, score.bend(z[k][i]), d[i]);
+                        for (int i = 0; i < 16; ++i) z[k][i] = fmaf(score.top, M::kColumns < 32 ? z[k][i] : score.bend(z[k][i]), d[i]);
                     } else {
 #pragma unroll
                         for (int i = 0; i < 16; ++i) z[k][i] = fmaf(score.in, z[k][i], d[i]);
@@ -380,7 +393,11 @@ __global__ __launch_bounds__(64 * WQ, (two_resident<T, SRC, DP>) ? 2 : 1) void s
     l += __shfl_xor(l, 32);
     LateParams &e = late_params();
 
-    if (q >= e.nq) return;
+    if constexpr (M::kColumns < 32) {
+#pragma unroll
+        for (int c = 0; c < NC / 32; ++c) M::fold(o[c]);
+    }
+    if (q >= e.nq || (lane & 31) >= M::kColumns) return;
     if (e.splits > 1) {
         const int64_t part = (int64_t)split * e.B * e.heads + bh;
         if (h == 0) {
@@ -405,7 +422,7 @@ __global__ __launch_bounds__(64 * WQ, (two_resident<T, SRC, DP>) ? 2 : 1) void s
 // Joins the partial results of a split call: M = max m_s, out = sum_s 2^(m_s - M) o_s / sum_s 2^(m_s - M) l_s.
 // A block joins QB queries; their parts' weights lie in LDS.  The other 256 / QB threads of a query are dealt to channels
 // (many queries, few parts) or, for at most 64 queries, to parts, whose sums meet in LDS in a fixed order.
-constexpr int kMaxSplits = 512, kManySplits = 64;
+constexpr int kMaxSplits = 1024, kManySplits = 64;
 template <typename T>
 __global__ __launch_bounds__(256) void soft_join_kernel(const Params p, int channels_per_block) {
     constexpr int QB = 32, kLanes = 256 / QB;
@@ -446,8 +463,9 @@ __global__ __launch_bounds__(256) void soft_join_kernel(const Params p, int chan
         p.lse[(int64_t)bh * p.nq + q] = some ? (top + log2f(l)) * kLn2 : -__builtin_inff();
 }
 
-// 8 queries x 32 part lanes, kJoinChannels channels a block.
-constexpr int kJoinChannels = 8;
+// 8 queries x 32 part lanes, 2 channels a block: latency is all there is, so many blocks with loads 16 at a time (1024 parts of
+// 256 channels: 7 us; 8 channels a block, a part after the other: 16 us).
+constexpr int kJoinChannels = 2;
 template <typename T>
 __global__ __launch_bounds__(256) void soft_join_few_kernel(const Params p) {
     constexpr int kPer = kMaxSplits / 32;                      // parts of a lane
@@ -474,20 +492,31 @@ __global__ __launch_bounds__(256) void soft_join_few_kernel(const Params p) {
     for (int i = 0; i < 32; ++i) top = fmaxf(top, part[0][i][qi]);
     if (top == -__builtin_inff()) top = 0.f;                   // no part has a cell, or all scores are NaN
     __syncthreads();
-    // parts past the last one count with weight 0, from the last one's place: every load may go out at once
+    // parts past the last one count with weight 0, from the first one's place: kBatch loads go out at once
+    constexpr int kBatch = 8;
     const int cq = in ? (int)q : 0;
+    const int64_t step = bhn * p.Dv * p.nq;
+    const float *first = p.part_o + ((int64_t)bh * p.Dv + c0) * p.nq + cq;
+    const int64_t second = c0 + 1 < p.Dv ? p.nq : 0;
 #pragma unroll
-    for (int i = 0; i < kPer; ++i) {
-        if (32 * i >= p.splits) break;                         // uniform
-        const int s = g + 32 * i;
-        const float w = s < p.splits ? exp2_(m[i] - top) : 0.f;
-        l = fmaf(w, ls[i], l);
-        const float *src = p.part_o + (((s < p.splits ? s : 0) * bhn + bh) * p.Dv + c0) * p.nq + cq;
-        float x[kJoinChannels];
+    for (int i0 = 0; i0 < kPer; i0 += kBatch) {
+        if (32 * i0 >= p.splits) break;                        // uniform
+        float x[kBatch][kJoinChannels];
 #pragma unroll
-        for (int c = 0; c < kJoinChannels; ++c) x[c] = src[(c0 + c < p.Dv ? c : 0) * p.nq];
+        for (int i = 0; i < kBatch; ++i) {
+            const int s = g + 32 * (i0 + i);
+            const float *src = first + (s < p.splits ? s : 0) * step;
+            x[i][0] = src[0];
+            x[i][1] = src[second];
+        }
 #pragma unroll
-        for (int c = 0; c < kJoinChannels; ++c) v[c] = s < p.splits ? fmaf(w, x[c], v[c]) : v[c];
+        for (int i = 0; i < kBatch; ++i) {
+            const bool there = g + 32 * (i0 + i) < p.splits;
+            const float w = there ? exp2_(m[i0 + i] - top) : 0.f;
+            l = fmaf(w, ls[i0 + i], l);
+#pragma unroll
+            for (int c = 0; c < kJoinChannels; ++c) v[c] = there ? fmaf(w, x[i][c], v[c]) : v[c];
+        }
     }
     part[0][g][qi] = l;
     __syncthreads();

@@ -8,9 +8,9 @@ namespace ispa_soft {
 template <typename T, typename SRC, int DP, int WQ, int MODE>
 int forward_one(Params p, hipStream_t stream) {
     static unsigned long long lds_allowed = 0;
-    const int lds = lds_bytes<Math<T, DP>, DP>(p.shared, 1);
+    const int lds = lds_bytes<Math<T, DP>, DP>(p.shared, 1, kOneBuffer<SRC, WQ>);
     const unsigned grid = (unsigned)((int64_t)p.B * p.heads * p.splits * p.blocks);
-    constexpr int NC = DP == 256 && !std::is_same_v<T, BF16> ? 128 : DP;
+    constexpr int NC = DP == 256 && !std::is_same_v<T, BF16> && !std::is_same_v<T, F32Q> ? 128 : DP;
     for (p.c0 = 0; p.c0 < p.Dv; p.c0 += NC)
         if (int rc = launch(soft_forward_kernel<T, SRC, DP, WQ, NC, MODE>, p, grid, 64 * WQ, lds, &lds_allowed, "soft_forward_kernel",
                             stream))
@@ -30,7 +30,7 @@ int forward_one(Params p, hipStream_t stream) {
 template <typename T, typename SRC, int DP>
 int forward_waves(const Params &p, int waves, hipStream_t stream) {
     // F32S: more than 64 queries and up to 128 channels; F32: the rest
-    if constexpr (std::is_same_v<T, F32S> || (std::is_same_v<T, F32> && DP == 256) || !std::is_same_v<T, F32>)
+    if constexpr (!std::is_same_v<T, F32Q> && (!std::is_same_v<T, F32> || DP == 256))
         if (waves > 1)
             return with_mode<T, DP>(p, true, [&](auto mode) { return forward_one<T, SRC, DP, 4, decltype(mode)::value>(p, stream); });
     if constexpr (!std::is_same_v<T, F32S>)

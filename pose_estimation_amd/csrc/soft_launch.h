@@ -17,7 +17,7 @@ struct Plan {
     int waves, blocks, splits;
 };
 
-constexpr int kMaxSplitCount = 512;
+constexpr int kMaxSplitCount = 1024;
 
 // Workgroups of four waves for more than 64 owned cells.  Up to that all the parallelism lies in the streamed tiles, and
 // four waves would stage for one.
@@ -32,7 +32,12 @@ inline Arithmetic arithmetic(bool f32, bool codes, int padded, int waves) {
 }
 inline int64_t tile_rows(Arithmetic a) { return a == kFloat ? 32 : 64; }
 
-// resident: workgroups of four waves that a compute unit holds.  The tiles are split so that the rounds of
+// Whether float32 queries against codes come as columns of planes (F32Q): as many as three times fit a wave's 32 columns, with
+// a free group for sums over rows of 16 lanes.  One query against 24 views of 128x128x256: 62 us, with three products
+// and a wave a SIMD 90 us.
+inline bool few_columns(bool f32, int64_t owned) { return f32 && owned <= 8; }
+
+// resident: workgroups that a compute unit holds.  The tiles are split so that the rounds of
 // workgroups that the 256 compute units work off, each as long as its tiles and about two more to start, are shortest; a
 // split costs its workgroup about four tiles more, for writing and joining its part.
 inline Plan make_plan(int64_t owned, int64_t groups, int64_t tiles, int resident) {
@@ -40,7 +45,7 @@ inline Plan make_plan(int64_t owned, int64_t groups, int64_t tiles, int resident
     plan.waves = waves_for(owned);
     plan.blocks = (int)((owned + 32 * plan.waves - 1) / (32 * plan.waves));
     plan.splits = 1;
-    const int64_t base = groups * plan.blocks, room = 256 * (plan.waves == 1 ? 4 : resident);
+    const int64_t base = groups * plan.blocks, room = 256 * resident;
     int64_t best = INT64_MAX;
     for (int64_t s = 1; s <= tiles && s <= kMaxSplitCount && (s == 1 || base * (s - 1) < 4 * room); ++s) {
         const int64_t cost = (base * s + room - 1) / room * ((tiles + s - 1) / s + (s > 1 ? 6 : 2));

@@ -125,8 +125,11 @@ int stream_map(Stream *s, Arithmetic a, const void *map, int64_t maps, int d, in
     return ispa::check_launch("soft_pack_kernel");
 }
 
-// Workgroups of four waves a compute unit holds: two where a lane's registers allow it.
-int resident(int dtype, int D, int Dv, bool backward) {
+// Workgroups a compute unit holds: two waves a SIMD where a lane's registers allow it, else one.
+int resident(int dtype, bool codes, bool backward, int D, int Dv, int64_t owned) {
+    if (waves_for(owned) == 1)
+        return codes && padded_channels(D, Dv) <= 128 && (dtype == ISPA_BF16 || few_columns(true, owned)) ? 8 : 4;
+    backward |= codes;
     return padded_channels(D, Dv) <= (dtype == ISPA_BF16 ? 128 : backward ? 0 : 64) ? 2 : 1;
 }
 
@@ -136,7 +139,7 @@ Arithmetic arithmetic_of(int dtype, bool codes, int D, int Dv, int64_t owned) {
 
 Plan plan_of(int dtype, bool codes, bool backward, int64_t groups, int D, int Dv, int64_t owned, int V, int64_t streamed) {
     const int64_t r = tile_rows(arithmetic_of(dtype, codes, D, Dv, owned));
-    return make_plan(owned, groups, (streamed + r - 1) / r * V, resident(dtype, D, Dv, codes || backward));
+    return make_plan(owned, groups, (streamed + r - 1) / r * V, resident(dtype, codes, backward, D, Dv, owned));
 }
 
 size_t forward_bytes(const Plan &plan, int B, int heads, int Dv, int64_t nq) {

@@ -53,6 +53,30 @@ __device__ __forceinline__ unsigned pack_bf16(float lo, float hi) {
     return __builtin_bit_cast(unsigned, __builtin_convertvector(v, bf16x2));
 }
 
+// An element whose row is the same for the wave and whose column is a lane's own: the row's address moves on in scalar
+// registers, the column's bytes stay in one vector register, and no address is multiplied out.
+template <typename E>
+using Global = __attribute__((address_space(1))) E;
+template <typename E>
+__device__ __forceinline__ Global<E> *at_column(E *row, unsigned bytes) {
+    typedef std::conditional_t<std::is_const_v<E>, const char, char> byte;
+    return (Global<E> *)((Global<byte> *)row + bytes);
+}
+
+// The same pointer in every lane, in scalar registers.
+template <typename E>
+__device__ __forceinline__ E *scalar(E *p) {
+    const uint64_t at = (uint64_t)p;
+    return reinterpret_cast<E *>((uint64_t)(unsigned)__builtin_amdgcn_readfirstlane((int)(uint32_t)at) |
+                                 (uint64_t)(unsigned)__builtin_amdgcn_readfirstlane((int)(uint32_t)(at >> 32)) << 32);
+}
+
+// Rows are walked one after the other: not all their addresses at once.
+template <typename E>
+__device__ __forceinline__ void next_row(E *&row) {
+    asm("" : "+s"(row));
+}
+
 // Keeps the code of a rare case behind its branch: turned into selects it would cost every tile three operations a cell.
 __device__ __forceinline__ void stay_branch() { asm volatile(""); }
 
@@ -72,6 +96,9 @@ struct F32S {               // streamed maps in three planes
 struct F32C {               // streamed codes, which one bfloat16 number holds exactly
     typedef float elem;
 };
+struct F32Q {               // streamed codes, up to 8 queries
+    typedef float elem;
+};
 struct I8 {                 // codes of a template store; the value is code * scale[cell]
     typedef signed char elem;
 };
@@ -83,6 +110,8 @@ __device__ __forceinline__ float load_float(const float *p) { return *p; }
 __device__ __forceinline__ float load_float(const unsigned short *p) { return bf16_to_float(*p); }
 __device__ __forceinline__ void store_float(float *p, float v) { *p = v; }
 __device__ __forceinline__ void store_float(unsigned short *p, float v) { *p = (unsigned short)pack_bf16(v, 0.f); }
+__device__ __forceinline__ void store_float(Global<float> *p, float v) { *p = v; }
+__device__ __forceinline__ void store_float(Global<unsigned short> *p, float v) { *p = (unsigned short)pack_bf16(v, 0.f); }
 
 template <typename S>
 __device__ __forceinline__ void decode4(unsigned w, float (&f)[4]) {
@@ -118,21 +147,26 @@ struct Math<BF16, DP> {
     static constexpr int kBytes = 2;             // of a streamed number in LDS
     static constexpr int kPlanes = 1;            // LDS tiles that hold one tile of the map
     static constexpr bool kWide = false;         // float32 maps or queries
+    static constexpr int kColumns = 32;          // owned cells of a wave
     struct Owned {                               // B operand of the first product: channels 16 s + 8 h .. + 7
         bf16x8 f[DP / 16];
     };
-    // base: a column of the map (always a real one); !ok: zeros
-    __device__ __forceinline__ static void load_owned(Owned &o, const unsigned short *base, int64_t ld, int d, bool ok, int h) {
-        const int64_t lane = 8 * h * ld;
+    // column `col` (always a real one) of `map`, rows of ld cells; !ok: zeros
+    __device__ __forceinline__ static void load_owned(Owned &o, const unsigned short *map, int col, int64_t ld, int d, bool ok, int h) {
+        const unsigned lane = (unsigned)(8 * h * (int)ld + col) * sizeof(*map);
+        map = scalar(map);
         each<DP / 16>([&](auto step) {
             constexpr int s = decltype(step)::value;
             unsigned short e[8];
-            const bool whole = 16 * s + 16 <= d;               // uniform: a row's address is a scalar's distance away
+            const bool whole = 16 * s + 16 <= d;               // uniform
 #pragma unroll
             for (int j = 0; j < 8; ++j) {
-                if (whole) e[j] = base[(16 * s + j) * ld + lane];
-                else e[j] = 16 * s + 8 * h + j < d ? base[(16 * s + j) * ld + lane] : (unsigned short)0;
+                if (whole) e[j] = *at_column(map, lane);
+                else e[j] = 16 * s + 8 * h + j < d ? *at_column(map, lane) : (unsigned short)0;
+                map += ld;
+                next_row(map);
             }
+            map += 8 * ld;
             u32x4 w;
 #pragma unroll
             for (int j = 0; j < 4; ++j) w[j] = ok ? (unsigned)e[2 * j] | ((unsigned)e[2 * j + 1] << 16) : 0u;
@@ -172,7 +206,7 @@ struct Math<BF16, DP> {
     __device__ __forceinline__ static void first(const char *tile, const Addr &a, int b0, const Owned &o, f32x16 (&acc)[N],
                                  const f32x16 &from = f32x16{}) {
         typedef __attribute__((address_space(3))) s16x4 *lds_ptr;
-        constexpr int kSteps = DP / 16, kAhead = DP == 256 ? 0 : 2;
+        constexpr int kSteps = DP / 16, kAhead = DP == 256 ? 0 : AHEAD ? 2 : 1;
         auto frag = [&](int n, int s) {
             union {
                 s16x4 q[2];
@@ -249,16 +283,22 @@ struct Math<F32, DP> {
     static constexpr int kBytes = 4;
     static constexpr int kPlanes = 1;
     static constexpr bool kWide = true;
+    static constexpr int kColumns = 32;
     struct Owned {                               // channel 2 s + h
         float f[DP / 2];
     };
-    __device__ __forceinline__ static void load_owned(Owned &o, const float *base, int64_t ld, int d, bool ok, int h) {
+    __device__ __forceinline__ static void load_owned(Owned &o, const float *map, int col, int64_t ld, int d, bool ok, int h) {
+        const unsigned first = (unsigned)col * sizeof(*map), lane = first + (unsigned)(h * (int)ld) * sizeof(*map);
+        map = scalar(map);
         each<DP / 2>([&](auto step) {
             constexpr int s = decltype(step)::value;
-            const int c = 2 * s + h;
-            const float x = base[(int64_t)(c < d ? c : d - 1) * ld];
-            o.f[s] = ok && c < d ? x : 0.f;
-            if (DP == 256 && s % 8 == 7) __builtin_amdgcn_sched_barrier(0);
+            // past the last channel the last row again: it meets zeros in LDS
+            const float x = *at_column(map, 2 * s + h < d ? lane : first);
+            if (2 * s + 2 < d) map += 2 * ld;
+            next_row(map);
+            o.f[s] = ok ? x : 0.f;
+            if constexpr (DP == 256 && s % 2 == 0) asm("" : "+a"(o.f[s]));      // see accumulator_side
+            if (DP == 256 && s % 4 == 3) __builtin_amdgcn_sched_barrier(0);
         });
     }
     __device__ __forceinline__ static void negate(Owned &o) {
@@ -346,23 +386,28 @@ struct SplitMath {
     static constexpr int kBytes = 2;
     static constexpr int kPlanes = PLANES;
     static constexpr bool kWide = true;
+    static constexpr int kColumns = 32;
     static constexpr int kTile = DP * kRowBytes;
     struct Owned {
         bf16x8 f[3][DP / 16];
     };
     typedef typename Narrow::Addr Addr;
     __device__ __forceinline__ static Addr addr(int lane) { return Narrow::addr(lane); }
-    __device__ __forceinline__ static void load_owned(Owned &o, const float *base, int64_t ld, int d, bool ok, int h) {
-        const int64_t lane = 8 * h * ld;
+    __device__ __forceinline__ static void load_owned(Owned &o, const float *map, int col, int64_t ld, int d, bool ok, int h) {
+        const unsigned lane = (unsigned)(8 * h * (int)ld + col) * sizeof(*map);
+        map = scalar(map);
         each<DP / 16>([&](auto step) {
             constexpr int s = decltype(step)::value;
             float e[8];
             const bool whole = 16 * s + 16 <= d;
 #pragma unroll
             for (int j = 0; j < 8; ++j) {
-                if (whole) e[j] = base[(16 * s + j) * ld + lane];
-                else e[j] = 16 * s + 8 * h + j < d ? base[(16 * s + j) * ld + lane] : 0.f;
+                if (whole) e[j] = *at_column(map, lane);
+                else e[j] = 16 * s + 8 * h + j < d ? *at_column(map, lane) : 0.f;
+                map += ld;
+                next_row(map);
             }
+            map += 8 * ld;
             u32x4 w[3];
 #pragma unroll
             for (int j = 0; j < 4; ++j) {
@@ -475,24 +520,100 @@ struct Math<F32S, DP> : SplitMath<DP, 3> {};
 template <int DP>
 struct Math<F32C, DP> : SplitMath<DP, 1> {};
 
+// Up to 8 float32 queries against codes: the three planes of a query are three of a wave's columns, 8 apart, instead of
+// three products (a third of the MFMAs and of the registers).  Sums over planes are sums over columns (fold).
+template <int DP>
+struct Math<F32Q, DP> : Math<BF16, DP> {
+    typedef Math<BF16, DP> Narrow;
+    typedef typename Narrow::Owned Owned;
+    typedef typename Narrow::Weights Weights;
+    static constexpr bool kWide = true;
+    static constexpr int kColumns = 8;
+    // The plane that this lane's column stands for; the fourth 8 columns hold zeros.
+    struct Plane {
+        unsigned m1, m2, keep;
+        __device__ __forceinline__ Plane() {
+            unsigned k = threadIdx.x;
+            asm volatile("" : "+v"(k));                        // formed where it is used: registers
+            k = (k >> 3) & 3;
+            m1 = k >= 1 ? 0xffff0000u : 0u;
+            m2 = k >= 2 ? 0xffff0000u : 0u;
+            keep = k == 3 ? 0u : ~0u;
+        }
+        __device__ __forceinline__ unsigned operator()(float x) const {          // in the upper half of the word
+            x -= __builtin_bit_cast(float, __builtin_bit_cast(unsigned, x) & m1);
+            x -= __builtin_bit_cast(float, __builtin_bit_cast(unsigned, x) & m2);
+            return __builtin_bit_cast(unsigned, x);
+        }
+        __device__ __forceinline__ unsigned operator()(float x, float y) const { return uppers((*this)(x), (*this)(y)) & keep; }
+    };
+    __device__ __forceinline__ static void load_owned(Owned &o, const float *map, int col, int64_t ld, int d, bool ok, int h) {
+        const unsigned lane = (unsigned)(8 * h * (int)ld + col) * sizeof(*map);
+        const Plane plane;
+        map = scalar(map);
+        each<DP / 16>([&](auto step) {
+            constexpr int s = decltype(step)::value;
+            float e[8];
+            const bool whole = 16 * s + 16 <= d;
+#pragma unroll
+            for (int j = 0; j < 8; ++j) {
+                if (whole) e[j] = *at_column(map, lane);
+                else e[j] = 16 * s + 8 * h + j < d ? *at_column(map, lane) : 0.f;
+                map += ld;
+                next_row(map);
+            }
+            map += 8 * ld;
+            u32x4 w;
+#pragma unroll
+            for (int j = 0; j < 4; ++j) w[j] = ok ? plane(e[2 * j], e[2 * j + 1]) : 0u;
+            o.f[s] = __builtin_bit_cast(bf16x8, w);
+            if constexpr (DP == 256) o.f[s] = accumulator_side(o.f[s]);
+            if (s % 4 == 3) __builtin_amdgcn_sched_barrier(0);
+        });
+    }
+    __device__ __forceinline__ static Weights weights(const float (&p)[16]) {
+        const Plane plane;
+        Weights w;
+#pragma unroll
+        for (int s = 0; s < 2; ++s) {
+            u32x4 v;
+#pragma unroll
+            for (int j = 0; j < 4; ++j) v[j] = plane(p[8 * s + 2 * j], p[8 * s + 2 * j + 1]);
+            w.f[s] = __builtin_bit_cast(bf16x8, v);
+        }
+        return w;
+    }
+    // every column of a query gets the sum of all three: its row of 16 lanes turned by 8, then the other row's
+    __device__ __forceinline__ static void fold(f32x16 &v) {
+#pragma unroll
+        for (int i = 0; i < 16; ++i) {
+            const float x = v[i];
+            const float a = x + __builtin_bit_cast(float, __builtin_amdgcn_update_dpp(0, __builtin_bit_cast(int, x), 0x128, 0xf, 0xf, false));
+            const auto b = __builtin_amdgcn_permlane16_swap(__builtin_bit_cast(unsigned, a), __builtin_bit_cast(unsigned, a), false, false);
+            const unsigned even = b[0], odd = b[1];
+            v[i] = __builtin_bit_cast(float, even) + __builtin_bit_cast(float, odd);
+        }
+    }
+};
+
 // Channel of output accumulator register i of a 32-channel block.
 __device__ __forceinline__ int out_channel(int i, int h) { return 8 * (i >> 2) + 4 * h + (i & 3); }
 
 // Stores 32-channel blocks of accumulators: channels c0 .. c0 + NC - 1 of column q of a map (d, n).
 template <int NC, typename E>
 __device__ __forceinline__ void store_columns(E *map, int64_t n, int q, int h, int c0, int d, const f32x16 (&o)[NC / 32]) {
-    E *at = map + 4 * h * n + q;
+    const unsigned lane = (unsigned)(4 * h * (int)n + q) * sizeof(E);
+    E *row = scalar(map + c0 * n);
     each<NC / 32>([&](auto block) {
         constexpr int c = decltype(block)::value;
-        if (c0 + 32 * c + 32 <= d) {                           // uniform: a channel's address is a scalar's distance away
+        const bool whole = c0 + 32 * c + 32 <= d;              // uniform
 #pragma unroll
-            for (int i = 0; i < 16; ++i) store_float(at + (c0 + 32 * c + out_channel(i, 0)) * n, o[c][i]);
-        } else {
-#pragma unroll
-            for (int i = 0; i < 16; ++i)
-                if (c0 + 32 * c + out_channel(i, h) < d) store_float(at + (c0 + 32 * c + out_channel(i, 0)) * n, o[c][i]);
+        for (int i = 0; i < 16; ++i) {
+            if (whole || c0 + 32 * c + out_channel(i, h) < d) store_float(at_column(row, lane), o[c][i]);
+            row += i % 4 < 3 ? n : 5 * n;
+            next_row(row);
         }
-        __builtin_amdgcn_sched_barrier(0);                     // bounds the addresses in registers
+        __builtin_amdgcn_sched_barrier(0);
     });
 }
 
@@ -509,39 +630,58 @@ struct Loader {
     static constexpr int kPer = DP * 8 / NT;
     typedef typename SRC::elem elem;
     typedef u32x2 raw;
+    typedef u32x2 Unaligned __attribute__((aligned(1)));
     static constexpr bool kAhead = kPer * (int)sizeof(raw) <= (DP == 256 ? 32 : 128);
     static constexpr int kBatch = kAhead ? kPer : DP == 256 ? 1 : kPer < 8 ? kPer : 8;
     static constexpr int kLoop = kAhead ? kPer / kBatch : 1;
     static_assert(NT == 64 || NT % 128 == 0, "");
     raw r[kBatch];
-    const elem *from;          // this thread's first segment
+    const elem *map;           // of the wave
+    unsigned from;             // this thread's first segment in it
     int ok;                    // cells of the segment that the map has
+    int back;                  // a segment that the row's end cuts is read this many cells before its place, up to that end
 
     __device__ __forceinline__ void rows(int i0, int64_t ld, int d) {
         const int row0 = threadIdx.x >> 3;
-        const elem *p = from + (int64_t)i0 * (NT / 8) * ld;
+        const elem *row = map + (int64_t)i0 * (NT / 8) * ld;
+        if (ld >= kN && (i0 + kBatch) * (NT / 8) <= d && __all(ok > 0)) {      // every lane loads: no branch between
+#pragma unroll
+            for (int i = 0; i < kBatch; ++i) {
+                r[i] = *(Global<const Unaligned> *)at_column(row, from);
+                row += (int64_t)(NT / 8) * ld;
+                next_row(row);
+            }
+            return;
+        }
+        stay_branch();
+        asm volatile("" : "+s"(d));                            // the rows' masks anew for each tile: kept, they fill the registers
 #pragma unroll
         for (int i = 0; i < kBatch; ++i) {
             raw v = {};
-            if (row0 + (i0 + i) * (NT / 8) < d) {
-                if (ok == kN) {
-                    __builtin_memcpy(&v, p, sizeof(raw));
-                } else if (ok > 0) {
-                    elem e[kN];
-#pragma unroll
-                    for (int j = 0; j < kN; ++j) e[j] = j < ok ? p[j] : (elem)0;
-                    __builtin_memcpy(&v, e, sizeof(raw));
+            if (ok > 0 && row0 + (i0 + i) * (NT / 8) < d) {
+                if (ld >= kN) {
+                    v = *(Global<const Unaligned> *)at_column(row, from);
+                } else {                                       // rows of fewer cells: byte by byte
+                    stay_branch();
+#pragma unroll 1
+                    for (int j = 0; j < (int)ld; ++j) {
+                        const uint64_t x = (uint64_t)(unsigned char)at_column(row, from)[j] << (8 * j);
+                        v |= __builtin_bit_cast(raw, x);
+                    }
                 }
             }
             r[i] = v;
-            p += (int64_t)(NT / 8) * ld;
+            row += (int64_t)(NT / 8) * ld;
+            next_row(row);
         }
     }
     __device__ __forceinline__ void load(const elem *base, int64_t ld, int d, int64_t cell0, int64_t n) {
         const int64_t at = cell0 + (threadIdx.x & 7) * kN;
         const int64_t left = n - at;
         ok = left >= kN ? kN : left > 0 ? (int)left : 0;
-        from = base + (int64_t)(threadIdx.x >> 3) * ld + at;
+        back = ok > 0 && ld >= kN ? kN - ok : 0;
+        map = scalar(base);
+        from = (unsigned)((int)(threadIdx.x >> 3) * (int)ld + (int)at - back);
         if constexpr (kAhead) rows(0, ld, d);
     }
     __device__ __forceinline__ void store(char *tile, int64_t ld, int d, uint64_t live) {
@@ -555,6 +695,12 @@ struct Loader {
 #pragma unroll kLoop
         for (int i0 = 0; i0 < kPer; i0 += kBatch) {
             if constexpr (!kAhead) rows(i0, ld, d);
+            if (__any(back > 0)) {
+                stay_branch();
+#pragma unroll
+                for (int i = 0; i < kBatch; ++i)
+                    r[i] = __builtin_bit_cast(raw, __builtin_bit_cast(uint64_t, r[i]) >> (8 * back));
+            }
 #pragma unroll
             for (int i = 0; i < kBatch; ++i) {
                 float x[4], y[4];

@@ -740,6 +740,39 @@ def test_store_match_falloff(sc, dtype, kind, c, heads, size, n):
 
 
 @gpu
+@pytest.mark.parametrize("dtype", [F32, BF16])
+@pytest.mark.parametrize("kind", ["int8", "fp8"])
+@pytest.mark.parametrize("n, c, heads, size, views", [(1, 128, 1, (1, 1), 2), (8, 128, 1, (1, 7), 1), (7, 40, 2, (1, 9), 3), (1, 256, 1, (23, 29), 4),
+                                                      (8, 256, 2, (40, 41), 3), (9, 64, 1, (2, 3), 2), (3, 5, 1, (64, 64), 30), (1, 12, 3, (130, 130), 5)])
+@pytest.mark.parametrize("cap, falloff", [(0.0, None), (6.0, None), (9.0, 0.02)])
+def test_store_match_few_queries(sc, dtype, kind, n, c, heads, size, views, cap, falloff):
+    """Up to 8 queries, rows of codes that end inside a tile or are shorter than a segment, features of any size."""
+    h, w = size
+    store = sc.TemplateStore(views, c, size, kind)
+    feats = rand(200, (views, c) + size, F32) * torch.exp(torch.randn((views, 1) + size, generator=torch.Generator().manual_seed(201)) * 0.3)
+    mask = silhouette(202, views, h, w)
+    mask[0, 0, 0] = True
+    store.write(range(views), feats, mask=mask)
+    q = rand(203, (2, c, n), dtype)
+    xy = torch.rand((2, n, 2), generator=torch.Generator().manual_seed(204)) * torch.tensor([w - 1.0, h - 1.0])
+    opts = dict(heads=heads, scale=14.0, cap=cap, falloff=falloff, query_xy=xy if falloff else None, num_query=[n, max(n - 2, 1)])
+    out, lse = store.soft_match(q.cuda(), [list(range(views))] * 2, return_lse=True, **opts)
+    values = np.broadcast_to(flat(store.read(range(views))).transpose(1, 0, 2).reshape(c, -1), (2, c, views * h * w))
+    taken = np.broadcast_to(mask.numpy().reshape(-1), (2, views * h * w))
+    if falloff:                                          # per view, joined by the log-sums
+        parts = [oracle(flat(q), values[:, :, i * h * w:(i + 1) * h * w], values[:, :, i * h * w:(i + 1) * h * w], heads, 14.0, cap,
+                        [falloff] * heads, host(xy), w, taken[:, i * h * w:(i + 1) * h * w], opts["num_query"]) for i in range(views)]
+        want_lse = np.logaddexp.reduce([p[1] for p in parts])
+        share = [np.repeat(np.where(np.isneginf(p[1]), 0, np.exp(p[1] - np.where(np.isneginf(want_lse), 0, want_lse))), c // heads, 1)
+                 for p in parts]
+        want, mag = sum(s * p[0] for s, p in zip(share, parts)), sum(s * p[2] for s, p in zip(share, parts))
+    else:
+        want, want_lse, mag = oracle(flat(q), values, values, heads, 14.0, cap, mask=taken, count=opts["num_query"])[:3]
+    near(out, want, mag, dtype, 1)
+    near_lse(lse, want_lse)
+
+
+@gpu
 def test_store_over_a_part_of_another(sc):
     """Views of a larger tensor, which start anywhere."""
     store = sc.TemplateStore(4, 9, (5, 7))
