@@ -4,6 +4,7 @@
 #include "soft_launch.h"
 
 namespace ispa_soft {
+static_assert(kMaxSplits == kMaxSplitCount, "the join reads every part");
 
 template <typename T, typename SRC, int DP, int WQ, int MODE>
 int forward_one(Params p, hipStream_t stream) {
