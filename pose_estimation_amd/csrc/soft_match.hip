@@ -26,62 +26,65 @@ int check_sizes(int dtype, int B, int heads, int D, int Dv, int64_t nq, int V, i
 
 size_t align256(size_t x) { return (x + 255) & ~(size_t)255; }
 
-// Copies maps (maps, d, n) into the form Direct wants: (maps, d8, ld) with d8 the next multiple of 8 rows and ld of 16 bytes,
-// zeros beside.  16 bytes a thread, read as they lie.
-template <typename T>
-__global__ __launch_bounds__(256) void soft_pack_kernel(const typename T::elem *src, typename T::elem *dst, int d, int d8, int n,
-                                                        int segs, int64_t total) {
-    typedef typename T::elem elem;
-    constexpr int kN = 16 / sizeof(elem);
-    const int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x;
-    if (i >= total) return;
-    const int row = (int)(i / segs), cell = (int)(i - (int64_t)row * segs) * kN;
-    const int map = row / d8, c = row - map * d8;
+// Maps (maps, d, n) to be copied into the form Direct wants: rows of `segs` 16-byte segments, d8 rows with d8 the next multiple of
+// 8, zeros beside; for kSplit three planes of bfloat16 numbers, (maps, 3, d8, ld).  One launch copies all maps of a call
+// that take the same arithmetic: its copies are a few us each, launches as much again (a float32 training step of 8 pairs of
+// 28x28x128 makes four copies, one of ragged bfloat16 maps six).
+constexpr int kMostCopies = 4;
+struct CopyJob {
+    const void *src;
+    void *dst;
+    int d, d8, n, segs;
+    int64_t total;             // segments of the copy (kSplit: of one plane)
+};
+struct CopyJobs {
+    CopyJob job[kMostCopies];
+    unsigned until[kMostCopies];       // the first block behind each job
+    int count;
+};
+
+// 16 bytes a thread, read as they lie.
+template <Arithmetic A>
+__global__ __launch_bounds__(256) void soft_copy_kernel(const CopyJobs jobs) {
+    int k = 0;
+    while (k + 1 < jobs.count && blockIdx.x >= jobs.until[k]) ++k;
+    const CopyJob &job = jobs.job[k];
+    const unsigned block = blockIdx.x - (k > 0 ? jobs.until[k - 1] : 0);
+    const int64_t i = (int64_t)block * 256 + threadIdx.x;
+    if (i >= job.total) return;
+    typedef std::conditional_t<A == kNarrow, unsigned short, float> elem;
+    constexpr int kN = A == kFloat ? 4 : 8;
+    const int row = (int)(i / job.segs), seg = (int)(i - (int64_t)row * job.segs), cell = seg * kN;
+    const int map = row / job.d8, c = row - map * job.d8;
     elem e[kN] = {};
-    if (c < d) {
-        const elem *at = src + ((int64_t)map * d + c) * n + cell;
-        if (cell + kN <= n) {
-            __builtin_memcpy(e, at, 16);
+    if (c < job.d) {
+        const elem *at = (const elem *)job.src + ((int64_t)map * job.d + c) * job.n + cell;
+        if (cell + kN <= job.n) {
+            __builtin_memcpy(e, at, sizeof(e));
         } else {
 #pragma unroll
             for (int j = 0; j < kN; ++j)
-                if (cell + j < n) e[j] = at[j];
+                if (cell + j < job.n) e[j] = at[j];
         }
     }
-    u32x4 v;
-    __builtin_memcpy(&v, e, 16);
-    *reinterpret_cast<u32x4 *>(dst + i * kN) = v;
-}
-
-// float32 maps as three planes of bfloat16 numbers (F32S), (maps, 3, d8, ld); 8 cells a thread.
-__global__ __launch_bounds__(256) void soft_split_kernel(const float *src, u32x4 *dst, int d, int d8, int n, int segs,
-                                                         int64_t total) {
-    const int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x;
-    if (i >= total) return;
-    const int row = (int)(i / segs), seg = (int)(i - (int64_t)row * segs), cell = seg * 8;
-    const int map = row / d8, c = row - map * d8;
-    float e[8] = {};
-    if (c < d) {
-        const float *at = src + ((int64_t)map * d + c) * n + cell;
-        if (cell + 8 <= n) {
-            __builtin_memcpy(e, at, 32);
-        } else {
+    u32x4 *dst = (u32x4 *)job.dst;
+    if constexpr (A == kSplit) {
+        u32x4 v[3];
 #pragma unroll
-            for (int j = 0; j < 8; ++j)
-                if (cell + j < n) e[j] = at[j];
+        for (int j = 0; j < 4; ++j) {
+            unsigned x[3], y[3];
+            split3(e[2 * j], x[0], x[1], x[2]);
+            split3(e[2 * j + 1], y[0], y[1], y[2]);
+#pragma unroll
+            for (int p = 0; p < 3; ++p) v[p][j] = uppers(x[p], y[p]);
         }
+#pragma unroll
+        for (int p = 0; p < 3; ++p) dst[(((int64_t)map * 3 + p) * job.d8 + c) * job.segs + seg] = v[p];
+    } else {
+        u32x4 v;
+        __builtin_memcpy(&v, e, 16);
+        dst[i] = v;
     }
-    u32x4 v[3];
-#pragma unroll
-    for (int j = 0; j < 4; ++j) {
-        unsigned x[3], y[3];
-        split3(e[2 * j], x[0], x[1], x[2]);
-        split3(e[2 * j + 1], y[0], y[1], y[2]);
-#pragma unroll
-        for (int k = 0; k < 3; ++k) v[k][j] = uppers(x[k], y[k]);
-    }
-#pragma unroll
-    for (int k = 0; k < 3; ++k) dst[(((int64_t)map * 3 + k) * d8 + c) * segs + seg] = v[k];
 }
 
 // Copies of maps in the workspace: three planes for kSplit; else only maps whose rows do not start on 16-byte borders or
@@ -102,28 +105,44 @@ Copies copies(Arithmetic a, int64_t maps, int d, int64_t n) {
     return c;
 }
 
-// The map for streaming; `at` moves past the copy, if there is one.
-int stream_map(Stream *s, Arithmetic a, const void *map, int64_t maps, int d, int64_t n, char **at, hipStream_t stream) {
-    const Copies c = copies(a, maps, d, n);
-    s->ld = c.ld;
-    s->d = c.d8;
-    s->map = map;
-    if (c.bytes == 0) return ISPA_OK;
-    const int segs = (int)(c.ld / (a == kFloat ? 4 : 8));
-    const int64_t rows = maps * c.d8, total = rows * segs;
-    ISPA_REQUIRE(rows < (1ll << 31) && total < (1ll << 32) - 256, "maps of %lld rows are too large for one call", (long long)rows);
-    const unsigned blocks = (unsigned)((total + 255) / 256);
-    if (a == kSplit)
-        soft_split_kernel<<<blocks, 256, 0, stream>>>((const float *)map, (u32x4 *)*at, d, c.d8, (int)n, segs, total);
-    else if (a == kFloat)
-        soft_pack_kernel<F32><<<blocks, 256, 0, stream>>>((const float *)map, (float *)*at, d, c.d8, (int)n, segs, total);
-    else
-        soft_pack_kernel<BF16><<<blocks, 256, 0, stream>>>((const unsigned short *)map, (unsigned short *)*at, d, c.d8, (int)n, segs,
-                                                           total);
-    s->map = *at;
-    *at += c.bytes;
-    return ispa::check_launch("soft_pack_kernel");
-}
+// The copies of a call: add() settles how a map is streamed, launch() makes the copies that were asked for.
+class Copier {
+public:
+    explicit Copier(char *workspace) : at(workspace) {}
+    int add(Stream *s, Arithmetic a, const void *map, int64_t maps, int d, int64_t n) {
+        const Copies c = copies(a, maps, d, n);
+        s->ld = c.ld;
+        s->d = c.d8;
+        s->map = map;
+        if (c.bytes == 0) return ISPA_OK;
+        const int segs = (int)(c.ld / (a == kFloat ? 4 : 8));
+        const int64_t rows = maps * c.d8, total = rows * segs;
+        CopyJobs &j = jobs[a];
+        const int64_t before = j.count > 0 ? j.until[j.count - 1] : 0, blocks = before + (total + 255) / 256;
+        ISPA_REQUIRE(rows < (1ll << 31) && blocks < (1ll << 32) / 256, "maps of %lld rows are too large for one call", (long long)rows);
+        j.job[j.count] = CopyJob{map, at, d, c.d8, (int)n, segs, total};
+        j.until[j.count++] = (unsigned)blocks;
+        s->map = at;
+        at += c.bytes;
+        return ISPA_OK;
+    }
+    int launch(hipStream_t stream) const {
+        if (int rc = one<kNarrow>(stream)) return rc;
+        if (int rc = one<kSplit>(stream)) return rc;
+        return one<kFloat>(stream);
+    }
+    char *at;                  // of the workspace, behind the copies
+
+private:
+    template <Arithmetic A>
+    int one(hipStream_t stream) const {
+        const CopyJobs &j = jobs[A];
+        if (j.count == 0) return ISPA_OK;
+        soft_copy_kernel<A><<<j.until[j.count - 1], 256, 0, stream>>>(j);
+        return ispa::check_launch("soft_copy_kernel");
+    }
+    CopyJobs jobs[3] = {};
+};
 
 // Workgroups a compute unit holds: two waves a SIMD where a lane's registers allow it, else one.
 int resident(int dtype, bool codes, bool backward, int D, int Dv, int64_t owned) {
@@ -194,13 +213,14 @@ int run_forward(Params &p, int dtype, Source source, void *workspace, size_t wor
     p.tiles = p.tiles_per_view * p.V;
     p.blocks = plan.blocks;
     p.splits = plan.splits;
-    char *at = (char *)workspace;
+    Copier copier((char *)workspace);
     if (maps) {
-        if (int rc = stream_map(&p.sk, a, p.k, bh, p.D, p.cells, &at, stream)) return rc;
+        if (int rc = copier.add(&p.sk, a, p.k, bh, p.D, p.cells)) return rc;
         if (!p.shared)
-            if (int rc = stream_map(&p.sv, a, p.v, bh, p.Dv, p.cells, &at, stream)) return rc;
+            if (int rc = copier.add(&p.sv, a, p.v, bh, p.Dv, p.cells)) return rc;
+        if (int rc = copier.launch(stream)) return rc;
     }
-    p.part_ml = (float *)at;
+    p.part_ml = (float *)copier.at;
     p.part_o = p.part_ml + (size_t)plan.splits * bh * p.nq * 2;
     if (maps) return dtype == ISPA_F32 ? forward_f32(p, plan.waves, stream) : forward_bf16(p, plan.waves, stream);
     return dtype == ISPA_F32 ? forward_codes_f32(p, source == kFp8, plan.waves, stream)
@@ -344,18 +364,19 @@ extern "C" int ispa_soft_match_backward(const void *q, const void *r, const void
     hipStream_t s = (hipStream_t)stream;
     const int64_t bh = (int64_t)B * heads;
     ISPA_REQUIRE((((uintptr_t)r | (uintptr_t)p.v | (uintptr_t)q | (uintptr_t)d_out) & 15) == 0, "maps must start on 16-byte borders");
-    char *at = (char *)workspace;
+    Copier copier((char *)workspace);
     const Arithmetic aq = arithmetic_of(dtype, false, D, Dv, nq), akv = arithmetic_of(dtype, false, D, Dv, cells);
-    if (int rc = stream_map(&p.sk, aq, r, bh, D, cells, &at, s)) return rc;
+    if (int rc = copier.add(&p.sk, aq, r, bh, D, cells)) return rc;
     if (!p.shared)
-        if (int rc = stream_map(&p.sv, aq, v, bh, Dv, cells, &at, s)) return rc;
+        if (int rc = copier.add(&p.sv, aq, v, bh, Dv, cells)) return rc;
     if (nq > 0) {
-        if (int rc = stream_map(&p.sq, akv, q, bh, D, nq, &at, s)) return rc;
-        if (int rc = stream_map(&p.so, akv, d_out, bh, Dv, nq, &at, s)) return rc;
+        if (int rc = copier.add(&p.sq, akv, q, bh, D, nq)) return rc;
+        if (int rc = copier.add(&p.so, akv, d_out, bh, Dv, nq)) return rc;
     }
-    float *delta = (float *)at;
+    if (int rc = copier.launch(s)) return rc;
+    float *delta = (float *)copier.at;
     p.delta = delta;
-    p.part_a = (float *)(at + align256(bh * nq * sizeof(float)));
+    p.part_a = (float *)(copier.at + align256(bh * nq * sizeof(float)));
     p.part_b = p.part_a + (pkv.splits > 1 ? (size_t)pkv.splits * bh * D * cells : 0);
     if (nq > 0) {
         const unsigned grid = (unsigned)((nq + 31) / 32 * bh);
