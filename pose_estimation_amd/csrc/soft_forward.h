@@ -300,7 +300,7 @@ __global__ __launch_bounds__(64 * WQ, (two_resident<T, SRC, DP, WQ>) ? 2 : 1) vo
                 }
                 if constexpr (MODE == kCapped) {
 #pragma unroll
-                    for (int i = 0; i < 16; ++i) z[k][i] = (-2.f * score.top) * score.r(z[k][i]);
+                    for (int i = 0; i < 16; ++i) z[k][i] = score.below_cap(z[k][i]);
                 } else if constexpr (MODE != kPlain) {
                     if constexpr (!std::is_same_v<T, BF16>) __builtin_amdgcn_sched_barrier(0);
                     float d[16];

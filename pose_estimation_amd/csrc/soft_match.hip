@@ -208,6 +208,7 @@ int run_forward(Params &p, int dtype, Source source, void *workspace, size_t wor
     const size_t need = copied + forward_bytes(plan, p.B, p.heads, p.Dv, p.nq);
     if (need > 0 && (workspace == nullptr || workspace_bytes < need))
         return ispa::fail(ISPA_EWORKSPACE, "workspace of %zu bytes, %zu needed", workspace_bytes, need);
+    ISPA_REQUIRE(need == 0 || ((uintptr_t)workspace & 255) == 0, "the workspace must start on a 256-byte border");
     ISPA_REQUIRE(!maps || (((uintptr_t)p.k | (uintptr_t)p.v) & 15) == 0, "maps must start on 16-byte borders");
     p.tiles_per_view = (int)((p.cells + tile_rows(a) - 1) / tile_rows(a));
     p.tiles = p.tiles_per_view * p.V;
@@ -337,6 +338,7 @@ extern "C" int ispa_soft_match_backward(const void *q, const void *r, const void
     const size_t need = backward_bytes(dtype, pq, pkv, B, heads, D, Dv, nq, cells);
     if (workspace_bytes < need || (need > 0 && workspace == nullptr))
         return ispa::fail(ISPA_EWORKSPACE, "workspace of %zu bytes, %zu needed", workspace_bytes, need);
+    ISPA_REQUIRE(need == 0 || ((uintptr_t)workspace & 255) == 0, "the workspace must start on a 256-byte border");
     Params p = {};
     p.q = q;
     p.k = r;

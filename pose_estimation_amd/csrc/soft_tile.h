@@ -902,16 +902,21 @@ struct Score {
     // kernels leave.  float32 keeps the relative error near 1e-7 too: below 0.6 the odd polynomial y + y^3 c(y^2), c
     // fitted to (tanh(y) / y - 1) / y^2 on [0, 0.36] by weighted least squares.
     static constexpr bool kExact = !std::is_same_v<T, BF16>;
-    float in, top, fall, in2;
+    float in, top, fall, in2, per;
     bool cap;
     __device__ __forceinline__ Score(const Params &p, int head) {
         cap = p.cap > 0.f;
         in = cap ? p.scale / p.cap : p.scale * kLog2e;
         in2 = in * (2.f * kLog2e);
         top = p.cap * kLog2e;
+        per = -0.5f / top;
         fall = p.falloff ? p.falloff[head] * kLog2e : 0.f;
     }
     __device__ __forceinline__ float r(float acc) const { return __builtin_amdgcn_rcpf(__builtin_amdgcn_exp2f(acc * in2) + 1.f); }
+    // -2 top r: what tanh leaves of the cap.  The factor rides in the sum under the reciprocal.
+    __device__ __forceinline__ float below_cap(float acc) const {
+        return __builtin_amdgcn_rcpf(fmaf(__builtin_amdgcn_exp2f(acc * in2), per, per));
+    }
     __device__ __forceinline__ float bend(float acc) const {
         const float far = fmaf(-2.f, r(acc), 1.f);
         if constexpr (!kExact) return far;

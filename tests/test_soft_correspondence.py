@@ -911,6 +911,7 @@ def test_abi_refusals():
     assert need > 0 and lib.ispa_soft_match_workspace_bytes(0, 1, 1, 300, 128, 1, 1, 16384) == 0
     assert match(d=128, dv=128, nq=1, cells=16384) == -3 and b"workspace" in lib.ispa_last_error()
     assert match(d=128, dv=128, nq=1, cells=16384, ws=1, size=need - 1) == -3
+    assert match(d=128, dv=128, nq=1, cells=16384, ws=1, size=need) == -1 and b"border" in lib.ispa_last_error()
     back = lambda **k: lib.ispa_soft_match_backward(1, 1, k.get("v"), 0, 1, 1, 64, 64, 10, 100, 10, 1.0, 0.0, None, None, None, None, 1, 1, 1,
                                                     None, 1, 1, k.get("dv"), None, 0, None)
     assert back(v=1) == -1 and b"come together" in lib.ispa_last_error()
