@@ -19,18 +19,22 @@ from . import _abi, _device as dv
 
 _CODES = {torch.float32: _abi.F32, torch.bfloat16: _abi.BF16}
 MAX_CHANNELS = _abi.SOFT_MAX_CHANNELS
+_HERE = contextlib.nullcontext()
 
 
 def _dims(x):
-    return tuple(x.shape) if hasattr(x, "shape") else np.shape(x)
+    try:
+        return tuple(x.shape)
+    except AttributeError:
+        return np.shape(x)
 
 
-def _elements(x, name):
-    """Cells of a feature map given as array or tensor; a shape check before anything touches the device."""
-    shape = _dims(x)
-    if len(shape) < 3:
-        raise ValueError(f"{name} must be (B,C,H,W) or (B,C,n), got {_dims(x)}")
-    return math.prod(shape[2:])
+def _map(x, name):
+    """Dimensions of a feature map given as array or tensor, and its cells; checked before anything touches the device."""
+    dims = _dims(x)
+    if len(dims) < 3:
+        raise ValueError(f"{name} must be (B,C,H,W) or (B,C,n), got {dims}")
+    return dims, math.prod(dims[2:])
 
 
 def _dtype(x, name):
@@ -44,10 +48,14 @@ def _dtype(x, name):
 def _place(x):
     """(device of the call, context that makes it the current one): where its first tensor lives, else the current one."""
     if dv.is_tensor(x) and x.is_cuda:
-        if x.device.index == torch.cuda.current_device():
-            return x.device, contextlib.nullcontext()
-        return x.device, torch.cuda.device(x.device)
-    return dv.device(), contextlib.nullcontext()
+        device = x.device
+        return device, _HERE if device.index == torch._C._cuda_getDevice() else torch.cuda.device(device)
+    return dv.device(), _HERE
+
+
+def _stream(device):
+    """Handle of the current stream.  torch.cuda.current_stream() builds an object around it, 2 us of a call of 25."""
+    return torch._C._cuda_getCurrentRawStream(device.index)
 
 
 def _on(x, dtype, device):
@@ -153,35 +161,39 @@ class _Call:
     """One soft_match call: its arguments checked (nothing touches the device), then as device tensors."""
 
     def __init__(self, query, ref, value, heads, scale, cap, falloff, query_xy, mask, num_query):
-        n, cells = _elements(query, "query"), _elements(ref, "ref")
-        b, c = _dims(query)[:2]
+        (q_dims, n), (r_dims, cells) = _map(query, "query"), _map(ref, "ref")
+        b, c = q_dims[:2]
         dtype = _dtype(query, "query")
         heads = int(heads)
-        if _dims(ref)[:2] != (b, c):
-            raise ValueError(f"query {_dims(query)} and ref {_dims(ref)} must share batch and channels")
-        if value is not None and (_elements(value, "value") != cells or _dims(value)[0] != b):
-            raise ValueError(f"value {_dims(value)} must have the batch and cells of ref {_dims(ref)}")
-        for x, name in ((ref, "ref"), (value, "value")):
-            if x is not None and _dtype(x, name) != dtype:
-                raise ValueError(f"{name} must have query's dtype {dtype}")
-        cv = c if value is None else _dims(value)[1]
+        if r_dims[:2] != (b, c):
+            raise ValueError(f"query {q_dims} and ref {r_dims} must share batch and channels")
+        if _dtype(ref, "ref") != dtype:
+            raise ValueError(f"ref must have query's dtype {dtype}")
+        cv = c
+        if value is not None:
+            v_dims, v_cells = _map(value, "value")
+            if v_cells != cells or v_dims[0] != b:
+                raise ValueError(f"value {v_dims} must have the batch and cells of ref {r_dims}")
+            if _dtype(value, "value") != dtype:
+                raise ValueError(f"value must have query's dtype {dtype}")
+            cv = v_dims[1]
         if heads < 1 or c < 1 or cv < 1 or c % heads or cv % heads:
             raise ValueError(f"{c} and {cv} channels do not split into {heads} heads")
         if c // heads > MAX_CHANNELS or cv // heads > MAX_CHANNELS:
             raise ValueError(f"at most {MAX_CHANNELS} channels per head")
         if cells < 1:
             raise ValueError("ref has no cells")
-        _check_mask(mask, b, _dims(ref)[2:])
-        grid = _dims(ref)[2:] if len(_dims(ref)) == 4 else None
+        _check_mask(mask, b, r_dims[2:])
+        grid = r_dims[2:] if len(r_dims) == 4 else None
         if scale is None:
             scale = (c // heads) ** -0.5
-        self.scale, self.cap = _scores(heads, scale, cap, falloff, query_xy, grid, _dims(query)[2:], b, n)
+        self.scale, self.cap = _scores(heads, scale, cap, falloff, query_xy, grid, q_dims[2:], b, n)
         num_query = _counts(num_query, b)
         self.raw = (query, ref, value, falloff, query_xy, mask, num_query)
         self.code = _CODES[dtype]
         self.dtype, self.b, self.heads, self.d, self.dv, self.n, self.cells = dtype, b, heads, c // heads, cv // heads, n, cells
         self.width = grid[1] if grid else cells
-        self.out_shape = (b, cv) + _dims(query)[2:]
+        self.out_shape = (b, cv) + q_dims[2:]
 
     def upload(self, device):
         query, ref, value, falloff, query_xy, mask, num_query = self.raw
@@ -217,7 +229,7 @@ class _Call:
         ws = _bytes(need, self.device)
         _abi.check(_abi.lib.ispa_soft_match(dv.ptr(self.q), dv.ptr(self.r), dv.ptr(self.v), *self._common(), dv.ptr(out),
                                             None if out32 is out else dv.ptr(out32), dv.ptr(lse), dv.ptr(ws), need,
-                                            dv.stream_ptr()))
+                                            _stream(self.device)))
         return out, out32, lse
 
     def backward(self, out32, lse, d_out, d_lse):
@@ -230,7 +242,7 @@ class _Call:
         ws = _bytes(need, self.device)
         _abi.check(_abi.lib.ispa_soft_match_backward(dv.ptr(self.q), dv.ptr(self.r), dv.ptr(self.v), *self._common(),
                                                      dv.ptr(out32), dv.ptr(lse), dv.ptr(d_out), dv.ptr(d_lse), dv.ptr(dq),
-                                                     dv.ptr(dr), dv.ptr(dval), dv.ptr(ws), need, dv.stream_ptr()))
+                                                     dv.ptr(dr), dv.ptr(dval), dv.ptr(ws), need, _stream(self.device)))
         return dq, dr, dval
 
 
@@ -383,7 +395,7 @@ class TemplateStore:
             v, f, m = self._index(views), _on(features, dtype, device), _mask(mask, device)
             _abi.check(_abi.lib.ispa_store_write(dv.ptr(f), _CODES[dtype], dv.ptr(m), dv.ptr(v), n, _KINDS[self.kind][0],
                                                  self.n_view, self.channels, self.codes.shape[2], dv.ptr(self.codes),
-                                                 dv.ptr(self.scales), dv.ptr(self.mask), dv.stream_ptr()))
+                                                 dv.ptr(self.scales), dv.ptr(self.mask), _stream(device)))
 
     def _read(self, views, dtype, features):
         views = self._views(views, 1)
@@ -395,7 +407,7 @@ class TemplateStore:
             mask = None if features else torch.empty((n,) + self.size, dtype=torch.uint8, device=device)
             _abi.check(_abi.lib.ispa_store_read(dv.ptr(self.codes), dv.ptr(self.scales), dv.ptr(self.mask), dv.ptr(v), n,
                                                 _KINDS[self.kind][0], self.n_view, self.channels, self.codes.shape[2],
-                                                _CODES[dtype], dv.ptr(out), dv.ptr(mask), dv.stream_ptr()))
+                                                _CODES[dtype], dv.ptr(out), dv.ptr(mask), _stream(device)))
             return out if features else mask
 
     def read(self, views, dtype=torch.float32):
@@ -414,8 +426,8 @@ class TemplateStore:
         """soft_match of query (B,C,Hq,Wq) or (B,C,n) against the stored views (B,V) of each item: one softmax over the
         cells of all V views, whose features are reference and value, read from their codes.  -1 stands for no
         view, the store's masks apply, and the other arguments are soft_match's.  No gradients flow."""
-        n = _elements(query, "query")
-        b, c = _dims(query)[:2]
+        dims, n = _map(query, "query")
+        b, c = dims[:2]
         dtype = _dtype(query, "query")
         heads = int(heads)
         if c != self.channels:
@@ -427,7 +439,7 @@ class TemplateStore:
             raise ValueError(f"views must be ({b},V), got {_dims(views)}")
         if scale is None:
             scale = (c // heads) ** -0.5
-        scale, cap = _scores(heads, scale, cap, falloff, query_xy, self.size, _dims(query)[2:], b, n)
+        scale, cap = _scores(heads, scale, cap, falloff, query_xy, self.size, dims[2:], b, n)
         count = _counts(num_query, b)
         as_tensor = dv.is_tensor(query)
         device, place = _place(self.codes)
@@ -435,7 +447,7 @@ class TemplateStore:
             q, v = _on(query.detach() if as_tensor else query, dtype, device), self._index(views)
             f, xy = _score_tensors(heads, falloff, query_xy, device)
             count = _count_tensor(count, device)
-            out = torch.empty((b, c) + _dims(query)[2:], dtype=dtype, device=device)
+            out = torch.empty((b, c) + dims[2:], dtype=dtype, device=device)
             lse = torch.empty((b, heads, n), dtype=torch.float32, device=device) if return_lse else None
             d, cells, code = c // heads, self.codes.shape[2], _CODES[dtype]
             need = _forward_bytes(code, b, heads, d, d, n, v.shape[1], cells)
@@ -443,6 +455,6 @@ class TemplateStore:
             _abi.check(_abi.lib.ispa_store_match(
                 dv.ptr(q), code, dv.ptr(self.codes), dv.ptr(self.scales), dv.ptr(self.mask), _KINDS[self.kind][0], dv.ptr(v),
                 v.shape[1], self.n_view, b, heads, d, n, cells, self.size[1], scale, cap, dv.ptr(f), dv.ptr(xy), dv.ptr(count),
-                dv.ptr(out), dv.ptr(lse), dv.ptr(ws), need, dv.stream_ptr()))
+                dv.ptr(out), dv.ptr(lse), dv.ptr(ws), need, _stream(device)))
             out = dv.back(out, as_tensor)
             return (out, dv.back(lse, as_tensor)) if return_lse else out
