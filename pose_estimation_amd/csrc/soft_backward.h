@@ -8,7 +8,7 @@
 //
 // What bounds it (MI355X): 16 pairs of 64x64x128, bfloat16, reference and value one map: forward 0.16, query gradient 0.19,
 // value's part 0.15, reference's 0.21 ms; matrix pipe 38 to 50 % busy, vector ALU 47 to 55 %, together 93 to 98 %.
-// float32, 8 pairs of 28x28x128: 0.22 ms for all, two to four tiles a workgroup, half of it the start and end of workgroups.
+// float32, 8 pairs of 28x28x128: 0.21 ms for all, two to four tiles a workgroup, half of it the start and end of workgroups.
 #pragma once
 #include "soft_forward.h"
 

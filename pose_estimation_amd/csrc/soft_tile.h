@@ -77,6 +77,29 @@ __device__ __forceinline__ void next_row(E *&row) {
     asm("" : "+s"(row));
 }
 
+// A lane's 8 channels of a 16-channel step, zeros past the last; `row` moves on by 16 rows.  whole: all 16 are there.
+template <typename E>
+__device__ __forceinline__ void eight_rows(const E *&row, unsigned lane, int64_t ld, bool whole, int channel, int d, E (&e)[8]) {
+    const E *at = row;
+    if (whole) {
+#pragma unroll
+        for (int j = 0; j < 8; ++j) {
+            e[j] = *at_column(at, lane);
+            at += ld;
+            next_row(at);
+        }
+    } else {
+#pragma unroll
+        for (int j = 0; j < 8; ++j) {
+            e[j] = channel + j < d ? *at_column(at, lane) : (E)0;
+            at += ld;
+            next_row(at);
+        }
+    }
+    row += 16 * ld;
+    next_row(row);
+}
+
 // Keeps the code of a rare case behind its branch: turned into selects it would cost every tile three operations a cell.
 __device__ __forceinline__ void stay_branch() { asm volatile(""); }
 
@@ -159,6 +182,7 @@ struct Math<BF16, DP> {
             constexpr int s = decltype(step)::value;
             unsigned short e[8];
             const bool whole = 16 * s + 16 <= d;               // uniform
+            // not eight_rows(), which sets the main loop of the forward kernel of 128 channels differently (64 pairs: 631 us for 595)
 #pragma unroll
             for (int j = 0; j < 8; ++j) {
                 if (whole) e[j] = *at_column(map, lane);
@@ -400,14 +424,7 @@ struct SplitMath {
             constexpr int s = decltype(step)::value;
             float e[8];
             const bool whole = 16 * s + 16 <= d;
-#pragma unroll
-            for (int j = 0; j < 8; ++j) {
-                if (whole) e[j] = *at_column(map, lane);
-                else e[j] = 16 * s + 8 * h + j < d ? *at_column(map, lane) : 0.f;
-                map += ld;
-                next_row(map);
-            }
-            map += 8 * ld;
+            eight_rows(map, lane, ld, whole, 16 * s + 8 * h, d, e);
             u32x4 w[3];
 #pragma unroll
             for (int j = 0; j < 4; ++j) {
@@ -555,14 +572,7 @@ struct Math<F32Q, DP> : Math<BF16, DP> {
             constexpr int s = decltype(step)::value;
             float e[8];
             const bool whole = 16 * s + 16 <= d;
-#pragma unroll
-            for (int j = 0; j < 8; ++j) {
-                if (whole) e[j] = *at_column(map, lane);
-                else e[j] = 16 * s + 8 * h + j < d ? *at_column(map, lane) : 0.f;
-                map += ld;
-                next_row(map);
-            }
-            map += 8 * ld;
+            eight_rows(map, lane, ld, whole, 16 * s + 8 * h, d, e);
             u32x4 w;
 #pragma unroll
             for (int j = 0; j < 4; ++j) w[j] = ok ? plane(e[2 * j], e[2 * j + 1]) : 0u;
@@ -606,12 +616,20 @@ __device__ __forceinline__ void store_columns(E *map, int64_t n, int q, int h, i
     E *row = scalar(map + c0 * n);
     each<NC / 32>([&](auto block) {
         constexpr int c = decltype(block)::value;
-        const bool whole = c0 + 32 * c + 32 <= d;              // uniform
+        if (c0 + 32 * c + 32 <= d) {                           // uniform
 #pragma unroll
-        for (int i = 0; i < 16; ++i) {
-            if (whole || c0 + 32 * c + out_channel(i, h) < d) store_float(at_column(row, lane), o[c][i]);
-            row += i % 4 < 3 ? n : 5 * n;
-            next_row(row);
+            for (int i = 0; i < 16; ++i) {
+                store_float(at_column(row, lane), o[c][i]);
+                row += i % 4 < 3 ? n : 5 * n;
+                next_row(row);
+            }
+        } else {
+#pragma unroll
+            for (int i = 0; i < 16; ++i) {
+                if (c0 + 32 * c + out_channel(i, h) < d) store_float(at_column(row, lane), o[c][i]);
+                row += i % 4 < 3 ? n : 5 * n;
+                next_row(row);
+            }
         }
         __builtin_amdgcn_sched_barrier(0);
     });
