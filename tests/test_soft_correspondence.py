@@ -376,6 +376,32 @@ def test_changed_mask_is_noticed(sc):
         out.sum().backward()
 
 
+@gpu
+def test_maps_beyond_32_bit_offsets(sc):
+    """The last of 9 items lies more than 2^31 numbers into the maps.  Its queries are cells of the map, so that one weight is
+    nearly 1 and its dP - Delta cancels: the errors go by the magnitudes before that, as everywhere here."""
+    b, c, h, scale = 9, 256, 1024, 25.0
+    g = torch.Generator(device="cuda").manual_seed(210)
+    r = torch.empty((b, c, h, h), dtype=BF16, device="cuda")
+    for i in range(b):
+        x = torch.randn((c, h, h), generator=g, device="cuda")
+        r[i] = x / x.square().sum(0).sqrt()
+    at = torch.randint(h * h, (5,), generator=g, device="cuda")
+    q = r.flatten(2)[:, :, at].contiguous()
+    d_out = torch.randn(q.shape, generator=g, device="cuda").to(BF16)
+    out, (dq, dr) = gradients(sc, q, r, None, d_out, None, scale=scale)
+    out, dq, dr = (x[-1].detach().flatten(1).double() for x in (out, dq, dr))
+    q, r, d = (x[-1].flatten(1).double() for x in (q, r, d_out))
+    p = torch.softmax(scale * q.T @ r, 1)
+    dp = d.T @ r
+    dx = scale * p * (dp - (p * dp).sum(1, keepdim=True))
+    size = scale * p * (dp.abs() + (p * dp.abs()).sum(1, keepdim=True))
+    for got, want, mag, roundings in ((out, r @ p.T, r.abs() @ p.T, 1), (dq, r @ dx.T, r.abs() @ size.T, 3),
+                                      (dr, q @ dx + d @ p, q.abs() @ size + d.abs() @ p, 3)):
+        err = (got - want).abs() - HALF[BF16] * (roundings * mag + want.abs()) - 1e-30
+        assert torch.isfinite(got).all() and float(err.max()) <= 0
+
+
 # ------------------------------------------------------------------------------------------------ streams and graphs
 @gpu
 @pytest.mark.parametrize("dtype", [F32, BF16])
