@@ -11,7 +11,7 @@ bool sizes_ok(int dtype, int B, int heads, int D, int Dv, int64_t nq, int V, int
     return (dtype == ISPA_F32 || dtype == ISPA_BF16) && B >= 0 && heads >= 1 && D >= 1 && D <= ISPA_SOFT_MAX_CHANNELS && Dv >= 1 &&
            Dv <= ISPA_SOFT_MAX_CHANNELS && nq >= 0 && nq < (1ll << 22) && V >= 0 && cells >= 1 && cells < (1ll << 22) &&
            (int64_t)B * heads < 65536 && V * ((cells + 31) / 32) < (1ll << 30) &&
-           (int64_t)B * heads * ((nq > cells ? nq : cells) / 32 + 1) < (1ll << 31) / kMaxSplitCount * 4;
+           (int64_t)B * heads * ((nq > cells ? nq : cells) / 32 + 1) < (1ll << 24);       // threads of a launch: 2^32
 }
 
 int check_sizes(int dtype, int B, int heads, int D, int Dv, int64_t nq, int V, int64_t cells) {
