@@ -87,7 +87,9 @@ int backward_sized(Params p, const Plan &dq, const Plan &dkv, hipStream_t stream
     p.blocks = dq.blocks;
     const int64_t rows = tile_rows(arithmetic(f32, false, DP, dq.waves));
     p.tiles = p.tiles_per_view = (int)((p.cells + rows - 1) / rows);
-    if (int rc = with_arithmetic<T, DP>(dq.waves, [&](auto t) { return dq_waves<decltype(t), DP>(p, dq.waves, stream); })) return rc;
+    // without queries there is no workgroup to launch; the gradients of the maps are still to be written (zeros)
+    if (p.nq > 0)
+        if (int rc = with_arithmetic<T, DP>(dq.waves, [&](auto t) { return dq_waves<decltype(t), DP>(p, dq.waves, stream); })) return rc;
     const int64_t bh = (int64_t)p.B * p.heads;
     if (p.parts)
         if (int rc = sum_parts<T>(p.part_a, nullptr, p.splits, bh * p.D * p.nq, p.scale, p.dq, stream)) return rc;

@@ -356,6 +356,22 @@ def test_only_the_wanted_gradients(sc, dtype):
 
 @gpu
 @pytest.mark.parametrize("dtype", [F32, BF16])
+@pytest.mark.parametrize("c, cv", [(32, 0), (32, 16), (128, 0), (256, 256)])
+def test_gradients_without_queries(sc, dtype, c, cv):
+    """An item set without a single query: its template gets zeros."""
+    for grid in ((3, 5), (20, 24)):
+        q, r, v = cuda(*inputs(dtype, 2, c, grid, 0, cv, seed=75))
+        q = q.flatten(2)[:, :, :0]
+        leaves = [x.detach().requires_grad_() for x in (q, r, v) if x is not None]
+        out, lse = sc.soft_match(*leaves, scale=5.0, return_lse=True)
+        got = torch.autograd.grad([out, lse], leaves, [torch.ones_like(out), torch.ones_like(lse)])
+        assert out.shape == (2, cv or c, 0) and lse.shape == (2, 1, 0) and got[0].shape == q.shape
+        for g, x in zip(got[1:], leaves[1:]):
+            assert g.shape == x.shape and g.dtype == dtype and (g == 0).all()
+
+
+@gpu
+@pytest.mark.parametrize("dtype", [F32, BF16])
 def test_runs_agree_bit_for_bit(sc, dtype):
     q, r, v = cuda(*inputs(dtype, 2, 128, (28, 28), 50, 0, seed=80))
     d_out = rand(81, (2, 128, 50), dtype, unit=False).cuda()
