@@ -12,11 +12,12 @@ constexpr int kFormed = DP == 256 && std::is_same_v<T, F32> ? 128 : DP;
 template <typename T, int DP, int WQ, int MODE>
 int dq_one(Params p, hipStream_t stream) {
     static unsigned long long lds_allowed = 0;
+    constexpr int kMost = most_lds_bytes<Math<T, DP>, DP>(2);
     const int lds = lds_bytes<Math<T, DP>, DP>(p.shared, 2);
     const unsigned grid = (unsigned)((int64_t)p.B * p.heads * p.splits * p.blocks);
     constexpr int NC = kFormed<T, DP>;
     for (p.c0 = 0; p.c0 < p.D; p.c0 += NC)
-        if (int rc = launch(soft_dq_kernel<T, DP, WQ, NC, MODE>, p, grid, 64 * WQ, lds, &lds_allowed, "soft_dq_kernel", stream))
+        if (int rc = launch(soft_dq_kernel<T, DP, WQ, NC, MODE>, p, grid, 64 * WQ, lds, kMost, &lds_allowed, "soft_dq_kernel", stream))
             return rc;
     return ISPA_OK;
 }
@@ -24,11 +25,11 @@ int dq_one(Params p, hipStream_t stream) {
 template <typename T, int DP, int WQ, int PART, int MODE>
 int dkv_one(Params p, int channels, hipStream_t stream) {
     static unsigned long long lds_allowed = 0;
-    const int lds = lds_bytes<Math<T, DP>, DP>(false, 2);
+    constexpr int kLds = lds_bytes<Math<T, DP>, DP>(false, 2);
     const unsigned grid = (unsigned)((int64_t)p.B * p.heads * p.splits * p.blocks);
     constexpr int NC = PART == 2 ? kFormed<T, DP> : DP;
     for (p.c0 = 0; p.c0 < channels; p.c0 += NC)
-        if (int rc = launch(soft_dkv_kernel<T, DP, WQ, PART, NC, MODE>, p, grid, 64 * WQ, lds, &lds_allowed, "soft_dkv_kernel",
+        if (int rc = launch(soft_dkv_kernel<T, DP, WQ, PART, NC, MODE>, p, grid, 64 * WQ, kLds, kLds, &lds_allowed, "soft_dkv_kernel",
                             stream))
             return rc;
     return ISPA_OK;

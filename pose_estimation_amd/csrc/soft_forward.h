@@ -91,6 +91,12 @@ constexpr int lds_bytes(bool shared, int phased_k, bool one = false) {
     const bool phased = kMayPhase<M> && !shared;
     return (phased ? phased_k : one ? 1 : 2) * (kTileBytes<M, DP> + kCellBytes) + (shared ? 0 : phased ? 1 : 2) * kTileBytes<M, DP>;
 }
+// The larger of both: a value map of its own may take less, as it is copied in phases.
+template <typename M, int DP>
+constexpr int most_lds_bytes(int phased_k) {
+    const int shared = lds_bytes<M, DP>(true, phased_k), own = lds_bytes<M, DP>(false, phased_k);
+    return shared > own ? shared : own;
+}
 
 // The tiles of one item and head: begin_* starts a tile's way into a buffer, end_* ends it.  Codes are reference and value.
 // PK: buffers of the reference's tiles where phased.

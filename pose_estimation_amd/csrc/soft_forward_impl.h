@@ -9,11 +9,14 @@ static_assert(kMaxSplits == kMaxSplitCount, "the join reads every part");
 template <typename T, typename SRC, int DP, int WQ, int MODE>
 int forward_one(Params p, hipStream_t stream) {
     static unsigned long long lds_allowed = 0;
-    const int lds = lds_bytes<Math<T, DP>, DP>(p.shared, 1, kOneBuffer<SRC, WQ>);
+    // codes are reference and value in one
+    constexpr bool kOne = kOneBuffer<SRC, WQ>;
+    constexpr int kMost = KeyTiles<Math<T, DP>, SRC>::kCodes ? lds_bytes<Math<T, DP>, DP>(true, 1, kOne) : most_lds_bytes<Math<T, DP>, DP>(1);
+    const int lds = lds_bytes<Math<T, DP>, DP>(p.shared, 1, kOne);
     const unsigned grid = (unsigned)((int64_t)p.B * p.heads * p.splits * p.blocks);
     constexpr int NC = DP == 256 && !std::is_same_v<T, BF16> && !std::is_same_v<T, F32Q> ? 128 : DP;
     for (p.c0 = 0; p.c0 < p.Dv; p.c0 += NC)
-        if (int rc = launch(soft_forward_kernel<T, SRC, DP, WQ, NC, MODE>, p, grid, 64 * WQ, lds, &lds_allowed, "soft_forward_kernel",
+        if (int rc = launch(soft_forward_kernel<T, SRC, DP, WQ, NC, MODE>, p, grid, 64 * WQ, lds, kMost, &lds_allowed, "soft_forward_kernel",
                             stream))
             return rc;
     if (p.splits == 1) return ISPA_OK;

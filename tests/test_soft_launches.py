@@ -69,3 +69,20 @@ for dtype in (_abi.F32, _abi.BF16):
                 n += backward(dtype, 2, 1, d, d, 0, cells, own)
 print(n)
 """)
+
+
+@pytest.mark.parametrize("own_first", [False, True])
+def test_lds_of_every_kernel_form(recorder, own_first):
+    """The same kernel serves calls with and without a value map, which take different amounts of LDS, in either order."""
+    run(recorder, f"""
+n = 0
+for own in {(True, False) if own_first else (False, True)}:
+    for dtype in (_abi.F32, _abi.BF16):
+        for d in (16, 64, 128, 256):
+            for nq in (1, 9, 64, 65, 500):
+                for cap, falloff in ((0.0, None), (5.0, None), (0.0, at), (50.0, at)):
+                    n += forward(dtype, 2, 1, d, d, nq, 4096, own, cap, falloff)
+                    n += backward(dtype, 2, 1, d, d, nq, 4096, own, cap, falloff)
+                    n += forward(dtype, 1, 2, d, d, nq, 60, own, cap, falloff) + backward(dtype, 1, 2, d, d, nq, 60, own, cap, falloff)
+print(n)
+""")
