@@ -54,16 +54,14 @@ __device__ __forceinline__ void probabilities(const Score<T> &score, const f32x1
     } else if constexpr (Score<T>::kExact) {
 #pragma unroll
         for (int i = 0; i < 16; ++i) {
-            const float th = score.bend(acc[i]);
-            slope[i] = fmaf(-th, th, 1.f);
+            const float th = score.bend(acc[i], slope[i]);
             w[i] = exp2_(fmaf(score.top, th, w[i]));
         }
     } else {
-        // tanh = 1 - 2 r: 1 - tanh^2 = 4 (r - r^2); the cap itself is in w
+        // tanh = 1 - 2 r; the cap itself is in w
 #pragma unroll
         for (int i = 0; i < 16; ++i) {
-            const float r = score.r(acc[i]);
-            slope[i] = 4.f * fmaf(-r, r, r);
+            const float r = score.r_slope(acc[i], slope[i]);
             w[i] = exp2_(fmaf(-2.f * score.top, r, w[i]));
         }
     }
@@ -77,14 +75,16 @@ __device__ __forceinline__ void weights(const Score<T> &score, const f32x16 &acc
     } else if constexpr (Score<T>::kExact) {
 #pragma unroll
         for (int i = 0; i < 16; ++i) {
-            const float th = score.bend(acc[i]);
-            w[i] = exp2_(fmaf(score.top, th, w[i])) * ((dp[i] - delta) * fmaf(-th, th, 1.f));
+            float slope;
+            const float th = score.bend(acc[i], slope);
+            w[i] = exp2_(fmaf(score.top, th, w[i])) * ((dp[i] - delta) * slope);
         }
     } else {
 #pragma unroll
         for (int i = 0; i < 16; ++i) {
-            const float r = score.r(acc[i]);
-            w[i] = exp2_(fmaf(-2.f * score.top, r, w[i])) * ((dp[i] - delta) * (4.f * fmaf(-r, r, r)));
+            float slope;
+            const float r = score.r_slope(acc[i], slope);
+            w[i] = exp2_(fmaf(-2.f * score.top, r, w[i])) * ((dp[i] - delta) * slope);
         }
     }
 }

@@ -855,6 +855,22 @@ def test_captured_store(sc):
         assert all(torch.equal(a, b) for a, b in zip(got, want))
 
 
+@gpu
+@pytest.mark.parametrize("dtype", [F32, BF16])
+@pytest.mark.parametrize("n, c", [(0, 32), (9, 32), (0, 256)])
+@pytest.mark.parametrize("ratio", [4.0, -4.0, 6.0, -6.0, 8.0, -8.0])
+def test_gradients_of_saturated_caps(sc, dtype, n, c, ratio):
+    """All cells alike, so that every score lies far in the cap, where 1 - tanh^2 is 1e-3 to 4e-7: its relative error counts.
+    It goes by twice that of scale x / cap, a sum of up to 256 terms times 8: 2 x 8 x 8 half steps of 2^-24, 8e-6."""
+    grid, cap = (12, 16), 7.0
+    q, r, v = inputs(dtype, 2, c, grid, n, 24, seed=220)
+    q, r = ((0.1 * x.float() + rand(223, (1, c) + (1,) * (x.dim() - 2), F32)).to(dtype) for x in (q, r))
+    d_out = rand(224, (2, 24) + tuple(q.shape[2:]), dtype, unit=False)
+    _, got = gradients(sc, *cuda(q, r, v, d_out), None, scale=ratio * cap, cap=cap)
+    want = oracle(flat(q), flat(r), flat(v), 1, ratio * cap, cap, d_out=flat(d_out))
+    check_gradients(got, want, dtype, False)
+
+
 # ------------------------------------------------------------------------------------------------ refusals (no GPU)
 def test_refusals(sc):
     q, r = torch.zeros((2, 8, 4, 4)), torch.zeros((2, 8, 5, 6))
