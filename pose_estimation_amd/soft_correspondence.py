@@ -157,6 +157,12 @@ def _mask(mask, device):
     return _on(mask, torch.uint8, device)
 
 
+def _fixed(x, name):
+    """Refuses a scale or cap whose derivative somebody waits for."""
+    if dv.is_tensor(x) and x.requires_grad and torch.is_grad_enabled():
+        raise ValueError(f"no gradient flows to {name}, a number (a learned temperature: multiply query by it; else detach it)")
+
+
 class _Call:
     """One soft_match call: its arguments checked (nothing touches the device), then as device tensors."""
 
@@ -185,6 +191,8 @@ class _Call:
             raise ValueError("ref has no cells")
         _check_mask(mask, b, r_dims[2:])
         grid = r_dims[2:] if len(r_dims) == 4 else None
+        _fixed(scale, "scale")
+        _fixed(cap, "cap")
         if scale is None:
             scale = (c // heads) ** -0.5
         self.scale, self.cap = _scores(heads, scale, cap, falloff, query_xy, grid, q_dims[2:], b, n)
@@ -291,7 +299,8 @@ def soft_match(query, ref, value=None, *, heads=1, scale=None, cap=0.0, falloff=
     the sum of exp(z): the match's confidence.  A query that is not real, or whose cells are all masked, gets 0 and -inf.
 
     Tensors that require gradients get them (out and lse, once; value None: ref's is the sum of both uses); no gradient
-    flows to falloff, query_xy or the masks.  Scores, sums and log-sums are float32; bfloat16 maps round the weights to
+    flows to falloff, query_xy or the masks, and a scale or cap that requires one is refused: they are numbers (a learned
+    temperature multiplies query).  Scores, sums and log-sums are float32; bfloat16 maps round the weights to
     bfloat16 for the product with the values.  Memory grows with the maps, not with their product, and results do
     not change from run to run."""
     as_tensor = dv.is_tensor(query)

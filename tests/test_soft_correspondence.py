@@ -914,6 +914,20 @@ def test_refusals(sc):
             sc.soft_match(call.pop("query"), call.pop("ref"), call.pop("value", None), **call)
 
 
+def test_learned_scale_and_cap_are_refused(sc):
+    q, r = torch.zeros((2, 8, 4, 4)), torch.zeros((2, 8, 5, 6))
+    learned = torch.tensor(3.0, requires_grad=True)
+    for x in (q, q.clone().requires_grad_()):
+        for name in ("scale", "cap"):
+            with pytest.raises(ValueError, match=f"no gradient flows to {name}"):
+                sc.soft_match(x, r, **{name: learned})
+    # where none is asked for they pass for the numbers they hold: on to the next check
+    with torch.no_grad(), pytest.raises(ValueError, match="do not lie on the reference grid"):
+        sc.soft_match(q, r, scale=learned, cap=learned, falloff=0.1)
+    with pytest.raises(ValueError, match="scale must be finite"):
+        sc.soft_match(q, r, scale=(learned / 0).detach())
+
+
 def test_store_refusals(sc):
     with pytest.raises(ValueError, match="kind"):
         sc.TemplateStore(1, 8, (4, 4), "int4")
