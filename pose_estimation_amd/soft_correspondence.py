@@ -14,6 +14,7 @@ import math
 
 import numpy as np
 import torch
+from torch.autograd import forward_ad
 
 from . import _abi, _device as dv
 
@@ -163,6 +164,12 @@ def _fixed(x, name):
         raise ValueError(f"no gradient flows to {name}, a number (a learned temperature: multiply query by it; else detach it)")
 
 
+def _no_tangents(*tensors):
+    """Refuses forward-mode derivatives: a dual tensor requires no gradient, and its tangent would be lost."""
+    if forward_ad._current_level >= 0 and any(dv.is_tensor(x) and forward_ad.unpack_dual(x).tangent is not None for x in tensors):
+        raise ValueError("soft_match has gradients (reverse mode) alone: no forward-mode tangents")
+
+
 class _Call:
     """One soft_match call: its arguments checked (nothing touches the device), then as device tensors."""
 
@@ -191,6 +198,7 @@ class _Call:
             raise ValueError("ref has no cells")
         _check_mask(mask, b, r_dims[2:])
         grid = r_dims[2:] if len(r_dims) == 4 else None
+        _no_tangents(query, ref, value, scale, cap)
         _fixed(scale, "scale")
         _fixed(cap, "cap")
         if scale is None:
@@ -298,7 +306,7 @@ def soft_match(query, ref, value=None, *, heads=1, scale=None, cap=0.0, falloff=
     Returns out (B,Cv,...) over query's cells in query's dtype, with return_lse also lse (B,heads,n) float32, the log of
     the sum of exp(z): the match's confidence.  A query that is not real, or whose cells are all masked, gets 0 and -inf.
 
-    Tensors that require gradients get them (out and lse, once; value None: ref's is the sum of both uses); no gradient
+    Tensors that require gradients get them (out and lse, once, in reverse mode; value None: ref's is the sum of both uses); no gradient
     flows to falloff, query_xy or the masks, and a scale or cap that requires one is refused: they are numbers (a learned
     temperature multiplies query).  Scores, sums and log-sums are float32; bfloat16 maps round the weights to
     bfloat16 for the product with the values.  Memory grows with the maps, not with their product, and results do

@@ -928,6 +928,24 @@ def test_learned_scale_and_cap_are_refused(sc):
         sc.soft_match(q, r, scale=(learned / 0).detach())
 
 
+def test_forward_mode_is_refused(sc):
+    from torch.autograd import forward_ad
+    q, r, v = torch.zeros((2, 8, 4, 4)), torch.zeros((2, 8, 5, 6)), torch.zeros((2, 4, 5, 6))
+    with forward_ad.dual_level():
+        dual = [forward_ad.make_dual(x, torch.ones_like(x)) for x in (q, r, v)]
+        for i in range(3):
+            with pytest.raises(ValueError, match="forward-mode"):
+                sc.soft_match(*(dual[j] if j == i else x for j, x in enumerate((q, r, v))))
+        with pytest.raises(ValueError, match="forward-mode"):
+            sc.soft_match(q, r, scale=forward_ad.make_dual(torch.tensor(2.0), torch.tensor(1.0)))
+        with pytest.raises(ValueError, match="heads"):   # a level alone changes nothing
+            sc.soft_match(q, r, v, heads=3)
+        with pytest.raises(ValueError, match="do not lie on the reference grid"):
+            sc.soft_match(q, r, v, falloff=0.1)
+    with pytest.raises(ValueError, match="forward-mode"):
+        torch.func.jvp(lambda x: sc.soft_match(x, r), (q,), (q,))
+
+
 def test_store_refusals(sc):
     with pytest.raises(ValueError, match="kind"):
         sc.TemplateStore(1, 8, (4, 4), "int4")
