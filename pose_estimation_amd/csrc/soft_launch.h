@@ -83,11 +83,11 @@ int with_mode(const Params &p, bool grid, F f) {
     return f(std::integral_constant<int, kGeneral>{});
 }
 
-// most: what the kernel's calls take at most.  The permission is asked for once per kernel and device, whichever call comes first.
+// most: what the kernel's calls take at most, which the first one that needs a permission asks for.
 template <typename K>
 int launch(K kernel, const Params &p, unsigned grid, int threads, int lds, int most, unsigned long long *lds_allowed, const char *what,
            hipStream_t stream) {
-    if (most > 65536)
+    if (lds > 65536)
         if (int rc = ispa::allow_dynamic_lds((const void *)kernel, most, lds_allowed)) return rc;
     kernel<<<grid, threads, lds, stream>>>(p);
     return ispa::check_launch(what);
