@@ -51,7 +51,7 @@ __device__ __forceinline__ void probabilities(const Score<T> &score, const f32x1
     if (MODE == kPlain || MODE == kRows || (MODE == kGeneral && !score.cap)) {
 #pragma unroll
         for (int i = 0; i < 16; ++i) w[i] = exp2_(fmaf(score.in, acc[i], w[i]));
-    } else if constexpr (Score<T>::kExact) {
+    } else if (Score<T>::kExact || (MODE == kGeneral && score.exact)) {
 #pragma unroll
         for (int i = 0; i < 16; ++i) {
             const float th = score.bend(acc[i], slope[i]);
@@ -72,7 +72,7 @@ __device__ __forceinline__ void weights(const Score<T> &score, const f32x16 &acc
     if (MODE == kPlain || MODE == kRows || (MODE == kGeneral && !score.cap)) {
 #pragma unroll
         for (int i = 0; i < 16; ++i) w[i] = exp2_(fmaf(score.in, acc[i], w[i])) * (dp[i] - delta);
-    } else if constexpr (Score<T>::kExact) {
+    } else if (Score<T>::kExact || (MODE == kGeneral && score.exact)) {
 #pragma unroll
         for (int i = 0; i < 16; ++i) {
             float slope;
@@ -93,7 +93,7 @@ template <typename T, int MODE>
 __device__ __forceinline__ float minus_lse(const Score<T> &score, float lse) {
     if (lse == -__builtin_inff()) return -__builtin_inff();    // no cells: weights 0
     const bool cap = MODE == kCapped || (MODE == kGeneral && score.cap);
-    return fmaf(-kLog2e, lse, !Score<T>::kExact && cap ? score.top : 0.f);
+    return fmaf(-kLog2e, lse, !Score<T>::kExact && cap && !(MODE == kGeneral && score.exact) ? score.top : 0.f);
 }
 
 // Both kernels can form their gradients for NC channels at a time, from p.c0 on.  A launch per half is what 256 float32

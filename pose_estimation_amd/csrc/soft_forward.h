@@ -310,13 +310,8 @@ __global__ __launch_bounds__(64 * WQ, (two_resident<T, SRC, DP, WQ>) ? 2 : 1) vo
                 } else if constexpr (MODE != kPlain) {
                     if constexpr (!std::is_same_v<T, BF16>) __builtin_amdgcn_sched_barrier(0);
                     float d[16];
-                    if (M::kColumns < 32 && score.cap) {       // tanh before there is a d: registers
-#pragma unroll
-                        for (int i = 0; i < 16; ++i) {
-                            z[k][i] = score.bend(z[k][i]);
-                            if (i % 8 == 7) __builtin_amdgcn_sched_barrier(0);
-                        }
-                    }
+                    constexpr bool kEarly = M::kColumns < 32 || (kCodes && !M::kWide);     // tanh before there is a d: registers
+                    if (kEarly && score.cap) score.template bend<true>(z[k]);
                     if (MODE == kRows || penalty.on) {
                         penalty(cell + 64, cell0, k, h, -off, d);
                     } else {
@@ -324,8 +319,9 @@ __global__ __launch_bounds__(64 * WQ, (two_resident<T, SRC, DP, WQ>) ? 2 : 1) vo
                         for (int i = 0; i < 16; ++i) d[i] = -off;
                     }
                     if (MODE == kGeneral && score.cap) {
+                        if constexpr (!kEarly) score.template bend<false>(z[k]);
 #pragma unroll
-                        for (int i = 0; i < 16; ++i) z[k][i] = fmaf(score.top, M::kColumns < 32 ? z[k][i] : score.bend(z[k][i]), d[i]);
+                        for (int i = 0; i < 16; ++i) z[k][i] = fmaf(score.top, z[k][i], d[i]);
                     } else {
 #pragma unroll
                         for (int i = 0; i < 16; ++i) z[k][i] = fmaf(score.in, z[k][i], d[i]);

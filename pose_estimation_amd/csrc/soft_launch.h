@@ -76,7 +76,7 @@ int with_mode(const Params &p, bool grid, F f) {
     if constexpr (DP <= 128) {
         if (!cap && !pen) return f(std::integral_constant<int, kPlain>{});
         if constexpr (std::is_same_v<T, BF16>)
-            if (cap && !pen && p.cap <= 32.f) return f(std::integral_constant<int, kCapped>{});
+            if (cap && !pen && p.cap <= kFixedCap) return f(std::integral_constant<int, kCapped>{});
         if (!cap && grid && p.W % Math<T, DP>::kCells == 0 && std::fabs(p.scale) > 1e-6f)
             return f(std::integral_constant<int, kRows>{});
     }

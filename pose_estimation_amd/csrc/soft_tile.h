@@ -908,22 +908,27 @@ __device__ __forceinline__ LateParams &late_params() {
 // What a kernel is built for: each sort of score has its own straight code, general ones branch at run time.
 enum Mode {
     kPlain = 0,       // no cap, no falloff
-    kCapped = 1,      // bfloat16, a cap of at most 32, no falloff
+    kCapped = 1,      // bfloat16, a cap of at most kFixedCap, no falloff
     kRows = 2,        // no cap, falloff on a grid whose rows the streamed groups of cells do not leave
     kGeneral = 3
 };
+constexpr float kFixedCap = 32.f;     // the cap stands for the maximum: weights are 2^(-2 cap log2 e) > 2^-93 at least
+constexpr float kPlainCap = 64.f;     // see Score
 
 // The scores of one item and head, in units of log2: z = bent - falloff d^2 with bent = in acc, or top tanh(in acc).
 template <typename T>
 struct Score {
-    // tanh(y) = 1 - 2 r, r = 1 / (exp(2 y) + 1), whose absolute error of 2e-7 is far below what the inputs of the bfloat16
-    // kernels leave.  float32 keeps the relative error near 1e-7 too: below 0.6 the odd polynomial y + y^3 c(y^2), c
-    // fitted to (tanh(y) / y - 1) / y^2 on [0, 0.36] by weighted least squares.
+    // tanh(y) = 1 - 2 r, r = 1 / (exp(2 y) + 1), has an absolute error of 2e-7, the cap's share of which is far below what the inputs of
+    // the bfloat16 kernels leave in a score as long as the cap is small: 1.3e-5 for kPlainCap.  float32, and bfloat16 above that
+    // (`exact`: 8 forward passes of 64x64x128 with a cap 143 us for 115, with gradients 640 for 490), keep the relative error near
+    // 1e-7 too: below 0.6 the odd polynomial y + y^3 c(y^2), c fitted to (tanh(y) / y - 1) / y^2 on [0, 0.36] by weighted least
+    // squares.
     static constexpr bool kExact = !std::is_same_v<T, BF16>;
     float in, top, fall, in2, per;
-    bool cap;
+    bool cap, exact;
     __device__ __forceinline__ Score(const Params &p, int head) {
         cap = p.cap > 0.f;
+        exact = kExact || p.cap > kPlainCap;
         in = cap ? p.scale / p.cap : p.scale * kLog2e;
         in2 = in * (2.f * kLog2e);
         top = p.cap * kLog2e;
@@ -944,9 +949,27 @@ struct Score {
         return x;
     }
     __device__ __forceinline__ float bend(float acc) const {
-        const float far = fmaf(-2.f, r(acc), 1.f);
-        if constexpr (!kExact) return far;
-        return near_zero(in * acc, far);
+        if constexpr (kExact) return bend_exact(acc);
+        return fmaf(-2.f, r(acc), 1.f);
+    }
+    __device__ __forceinline__ float bend_exact(float acc) const { return near_zero(in * acc, fmaf(-2.f, r(acc), 1.f)); }
+    // 16 products to tanh, by what the cap asks for.  TIGHT: a few at a time, where registers are short
+    template <bool TIGHT>
+    __device__ __forceinline__ void bend(f32x16 &acc) const {
+        if (!kExact && exact) {                                // uniform
+            stay_branch();
+#pragma unroll
+            for (int i = 0; i < 16; ++i) {
+                acc[i] = bend_exact(acc[i]);
+                if (TIGHT && i % 4 == 3) __builtin_amdgcn_sched_barrier(0);
+            }
+        } else {
+#pragma unroll
+            for (int i = 0; i < 16; ++i) {
+                acc[i] = bend(acc[i]);
+                if (TIGHT && i % 8 == 7) __builtin_amdgcn_sched_barrier(0);
+            }
+        }
     }
     // tanh(y), and its slope
     __device__ __forceinline__ float bend(float acc, float &slope) const {

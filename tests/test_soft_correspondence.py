@@ -871,6 +871,28 @@ def test_gradients_of_saturated_caps(sc, dtype, n, c, ratio):
     check_gradients(got, want, dtype, False)
 
 
+@gpu
+@pytest.mark.parametrize("dtype", [F32, BF16])
+@pytest.mark.parametrize("n, c", [(0, 48), (5, 48), (0, 256)])
+@pytest.mark.parametrize("cap", [33.0, 64.0, 1e3, 1e5, 1e7])
+@pytest.mark.parametrize("falloff", [None, 0.03])
+def test_caps_that_hardly_bend(sc, dtype, n, c, cap, falloff):
+    """A cap far above the scores leaves them as they are: its tanh counts with the cap's size."""
+    grid = (15, 16)
+    q, r, v = inputs(dtype, 2, c, grid, n, 40, seed=230)
+    nq = n or 240
+    xy = torch.rand((2, n, 2), generator=torch.Generator().manual_seed(231)) * 14 if n and falloff else None
+    d_out, d_lse = rand(232, (2, 40) + tuple(q.shape[2:]), dtype, unit=False), rand(233, (2, 1, nq), F32, unit=False)
+    opts = dict(scale=30.0, cap=cap, falloff=falloff, query_xy=xy)
+    _, lse = sc.soft_match(*cuda(q, r, v), return_lse=True, **opts)
+    out, got = gradients(sc, *cuda(q, r, v, d_out, d_lse), **opts)
+    want = oracle(flat(q), flat(r), flat(v), 1, 30.0, cap, None if falloff is None else [falloff], None if xy is None else host(xy), 16,
+                  d_out=flat(d_out), d_lse=host(d_lse))
+    near(out, want[0], want[2], dtype, 1)
+    near_lse(lse, want[1])
+    check_gradients(got, want, dtype, False)
+
+
 # ------------------------------------------------------------------------------------------------ refusals (no GPU)
 def test_refusals(sc):
     q, r = torch.zeros((2, 8, 4, 4)), torch.zeros((2, 8, 5, 6))
