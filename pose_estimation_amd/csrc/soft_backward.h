@@ -61,8 +61,8 @@ __device__ __forceinline__ void probabilities(const Score<T> &score, const f32x1
         // tanh = 1 - 2 r; the cap itself is in w
 #pragma unroll
         for (int i = 0; i < 16; ++i) {
-            const float r = score.r_slope(acc[i], slope[i]);
-            w[i] = exp2_(fmaf(-2.f * score.top, r, w[i]));
+            const float x = score.two_r(acc[i], slope[i]);
+            w[i] = exp2_(fmaf(-score.top, x, w[i]));
         }
     }
 }
@@ -83,8 +83,8 @@ __device__ __forceinline__ void weights(const Score<T> &score, const f32x16 &acc
 #pragma unroll
         for (int i = 0; i < 16; ++i) {
             float slope;
-            const float r = score.r_slope(acc[i], slope);
-            w[i] = exp2_(fmaf(-2.f * score.top, r, w[i])) * ((dp[i] - delta) * slope);
+            const float x = score.two_r(acc[i], slope);
+            w[i] = exp2_(fmaf(-score.top, x, w[i])) * ((dp[i] - delta) * slope);
         }
     }
 }

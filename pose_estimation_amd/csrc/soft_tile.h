@@ -940,12 +940,12 @@ struct Score {
     __device__ __forceinline__ float below_cap(float acc) const {
         return __builtin_amdgcn_rcpf(fmaf(__builtin_amdgcn_exp2f(acc * in2), per, per));
     }
-    // r and the slope 1 - tanh^2 = 4 e r^2 with e = exp(2 y): of two factors, so that nothing cancels far in the cap, where
+    // 2 r and the slope 1 - tanh^2 = e (2 r)^2 with e = exp(2 y): of factors, so that nothing cancels far in the cap, where
     // 1 - tanh^2 from a rounded tanh, and r - r^2 from an r near 1, lose all their bits.  e is kept finite (beside 2^126 the slope
     // is below 2^-124).
-    __device__ __forceinline__ float r_slope(float acc, float &slope) const {
-        const float e = __builtin_amdgcn_exp2f(fminf(acc * in2, 126.f)), x = __builtin_amdgcn_rcpf(e + 1.f);
-        slope = (4.f * x) * (e * x);
+    __device__ __forceinline__ float two_r(float acc, float &slope) const {
+        const float e = __builtin_amdgcn_exp2f(fminf(acc * in2, 126.f)), x = __builtin_amdgcn_rcpf(fmaf(e, 0.5f, 0.5f));
+        slope = x * (e * x);
         return x;
     }
     __device__ __forceinline__ float bend(float acc) const {
@@ -973,7 +973,7 @@ struct Score {
     }
     // tanh(y), and its slope
     __device__ __forceinline__ float bend(float acc, float &slope) const {
-        const float y = in * acc, th = near_zero(y, fmaf(-2.f, r_slope(acc, slope), 1.f));
+        const float y = in * acc, th = near_zero(y, 1.f - two_r(acc, slope));
         slope = fabsf(y) < 0.6f ? fmaf(-th, th, 1.f) : slope;
         return th;
     }
