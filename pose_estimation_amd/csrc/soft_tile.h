@@ -992,17 +992,19 @@ struct Score {
 // kRows: streamed cells lie on the grid in groups of kCells successive ones, whose rows' width is a multiple of that: a
 // group stays in one row.  bfloat16: d^2 grows along it by a quadratic, whose own part, -falloff j^2, is the same in every
 // group and lies in the accumulators' start (`from`), so that one operation a cell is left (FROM: where 16 registers are
-// left for it).  Its parts cancel near the query, which leaves falloff 64 2^-23 of error in a score: below a weight's
-// rounding up to a falloff of 250, but not below float32's; float32 takes the distances as they are.
+// left for it).  Its parts cancel near the query, which leaves falloff 64 2^-23 of error in a score: 8e-6 for kGentle.  float32,
+// and bfloat16 above that (`steep`), take the distances as they are.
 // kGeneral: places read from LDS (`cell`: 64 x, 64 y).
 template <typename M, int MODE, bool FROM = true>
 struct Penalty {
     static constexpr bool kQuadratic = !M::kWide;
-    bool on;
+    static constexpr float kGentle = 1.f;
+    bool on, steep;
     float fall, x, y, width, per_width;
     __device__ __forceinline__ Penalty(const Params &p, float fall_, float x_, float y_) {
         on = MODE == kRows || (MODE == kGeneral && p.falloff != nullptr);
         fall = fall_;
+        steep = !kQuadratic || fabsf(fall) > kGentle * kLog2e;
         x = x_;
         y = y_;
         width = (float)p.W;
@@ -1012,7 +1014,7 @@ struct Penalty {
     __device__ __forceinline__ f32x16 from(float in) const {
         f32x16 v = {};
         if constexpr (MODE == kRows && FROM && kQuadratic) {
-            const float f = -fall / in;
+            const float f = steep ? 0.f : -fall / in;
 #pragma unroll
             for (int i = 0; i < 16; ++i) v[i] = f * (float)((i % M::kCells) * (i % M::kCells));
         }
@@ -1026,7 +1028,7 @@ struct Penalty {
                 const float c = (float)(cell0 + 32 * k + M::cell(g, h));
                 const float cy = floorf((c + 0.5f) * per_width);
                 const float cx = fmaf(-width, cy, c), dx = cx - x, dy = cy - y;
-                if constexpr (!kQuadratic) {
+                if (steep) {                                   // uniform
                     const float yy = dy * dy;
 #pragma unroll
                     for (int j = 0; j < M::kCells; ++j) {

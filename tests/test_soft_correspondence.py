@@ -893,6 +893,45 @@ def test_caps_that_hardly_bend(sc, dtype, n, c, cap, falloff):
     check_gradients(got, want, dtype, False)
 
 
+@gpu
+@pytest.mark.parametrize("dtype", [F32, BF16])
+@pytest.mark.parametrize("cap", [0.0, 6.0])
+@pytest.mark.parametrize("grid", [(40, 48), (31, 45)])
+@pytest.mark.parametrize("falloff", [1.0, 40.0, 1e3, 3e4])
+def test_steep_falloff_on_the_grid(sc, dtype, falloff, grid, cap):
+    """Queries on cells: the distance of the cell that counts is 0, so scores are as exact as without a falloff, however far
+    those of the cells before it lie below."""
+    q, r, v = inputs(dtype, 1, 32, grid, 0, 8, seed=240)
+    n = grid[0] * grid[1]
+    d_out, d_lse = rand(241, (1, 8) + grid, dtype, unit=False), rand(242, (1, 1, n), F32, unit=False)
+    opts = dict(scale=12.0, falloff=falloff, cap=cap)
+    _, lse = sc.soft_match(*cuda(q, r, v), return_lse=True, **opts)
+    out, got = gradients(sc, *cuda(q, r, v, d_out, d_lse), **opts)
+    want = oracle(flat(q), flat(r), flat(v), 1, 12.0, cap, [falloff], None, grid[1], d_out=flat(d_out), d_lse=host(d_lse))
+    near(out, want[0], want[2], dtype, 1)
+    near_lse(lse, want[1])
+    check_gradients(got, want, dtype, False)
+
+
+@gpu
+@pytest.mark.parametrize("dtype", [F32, BF16])
+@pytest.mark.parametrize("grid", [(40, 48), (31, 45)])
+@pytest.mark.parametrize("n", [7, 50, 200])
+@pytest.mark.parametrize("falloff", [1.0, 1e3, 3e4])
+def test_store_match_steep_falloff(sc, dtype, falloff, n, grid):
+    """The same against a stored view: queries on whole cells of the grid."""
+    store = sc.TemplateStore(1, 32, grid)
+    store.write([0], rand(250, (1, 32) + grid, F32))
+    q = rand(251, (1, 32, n), dtype)
+    g = torch.Generator().manual_seed(252)
+    xy = torch.stack([torch.randint(grid[1], (1, n), generator=g), torch.randint(grid[0], (1, n), generator=g)], 2).float()
+    out, lse = store.soft_match(q.cuda(), [[0]], scale=12.0, falloff=falloff, query_xy=xy, return_lse=True)
+    values = flat(store.read([0]))
+    want = oracle(flat(q), values, values, 1, 12.0, 0.0, [falloff], host(xy), grid[1])
+    near(out, want[0], want[2], dtype, 1)
+    near_lse(lse, want[1])
+
+
 # ------------------------------------------------------------------------------------------------ refusals (no GPU)
 def test_refusals(sc):
     q, r = torch.zeros((2, 8, 4, 4)), torch.zeros((2, 8, 5, 6))
