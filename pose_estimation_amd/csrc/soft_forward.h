@@ -194,9 +194,8 @@ constexpr bool two_resident = std::is_same_v<SRC, BF16> || (kOneBuffer<SRC, WQ> 
 // How far (in units of log2) a query's largest score may rise above the maximum that its sums are kept against before they
 // are rescaled: weights stay below 2^8, and nearly all tiles leave the accumulators alone.
 constexpr float kSlack = 8.f;
-// A tile whose scores rise by more than this over what they were formed against is formed anew: their rounding goes by the
-// rise, which a steep falloff makes far larger than the scores that count.  float32 only: 2^-24 of any rise below 2^16 is
-// lost in bfloat16's weights.
+// A tile whose scores rise by more than this over what they were formed against is formed anew, against its own largest: their
+// rounding goes by the rise, which a steep falloff makes far larger than the scores that count.
 constexpr float kFar = 64.f;
 
 // NC: value channels that one launch forms, from p.c0 on (256 float32 channels take two launches, for the registers).
@@ -279,10 +278,8 @@ __global__ __launch_bounds__(64 * WQ, (two_resident<T, SRC, DP, WQ>) ? 2 : 1) vo
         const int cell0 = next_cell0;
         const char *ktile = feed.k(i), *vtile = feed.v(i);
         const float *cell = feed.cell(i);
-        f32x16 z[kBlocks];
-        bool again = live != 0;
-        while (again) {
-            again = false;
+        f32x16 z[kBlocks] = {};
+        auto form = [&]() __attribute__((always_inline)) {
             // z: scores relative to off.  kPlain: the products, scaled in the exponent.  kCapped: relative to the cap, which
             // stands for the maximum: weights are 2^(-2 cap) > 2^-93 at least.
             if constexpr (DP == 256 && kBlocks == 2) {         // block by block: fewer fragments in registers
@@ -338,18 +335,34 @@ __global__ __launch_bounds__(64 * WQ, (two_resident<T, SRC, DP, WQ>) ? 2 : 1) vo
                         z[k][i] = bits & (1u << M::cell(i, 0)) ? z[k][i] : -__builtin_inff();
                 }
             }
+        };
+        auto largest = [&]() __attribute__((always_inline)) {
+            float top = -__builtin_inff();
+#pragma unroll
+            for (int k = 0; k < kBlocks; ++k)
+#pragma unroll
+                for (int i = 0; i < 16; ++i) top = fmaxf(top, z[k][i]);
+            if (MODE == kPlain) top = fmaf(top, score.in, -off);
+            return fmaxf(top, __shfl_xor(top, 32));
+        };
+        if (live != 0) {
+            form();
             if constexpr (MODE == kCapped) {
                 m = score.top;
             } else {
-                float top = -__builtin_inff();
-#pragma unroll
-                for (int k = 0; k < kBlocks; ++k)
-#pragma unroll
-                    for (int i = 0; i < 16; ++i) top = fmaxf(top, z[k][i]);
-                if (MODE == kPlain) top = fmaf(top, score.in, -off);
-                top = fmaxf(top, __shfl_xor(top, 32));
+                float top = largest();
                 if (__any(top > room)) {
                     stay_branch();
+                    bool far = false;
+                    if constexpr (MODE == kRows || MODE == kGeneral) {
+                        far = off != 0.f && top > kFar;        // there is a maximum, and the tile lies far above it
+                        if (__any(far)) {
+                            stay_branch();
+                            off = far ? off + top : off;                   // rounded by what a rise takes: z tells how far it is off
+                            form();
+                            top = largest();
+                        }
+                    }
                     const float m_new = fmaxf(m, top + off);
                     const float fix = m == -__builtin_inff() ? 0.f : exp2_(m - m_new);
                     m = m_new;
@@ -361,12 +374,14 @@ __global__ __launch_bounds__(64 * WQ, (two_resident<T, SRC, DP, WQ>) ? 2 : 1) vo
                     for (int c = 0; c < NC / 32; ++c)
 #pragma unroll
                         for (int i = 0; i < 16; ++i) o[c][i] *= fix;
-                    if constexpr (M::kWide && MODE != kPlain) again = __any(was != 0.f && off - was > kFar);
-                    if constexpr (MODE != kPlain)
+                    if constexpr (MODE != kPlain) {
+                        // beyond 2^24 the maximum cannot follow the tile's largest score, which still is what weights go by
+                        const float rise = off - was, lift = (far || top > 0.f) && fabsf(top - rise) > 1.f ? top : rise;
 #pragma unroll
                         for (int k = 0; k < kBlocks; ++k)
 #pragma unroll
-                            for (int i = 0; i < 16; ++i) z[k][i] -= off - was;
+                            for (int i = 0; i < 16; ++i) z[k][i] -= lift;
+                    }
                 }
             }
         }
@@ -404,6 +419,12 @@ __global__ __launch_bounds__(64 * WQ, (two_resident<T, SRC, DP, WQ>) ? 2 : 1) vo
     }
     l += __shfl_xor(l, 32);
     LateParams &e = late_params();
+    int late_lane = lane;
+    if constexpr (M::kColumns < 32) {                          // formed anew: a register less through the loop
+        late_lane = threadIdx.x & 63;
+        asm volatile("" : "+v"(late_lane));
+    }
+    const int late_h = late_lane >> 5;
 
     if constexpr (M::kColumns < 32) {
 #pragma unroll
@@ -412,11 +433,11 @@ __global__ __launch_bounds__(64 * WQ, (two_resident<T, SRC, DP, WQ>) ? 2 : 1) vo
     if (q >= e.nq || (lane & 31) >= M::kColumns) return;
     if (e.splits > 1) {
         const int64_t part = (int64_t)split * e.B * e.heads + bh;
-        if (h == 0) {
+        if (late_h == 0) {
             const float2 ml = q_ok ? make_float2(m, l) : make_float2(-__builtin_inff(), 0.f);
             *reinterpret_cast<float2 *>(e.part_ml + (part * e.nq + q) * 2) = ml;
         }
-        store_columns<NC>(e.part_o + part * e.Dv * e.nq, e.nq, q, h, e.c0, e.Dv, o);
+        store_columns<NC>(e.part_o + part * e.Dv * e.nq, e.nq, q, late_h, e.c0, e.Dv, o);
         return;
     }
     const bool some = q_ok && l != 0.f;                        // l is 0 only where no cell takes part (NaN is not)
@@ -425,9 +446,9 @@ __global__ __launch_bounds__(64 * WQ, (two_resident<T, SRC, DP, WQ>) ? 2 : 1) vo
     for (int c = 0; c < NC / 32; ++c)
 #pragma unroll
         for (int i = 0; i < 16; ++i) o[c][i] = some ? o[c][i] * inv : 0.f;
-    store_columns<NC>((typename T::elem *)e.out + (int64_t)bh * e.Dv * e.nq, e.nq, q, h, e.c0, e.Dv, o);
-    if (e.out32 != nullptr) store_columns<NC>(e.out32 + (int64_t)bh * e.Dv * e.nq, e.nq, q, h, e.c0, e.Dv, o);
-    if (h == 0 && e.lse != nullptr)
+    store_columns<NC>((typename T::elem *)e.out + (int64_t)bh * e.Dv * e.nq, e.nq, q, late_h, e.c0, e.Dv, o);
+    if (e.out32 != nullptr) store_columns<NC>(e.out32 + (int64_t)bh * e.Dv * e.nq, e.nq, q, late_h, e.c0, e.Dv, o);
+    if (late_h == 0 && e.lse != nullptr)
         e.lse[(int64_t)bh * e.nq + q] = some ? (m + log2f(l)) * kLn2 : -__builtin_inff();
 }
 

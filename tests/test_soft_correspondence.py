@@ -932,6 +932,32 @@ def test_store_match_steep_falloff(sc, dtype, falloff, n, grid):
     near_lse(lse, want[1])
 
 
+@gpu
+@pytest.mark.parametrize("dtype", [F32, BF16])
+@pytest.mark.parametrize("stored", [False, True])
+@pytest.mark.parametrize("grid", [(40, 48), (31, 45)])
+@pytest.mark.parametrize("n, items", [(0, 48), (50, 1100)])
+@pytest.mark.parametrize("falloff", [40.0, 3e4, 3e7])
+def test_scores_that_rise_late(sc, dtype, stored, grid, n, items, falloff):
+    """Workgroups that walk the whole map, over cells whose scores lie up to 1e11 below those that count.  All items are alike."""
+    q, r, _ = inputs(dtype, 1, 32, grid, n, 0, seed=260)
+    g = torch.Generator().manual_seed(261)
+    xy = torch.stack([torch.randint(grid[1], (1, n), generator=g), torch.randint(grid[0], (1, n), generator=g)], 2).float() if n else None
+    opts = dict(scale=12.0, falloff=falloff, query_xy=xy.expand(items, -1, -1).contiguous() if n else None, return_lse=True)
+    many = q.cuda().expand((items,) + tuple(q.shape[1:])).contiguous()
+    if stored:
+        store = sc.TemplateStore(1, 32, grid)
+        store.write([0], r)
+        out, lse = store.soft_match(many, [[0]] * items, **opts)
+        r = store.read([0])
+    else:
+        out, lse = sc.soft_match(many, r.cuda().expand((items,) + tuple(r.shape[1:])), **opts)
+    want = oracle(flat(q), flat(r), flat(r), 1, 12.0, 0.0, [falloff], host(xy) if n else None, grid[1])
+    near(out[:1], want[0], want[2], dtype, 1)
+    near_lse(lse[:1], want[1])
+    assert (out == out[:1]).all() and (lse == lse[:1]).all()
+
+
 # ------------------------------------------------------------------------------------------------ refusals (no GPU)
 def test_refusals(sc):
     q, r = torch.zeros((2, 8, 4, 4)), torch.zeros((2, 8, 5, 6))
