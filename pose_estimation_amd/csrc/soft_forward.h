@@ -342,15 +342,16 @@ __global__ __launch_bounds__(64 * WQ, (two_resident<T, SRC, DP, WQ>) ? 2 : 1) vo
             for (int k = 0; k < kBlocks; ++k)
 #pragma unroll
                 for (int i = 0; i < 16; ++i) top = fmaxf(top, z[k][i]);
-            if (MODE == kPlain) top = fmaf(top, score.in, -off);
             return fmaxf(top, __shfl_xor(top, 32));
         };
+        float rel = off;                                       // kPlain: what the exponents are relative to
         if (live != 0) {
             form();
             if constexpr (MODE == kCapped) {
                 m = score.top;
             } else {
-                float top = largest();
+                const float peak = largest();
+                float top = MODE == kPlain ? fmaf(peak, score.in, -off) : peak;
                 if (__any(top > room)) {
                     stay_branch();
                     bool far = false;
@@ -364,7 +365,8 @@ __global__ __launch_bounds__(64 * WQ, (two_resident<T, SRC, DP, WQ>) ? 2 : 1) vo
                         }
                     }
                     const float m_new = fmaxf(m, top + off);
-                    const float fix = m == -__builtin_inff() ? 0.f : exp2_(m - m_new);
+                    const bool first = m == -__builtin_inff();
+                    const float fix = first ? 0.f : exp2_(m - m_new);
                     m = m_new;
                     room = m == -__builtin_inff() ? m : kSlack;
                     const float was = off;
@@ -374,8 +376,19 @@ __global__ __launch_bounds__(64 * WQ, (two_resident<T, SRC, DP, WQ>) ? 2 : 1) vo
                     for (int c = 0; c < NC / 32; ++c)
 #pragma unroll
                         for (int i = 0; i < 16; ++i) o[c][i] *= fix;
-                    if constexpr (MODE != kPlain) {
-                        // beyond 2^24 the maximum cannot follow the tile's largest score, which still is what weights go by
+                    // beyond 2^24 the maximum cannot follow the tile's largest score, which still is what weights go by
+                    if constexpr (MODE == kPlain) {
+                        rel = off;
+                        const bool beyond = (first || top > 0.f) && peak > -__builtin_inff() && fabsf(fmaf(peak, score.in, -off)) > 1.f;
+                        if (__any(beyond)) {
+                            stay_branch();
+                            rel = beyond ? 0.f : off;
+#pragma unroll
+                            for (int k = 0; k < kBlocks; ++k)
+#pragma unroll
+                                for (int i = 0; i < 16; ++i) z[k][i] -= beyond ? peak : 0.f;
+                        }
+                    } else {
                         const float rise = off - was, lift = (far || top > 0.f) && fabsf(top - rise) > 1.f ? top : rise;
 #pragma unroll
                         for (int k = 0; k < kBlocks; ++k)
@@ -400,7 +413,7 @@ __global__ __launch_bounds__(64 * WQ, (two_resident<T, SRC, DP, WQ>) ? 2 : 1) vo
                 float w[16];
 #pragma unroll
                 for (int i = 0; i < 16; ++i) {
-                    w[i] = exp2_(MODE == kPlain ? fmaf(score.in, z[k][i], -off) : z[k][i]);
+                    w[i] = exp2_(MODE == kPlain ? fmaf(score.in, z[k][i], -rel) : z[k][i]);
                     sum[i & 1] += w[i];
                 }
                 if constexpr (kCodes) {

@@ -958,6 +958,33 @@ def test_scores_that_rise_late(sc, dtype, stored, grid, n, items, falloff):
     assert (out == out[:1]).all() and (lse == lse[:1]).all()
 
 
+@gpu
+@pytest.mark.parametrize("dtype", [F32, BF16])
+@pytest.mark.parametrize("n", [5, 100])
+@pytest.mark.parametrize("cap", [0.0, 1e9])
+@pytest.mark.parametrize("scale", [1e6, -1e8, 1e9, -1e12, 1e20])
+def test_scores_of_any_size(sc, dtype, n, cap, scale):
+    """Scores whose float32 steps are wider than the exponents of the softmax: the largest one takes all."""
+    q, r, v = inputs(dtype, 1, 32, (20, 20), n, 16, seed=270)
+    mask = silhouette(271, 1, 20, 20)
+    mask[0, :5] = False                                  # tiles without a cell first
+    out, lse = sc.soft_match(*cuda(q, r, v), scale=scale, cap=cap, mask=mask.cuda(), return_lse=True)
+    want = oracle(flat(q), flat(r), flat(v), 1, scale, cap, mask=mask.numpy())
+    # a score is a sum of 32 rounded terms, and rounded as it is stored: 40 2^-24 of the largest at most
+    assert np.isfinite(host(out)).all() and np.abs(host(lse) / want[1] - 1).max() <= 40 * 2.0 ** -24
+    x = scale * flat(q)[0].T @ flat(r)[0][:, mask.numpy().reshape(-1)]
+    z = np.sort(cap * np.tanh(x / cap) if cap else x, 1)
+    clear = z[:, -1] - z[:, -2] > 100 * 2.0 ** -24 * np.abs(z).max() + 100
+    assert clear.any() or cap
+    # the one weight is 2^x with |x| <= 1, not 1, and is divided by itself: w v, 1 / l and their product are rounded as any weight's
+    # are, so that the bound is near's (float32: 3 half steps and what the planes' product leaves out, 8 half steps, below 2e-5)
+    slack = 2e-5 if dtype == F32 else HALF[dtype]
+    err = np.abs(flat(out) - want[0])[0][:, clear]
+    assert (err <= (slack + HALF[dtype]) * np.abs(want[0][0][:, clear])).all()
+    # no average leaves the values' range
+    assert np.abs(host(out)).max() <= np.abs(host(v)).max() * (1 + slack + HALF[dtype])
+
+
 # ------------------------------------------------------------------------------------------------ refusals (no GPU)
 def test_refusals(sc):
     q, r = torch.zeros((2, 8, 4, 4)), torch.zeros((2, 8, 5, 6))
