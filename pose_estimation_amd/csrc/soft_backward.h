@@ -45,24 +45,28 @@ __global__ __launch_bounds__(256) void soft_delta_kernel(const Params p, const f
     delta[bh * p.nq + q] = some ? s : 0.f;
 }
 
+// A weight from its log in units of log2.  The log-sum is off by its own rounding, 2^-24 of itself: scores beyond 2^31 would
+// overflow without the bound (which costs nothing: a modifier of the instruction).
+__device__ __forceinline__ float probability(float x) { return __builtin_amdgcn_fmed3f(exp2_(x), 0.f, 1.f); }
+
 // From products `acc` and w = -(falloff d^2) + minus_lse: w = P and the slope 1 - tanh^2, or at once dx / scale with dP in `dp`.
 template <typename T, int MODE>
 __device__ __forceinline__ void probabilities(const Score<T> &score, const f32x16 &acc, float (&w)[16], float (&slope)[16]) {
     if (MODE == kPlain || MODE == kRows || (MODE == kGeneral && !score.cap)) {
 #pragma unroll
-        for (int i = 0; i < 16; ++i) w[i] = exp2_(fmaf(score.in, acc[i], w[i]));
+        for (int i = 0; i < 16; ++i) w[i] = probability(fmaf(score.in, acc[i], w[i]));
     } else if (Score<T>::kExact || (MODE == kGeneral && score.exact)) {
 #pragma unroll
         for (int i = 0; i < 16; ++i) {
             const float th = score.bend(acc[i], slope[i]);
-            w[i] = exp2_(fmaf(score.top, th, w[i]));
+            w[i] = probability(fmaf(score.top, th, w[i]));
         }
     } else {
         // tanh = 1 - 2 r; the cap itself is in w
 #pragma unroll
         for (int i = 0; i < 16; ++i) {
             const float x = score.two_r(acc[i], slope[i]);
-            w[i] = exp2_(fmaf(-score.top, x, w[i]));
+            w[i] = probability(fmaf(-score.top, x, w[i]));
         }
     }
 }
@@ -71,20 +75,20 @@ __device__ __forceinline__ void weights(const Score<T> &score, const f32x16 &acc
                                         float delta) {
     if (MODE == kPlain || MODE == kRows || (MODE == kGeneral && !score.cap)) {
 #pragma unroll
-        for (int i = 0; i < 16; ++i) w[i] = exp2_(fmaf(score.in, acc[i], w[i])) * (dp[i] - delta);
+        for (int i = 0; i < 16; ++i) w[i] = probability(fmaf(score.in, acc[i], w[i])) * (dp[i] - delta);
     } else if (Score<T>::kExact || (MODE == kGeneral && score.exact)) {
 #pragma unroll
         for (int i = 0; i < 16; ++i) {
             float slope;
             const float th = score.bend(acc[i], slope);
-            w[i] = exp2_(fmaf(score.top, th, w[i])) * ((dp[i] - delta) * slope);
+            w[i] = probability(fmaf(score.top, th, w[i])) * ((dp[i] - delta) * slope);
         }
     } else {
 #pragma unroll
         for (int i = 0; i < 16; ++i) {
             float slope;
             const float x = score.two_r(acc[i], slope);
-            w[i] = exp2_(fmaf(-score.top, x, w[i])) * ((dp[i] - delta) * slope);
+            w[i] = probability(fmaf(-score.top, x, w[i])) * ((dp[i] - delta) * slope);
         }
     }
 }

@@ -985,6 +985,23 @@ def test_scores_of_any_size(sc, dtype, n, cap, scale):
     assert np.abs(host(out)).max() <= np.abs(host(v)).max() * (1 + slack + HALF[dtype])
 
 
+@gpu
+@pytest.mark.parametrize("dtype", [F32, BF16])
+@pytest.mark.parametrize("n", [5, 100])
+@pytest.mark.parametrize("opts", [dict(), dict(cap=1e9), dict(falloff=0.05), dict(cap=1e13, falloff=0.05)])
+@pytest.mark.parametrize("scale", [1e9, -1e12, 1e20])
+def test_gradients_of_scores_of_any_size(sc, dtype, n, opts, scale):
+    """A weight formed from a log-sum that is wider rounded than an exponent is still a weight: at most 1."""
+    q, r, v = inputs(dtype, 1, 32, (20, 24), n, 16, seed=280)
+    if "falloff" in opts:
+        opts = opts | dict(query_xy=torch.rand((1, n, 2), generator=torch.Generator().manual_seed(281)) * 19)
+    d_out = rand(282, (1, 16, n), dtype, unit=False)
+    out, got = gradients(sc, *cuda(q, r, v, d_out), None, scale=scale, **opts)
+    assert np.isfinite(host(out)).all() and all(np.isfinite(host(g)).all() for g in got)
+    most = np.abs(host(d_out)).sum(2)[:, :, None, None]
+    assert (np.abs(host(got[2])) <= most * (1 + n * HALF[dtype])).all()
+
+
 # ------------------------------------------------------------------------------------------------ refusals (no GPU)
 def test_refusals(sc):
     q, r = torch.zeros((2, 8, 4, 4)), torch.zeros((2, 8, 5, 6))
