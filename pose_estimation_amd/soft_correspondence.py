@@ -19,6 +19,7 @@ from torch.autograd import forward_ad
 from . import _abi, _device as dv
 
 _CODES = {torch.float32: _abi.F32, torch.bfloat16: _abi.BF16}
+_COUNTS = {torch.uint8, torch.int8, torch.uint16, torch.int16, torch.uint32, torch.int32, torch.int64}
 MAX_CHANNELS = _abi.SOFT_MAX_CHANNELS
 _HERE = contextlib.nullcontext()
 
@@ -125,7 +126,7 @@ def _counts(num_query, batch):
     t = num_query if dv.is_tensor(num_query) else np.asarray(num_query)
     if math.prod(t.shape) != batch:
         raise ValueError("num_query must hold one count per batch item")
-    if t.dtype.is_floating_point if dv.is_tensor(t) else t.size and t.dtype.kind not in "iu":
+    if t.dtype not in _COUNTS if dv.is_tensor(t) else t.size and t.dtype.kind not in "iu":
         raise ValueError("num_query must hold integers")
     return t.reshape(-1)
 
@@ -135,8 +136,10 @@ def _count_tensor(num_query, device):
     if num_query is None:
         return None
     low, high = -1, 2 ** 31 - 1
-    num_query = num_query.clamp(low, high) if dv.is_tensor(num_query) and num_query.dtype == torch.int64 else \
-        num_query if dv.is_tensor(num_query) else np.clip(num_query, low, high)
+    if not dv.is_tensor(num_query):
+        num_query = np.clip(num_query, low, high)
+    elif num_query.dtype in (torch.uint32, torch.int64):
+        num_query = num_query.to(torch.int64).clamp(low, high)
     return _on(num_query, torch.int32, device)
 
 

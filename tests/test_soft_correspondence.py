@@ -1002,6 +1002,18 @@ def test_gradients_of_scores_of_any_size(sc, dtype, n, opts, scale):
     assert (np.abs(host(got[2])) <= most * (1 + n * HALF[dtype])).all()
 
 
+@gpu
+@pytest.mark.parametrize("dtype", [torch.uint8, torch.int8, torch.uint16, torch.int16, torch.uint32, torch.int32, torch.int64])
+def test_counts_of_every_type(sc, dtype):
+    """A count above every query map means all of it, also one that int32 does not hold."""
+    q, r, _ = inputs(F32, 2, 16, (5, 6), 40, seed=290)
+    most = min(torch.iinfo(dtype).max, 2 ** 63 - 1)
+    count = torch.from_numpy(np.array([most, 7], dtype=str(dtype).split(".")[1]))
+    want = sc.soft_match(*cuda(q, r), num_query=[40, 7])
+    for x in (count, count.cuda()):
+        assert torch.equal(sc.soft_match(*cuda(q, r), num_query=x), want)
+
+
 # ------------------------------------------------------------------------------------------------ refusals (no GPU)
 def test_refusals(sc):
     q, r = torch.zeros((2, 8, 4, 4)), torch.zeros((2, 8, 5, 6))
@@ -1043,6 +1055,15 @@ def test_refusals(sc):
         call = dict(query=q, ref=r) | args
         with pytest.raises(ValueError, match=match):
             sc.soft_match(call.pop("query"), call.pop("ref"), call.pop("value", None), **call)
+
+
+def test_counts_of_other_types_are_refused(sc):
+    q, r = torch.zeros((2, 8, 4, 4)), torch.zeros((2, 8, 5, 6))
+    for dtype in (torch.bool, torch.complex64, torch.uint64, torch.float16):
+        with pytest.raises(ValueError, match="num_query must hold integers"):
+            sc.soft_match(q, r, num_query=torch.ones(2).to(dtype))
+    with pytest.raises(ValueError, match="num_query must hold integers"):
+        sc.soft_match(q, r, num_query=[True, False])
 
 
 def test_learned_scale_and_cap_are_refused(sc):
