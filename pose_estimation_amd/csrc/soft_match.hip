@@ -188,6 +188,7 @@ size_t backward_bytes(int dtype, const Plan &dq, const Plan &dkv, int B, int hea
 
 int check_score(float scale, float cap, const float *falloff, int W) {
     ISPA_REQUIRE(std::isfinite(scale) && std::isfinite(cap) && cap >= 0.f, "scale %g, cap %g: finite, cap >= 0 wanted", scale, cap);
+    ISPA_REQUIRE(cap == 0.f || (cap >= 1e-30f && std::fabs(scale) <= 1e30 * cap), "cap %g is too small for scale %g", cap, scale);
     ISPA_REQUIRE(falloff == nullptr || W >= 1, "falloff needs the map's width");
     return ISPA_OK;
 }

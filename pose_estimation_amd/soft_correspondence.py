@@ -96,6 +96,8 @@ def _scores(heads, scale, cap, falloff, query_xy, grid, query_shape, batch, n):
         raise ValueError(f"scale must be finite, got {scale}")
     if not (math.isfinite(cap) and cap >= 0):
         raise ValueError(f"cap must be finite and not negative (0 or None: no cap), got {cap}")
+    if 0 < cap and (cap < 1e-30 or abs(scale) > 1e30 * cap):   # 0 or an infinite quotient in float32
+        raise ValueError(f"cap {cap} is too small for scale {scale}")
     if falloff is not None:
         if grid is None:
             raise ValueError("falloff needs a reference map (B,C,H,W): distances are taken on its grid")
@@ -103,8 +105,8 @@ def _scores(heads, scale, cap, falloff, query_xy, grid, query_shape, batch, n):
             raise ValueError(f"falloff: queries {query_shape} do not lie on the reference grid {grid}; give query_xy")
         if not np.isscalar(falloff) and _dims(falloff) != (heads,):
             raise ValueError(f"falloff must be a number or hold one value per head ({heads})")
-        if not dv.is_tensor(falloff) and not np.isfinite(np.asarray(falloff, np.float64)).all():
-            raise ValueError(f"falloff must be finite, got {falloff}")
+        if not dv.is_tensor(falloff) and not (np.abs(np.asarray(falloff, np.float64)) < 1e38).all():
+            raise ValueError(f"falloff must be finite in float32, got {falloff}")
         if query_xy is not None and _dims(query_xy) != (batch, n, 2):
             raise ValueError(f"query_xy must be ({batch},{n},2), got {_dims(query_xy)}")
     return scale, cap

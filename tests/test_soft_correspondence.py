@@ -1066,6 +1066,18 @@ def test_counts_of_other_types_are_refused(sc):
         sc.soft_match(q, r, num_query=[True, False])
 
 
+def test_numbers_that_float32_does_not_hold_are_refused(sc):
+    from pose_estimation_amd import _abi
+    q, r = torch.zeros((2, 8, 5, 6)), torch.zeros((2, 8, 5, 6))
+    for args, match in [(dict(cap=1e-50), "too small"), (dict(cap=1e-31), "too small"), (dict(cap=1e-5, scale=-1e26), "too small"),
+                        (dict(falloff=1e39), "finite in float32"), (dict(falloff=[-1e38]), "finite in float32")]:
+        with pytest.raises(ValueError, match=match):
+            sc.soft_match(q, r, **args)
+    for cap, scale in ((1e-31, 1.0), (1e-5, -1e26)):
+        assert _abi.lib.ispa_soft_match(1, 1, None, 0, 1, 1, 64, 64, 10, 100, 10, scale, cap, None, None, None, None, 1, None, None, None, 0,
+                                        None) == -1 and b"too small" in _abi.lib.ispa_last_error()
+
+
 def test_learned_scale_and_cap_are_refused(sc):
     q, r = torch.zeros((2, 8, 4, 4)), torch.zeros((2, 8, 5, 6))
     learned = torch.tensor(3.0, requires_grad=True)
