@@ -824,11 +824,10 @@ struct Direct {
         const uint32_t hi = (uint32_t)__builtin_amdgcn_readfirstlane((int)(uint32_t)(sbase >> 32));
         const uint32_t lo = (uint32_t)__builtin_amdgcn_readfirstlane((int)(uint32_t)sbase);
         const unsigned m0 = (unsigned)__builtin_amdgcn_readfirstlane((int)dst);
-        // nothing else in these kernels uses m0 (LDS instructions do not read it)
         asm volatile("s_mov_b32 m0, %1\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %0, %2"
                      :
                      : "v"(voff), "s"(m0), "s"((uint64_t)hi << 32 | lo)
-                     : "memory");
+                     : "memory", "m0");
     }
     __device__ __forceinline__ static void wait() { asm volatile("s_waitcnt vmcnt(0)" ::: "memory"); }
     // After wait(): zeros for the cells that take no part (see Loader), in the segments this lane itself has copied.
