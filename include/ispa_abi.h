@@ -380,15 +380,16 @@ int ispa_prune_points_2d(double *coords, int B, int64_t n, const uint8_t *flags,
  *   P = softmax over the cells j that take part;   out_ci = sum_j P_ij v_cj;   lse_i = log sum_j exp(z_ij)
  * q (B, heads*D, nq), r (B, heads*D, cells), v (B, heads*Dv, cells) of one dtype, ISPA_F32 or ISPA_BF16; head h has
  * channels [h*D, (h+1)*D).  v NULL: r is the value map too (Dv = D).  D and Dv: 1 to ISPA_SOFT_MAX_CHANNELS.
- * cap: 0 (none) or at least 1e-30 and 1e-30 |scale|.  falloff (heads) f32 or NULL; query_xy (B,nq,2) f32 [x, y] in cells, or NULL: query i lies on cell i.
+ * cap: 0 (none) or at least 1e-30 and 1e-30 |scale|.  falloff (heads) f32 or NULL; query_xy (B,nq,2) f32 [x, y] in cells, or
+ * NULL: query i lies on cell i.
  * mask (B,cells) u8 or NULL: a cell with 0 takes no part, whatever its features hold; all others are to be finite, and
  * falloff and query_xy of real queries too.
  * num_query (B) i32 or NULL: only the first num_query[b] queries are real.
  * out (B, heads*Dv, nq) of the dtype; out32 (optional) the same in float32 before its rounding, which the backward call
  * wants; lse (optional) (B,heads,nq) f32.  A query that is not real or has no cell gets out 0 and lse -inf.
  * Sums, maxima and log-sums are float32; with ISPA_BF16 the softmax weights are rounded to bfloat16 for the
- * product with v (and the gradients' weights for theirs).  Few queries: the cells are split over workgroups and the parts joined by a second launch, in a fixed
- * order (results do not change from run to run).  q, r, v (and d_out below) start on 16-byte borders.  workspace (256-byte
+ * product with v (and the gradients' weights for theirs).  Few queries: the cells are split over workgroups and the parts
+ * joined by a second launch, in a fixed order (results do not change from run to run).  q, r, v (and d_out below) start on 16-byte borders.  workspace (256-byte
  * aligned): ispa_soft_match_workspace_bytes(...) with views = 1. */
 #define ISPA_SOFT_MAX_CHANNELS 256
 size_t ispa_soft_match_workspace_bytes(int dtype, int B, int heads, int D, int Dv, int64_t nq, int views, int64_t cells);

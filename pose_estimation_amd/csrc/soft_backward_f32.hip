@@ -1,4 +1,4 @@
-// Soft correspondence, backward kernels on float32 MFMAs.
+// Soft correspondence, backward kernels of float32 maps (bfloat16 MFMAs on three planes, float32 MFMAs: see Arithmetic).
 #include "soft_backward_impl.h"
 
 namespace ispa_soft {

@@ -2,13 +2,13 @@
 // running maximum m and sum l per query (float32, in units of log2).
 //
 // What bounds it (MI355X):
-//   bfloat16, many queries: 64 pairs of 64x64x128 with a falloff 0.59 to 0.61 ms, 0.91 PFLOP/s, 66 % of what a large matrix product
-//   reaches.  The matrix pipe is busy 43 % of the cycles and the vector ALU 55 %, one after the other: two waves a SIMD, with
-//   unequal priorities, hide waits but not each other's issue.  Hence one operation a cell for the falloff (Penalty), the
-//   lazy rescale (kSlack), the fixed maximum of kCapped.  Reading value fragments ahead, or exponentials between the
-//   products, cost 3 to 5 % more cycles.
-//   float32, many queries: six bfloat16 products for one, 64x64x128 58 to 60 us, 145 TFLOP/s, where a float32 matrix product
-//   reaches 153; copying the maps into planes takes 4 us of it.
+//   bfloat16, many queries: 64 pairs of 64x64x128 with a falloff 0.58 to 0.62 ms, by the card, 0.89 to 0.95 PFLOP/s, 64 to 69 % of
+//   what a large matrix product reaches.  The matrix pipe is busy 43 % of the cycles and the vector ALU 54 %, one after the
+//   other: two waves a SIMD, with unequal priorities, hide waits but not each other's issue.  Hence one operation a cell for
+//   the falloff (Penalty), the lazy rescale (kSlack), the fixed maximum of kCapped.  Reading value fragments ahead, or
+//   exponentials between the products, cost 3 to 5 % more cycles.
+//   float32, many queries: six bfloat16 products for one, 64x64x128 58 to 62 us, 139 to 148 TFLOP/s, where a float32 matrix
+//   product reaches 153; copying the maps into planes takes 4 us of it.
 //   few queries: 10 against 28x28x128 in 12 us and 4 to join: a launch, a query column's loads, one tile, its stores.
 #pragma once
 #include "soft_tile.h"

@@ -33,7 +33,7 @@ inline Arithmetic arithmetic(bool f32, bool codes, int padded, int waves) {
 inline int64_t tile_rows(Arithmetic a) { return a == kFloat ? 32 : 64; }
 
 // Whether float32 queries against codes come as columns of planes (F32Q): as many as three times fit a wave's 32 columns, with
-// a free group for sums over rows of 16 lanes.  One query against 24 views of 128x128x256: 61 us, with three products
+// a free group for sums over rows of 16 lanes.  One query against 24 views of 128x128x256: 58 us, with three products
 // and a wave a SIMD 90 us.
 inline bool few_columns(bool f32, int64_t owned) { return f32 && owned <= 8; }
 

@@ -450,7 +450,9 @@ struct SplitMath {
                 o.f[x][s] = __builtin_bit_cast(bf16x8, __builtin_bit_cast(u32x4, o.f[x][s]) ^ 0x80008000u);
         });
     }
-    // Planes x of one side and y of the other are multiplied where x + y < 3: what is left out lies below 2^-24.
+    // Planes x of one side and y of the other are multiplied where x + y < 3.  Planes are cut, not rounded: what is left out, mid lo
+    // and lo mid in the main, has the product's sign and is 2^-21 of it at worst (7.8 half steps of float32), 2^-24.5 on
+    // average.  Sums come out as near to 64 bits as those of float32 MFMAs (64x64x128: 2.8e-7, a float32 matrix product 1.3e-6).
     template <int N, bool AHEAD = true>
     __device__ __forceinline__ static void first(const char *tile, const Addr &a, int b0, const Owned &o, f32x16 (&acc)[N],
                                                  const f32x16 &from = f32x16{}) {
@@ -919,7 +921,7 @@ template <typename T>
 struct Score {
     // tanh(y) = 1 - 2 r, r = 1 / (exp(2 y) + 1), has an absolute error of 2e-7, the cap's share of which is far below what the inputs of
     // the bfloat16 kernels leave in a score as long as the cap is small: 1.3e-5 for kPlainCap.  float32, and bfloat16 above that
-    // (`exact`: 8 forward passes of 64x64x128 with a cap 143 us for 115, with gradients 640 for 490), keep the relative error near
+    // (`exact`: 8 pairs of 64x64x128 forward 140 us for 109, with gradients 622 for 484), keep the relative error near
     // 1e-7 too: below 0.6 the odd polynomial y + y^3 c(y^2), c fitted to (tanh(y) / y - 1) / y^2 on [0, 0.36] by weighted least
     // squares.
     static constexpr bool kExact = !std::is_same_v<T, BF16>;

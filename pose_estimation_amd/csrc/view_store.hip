@@ -51,8 +51,10 @@ __device__ __forceinline__ unsigned char encode(float v) {
 }
 
 // A block takes 64 cells of one view, a wave's lanes side by side, and its waves share the channels: 4 to read, 8 to write.
-// Memory bounds both: 24 views of 56x56x128 float32, 48 MB either way, are written in 14.6 us (3.3 TB/s) and read in 9 to 11 us
-// (a large copy: 4.8 TB/s).  (16 or 4 bytes a lane, four cells to a thread, took longer both ways: 13.7 us for 9.2 to
+// 24 views of 56x56x128 float32, 48 MB either way, are written in 14.7 us (3.3 TB/s) and read in 9 to 11 us (4.4 to 5.3; a large copy:
+// 4.8 TB/s).  Memory bounds the read.  The write has the vector ALU busy 66 % of the cycles with settling codes, and its waves
+// wait half of theirs; 17 views of 31x47x200 bfloat16 into e4m3, 15 MB, take 20 us, with 42 % and two thirds: too few waves to
+// hide the steps of a code behind each other.  (16 or 4 bytes a lane, four cells to a thread, took longer both ways: 13.7 us for 9.2 to
 // read them, 23.6 us for 18.6 to write them: fewer lanes to a row.)
 constexpr int kCellsPer = 64, kGroups = kThreads / kCellsPer, kWriters = 8;
 

@@ -314,8 +314,9 @@ def soft_match(query, ref, value=None, *, heads=1, scale=None, cap=0.0, falloff=
     Tensors that require gradients get them (out and lse, once, in reverse mode; value None: ref's is the sum of both uses); no gradient
     flows to falloff, query_xy or the masks, and a scale or cap that requires one is refused: they are numbers (a learned
     temperature multiplies query).  Scores, sums and log-sums are float32; bfloat16 maps round the weights to
-    bfloat16 for the product with the values.  Memory grows with the maps, not with their product, and results do
-    not change from run to run."""
+    bfloat16 for the product with the values.  Gradients form their weights from the log-sums, which are off by 2^-24 of
+    themselves, as the scores are: scores far beyond 1e5 have no gradients to speak of.  Memory grows with the maps, not with
+    their product, and results do not change from run to run."""
     as_tensor = dv.is_tensor(query)
     call = _Call(query, ref, value, heads, scale, cap, falloff, query_xy, mask, num_query)
     if torch.is_grad_enabled() and any(dv.is_tensor(x) and x.requires_grad for x in (query, ref, value)):
@@ -339,7 +340,8 @@ class TemplateStore:
 
     codes (n_view,C,H*W) int8 or float8_e4m3fn, scales (n_view,H*W) float32, mask (n_view,H*W) uint8, on one device.
     A cell's channels share the scale max|x| / 127 ("fp8": / 448); the value is code * scale, so an int8 code is off
-    by at most half a scale, an e4m3 one by 2^-4 of itself.  Views not yet written have no cells.
+    by at most half a scale, an e4m3 one by 2^-4 of x or, below 2^-6 scales, by 2^-10 scales.  Views not yet written have no
+    cells.
 
     Calls run on the current stream; a store that several streams use is ordered by the caller, like any tensor."""
 
