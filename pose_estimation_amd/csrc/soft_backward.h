@@ -1,10 +1,11 @@
 // Soft correspondence, backward.  With P recomputed from the stored log-sum (see soft_tile.h for the tile scheme):
 //   delta_i = sum_c do_ci o_ci - dlse_i      dP_ij = sum_c do_ci v_cj      dx_ij = P_ij (dP_ij - delta_i) (1 - tanh^2)
 //   dq_ci = scale sum_j dx_ij k_cj           dk_cj = scale sum_i dx_ij q_ci           dv_cj = sum_i P_ij do_ci
-// Two kernels, one per owned side: scores and dP are formed twice (7 products instead of 5; 8 where the gradients of reference and
-// value take a launch each, see dkv_two_launches: scores three times), and in exchange no gradient is summed with atomics - every sum has a fixed order and two runs agree bit for bit.  P and dx are rounded to bfloat16 for
-// the products of bfloat16 maps (2^-9 of a weight on average, beside the result's own rounding; in two terms of bfloat16
-// the kernels of up to 64 channels took 30 to 40 % longer).
+// Two kernels, one per owned side: scores and dP are formed twice (7 products instead of 5; 8 where the gradients of reference
+// and value take a launch each, see dkv_two_launches: scores three times), and in exchange no gradient is summed with
+// atomics - every sum has a fixed order and two runs agree bit for bit.  P and dx are rounded to bfloat16 for the products of
+// bfloat16 maps (2^-9 of a weight on average, beside the result's own rounding; in two terms of bfloat16 the kernels of up to
+// 64 channels took 30 to 40 % longer).
 //
 // What bounds it (MI355X): 16 pairs of 64x64x128, bfloat16, reference and value one map: forward 0.16, query gradient 0.19,
 // value's part 0.16, reference's 0.22 ms; in the gradients the matrix pipe is 38 to 47 % busy, the vector ALU 44 to 54 %,
